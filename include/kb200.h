@@ -35,7 +35,7 @@
 extern "C" {
 #endif
 
-#define KB200_ABI_VERSION 5
+#define KB200_ABI_VERSION 6
 
 #define KB200_MAX_RANK 6      /* iteration dims after the host collapsed contiguous ones */
 #define KB200_MAX_OPERANDS 12 /* distinct tensors one fused kernel touches */
@@ -48,7 +48,8 @@ typedef enum kb200_status {
   KB200_ERR_BOUNDS = -3,      /* an operand's span leaves the buffer it is bound to */
   KB200_ERR_CUDA = -4,        /* a CUDA call failed; message carries cudaGetErrorString */
   KB200_ERR_UNBOUND = -5,     /* launch before kb200_plan_bind */
-  KB200_ERR_DEVICE_WAIT = -6  /* a bounded device-side wait ran out (see kb200_plan_status) */
+  KB200_ERR_DEVICE_WAIT = -6, /* a bounded device-side wait ran out (see kb200_plan_status) */
+  KB200_ERR_PAGES = -7        /* a cache had fewer free pages than were asked for (see kb200_cache_status; maps to MemoryError) */
 } kb200_status;
 
 /* Where a tensor lives.  Mirrors the `bases` keys of the reference's Launch
@@ -339,6 +340,120 @@ int kb200_matmul_bf16_static(const float* a, const float* b, float* c, int64_t m
  * last kb200_matmul_bf16_static call that passed status_word == NULL ran out on the current device
  * (a blocking 4-byte copy; allocates nothing).  No counterpart in the reference. */
 int kb200_matmul_bf16_static_status(void);
+
+/* ---- keys and values in pages ----------------------------------------------------------------
+ * What a compiled graph cannot do: keep K and V between calls, so that the next tokens of a sequence cost their own rows
+ * only.  No counterpart in the reference.  A cache holds `sequences` sequences of a model's `layers` layers in pages of
+ * `page_tokens` tokens; which pages a sequence has is the same in all layers.
+ *
+ *   pool    [layers, 2 (K, V), pages, kv_heads, page_tokens, head_dim] of `dtype`, 16-byte aligned
+ *   table   [sequences, max_pages]: the pages of a sequence in the order of its tokens, -1 behind them
+ *   held    [sequences]: how many pages that is
+ *   lengths [sequences]: committed tokens.  Drafted ones are written behind them (kb200_cache_append) and become
+ *           committed by kb200_cache_accept.
+ *   refs    [pages]: how many sequences hold the page (0 = free; a caller may keep pages for itself by counting them)
+ *
+ * All of it is device memory of the caller's, int32 but for the pool, consistent when the cache is created (an empty cache: table -1, the
+ * rest 0; the pool may hold anything) and changed by these functions only, or by the caller between them.  Sequences may
+ * share pages (kb200_cache_fork); what is written is made the writer's own first (kb200_cache_reserve).
+ *
+ * Every operation is enqueued on `cuda_stream`, reads its arguments and the cache's state on the device, and neither
+ * allocates nor synchronises: capturable, and a replayed graph follows what the tables hold then.  Operations that change a cache use scratch
+ * of its own and are ordered by the caller, like the launches of one plan; kb200_cache_attend only reads it and takes its
+ * workspace from the caller, so that calls may overlap.  Page numbers and
+ * indexes that are out of range are never followed: what they stand for is left out (a page of the table: read as zeros) and
+ * said in the status word. */
+typedef struct kb200_cache kb200_cache;
+
+typedef enum kb200_dtype { KB200_DTYPE_FP32 = 0, KB200_DTYPE_BF16 = 1, KB200_DTYPE_FP16 = 2 } kb200_dtype;
+
+typedef struct kb200_cache_desc {
+  int32_t dtype;        /* kb200_dtype */
+  int32_t layers;
+  int32_t sequences;
+  int32_t max_pages;    /* columns of the table; max_pages * page_tokens < 2^30 */
+  int32_t pages;
+  int32_t kv_heads;
+  int32_t page_tokens;  /* 8, 16, 32, 64, 128 or 256 */
+  int32_t head_dim;     /* a multiple of 16 up to 256 */
+  void* pool;
+  uint64_t pool_bytes;
+  int32_t* table;
+  int32_t* held;
+  int32_t* lengths;
+  int32_t* refs;
+} kb200_cache_desc;
+
+/* Rows of new tokens, [batch, tokens, heads, head_dim] with head_dim contiguous; strides in elements, each a multiple of 16
+ * bytes like the address. */
+typedef struct kb200_rows {
+  void* data;
+  int32_t dtype;        /* the cache's, or KB200_DTYPE_FP32: rounded to it */
+  int32_t heads;
+  int64_t stride[3];
+} kb200_rows;
+
+/* Bits of a cache's status word, by which kb200_cache_status tells what was left out. */
+typedef enum kb200_cache_fault {
+  KB200_CACHE_NO_PAGES = 1,   /* kb200_cache_reserve: fewer free pages than needed; nothing was reserved */
+  KB200_CACHE_TOO_LONG = 2,   /* ... a sequence would need more than max_pages; nothing was reserved */
+  KB200_CACHE_BAD_INDEX = 4,  /* a sequence, count, kept token or page out of range, a sequence given twice to kb200_cache_append */
+  KB200_CACHE_NO_ROOM = 8,    /* a token's position has no page (see kb200_cache_reserve) */
+  KB200_CACHE_SHARED = 16     /* a write into a page that another sequence holds as well */
+} kb200_cache_fault;
+
+/* Whether kb200_cache_create takes the description; needs no GPU. */
+int kb200_cache_check(const kb200_cache_desc* desc);
+
+/* Checks the description, allocates the cache's scratch and status word on `device`.  The tables are not touched. */
+int kb200_cache_create(const kb200_cache_desc* desc, int device, kb200_cache** out);
+
+/* For every sequence s at once: it becomes what sequence sources[s] was before the call, sharing its pages; -1 leaves it
+ * empty, s as it is.  Pages that nobody holds any more are free.  sources: [sequences]. */
+int kb200_cache_fork(kb200_cache* cache, const int32_t* sources, void* cuda_stream);
+
+/* Room for counts[s] tokens behind every sequence's committed ones, in pages of its own: pages that it lacks, and shared ones
+ * in that range, are taken from the free pages, lowest first, in the order of the sequences and of their tokens.  A shared page all of whose
+ * holders write in this call stays with the lowest of them.  The committed tokens of a replaced page are copied, in all layers; what lay behind
+ * them is not kept.  All or nothing: if the pages do not suffice the cache stays as it is.  counts: [sequences]. */
+int kb200_cache_reserve(kb200_cache* cache, const int32_t* counts, void* cuda_stream);
+
+/* Keeps the first lengths[s] tokens of every sequence and frees the pages behind them; a negative entry leaves the sequence
+ * as it is.  lengths: [sequences]; the cache's own array gives back what was reserved and not used. */
+int kb200_cache_truncate(kb200_cache* cache, const int32_t* lengths, void* cuda_stream);
+
+/* Moves pages so that those in use come first: the used pages behind their own number fill the free ones before it, both in
+ * ascending order.  Sequences see the same tokens; the pages behind are free and keep what they held. */
+int kb200_cache_compact(kb200_cache* cache, void* cuda_stream);
+
+/* Writes K and V of new tokens of one layer: token i < counts[b] of batch row b goes to position lengths[slots[b]] + i.
+ * counts NULL: all `tokens`; slots NULL: row b is sequence b.  Needs room (kb200_cache_reserve). */
+int kb200_cache_append(kb200_cache* cache, int layer, const kb200_rows* k, const kb200_rows* v, int rows, int tokens,
+                       const int32_t* counts, const int32_t* slots, void* cuda_stream);
+
+/* Commits counts[s] of the tokens drafted behind each sequence: those with the ascending indexes kept[s * kept_width + i], which
+ * are moved together in all layers (kept NULL: the first ones, which stay where they are), and frees the pages behind them.
+ * A sequence whose entries are not ascending, or have no pages, or would move within shared pages, stays as it is. */
+int kb200_cache_accept(kb200_cache* cache, const int32_t* counts, const int32_t* kept, int kept_width, void* cuda_stream);
+
+/* Attention of drafted tokens: out[b, i, h] = sum_j softmax_j(scale * q[b, i, h] . k[j, g]) v[j, g], g = h * kv_heads / heads, over
+ * the committed tokens j of sequence slots[b] and over the drafted ones t < counts[b] behind them with
+ * mask[b * mask_stride[0] + i * mask_stride[1] + t * mask_stride[2]] != 0 (bytes; mask NULL: t <= i).  Tokens that a row does not see
+ * contribute nothing, whatever they hold.  A row that sees nothing, and rows i >= counts[b], are 0.  One token per sequence is ordinary decoding.
+ * q and out: [rows, tokens, heads, head_dim]; out has the cache's type, q that or float32 (rounded to it).  Products of 16-bit types are
+ * summed in float32, the weights rounded to that type in front of V; float32 is multiplied as in the plans' FP32 precision (three products
+ * of split operands; NaN where a row sees infinities).
+ * workspace: kb200_cache_attend_workspace bytes, 16-byte aligned, used by this call alone until it has run. */
+uint64_t kb200_cache_attend_workspace(const kb200_cache* cache, int rows, int tokens, int heads);
+int kb200_cache_attend(kb200_cache* cache, int layer, const kb200_rows* q, const kb200_rows* out, int rows, int tokens,
+                       const uint8_t* mask, const int64_t* mask_stride, const int32_t* counts, const int32_t* slots, float scale,
+                       void* workspace, uint64_t workspace_bytes, void* cuda_stream);
+
+/* After the caller synchronised: 0, or what the operations since the last call left out (KB200_ERR_PAGES where pages
+ * were short, else KB200_ERR_BOUNDS; the text names the bits).  A blocking 4-byte copy; clears the status word. */
+int kb200_cache_status(kb200_cache* cache);
+
+void kb200_cache_destroy(kb200_cache* cache);
 
 #ifdef __cplusplus
 }

@@ -16,7 +16,7 @@ import subprocess
 import sysconfig
 from pathlib import Path
 
-ABI_VERSION = 5
+ABI_VERSION = 6
 MAX_RANK, MAX_OPERANDS, MAX_TAPE = 6, 12, 96
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -46,7 +46,7 @@ OPCODES = {
     "rsqrt": 17, "sqrt": 18, "copy": 19, "reduce_sum": 20, "reduce_max": 21, "STORE": 22,
 }
 STATUS_EXC = {-1: ValueError, -2: NotImplementedError, -3: ValueError, -4: RuntimeError, -5: RuntimeError,
-              -6: RuntimeError}
+              -6: RuntimeError, -7: MemoryError}
 
 
 class TapeOp(C.Structure):
@@ -65,6 +65,16 @@ class KernelDesc(C.Structure):
                 ("a_slot", C.c_int32), ("b_slot", C.c_int32), ("n_operands", C.c_int32), ("n_tape", C.c_int32),
                 ("operands", Operand * MAX_OPERANDS), ("tape", TapeOp * MAX_TAPE),
                 ("cfg", C.c_int32 * 8), ("name", C.c_char * 32)]
+
+
+class CacheDesc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("layers", C.c_int32), ("sequences", C.c_int32), ("max_pages", C.c_int32), ("pages", C.c_int32),
+                ("kv_heads", C.c_int32), ("page_tokens", C.c_int32), ("head_dim", C.c_int32), ("pool", C.c_void_p),
+                ("pool_bytes", C.c_uint64), ("table", C.c_void_p), ("held", C.c_void_p), ("lengths", C.c_void_p), ("refs", C.c_void_p)]
+
+
+class Rows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("dtype", C.c_int32), ("heads", C.c_int32), ("stride", C.c_int64 * 3)]
 
 
 EXPORTS = {
@@ -90,6 +100,20 @@ EXPORTS = {
     "kb200_matmul_bf16_static": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int64,
                                            C.c_void_p, C.c_void_p]),
     "kb200_matmul_bf16_static_status": (C.c_int, []),
+    "kb200_cache_check": (C.c_int, [C.POINTER(CacheDesc)]),
+    "kb200_cache_create": (C.c_int, [C.POINTER(CacheDesc), C.c_int, C.POINTER(C.c_void_p)]),
+    "kb200_cache_fork": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "kb200_cache_reserve": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "kb200_cache_truncate": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "kb200_cache_compact": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "kb200_cache_append": (C.c_int, [C.c_void_p, C.c_int, C.POINTER(Rows), C.POINTER(Rows), C.c_int, C.c_int, C.c_void_p, C.c_void_p,
+                                     C.c_void_p]),
+    "kb200_cache_accept": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
+    "kb200_cache_attend_workspace": (C.c_uint64, [C.c_void_p, C.c_int, C.c_int, C.c_int]),
+    "kb200_cache_attend": (C.c_int, [C.c_void_p, C.c_int, C.POINTER(Rows), C.POINTER(Rows), C.c_int, C.c_int, C.c_void_p,
+                                     C.POINTER(C.c_int64), C.c_void_p, C.c_void_p, C.c_float, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "kb200_cache_status": (C.c_int, [C.c_void_p]),
+    "kb200_cache_destroy": (None, [C.c_void_p]),
 }
 
 _lib = None
