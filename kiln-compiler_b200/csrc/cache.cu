@@ -757,6 +757,7 @@ KB200_EXPORT int kb200_cache_status(kb200_cache* handle) {
   KB200_CUDA(cudaMemcpy(&word, c.view.status, sizeof(int), cudaMemcpyDeviceToHost));
   if (word == 0) return KB200_OK;
   KB200_CUDA(cudaMemset(c.view.status, 0, sizeof(int)));
+  if (word & kCacheWaitFault) return fail(KB200_ERR_DEVICE_WAIT, "a bounded device-side wait of kb200_cache_attend ran out");
   return fail(word & KB200_CACHE_NO_PAGES ? KB200_ERR_PAGES : KB200_ERR_BOUNDS, "cache:%s%s%s%s%s",
               word & KB200_CACHE_NO_PAGES ? " fewer free pages than were to be reserved;" : "",
               word & KB200_CACHE_TOO_LONG ? " a sequence would need more than max_pages;" : "",

@@ -1,6 +1,7 @@
 // The paged K/V cache: what its operations (cache.cu) and the attention over it (cache_attention.cu) share.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -17,6 +18,8 @@ struct CacheView {
   int row_chunks;          // 16-byte chunks of a token's row
 };
 
+constexpr int kCacheWaitFault = 1 << 16;      // a bounded wait of the attention ran out (beside kb200_cache_fault in the status word)
+
 struct Cache {
   CacheView view;
   int dtype = 0;
@@ -32,10 +35,10 @@ struct Cache {
   int32_t* page_b = nullptr;         // [pages]
   int4* copies = nullptr;            // pages to copy: from, to, tokens
   int* counters = nullptr;           // see cache.cu
-  int attention_resident[3] = {};    // CTAs to an SM of the attention kernel, by the size of its row tiles
+  CUtensorMap map;                   // the pool: elements of a row, rows of a page (head by head), pages of K and of V layer by layer
 };
 
-int cache_attention_prepare(Cache& c);       // (cache_attention.cu) the kernels' limits, on the current device
+int cache_attention_prepare(Cache& c);       // (cache_attention.cu) the pool's map and the kernels' limits, on the current device
 
 // This thread's device for the duration of a call.
 struct DeviceGuard {

@@ -40,13 +40,10 @@ template <int ROWS, int TILE>
 __device__ __forceinline__ CacheItems cache_items(const CacheAttnParams& p, int b) {
   CacheItems r{};
   const int slot = p.slots != nullptr ? p.slots[b] : b;
-  if ((unsigned)slot >= (unsigned)p.c.sequences) {
-    cache_fault(p.c, KB200_CACHE_BAD_INDEX);
-    return r;
-  }
   int count = p.counts != nullptr ? p.counts[b] : p.tokens;
-  if (count < 0 || count > p.tokens) {
+  if ((unsigned)slot >= (unsigned)p.c.sequences || count < 0 || count > p.tokens) {
     cache_fault(p.c, KB200_CACHE_BAD_INDEX);
+    if ((unsigned)slot >= (unsigned)p.c.sequences) return r;
     count = min(max(count, 0), p.tokens);
   }
   const int64_t room = (int64_t)min(max(p.c.held[slot], 0), p.c.max_pages) << p.c.page_log2;
@@ -61,6 +58,103 @@ __device__ __forceinline__ CacheItems cache_items(const CacheAttnParams& p, int 
   r.key_tiles = max(1, (r.end + TILE - 1) / TILE);
   r.units = (int64_t)r.row_tiles * r.key_tiles * p.c.kv_heads;
   return r;
+}
+
+// Where a run is: an item (batch row, key head, row tile) and a key tile of it.
+struct CacheCursor {
+  int b, head, row_tile, tile;
+  CacheItems it;
+};
+// To the next item.
+template <int ROWS, int TILE>
+__device__ __forceinline__ void next_item(const CacheAttnParams& p, CacheCursor& u) {
+  u.tile = 0;
+  if (++u.row_tile < u.it.row_tiles) return;
+  u.row_tile = 0;
+  if (++u.head < p.c.kv_heads) return;
+  u.head = 0;
+  while (++u.b < p.rows) {
+    u.it = cache_items<ROWS, TILE>(p, u.b);
+    if (u.it.units > 0) return;
+  }
+}
+
+struct CacheRun {
+  int64_t all, lo, hi;             // units of the call, of this CTA
+  int parts;                       // CTAs that have any
+  CacheCursor at;
+};
+struct CacheRunShared {
+  int64_t sums[32], rest;
+  int b;
+  CacheItems it;
+};
+
+// The run of CTA `part`, by all threads of a CTA of THREADS; false: it has none.
+template <int ROWS, int TILE, int THREADS>
+__device__ __forceinline__ bool find_run(const CacheAttnParams& p, int part, CacheRunShared& shared, CacheRun* run) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool one_round = p.rows <= THREADS;
+  int64_t base = 0, from = 0;
+  CacheItems it{};
+  for (int pass = 0; pass < 2; ++pass) {
+    if (pass == 0 || !one_round) {
+      base = 0;
+      for (int b0 = 0; b0 < p.rows; b0 += THREADS) {
+        const int b = b0 + threadIdx.x;
+        if (b < p.rows) it = cache_items<ROWS, TILE>(p, b);
+        else it.units = 0;
+        int64_t sum = it.units;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+          const int64_t below = __shfl_up_sync(0xffffffffu, sum, d);
+          if (lane >= d) sum += below;
+        }
+        __syncthreads();
+        if (lane == 31) shared.sums[warp] = sum;
+        __syncthreads();
+        int64_t before = 0, total = 0;
+#pragma unroll
+        for (int w = 0; w < THREADS / 32; ++w) {
+          before += w < warp ? shared.sums[w] : 0;
+          total += shared.sums[w];
+        }
+        from = base + before + sum - it.units;
+        if (pass == 1 && run->lo >= from && run->lo < from + it.units) shared.b = b, shared.rest = run->lo - from, shared.it = it;
+        base += total;
+      }
+    } else if (run->lo >= from && run->lo < from + it.units) {
+      shared.b = threadIdx.x, shared.rest = run->lo - from, shared.it = it;
+    }
+    if (pass == 0) {
+      run->all = base;
+      run->parts = (int)min((int64_t)p.parts, (base + p.min_units - 1) / p.min_units);
+      if (part >= run->parts) return false;
+      run->lo = base * part / run->parts;
+      run->hi = base * (part + 1) / run->parts;
+    }
+  }
+  __syncthreads();
+  CacheCursor& at = run->at;
+  at.b = shared.b;
+  at.it = shared.it;
+  int64_t rest = shared.rest;
+  const int64_t per_head = (int64_t)at.it.row_tiles * at.it.key_tiles;
+  at.head = (int)(rest / per_head);
+  rest -= at.head * per_head;
+  at.row_tile = (int)(rest / at.it.key_tiles);
+  at.tile = (int)(rest - (int64_t)at.row_tile * at.it.key_tiles);
+  return true;
+}
+
+// An item's row: the token and, of the heads that share its key head, the one.
+struct CacheRow {
+  int token, head;
+};
+template <int ROWS>
+__device__ __forceinline__ CacheRow row_of(const CacheAttnParams& p, const CacheCursor& at, int row) {
+  const int r = at.row_tile * ROWS + row, token = r / p.group;
+  return CacheRow{token, at.head * p.group + r - token * p.group};
 }
 #endif
 

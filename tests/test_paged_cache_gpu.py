@@ -310,6 +310,10 @@ SHAPES = [
     (F16, [2049], [5], 4, 8, 16, 256),
     (BF16, [900, 33, 0, 257] * 20, [1] * 80, 1, 1, 64, 32),    # more rows than CTAs look at in one round is 128
     (BF16, [33, 5, 64] * 50, [2, 1, 3] * 50, 1, 2, 64, 16),
+    (BF16, [2900, 2000, 3100, 1, 2500, 2999, 130, 3000], [1, 2, 3, 2, 1, 1, 3, 2], 16, 2, 128, 16),      # dozens of tiles to a CTA
+    (F32, [1900, 1200, 1, 1777], [2, 1, 2, 3], 32, 1, 64, 32),
+    (F16, [1500, 1600, 1700], [9, 9, 3], 16, 3, 128, 64),
+    (BF16, [1000, 2000], [40, 33], 16, 1, 64, 16),
 ]
 
 
