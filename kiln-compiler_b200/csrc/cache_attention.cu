@@ -2,116 +2,49 @@
 // each sequence, one pass over its keys with a running maximum and sum.
 //
 // What bounds it: the cache's bytes.  A key head's K and V are read once for all query rows that share them (drafted tokens x heads per key head).
-// Products run on the tensor cores by warp (mma.sync): the rows of a decoding step do not fill more.
+// Products run by warp (cache_attention_math.cuh): the rows of a decoding step do not fill larger units.
 //
 // A CTA has one producer warp and up to six consumer warps (from the eighth on a scheduler holds three warps and a thread 168 registers) and walks its run of key tiles (cache_attention.h).  The producer brings
 // tiles of K and V through a tensor map of the pool, page by page, as far ahead as the ring of stages goes, across the borders of sequences and
-// heads.  A consumer warp takes a WHOLE tile for 16 query rows and keeps maxima, sums and output rows in registers; the
+// heads.  A consumer warp takes a WHOLE tile for up to 16 query rows and keeps maxima, sums and output rows in registers; the
 // warps' sums are joined at the end of an item only.  Every stage of the ring belongs to one warp (or the group of warps with the other rows of the row
 // tile), which therefore sees each of its fillings: a barrier's parity tells no more than the last one.  (With the tile's keys divided among the warps, and copies issued by them, a warp
 // paid the rescaling, the shuffles and the addresses for 16 keys instead of 64: 985 instructions per warp and tile at 5.8 cycles each, two warps to
 // a scheduler, 187 us for 32 sequences of up to 8192 tokens, 52 % of the bandwidth.)
 //
 // Scores, maxima, sums and output rows are float32.  16-bit caches: the weights of a tile are rounded to the cache's type for the product with V
-// (half a step, 2^-9 for bfloat16, of every summand; the sum of the weights is kept of the unrounded ones).  float32 caches: both operands of both
-// products as a TF32 head and tail, three products, what is dropped is 2^-22 of a summand; the tensor core cuts
-// off what does not fit a sum, so products with tails are summed apart from those of heads, and a tile's rows start from zero and are added by FMA.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <math_constants.h>
-
+// (half a step, 2^-9 for bfloat16, of every summand; the sum of the weights is kept of the unrounded ones).  float32 caches are not rounded anywhere.
 #include <algorithm>
-#include <type_traits>
+#include <cmath>
 
-#include "cache_attention.h"
-#include "tc_common.cuh"
+#include "cache_attention_math.cuh"
 
 #define KB200_EXPORT extern "C" __attribute__((visibility("default")))
 
 namespace kb200 {
 namespace {
 
-using namespace tc;
+using namespace cache_math;
 
-// Sizes by type and padded head width.  A tile is blocks of 128-byte columns, as the map's 128-byte swizzle wants them: K's, then V's.
-template <typename T, int DP, int RG>
+// Warps, ring and shared memory by what the warps do; RG: groups of warps with other rows of the same row tile.
+template <typename Math, int RG>
 struct Shape {
+  using T = typename Math::Type;
+  using G = Tile<T, Math::kDim>;
   static constexpr bool kWide = sizeof(T) == 4;
-  static constexpr int kGroups = RG == 4 ? 1 : DP > 128 ? 6 / RG - 1 : 6 / RG;     // of warps, each for tiles of its own
+  // groups of warps, each for tiles of its own: as many as there are stages, with what a warp keeps in shared memory beside them
+  static constexpr int kMost = kWide ? (Math::kDim <= 64 ? 5 : Math::kDim <= 128 ? 4 : 3) : Math::kDim > 128 ? 5 : 6;
+  static constexpr int kGroups = RG == 4 ? 1 : kMost / RG;
   static constexpr int kWarps = kGroups * RG;                            // consumers
-  static constexpr bool kKeepsQ = !kWide || DP <= 64;                    // query rows in registers
   static constexpr int kThreads = 32 * (kWarps + 1);
-  static constexpr int kBlocks = DP * (int)sizeof(T) / 128;
-  static constexpr int kTile = kBlocks <= 2 ? 64 : 128 / kBlocks;        // keys: 16 KB of K and of V at most
-  static constexpr int kBlockBytes = kTile * 128;
-  static constexpr int kStageBytes = 2 * kBlocks * kBlockBytes;
-  static constexpr int kStages = kGroups * ((DP > 128 ? 160 : 192) * 1024 / kStageBytes / kGroups);      // (a multiple: see above)
   static constexpr int kSlots = 2;                                       // warps whose rows are in shared memory at a time when sums are joined
-  static constexpr int kSlotRow = DP + 4;                                // floats
-  static constexpr int kSmem = kStages * kStageBytes + kSlots * 16 * kSlotRow * 4;
+  static constexpr int kSlotFloats = Math::kOut * 32;
+  static constexpr int kQuery = kWide ? Math::kRows * Math::kDim : 0, kWeights = kWide ? G::kKeys * Math::kRows : 0;      // floats of a warp
+  static constexpr int kBeside = (kSlots * kSlotFloats + kWarps * (kQuery + kWeights)) * 4;
+  static constexpr int kStages = kGroups * ((222 * 1024 - kBeside) / G::kBytes / kGroups);      // (a multiple: see above)
+  static constexpr int kSmem = kStages * G::kBytes + kBeside;
+  static constexpr int kRows = Math::kRows * RG;                         // of a row tile
 };
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
-}
-__device__ __forceinline__ void ldmatrix4_t(uint32_t (&r)[4], uint32_t at) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
-}
-template <typename T>
-__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// x as a TF32 head, rounded to nearest, and the rest, rounded as well.
-__device__ __forceinline__ void split(float x, uint32_t* head, uint32_t* tail) {
-  uint32_t h, t;
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(h) : "f"(x));
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(t) : "f"(x - __uint_as_float(h)));
-  *head = h;
-  *tail = t;
-}
-template <typename T>
-__device__ __forceinline__ uint32_t pack(float a, float b) {
-  if constexpr (std::is_same<T, __half>::value) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  } else {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-}
-template <typename T>
-__device__ __forceinline__ void store2(T* to, float a, float b) {
-  if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(to) = make_float2(a, b);
-  else *reinterpret_cast<uint32_t*>(to) = pack<T>(a, b);
-}
-// Does one of the elements in a 32-bit word hold an infinity or NaN?
-template <typename T>
-__device__ __forceinline__ bool not_finite(uint32_t w) {
-  if constexpr (sizeof(T) == 4) return (w & 0x7f800000u) == 0x7f800000u;
-  else if constexpr (std::is_same<T, __half>::value) return (w & 0x7c000000u) == 0x7c000000u || (w & 0x7c00u) == 0x7c00u;
-  else return (w & 0x7f800000u) == 0x7f800000u || (w & 0x7f80u) == 0x7f80u;
-}
-template <typename T>
-__device__ __forceinline__ float to_float(T x) {
-  if constexpr (std::is_same<T, float>::value) return x;
-  else if constexpr (std::is_same<T, __half>::value) return __half2float(x);
-  else return __bfloat162float(x);
-}
 
 // A wait of 2^31 cycles at most, about a second (a poll may suspend the thread, so a number of polls says little).
 __device__ __forceinline__ bool wait_a_second(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
@@ -133,22 +66,21 @@ __device__ __forceinline__ bool wait_a_second(uint32_t bar, uint32_t parity, vol
 }
 
 // A part: ROWS output rows (not divided by their sums), then their maxima and sums.
-template <int DP, int ROWS>
-constexpr int64_t part_floats() { return (int64_t)ROWS * (DP + 2); }
+constexpr int64_t part_floats(int dim, int rows) { return (int64_t)rows * (dim + 2); }
 
-template <typename T, int DP, int RG>
-__global__ void __launch_bounds__(Shape<T, DP, RG>::kThreads, 1)
+template <typename Math, int RG>
+__global__ void __launch_bounds__(Shape<Math, RG>::kThreads, 1)
 cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CacheAttnParams p) {
-  using Z = Shape<T, DP, RG>;
-  constexpr int KG = Z::kGroups, ROWS = 16 * RG, TILE = Z::kTile;      // groups of warps by keys, by rows
-  constexpr int NT = TILE / 8, DT = DP / 8;        // 8-wide column tiles of a warp's scores, of its output rows
-  constexpr bool kWide = Z::kWide;
+  using Z = Shape<Math, RG>;
+  using T = typename Math::Type;
+  using G = typename Z::G;
+  constexpr int KG = Z::kGroups, ROWS = Z::kRows, TILE = G::kKeys, DP = Math::kDim;
   static_assert(Z::kStages > 0 && Z::kStages % KG == 0 && (KG == 1 || Z::kSlots % RG == 0), "a stage belongs to one group, a slot to a warp of each row group");
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[2 * Z::kStages];
   __shared__ CacheRunShared found;
-  __shared__ uint32_t sees[Z::kWarps][16][2];      // a tile with drafted tokens under a mask: which row sees which key
-  __shared__ float states[Z::kWarps][16][2];
+  __shared__ uint32_t sees[Z::kWarps][Math::kRows][2];      // a tile with drafted tokens under a mask: which row sees which key
+  __shared__ float states[Z::kWarps][Math::kRows][2];
   __shared__ int abort_flag;
 
   const int lane = threadIdx.x & 31, warp = warp_index();
@@ -195,28 +127,29 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
         }
         const int stage = u % Z::kStages;
         if (!wait(empty + 8 * stage, ((u / Z::kStages) & 1) ^ 1)) break;
-        const uint32_t to = stage0 + stage * Z::kStageBytes, bar = full + 8 * stage;
-        if (lane == 0) mbar_expect_tx(bar, Z::kStageBytes);
+        const uint32_t to = stage0 + stage * G::kBytes, bar = full + 8 * stage;
+        if (lane == 0) mbar_expect_tx(bar, G::kBytes);
         __syncwarp();
         // K and V of every box, block by block: as many loads as there are, spread over the lanes
         const int in_page = now.tile * TILE & ((1 << p.c.page_log2) - 1);
-        for (int i0 = 0; i0 < boxes * Z::kBlocks * 2; i0 += 32) {
-          const int i = i0 + lane, which = i & 1, block = (i >> 1) % Z::kBlocks, j = (i >> 1) / Z::kBlocks;
+        for (int i0 = 0; i0 < boxes * G::kBlocks * 2; i0 += 32) {
+          const int i = i0 + lane, which = i & 1, block = (i >> 1) % G::kBlocks, j = (i >> 1) / G::kBlocks;
           const int page = __shfl_sync(0xffffffffu, my_page, (first + j) & 31);
-          if (i < boxes * Z::kBlocks * 2)
-            tma_load_3d(to + which * Z::kBlocks * Z::kBlockBytes + block * Z::kBlockBytes + j * box * 128, &map, bar, block * (128 / (int)sizeof(T)),
+          if (i < boxes * G::kBlocks * 2)
+            tma_load_3d(to + which * G::kHalf + block * G::kBlockBytes + j * box * 128, &map, bar, block * (128 / (int)sizeof(T)),
                         (now.head << p.c.page_log2) + in_page, page < 0 ? none : (p.layer * 2 + which) * p.c.pages + page);
         }
         ++u;
-        --left;
-        if (++now.tile == now.it.key_tiles) next_item<ROWS, TILE>(p, now);
+        const bool ends = ++now.tile == now.it.key_tiles;
+        if (ends || !p.whole) --left;
+        if (ends && left > 0) next_item<ROWS, TILE>(p, now);
       }
     }
   } else {
     // ---------------- consumers ----------------
     const int row_group = warp % RG, key_group = warp / RG;
-    const int g = lane >> 2, t4 = lane & 3;          // fragment coordinates
-    float* const slots = reinterpret_cast<float*>(smem + Z::kStages * Z::kStageBytes);
+    float* const slots = reinterpret_cast<float*>(smem + Z::kStages * G::kBytes);
+    float* const query = slots + Z::kSlots * Z::kSlotFloats + warp * (Z::kQuery + Z::kWeights);
     auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(32 * Z::kWarps) : "memory"); };
 
     // rows behind a sequence's drafted tokens
@@ -230,390 +163,91 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
       }
     }
 
-    const int row = row_group * 16 + g;              // this thread's rows of the row tile: row and row + 8
-    uint32_t q16[kWide ? 1 : DP / 16][4];
-    float q32[kWide && Z::kKeepsQ ? DP / 8 : 1][4];
-    const float* q_from[2] = {nullptr, nullptr};     // ... or where they are
-    float o[DT][4], m[2], l[2];
-    int rows_here = 0;                               // of the item's row tile
-    auto begin = [&]() {
-      rows_here = min(ROWS, now.it.count * p.group - now.row_tile * ROWS);
-#pragma unroll
-      for (int i = 0; i < DT; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
-      m[0] = m[1] = -CUDART_INF_F;
-      l[0] = l[1] = 0.0f;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const bool there = row + 8 * half < rows_here;
-        const CacheRow r = row_of<ROWS>(p, now, there ? row + 8 * half : 0);
-        const int64_t at = now.b * p.q_stride[0] + r.token * p.q_stride[1] + r.head * p.q_stride[2];
-        if constexpr (kWide) {
-          // dims 2t and 2t + 1 of eight stand in fragment columns t and t + 4, in both operands: 64-bit loads
-          if constexpr (Z::kKeepsQ) {
-#pragma unroll
-            for (int k = 0; k < DP / 8; ++k) {
-              const float2 x = there && k * 8 < p.c.head_dim ? reinterpret_cast<const float2*>(static_cast<const float*>(p.q) + at)[k * 4 + t4] : make_float2(0, 0);
-              q32[k][half] = x.x;
-              q32[k][2 + half] = x.y;
-            }
-          } else {
-            q_from[half] = there ? static_cast<const float*>(p.q) + at : nullptr;
-          }
-        } else {
-          auto pair = [&](int i) {                   // two elements
-            if (!p.q_fp32) return reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.q) + at)[i];
-            const float2 x = reinterpret_cast<const float2*>(static_cast<const float*>(p.q) + at)[i];
-            return pack<T>(x.x, x.y);
-          };
-#pragma unroll
-          for (int k = 0; k < DP / 16; ++k) {
-            const bool in = there && k * 16 < p.c.head_dim;
-            q16[k][half] = in ? pair(k * 8 + t4) : 0u;
-            q16[k][2 + half] = in ? pair(k * 8 + 4 + t4) : 0u;
-          }
-        }
-      }
-    };
+    Math math;
+    Place at{nullptr, nullptr, 0, 0, row_group * Math::kRows, 0, warp, lane, row_group, key_group};
 
-    // ---- a tile ----
-    auto compute = [&](int tile, uint32_t k_tile, uint32_t v_tile) {
-      float s[NT][4];
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[i][j] = 0.0f;
-      if constexpr (!kWide) {
-        const uint32_t at = k_tile + ((lane >> 4) * 8 + (lane & 7)) * 128;
-#pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-          const uint32_t in_row = (k / 4) * Z::kBlockBytes + ((((k % 4) * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
-#pragma unroll
-          for (int n = 0; n < NT; n += 2) {
-            uint32_t b[4];
-            ldmatrix4(b, at + n * 8 * 128 + in_row);
-            mma16<T>(s[n], q16[k], b[0], b[1]);
-            mma16<T>(s[n + 1], q16[k], b[2], b[3]);
-          }
-        }
-      } else {
-        float low[NT][4];
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) low[i][j] = 0.0f;
-        const uint8_t* const at = smem + (k_tile - stage0) + g * 128 + (t4 & 1) * 8;
-#pragma unroll
-        for (int k = 0; k < DP / 8; ++k) {
-          const int in_row = (k / 4) * Z::kBlockBytes + ((((k % 4) * 2 + (t4 >> 1)) ^ g) << 4);
-          uint32_t ah[4], al[4];
-          if constexpr (Z::kKeepsQ) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) split(q32[k][j], ah + j, al + j);
-          } else {
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const float2 x = q_from[half] != nullptr && k * 8 < p.c.head_dim ? reinterpret_cast<const float2*>(q_from[half])[k * 4 + t4] : make_float2(0, 0);
-              split(x.x, ah + half, al + half);
-              split(x.y, ah + 2 + half, al + 2 + half);
-            }
-          }
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const float2 x = *reinterpret_cast<const float2*>(at + n * 8 * 128 + in_row);
-            uint32_t bh[2], bl[2];
-            split(x.x, bh + 0, bl + 0);
-            split(x.y, bh + 1, bl + 1);
-            mma_tf32(low[n], al, bh[0], bh[1]);
-            mma_tf32(low[n], ah, bl[0], bl[1]);
-            mma_tf32(s[n], ah, bh[0], bh[1]);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[i][j] += low[i][j];
-      }
-
-      const int key0 = tile * TILE;
-      const bool drafted = key0 + TILE > min(now.it.length, now.it.end);
-      bool infinite = false;
-      unsigned long long shows[2] = {~0ull, ~0ull};  // the tile's keys that rows g and g + 8 see
-      if (drafted) {
-        if (p.mask == nullptr) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int n = min(now.it.end, now.it.length + row_of<ROWS>(p, now, row + 8 * h).token + 1) - key0;
-            shows[h] = n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
-          }
-        } else {
-          // a ballot per row and 32 keys, all loads in flight together (where there is nothing to look up they read the mask's first byte)
-          uint8_t bytes[16][(TILE + 31) / 32];
-          const uint8_t* const mask = p.mask + now.b * p.mask_stride[0];
-          const int first = now.row_tile * ROWS + row_group * 16;
-          int token = first / p.group, in_group = first - token * p.group;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-#pragma unroll
-            for (int w = 0; w < (TILE + 31) / 32; ++w) {
-              const int j = key0 + w * 32 + lane - now.it.length;
-              const bool looked_up = j >= 0 && j < now.it.count && row_group * 16 + i < rows_here;
-              bytes[i][w] = *(looked_up ? mask + token * p.mask_stride[1] + j * p.mask_stride[2] : p.mask);
-            }
-            if (++in_group == p.group) in_group = 0, ++token;
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-#pragma unroll
-            for (int w = 0; w < (TILE + 31) / 32; ++w) {
-              const int key = key0 + w * 32 + lane;
-              const bool visible = key < now.it.length || (bytes[i][w] != 0 && row_group * 16 + i < rows_here);
-              const uint32_t word = __ballot_sync(0xffffffffu, visible && key < now.it.end && w * 32 + lane < TILE);
-              if (lane == 0) sees[warp][i][w] = word;
-            }
-          __syncwarp();
-#pragma unroll
-          for (int h = 0; h < 2; ++h) shows[h] = sees[warp][g + 8 * h][0] | (TILE > 32 ? (unsigned long long)sees[warp][g + 8 * h][1] << 32 : 0ull);
-          __syncwarp();
-        }
-        // V behind the sequence's end is what an earlier tenant left, and V of a drafted token that some rows do not see may hold infinities or NaN; 0 times
-        // those is NaN.  The former become zeros here, the latter below.
-        const int last = now.it.end - key0;
-        bool odd = false;
-#pragma unroll 8
-        for (int i = lane; i < TILE * Z::kBlocks * 8; i += 32) {
-          const int key = i / (Z::kBlocks * 8), chunk = i % (Z::kBlocks * 8);
-          uint4* const x = reinterpret_cast<uint4*>(smem + (v_tile - stage0) + (chunk / 8) * Z::kBlockBytes + key * 128 + (((chunk % 8) ^ (key & 7)) << 4));
-          if (RG == 1 && key >= last) *x = make_uint4(0, 0, 0, 0);
-          else if (key < last) odd = odd || not_finite<T>(x->x) || not_finite<T>(x->y) || not_finite<T>(x->z) || not_finite<T>(x->w);
-        }
-        infinite = __any_sync(0xffffffffu, odd) != 0;
-        __syncwarp();
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int key = n * 8 + t4 * 2 + (j & 1);
-            if (!(shows[j >> 1] >> key & 1)) s[n][j] = -CUDART_INF_F;
-          }
-      }
-
-      // ---- softmax: two rows of a thread, their keys over the four lanes of a group ----
-      float top[2] = {-CUDART_INF_F, -CUDART_INF_F}, shift[2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) top[j >> 1] = fmaxf(top[j >> 1], s[n][j]);
-      float alpha[2] = {1.0f, 1.0f};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2)) * p.scale_log2;
-      }
-      const bool grown = __any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1]);
-      if (grown) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          top[h] = fmaxf(top[h], m[h]);
-          alpha[h] = top[h] == -CUDART_INF_F ? 1.0f : ex2(m[h] - top[h]);
-          m[h] = top[h];
-          l[h] *= alpha[h];
-        }
-        if constexpr (!kWide)
-#pragma unroll
-          for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[d][j] *= alpha[j >> 1];
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) shift[h] = m[h] == -CUDART_INF_F ? 0.0f : -m[h];          // nothing seen so far: every weight is 2^-inf
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s[n][j] = ex2(fmaf(s[n][j], p.scale_log2, shift[j >> 1]));
-          l[j >> 1] += s[n][j];
-        }
-
-      auto v_at = [&](int key, int d) -> T* {
-        const int byte = d * (int)sizeof(T);
-        return reinterpret_cast<T*>(smem + (v_tile - stage0) + (byte / 128) * Z::kBlockBytes + key * 128 + ((((byte % 128) >> 4) ^ (key & 7)) << 4) + byte % 16);
-      };
-      // Elements that are not finite are added to the rows that see them one by one, and are zero in the product.
-      if (infinite) {
-        if constexpr (kWide)
-#pragma unroll
-          for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[d][j] *= alpha[j >> 1];
-        alpha[0] = alpha[1] = 1.0f;
-        for (int key = 0; key < TILE; ++key)
-#pragma unroll
-          for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float x = to_float(*v_at(key, d * 8 + t4 * 2 + (j & 1)));
-              if (!(fabsf(x) < CUDART_INF_F) && (shows[j >> 1] >> key & 1)) o[d][j] += x;
-            }
-      }
-      if (drafted && (RG > 1 || infinite)) {
-        // (warps of other rows read the same tile: each waits for all to have seen it as it was)
-        if (RG > 1) asm volatile("bar.sync %0, %1;" ::"r"(2 + key_group), "n"(32 * RG) : "memory");
-        else __syncwarp();
-        const int last = now.it.end - key0;
-        for (int i = row_group * 32 + lane; i < TILE * DP; i += 32 * RG) {
-          T* const x = v_at(i / DP, i % DP);
-          if (i / DP >= last || !(fabsf(to_float(*x)) < CUDART_INF_F)) *x = T(0.0f);
-        }
-        if (RG > 1) asm volatile("bar.sync %0, %1;" ::"r"(2 + key_group), "n"(32 * RG) : "memory");
-        else __syncwarp();
-      }
-
-      // ---- P V ----
-      if constexpr (!kWide) {
-        const uint32_t at = v_tile + (((lane >> 3) & 1) * 8 + (lane & 7)) * 128;
-#pragma unroll
-        for (int k = 0; k < NT / 2; ++k) {
-          const uint32_t a[4] = {pack<T>(s[2 * k][0], s[2 * k][1]), pack<T>(s[2 * k][2], s[2 * k][3]), pack<T>(s[2 * k + 1][0], s[2 * k + 1][1]),
-                                 pack<T>(s[2 * k + 1][2], s[2 * k + 1][3])};
-#pragma unroll
-          for (int d = 0; d < DT; d += 2) {
-            uint32_t b[4];
-            ldmatrix4_t(b, at + k * 16 * 128 + (d / 8) * Z::kBlockBytes + (((d % 8 + (lane >> 4)) ^ (lane & 7)) << 4));
-            mma16<T>(o[d], a, b[0], b[1]);
-            mma16<T>(o[d + 1], a, b[2], b[3]);
-          }
-        }
-      } else {
-        // keys 2t and 2t + 1 of eight stand in fragment columns t and t + 4: the scores are where the product wants them
-        uint32_t ah[NT][4], al[NT][4];
-#pragma unroll
-        for (int k = 0; k < NT; ++k) {
-          split(s[k][0], ah[k] + 0, al[k] + 0);
-          split(s[k][2], ah[k] + 1, al[k] + 1);
-          split(s[k][1], ah[k] + 2, al[k] + 2);
-          split(s[k][3], ah[k] + 3, al[k] + 3);
-        }
-        const uint8_t* const at = smem + (v_tile - stage0) + 2 * t4 * 128 + (g & 3) * 4;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          float high[4] = {0.0f, 0.0f, 0.0f, 0.0f}, low[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          const int block = (d / 4) * Z::kBlockBytes, chunk = (d % 4) * 2 + (g >> 2);
-#pragma unroll
-          for (int k = 0; k < NT; ++k) {
-            uint32_t bh[2], bl[2];
-            split(*reinterpret_cast<const float*>(at + block + k * 8 * 128 + ((chunk ^ (2 * t4)) << 4)), bh + 0, bl + 0);
-            split(*reinterpret_cast<const float*>(at + block + (k * 8 + 1) * 128 + ((chunk ^ (2 * t4 + 1)) << 4)), bh + 1, bl + 1);
-            mma_tf32(low, al[k], bh[0], bh[1]);
-            mma_tf32(low, ah[k], bl[0], bl[1]);
-            mma_tf32(high, ah[k], bh[0], bh[1]);
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[d][j] = fmaf(o[d][j], alpha[j >> 1], high[j] + low[j]);
-        }
-      }
-      if (drafted) fence_async_smem();               // (the zeros, in front of the next copy to this stage)
-    };
-
-    // ---- the end of an item, or of the run inside one: the warps' sums, then the rows or a part ----
-    // `order`: this warp's place among those that had a tile of it, in the order of the keys.
+    // The end of an item, or of the run inside one: the warps' sums, then the rows or a part.  `order`: this warp's place among those that had a tile of
+    // it, in the order of the keys.
     auto finish = [&](int order, int tiles, bool whole, int64_t part) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-        if (l[h] != l[h]) m[h] = 0.0f;               // (NaN, which a maximum passes over, reaches the result)
-      }
+      math.sum_up();
       int n = min(KG, tiles);                        // groups of keys that had a tile
       if (n > 1) {
         // to the largest maximum
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          if (t4 == 0) states[order * RG + row_group][g + 8 * h][0] = m[h];
+        math.states(lane, [&](int row, float top, float) { states[order * RG + row_group][row][0] = top; });
         meet();
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        math.rescale(lane, [&](int row) {
           float top = -CUDART_INF_F;
-          for (int w = 0; w < n; ++w) top = fmaxf(top, states[w * RG + row_group][g + 8 * h][0]);
-          const float mine = m[h] == -CUDART_INF_F ? 0.0f : ex2(m[h] - top);
-          l[h] *= mine;
-          m[h] = top;
-#pragma unroll
-          for (int d = 0; d < DT; ++d) o[d][2 * h] *= mine, o[d][2 * h + 1] *= mine;
-          if (t4 == 0) states[order * RG + row_group][g + 8 * h][1] = l[h];
-        }
+          for (int w = 0; w < n; ++w) top = fmaxf(top, states[w * RG + row_group][row][0]);
+          return top;
+        });
+        math.states(lane, [&](int row, float, float sum) { states[order * RG + row_group][row][1] = sum; });
         while (n > 1) {                              // the upper half's rows go to the lower half, as many at a time as there are slots
           const int half = (n + 1) / 2;
           for (int from = half; from < n; from += Z::kSlots / RG) {
             const int to = min(n, from + Z::kSlots / RG);
-            float* const slot = slots + ((order >= half ? order - from : order + half - from) * RG + row_group) * 16 * Z::kSlotRow + t4 * 2;
-            if (order >= from && order < to)
-#pragma unroll
-              for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) *reinterpret_cast<float2*>(slot + (g + 8 * h) * Z::kSlotRow + d * 8) = make_float2(o[d][2 * h], o[d][2 * h + 1]);
+            float* const slot = slots + ((order >= half ? order - from : order + half - from) * RG + row_group) * Z::kSlotFloats + lane;
+            if (order >= from && order < to) math.each_out([&](int i, float x) { slot[i * 32] = x; });
             meet();
-            if (order + half >= from && order + half < to)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                  const float2 x = *reinterpret_cast<const float2*>(slot + (g + 8 * h) * Z::kSlotRow + d * 8);
-                  o[d][2 * h] += x.x;
-                  o[d][2 * h + 1] += x.y;
-                }
-                l[h] += states[(order + half) * RG + row_group][g + 8 * h][1];
-                __syncwarp();
-                if (t4 == 0) states[order * RG + row_group][g + 8 * h][1] = l[h];
-              }
+            if (order + half >= from && order + half < to) {
+              math.each_out([&](int i, float& x) { x += slot[i * 32]; });
+              math.add_sums(lane, [&](int row) { return states[(order + half) * RG + row_group][row][1]; });
+              __syncwarp();
+              math.states(lane, [&](int row, float, float sum) { states[order * RG + row_group][row][1] = sum; });
+            }
             meet();
           }
           n = half;
         }
       }
       if (order != 0) return;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (row + 8 * h >= rows_here) continue;
+      math.each_row(lane, [&](int row, float sum, float top, bool once, auto&& columns) {
+        row += at.row0;
+        if (row >= at.rows_here) return;
         if (whole) {
-          const float inv = l[h] == 0.0f ? 0.0f : 1.0f / l[h];
-          const CacheRow r = row_of<ROWS>(p, now, row + 8 * h);
-          T* const to = static_cast<T*>(p.out) + now.b * p.out_stride[0] + r.token * p.out_stride[1] + r.head * p.out_stride[2] + t4 * 2;
-#pragma unroll
-          for (int d = 0; d < DT; ++d)
-            if (d * 8 < p.c.head_dim) store2<T>(to + d * 8, o[d][2 * h] * inv, o[d][2 * h + 1] * inv);
+          const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+          const CacheRow r = row_of<ROWS>(p, now, row);
+          T* const to = static_cast<T*>(p.out) + now.b * p.out_stride[0] + r.token * p.out_stride[1] + r.head * p.out_stride[2];
+          columns([&](int d, float x, float y) {
+            if (d < p.c.head_dim) store2<T>(to + d, x * inv, y * inv);
+          });
         } else {
           float* const to = p.partial + part * p.partial_floats;
-#pragma unroll
-          for (int d = 0; d < DT; ++d)
-            if (d * 8 < p.c.head_dim) *reinterpret_cast<float2*>(to + (int64_t)(row + 8 * h) * DP + d * 8 + t4 * 2) = make_float2(o[d][2 * h], o[d][2 * h + 1]);
-          if (t4 == 0) to[ROWS * DP + row + 8 * h] = m[h], to[ROWS * DP + ROWS + row + 8 * h] = l[h];
+          columns([&](int d, float x, float y) {
+            if (d < p.c.head_dim) *reinterpret_cast<float2*>(to + (int64_t)row * DP + d) = make_float2(x, y);
+          });
+          if (once) to[ROWS * DP + row] = top, to[ROWS * DP + ROWS + row] = sum;
         }
-      }
+      });
     };
 
     int64_t left = any ? run.hi - run.lo : 0;
     uint32_t u0 = 0;
     while (left > 0) {
-      const int tiles = (int)min(left, (int64_t)now.it.key_tiles - now.tile);      // of this item, in this run
-      begin();
+      const int tiles = p.whole ? now.it.key_tiles : (int)min(left, (int64_t)now.it.key_tiles - now.tile);      // of this item, in this run
+      at.rows_here = min(ROWS, now.it.count * p.group - now.row_tile * ROWS);
+      at.sure = min(now.it.length, now.it.end);
+      if constexpr (Z::kWide) math.template begin<ROWS>(p, now, at, query);
+      else math.template begin<ROWS>(p, now, at);
       const int order = (int)((key_group + KG - u0 % KG) % KG);
       for (int i = order; i < tiles; i += KG) {
         const uint32_t u = u0 + i, stage = u % Z::kStages;
+        at.key0 = (now.tile + i) * TILE;
         if (wait(full + 8 * stage, (u / Z::kStages) & 1)) {
-          const uint32_t k_tile = stage0 + stage * Z::kStageBytes;
-          compute(now.tile + i, k_tile, k_tile + Z::kBlocks * Z::kBlockBytes);
+          at.k = smem + stage * G::kBytes;
+          at.v = at.k + G::kHalf;
+          if constexpr (Z::kWide) math.template tile<ROWS>(p, now, at, sees[warp], query, query + Z::kQuery);
+          else math.template tile<ROWS>(p, now, at, sees[warp]);
           __syncwarp();
           if (lane == 0) mbar_arrive(empty + 8 * stage);
-        } else if (RG > 1 && (now.tile + i + 1) * TILE > min(now.it.length, now.it.end)) {
-          for (int j = 0; j < 2; ++j) asm volatile("bar.sync %0, %1;" ::"r"(2 + key_group), "n"(32 * RG) : "memory");
+        } else if (RG > 1 && at.key0 + TILE > at.sure) {         // (the meetings of a tile with drafted tokens)
+          meet_rows<RG>(key_group);
+          meet_rows<RG>(key_group);
         }
       }
       // a part that begins with the run is the run's first, else its second
       finish(order, tiles, now.tile == 0 && tiles == now.it.key_tiles, 2 * (int64_t)blockIdx.x + (u0 == 0 ? 0 : 1));
       u0 += tiles;
-      left -= tiles;
+      left -= p.whole ? 1 : tiles;
       if (left > 0) next_item<ROWS, TILE>(p, now);
     }
   }
@@ -626,7 +260,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
 }
 
 // Joins the parts of an item.  CTA x sees to the item that ends in the run of CTA x of the first launch and began before it.
-constexpr int kJoinThreads = 128;
+constexpr int kJoinThreads = 128, kJoinAtOnce = 8;      // parts whose loads are in flight together
 
 template <typename T, int DP, int ROWS, int TILE>
 __global__ void __launch_bounds__(kJoinThreads) cache_attention_join_kernel(const __grid_constant__ CacheAttnParams p) {
@@ -643,18 +277,35 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attention_join_kernel(cons
   for (int i = blockIdx.y * kJoinThreads + threadIdx.x; i < rows_here * (DP / 4); i += gridDim.y * kJoinThreads) {
     const int row = i / (DP / 4), d = i % (DP / 4) * 4;
     if (d >= p.c.head_dim) continue;
+    // (a run that the item begins in, but not with, has left it as its second part)
+    const int later = run.all * first / run.parts != begins ? 1 : 0;
     float top = -CUDART_INF_F, sum = 0.0f;
     float4 x = make_float4(0, 0, 0, 0);
-    for (int r = first; r <= (int)blockIdx.x; ++r) {
-      // (a run that the item begins in, but not with, has left it as its second part)
-      const int64_t slot = 2 * (int64_t)r + (r == first && run.all * r / run.parts != begins ? 1 : 0);
-      const float* const part = p.partial + slot * p.partial_floats;
-      const float m = part[ROWS * DP + row], l = part[ROWS * DP + ROWS + row];
-      if (m == -CUDART_INF_F) continue;
-      const float4 y = *reinterpret_cast<const float4*>(part + (int64_t)row * DP + d);
-      const float next = fmaxf(top, m), a = ex2(top - next), b = ex2(m - next);
-      sum = sum * a + l * b;
-      x.x = x.x * a + y.x * b, x.y = x.y * a + y.y * b, x.z = x.z * a + y.z * b, x.w = x.w * a + y.w * b;
+    for (int r0 = first; r0 <= (int)blockIdx.x; r0 += kJoinAtOnce) {
+      float m[kJoinAtOnce], l[kJoinAtOnce], next = top;
+      float4 y[kJoinAtOnce];
+#pragma unroll
+      for (int j = 0; j < kJoinAtOnce; ++j) {
+        const int r = min(r0 + j, (int)blockIdx.x);
+        const float* const part = p.partial + (2 * (int64_t)r + (r == first ? later : 0)) * p.partial_floats;
+        m[j] = part[ROWS * DP + row];
+        l[j] = part[ROWS * DP + ROWS + row];
+        y[j] = *reinterpret_cast<const float4*>(part + (int64_t)row * DP + d);
+      }
+#pragma unroll
+      for (int j = 0; j < kJoinAtOnce; ++j) {
+        if (r0 + j > (int)blockIdx.x) m[j] = -CUDART_INF_F;
+        next = fmaxf(next, m[j]);
+      }
+      if (next == -CUDART_INF_F) continue;           // nothing seen so far
+      const float a = ex2(top - next);
+      sum *= a, x.x *= a, x.y *= a, x.z *= a, x.w *= a;
+#pragma unroll
+      for (int j = 0; j < kJoinAtOnce; ++j) {
+        if (m[j] == -CUDART_INF_F) continue;
+        const float b = ex2(m[j] - next);
+        sum += l[j] * b, x.x += y[j].x * b, x.y += y[j].y * b, x.z += y[j].z * b, x.w += y[j].w * b;
+      }
       top = next;
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -671,41 +322,51 @@ struct Variant {
   void (*kernel)(CUtensorMap, CacheAttnParams);
   void (*join)(CacheAttnParams);
   int threads, smem, rows, tile;   // rows and keys of a tile
+  int groups;                      // tiles at work at once
   int64_t part_floats;
 };
 
-template <typename T, int DP, int RG>
+template <typename Math, int RG>
 Variant variant() {
-  using Z = Shape<T, DP, RG>;
-  return Variant{cache_attention_kernel<T, DP, RG>, cache_attention_join_kernel<T, DP, 16 * RG, Z::kTile>, Z::kThreads, Z::kSmem, 16 * RG, Z::kTile,
-                 part_floats<DP, 16 * RG>()};
+  using Z = Shape<Math, RG>;
+  return Variant{cache_attention_kernel<Math, RG>, cache_attention_join_kernel<typename Math::Type, Math::kDim, Z::kRows, Z::G::kKeys>, Z::kThreads, Z::kSmem,
+                 Z::kRows, Z::G::kKeys, Z::kGroups, part_floats(Math::kDim, Z::kRows)};
 }
 
-// Tiles of 16, 32 and 64 query rows.
+// By the rows of an item, up to 64 to a row tile.
 template <typename T, int DP>
-Variant variant_of(int index) { return index == 0 ? variant<T, DP, 1>() : index == 1 ? variant<T, DP, 2>() : variant<T, DP, 4>(); }
+Variant variant_of(int rows) {
+  if constexpr (sizeof(T) == 4)
+    return rows <= 2 ? variant<FmaMath<DP, 2, 1>, 1>() : rows <= 4 ? variant<FmaMath<DP, 4, 1>, 1>() : rows <= 8 ? variant<FmaMath<DP, 8, 1>, 1>()
+           : rows <= 16 ? variant<FmaMath<DP, 16, 1>, 1>() : rows <= 32 ? variant<FmaMath<DP, 16, 2>, 2>() : variant<FmaMath<DP, 16, 4>, 4>();
+  else
+    return rows <= 16 ? variant<MmaMath<T, DP, 1>, 1>() : rows <= 32 ? variant<MmaMath<T, DP, 2>, 2>() : variant<MmaMath<T, DP, 4>, 4>();
+}
 template <typename T>
-Variant variant_of(int head_dim, int index) {
-  return head_dim <= 64 ? variant_of<T, 64>(index) : head_dim <= 128 ? variant_of<T, 128>(index) : variant_of<T, 256>(index);
+Variant variant_of(int head_dim, int rows) {
+  return head_dim <= 64 ? variant_of<T, 64>(rows) : head_dim <= 128 ? variant_of<T, 128>(rows) : variant_of<T, 256>(rows);
 }
-Variant variant_at(const Cache& c, int index) {
-  return c.dtype == KB200_DTYPE_FP32 ? variant_of<float>(c.view.head_dim, index)
-         : c.dtype == KB200_DTYPE_BF16 ? variant_of<__nv_bfloat16>(c.view.head_dim, index) : variant_of<__half>(c.view.head_dim, index);
+Variant variant_for(const Cache& c, int rows) {
+  return c.dtype == KB200_DTYPE_FP32 ? variant_of<float>(c.view.head_dim, rows)
+         : c.dtype == KB200_DTYPE_BF16 ? variant_of<__nv_bfloat16>(c.view.head_dim, rows) : variant_of<__half>(c.view.head_dim, rows);
 }
+Variant variant_for(const Cache& c, int tokens, int heads) { return variant_for(c, tokens * (heads / c.view.kv_heads)); }
 
-// As many rows to a tile as there are: every row tile reads the keys again.
-int variant_index(const Cache& c, int tokens, int heads) {
-  const int64_t rows = (int64_t)tokens * (heads / c.view.kv_heads);
-  return rows <= 16 ? 0 : rows <= 32 ? 1 : 2;
-}
-
-// CTAs that share the work: all that fit, but no more than there can be units.
-int parts_of(const Cache& c, const Variant& v, int rows, int tokens, int heads) {
+// How a call is divided: a CTA per SM, but no more than have a tile for each of their warps.
+struct Division {
+  int parts, min_units;
+  bool whole;
+};
+Division division_of(const Cache& c, const Variant& v, int rows, int tokens, int heads) {
   const int64_t row_tiles = ((int64_t)tokens * (heads / c.view.kv_heads) + v.rows - 1) / v.rows;
   const int64_t tiles = (((int64_t)c.view.max_pages << c.view.page_log2) + v.tile - 1) / v.tile;
-  const double units = (double)rows * c.view.kv_heads * row_tiles * tiles;
-  return (int)std::min<double>(units, (double)c.sm_count);
+  Division d{0, 1, tiles <= v.groups};
+  if (!d.whole) d.min_units = v.groups;
+  const double units = (double)rows * c.view.kv_heads * row_tiles * (d.whole ? 1 : tiles);
+  d.parts = (int)std::min<double>(std::ceil(units / d.min_units), (double)c.sm_count);
+  return d;
 }
+uint64_t workspace_of(const Variant& v, const Division& d) { return d.whole ? 0 : (uint64_t)d.parts * 2 * v.part_floats * sizeof(float); }
 
 Cache* cache_of(const kb200_cache* c) { return reinterpret_cast<Cache*>(const_cast<kb200_cache*>(c)); }
 
@@ -720,7 +381,7 @@ int cache_attention_prepare(Cache& c) {
   const EncodeFn encode = encode_fn();
   if (encode == nullptr) return fail(KB200_ERR_CUDA, "kb200_cache_create: the driver has no cuTensorMapEncodeTiled");
   const CacheView& v = c.view;
-  const int page = 1 << v.page_log2, columns = 128 / c.element, tile = variant_at(c, 0).tile;
+  const int page = 1 << v.page_log2, columns = 128 / c.element, tile = variant_for(c, 1).tile;
   const cuuint64_t dims[3] = {(cuuint64_t)v.head_dim, (cuuint64_t)v.kv_heads * page, (cuuint64_t)v.layers * 2 * v.pages};
   const cuuint64_t strides[2] = {(cuuint64_t)v.head_dim * c.element, dims[1] * v.head_dim * c.element};
   const cuuint32_t box[3] = {(cuuint32_t)columns, (cuuint32_t)std::min(page, tile), 1}, steps[3] = {1, 1, 1};
@@ -731,8 +392,8 @@ int cache_attention_prepare(Cache& c) {
   const CUresult r = encode(&c.map, type, 3, v.pool, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(KB200_ERR_UNSUPPORTED, "kb200_cache_create: the pool cannot be described to the copy engine (error %d)", (int)r);
-  for (int i = 0; i < 3; ++i) {
-    const Variant of = variant_at(c, i);
+  for (int rows = 2; rows <= 64; rows *= 2) {
+    const Variant of = variant_for(c, rows);
     KB200_CUDA(cudaFuncSetAttribute(of.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, of.smem));
   }
   return KB200_OK;
@@ -746,9 +407,8 @@ KB200_EXPORT uint64_t kb200_cache_attend_workspace(const kb200_cache* handle, in
   if (handle == nullptr) return 0;
   const Cache& c = *cache_of(handle);
   if (!call_ok(c, rows, tokens, heads) || rows == 0 || tokens == 0) return 0;
-  const int index = variant_index(c, tokens, heads);
-  const Variant v = variant_at(c, index);
-  return (uint64_t)parts_of(c, v, rows, tokens, heads) * 2 * v.part_floats * sizeof(float);
+  const Variant v = variant_for(c, tokens, heads);
+  return workspace_of(v, division_of(c, v, rows, tokens, heads));
 }
 
 KB200_EXPORT int kb200_cache_attend(kb200_cache* handle, int layer, const kb200_rows* q, const kb200_rows* out, int rows, int tokens,
@@ -769,11 +429,10 @@ KB200_EXPORT int kb200_cache_attend(kb200_cache* handle, int layer, const kb200_
   }
   if (mask != nullptr && mask_stride == nullptr) return fail(KB200_ERR_ARGUMENT, "kb200_cache_attend: a mask without strides");
   if (!(scale > 0.0f) || !(scale < 1e30f)) return fail(KB200_ERR_ARGUMENT, "kb200_cache_attend: scale must be positive and finite");
-  const int index = variant_index(c, tokens, q->heads);
-  const Variant v = variant_at(c, index);
-  const int parts = parts_of(c, v, rows, tokens, q->heads);
-  const uint64_t need = (uint64_t)parts * 2 * v.part_floats * sizeof(float);
-  if (workspace == nullptr || !tc::aligned16(workspace) || workspace_bytes < need)
+  const Variant v = variant_for(c, tokens, q->heads);
+  const Division d = division_of(c, v, rows, tokens, q->heads);
+  const uint64_t need = workspace_of(v, d);
+  if (need > 0 && (workspace == nullptr || !tc::aligned16(workspace) || workspace_bytes < need))
     return fail(KB200_ERR_ARGUMENT, "kb200_cache_attend: a workspace of %llu bytes on 16 bytes is needed", (unsigned long long)need);
   const DeviceGuard guard(c.device);
   if (guard.error != cudaSuccess) return cuda_fail(guard.error, "kb200_cache_attend");
@@ -793,11 +452,12 @@ KB200_EXPORT int kb200_cache_attend(kb200_cache* handle, int layer, const kb200_
   p.tokens = tokens;
   p.heads = q->heads;
   p.group = q->heads / c.view.kv_heads;
-  p.parts = parts;
-  p.min_units = 2;
+  p.parts = d.parts;
+  p.min_units = d.min_units;
+  p.whole = d.whole;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.q_fp32 = q->dtype != c.dtype;
-  KB200_CUDA(launch_kernel(true, v.kernel, dim3(parts), dim3(v.threads), v.smem, s, c.map, p));
-  KB200_CUDA(launch_kernel(true, v.join, dim3(parts, v.rows / 8), dim3(kJoinThreads), 0, s, p));
+  KB200_CUDA(launch_kernel(true, v.kernel, dim3(d.parts), dim3(v.threads), v.smem, s, c.map, p));
+  if (!d.whole) KB200_CUDA(launch_kernel(true, v.join, dim3(d.parts, std::max(1, v.rows / 8)), dim3(kJoinThreads), 0, s, p));
   return KB200_OK;
 }

@@ -19,6 +19,7 @@ struct CacheAttnParams {
   int parts;                               // CTAs that share the work at most
   int min_units;                           // ... each this many units at least
   float scale_log2;
+  bool whole;                              // items are not divided: no parts
   bool q_fp32;                             // q is float32 where the cache is not
 };
 
@@ -26,7 +27,8 @@ struct CacheAttnParams {
 // of a call, sequence by sequence, key head by key head, row tile by row tile, are divided into equal runs of neighbours, one
 // per CTA, whatever the sequences' lengths are: a ragged batch keeps all SMs busy to the end.  A run that starts or ends inside an item (a
 // row tile of a head of a sequence) leaves its part of the softmax in the workspace, at most two parts per CTA; the
-// second launch joins them in the order of the keys.
+// second launch joins them in the order of the keys.  Where no sequence can have more tiles than a CTA works on at once the units are whole items, and there is
+// nothing to join.
 
 struct CacheItems {                        // of one batch row
   int slot, length, count;                 // committed and drafted tokens
@@ -56,7 +58,7 @@ __device__ __forceinline__ CacheItems cache_items(const CacheAttnParams& p, int 
   if (r.end < length + count) cache_fault(p.c, KB200_CACHE_NO_ROOM);
   r.row_tiles = (count * p.group + ROWS - 1) / ROWS;
   r.key_tiles = max(1, (r.end + TILE - 1) / TILE);
-  r.units = (int64_t)r.row_tiles * r.key_tiles * p.c.kv_heads;
+  r.units = (int64_t)r.row_tiles * (p.whole ? 1 : r.key_tiles) * p.c.kv_heads;
   return r;
 }
 
@@ -139,11 +141,12 @@ __device__ __forceinline__ bool find_run(const CacheAttnParams& p, int part, Cac
   at.b = shared.b;
   at.it = shared.it;
   int64_t rest = shared.rest;
-  const int64_t per_head = (int64_t)at.it.row_tiles * at.it.key_tiles;
+  const int item = p.whole ? 1 : at.it.key_tiles;
+  const int64_t per_head = (int64_t)at.it.row_tiles * item;
   at.head = (int)(rest / per_head);
   rest -= at.head * per_head;
-  at.row_tile = (int)(rest / at.it.key_tiles);
-  at.tile = (int)(rest - (int64_t)at.row_tile * at.it.key_tiles);
+  at.row_tile = (int)(rest / item);
+  at.tile = (int)(rest - (int64_t)at.row_tile * item);
   return true;
 }
 

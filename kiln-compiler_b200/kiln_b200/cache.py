@@ -196,9 +196,9 @@ class PagedCache:
             raise ValueError("out requires a gradient")
         direct, out_rows = self._tokens("out", out)
         n_bytes = self._lib.kb200_cache_attend_workspace(self._cache, rows, tokens, heads)
-        workspace = torch.empty(max(n_bytes, 16), dtype=torch.uint8, device=self.device)
+        workspace = torch.empty(n_bytes, dtype=torch.uint8, device=self.device) if n_bytes else None
         _cabi.check(self._lib.kb200_cache_attend(self._cache, layer, q_rows, out_rows, rows, tokens, self._at(mask), strides, self._at(counts), self._at(slots),
-                                                 self.head_dim ** -0.5 if scale is None else scale, workspace.data_ptr(), n_bytes, self._stream()), self._lib)
+                                                 self.head_dim ** -0.5 if scale is None else scale, self._at(workspace), n_bytes, self._stream()), self._lib)
         if direct.data_ptr() != out.data_ptr():
             out.copy_(direct)
         return out

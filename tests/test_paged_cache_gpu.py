@@ -552,11 +552,12 @@ def test_many_calls_leave_the_allocator_as_it_was():
 def test_c_entry_refuses_short_workspaces():
     import ctypes as C
 
-    cache, q = filled([300], [2], dtype=BF16, kv_heads=2, head_dim=64)
+    cache, q = filled([3000], [2], dtype=BF16, kv_heads=2, head_dim=64)
     q = q.to(BF16)
     lib = _cabi.load()
     n = lib.kb200_cache_attend_workspace(cache._cache, 1, 2, 2)
     rows = cache._tokens("q", q)[1]
+    assert n > 0
     space = torch.empty(n + 16, dtype=torch.uint8, device="cuda")
     out = torch.empty_like(q)
     out_rows = cache._tokens("out", out)[1]
