@@ -39,7 +39,7 @@ struct Shape {
   static constexpr int kThreads = 32 * (kWarps + 1);
   static constexpr int kSlots = 2;                                       // warps whose rows are in shared memory at a time when sums are joined
   static constexpr int kSlotFloats = Math::kOut * 32;
-  static constexpr int kQuery = kWide ? Math::kRows * Math::kDim : 0, kWeights = kWide ? G::kKeys * Math::kRows : 0;      // floats of a warp
+  static constexpr int kQuery = kWide ? Math::kRows * Math::kDim : 0, kWeights = kWide ? G::kKeys * (Math::kRows + 4) : 0;      // floats of a warp
   static constexpr int kBeside = (kSlots * kSlotFloats + kWarps * (kQuery + kWeights)) * 4;
   static constexpr int kStages = kGroups * ((222 * 1024 - kBeside) / G::kBytes / kGroups);      // (a multiple: see above)
   static constexpr int kSmem = kStages * G::kBytes + kBeside;
@@ -65,8 +65,9 @@ __device__ __forceinline__ bool wait_a_second(uint32_t bar, uint32_t parity, vol
   }
 }
 
-// A part: ROWS output rows (not divided by their sums), then their maxima and sums.
-constexpr int64_t part_floats(int dim, int rows) { return (int64_t)rows * (dim + 2); }
+// A part, by groups of rows: a warp's output registers, not divided by their sums, then its rows' maxima and sums.
+template <typename Math>
+constexpr int kPartOfWarp = Math::kOut * 32 + 2 * Math::kRows;
 
 template <typename Math, int RG>
 __global__ void __launch_bounds__(Shape<Math, RG>::kThreads, 1)
@@ -74,13 +75,15 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
   using Z = Shape<Math, RG>;
   using T = typename Math::Type;
   using G = typename Z::G;
-  constexpr int KG = Z::kGroups, ROWS = Z::kRows, TILE = G::kKeys, DP = Math::kDim;
+  constexpr int KG = Z::kGroups, ROWS = Z::kRows, TILE = G::kKeys;
   static_assert(Z::kStages > 0 && Z::kStages % KG == 0 && (KG == 1 || Z::kSlots % RG == 0), "a stage belongs to one group, a slot to a warp of each row group");
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[2 * Z::kStages];
   __shared__ CacheRunShared found;
-  __shared__ uint32_t sees[Z::kWarps][Math::kRows][2];      // a tile with drafted tokens under a mask: which row sees which key
-  __shared__ float states[Z::kWarps][Math::kRows][2];
+  __shared__ uint2 sees[Z::kWarps][16];            // a tile with drafted tokens: which row sees which key
+  __shared__ float2 states[Z::kWarps][Math::kRows];       // maxima and sums, by place in an item that several groups had a tile of
+  __shared__ float2 own_states[Z::kWarps][Math::kRows];   // ... of all of them, or of a warp that had it alone: others may be at other items
+  __shared__ float factors[Z::kWarps][Math::kRows];
   __shared__ int abort_flag;
 
   const int lane = threadIdx.x & 31, warp = warp_index();
@@ -171,16 +174,24 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
     auto finish = [&](int order, int tiles, bool whole, int64_t part) {
       math.sum_up();
       int n = min(KG, tiles);                        // groups of keys that had a tile
+      math.put_states(lane, n > 1 ? states[order * RG + row_group] : own_states[warp]);
       if (n > 1) {
-        // to the largest maximum
-        math.states(lane, [&](int row, float top, float) { states[order * RG + row_group][row][0] = top; });
         meet();
-        math.rescale(lane, [&](int row) {
-          float top = -CUDART_INF_F;
-          for (int w = 0; w < n; ++w) top = fmaxf(top, states[w * RG + row_group][row][0]);
-          return top;
-        });
-        math.states(lane, [&](int row, float, float sum) { states[order * RG + row_group][row][1] = sum; });
+        // to the largest maximum
+        float factor = 0.0f;
+        float2 all = make_float2(-CUDART_INF_F, 0.0f);
+        const int row = lane % Math::kRows;
+        const float top = states[order * RG + row_group][row].x;
+        for (int w = 0; w < n; ++w) all.x = fmaxf(all.x, states[w * RG + row_group][row].x);
+        for (int w = 0; w < n; ++w) {
+          const float2 state = states[w * RG + row_group][row];
+          if (state.x != -CUDART_INF_F) all.y += state.y * ex2(state.x - all.x);
+        }
+        if (top != -CUDART_INF_F) factor = ex2(top - all.x);
+        if (lane < Math::kRows) factors[warp][lane] = factor;
+        meet();                                      // (which also says that the states have been read)
+        math.rescale(lane, factors[warp]);
+        if (lane < Math::kRows) own_states[warp][lane] = all;
         while (n > 1) {                              // the upper half's rows go to the lower half, as many at a time as there are slots
           const int half = (n + 1) / 2;
           for (int from = half; from < n; from += Z::kSlots / RG) {
@@ -188,36 +199,21 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
             float* const slot = slots + ((order >= half ? order - from : order + half - from) * RG + row_group) * Z::kSlotFloats + lane;
             if (order >= from && order < to) math.each_out([&](int i, float x) { slot[i * 32] = x; });
             meet();
-            if (order + half >= from && order + half < to) {
-              math.each_out([&](int i, float& x) { x += slot[i * 32]; });
-              math.add_sums(lane, [&](int row) { return states[(order + half) * RG + row_group][row][1]; });
-              __syncwarp();
-              math.states(lane, [&](int row, float, float sum) { states[order * RG + row_group][row][1] = sum; });
-            }
+            if (order + half >= from && order + half < to) math.each_out([&](int i, float& x) { x += slot[i * 32]; });
             meet();
           }
           n = half;
         }
       }
+      __syncwarp();
       if (order != 0) return;
-      math.each_row(lane, [&](int row, float sum, float top, bool once, auto&& columns) {
-        row += at.row0;
-        if (row >= at.rows_here) return;
-        if (whole) {
-          const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-          const CacheRow r = row_of<ROWS>(p, now, row);
-          T* const to = static_cast<T*>(p.out) + now.b * p.out_stride[0] + r.token * p.out_stride[1] + r.head * p.out_stride[2];
-          columns([&](int d, float x, float y) {
-            if (d < p.c.head_dim) store2<T>(to + d, x * inv, y * inv);
-          });
-        } else {
-          float* const to = p.partial + part * p.partial_floats;
-          columns([&](int d, float x, float y) {
-            if (d < p.c.head_dim) *reinterpret_cast<float2*>(to + (int64_t)row * DP + d) = make_float2(x, y);
-          });
-          if (once) to[ROWS * DP + row] = top, to[ROWS * DP + ROWS + row] = sum;
-        }
-      });
+      if (whole) {
+        math.template write<ROWS>(p, now, at, own_states[warp], query);
+      } else {
+        float* const to = p.partial + part * p.partial_floats + row_group * kPartOfWarp<Math>;
+        math.each_out([&](int i, float x) { to[i * 32 + lane] = x; });
+        if (lane < Math::kRows) reinterpret_cast<float2*>(to + Math::kOut * 32)[lane] = own_states[warp][lane];
+      }
     };
 
     int64_t left = any ? run.hi - run.lo : 0;
@@ -229,19 +225,19 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
       if constexpr (Z::kWide) math.template begin<ROWS>(p, now, at, query);
       else math.template begin<ROWS>(p, now, at);
       const int order = (int)((key_group + KG - u0 % KG) % KG);
+      uint32_t ahead = 0u;
+      if (p.mask != nullptr && p.tokens <= kMaskAhead && order < tiles && (now.tile + tiles) * TILE > at.sure)
+        ahead = mask_word<ROWS>(p, now, at, (lane >> 4) * 32);
       for (int i = order; i < tiles; i += KG) {
         const uint32_t u = u0 + i, stage = u % Z::kStages;
         at.key0 = (now.tile + i) * TILE;
         if (wait(full + 8 * stage, (u / Z::kStages) & 1)) {
           at.k = smem + stage * G::kBytes;
           at.v = at.k + G::kHalf;
-          if constexpr (Z::kWide) math.template tile<ROWS>(p, now, at, sees[warp], query, query + Z::kQuery);
-          else math.template tile<ROWS>(p, now, at, sees[warp]);
+          if constexpr (Z::kWide) math.template tile<ROWS>(p, now, at, ahead, sees[warp], query, query + Z::kQuery);
+          else math.template tile<ROWS>(p, now, at, ahead, sees[warp]);
           __syncwarp();
           if (lane == 0) mbar_arrive(empty + 8 * stage);
-        } else if (RG > 1 && at.key0 + TILE > at.sure) {         // (the meetings of a tile with drafted tokens)
-          meet_rows<RG>(key_group);
-          meet_rows<RG>(key_group);
         }
       }
       // a part that begins with the run is the run's first, else its second
@@ -262,8 +258,10 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
 // Joins the parts of an item.  CTA x sees to the item that ends in the run of CTA x of the first launch and began before it.
 constexpr int kJoinThreads = 128, kJoinAtOnce = 8;      // parts whose loads are in flight together
 
-template <typename T, int DP, int ROWS, int TILE>
+template <typename Math, int RG>
 __global__ void __launch_bounds__(kJoinThreads) cache_attention_join_kernel(const __grid_constant__ CacheAttnParams p) {
+  using T = typename Math::Type;
+  constexpr int DP = Math::kDim, ROWS = Math::kRows * RG, TILE = Tile<T, DP>::kKeys;
   __shared__ CacheRunShared found;
   pdl_wait();
   pdl_launch_dependents();
@@ -277,6 +275,8 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attention_join_kernel(cons
   for (int i = blockIdx.y * kJoinThreads + threadIdx.x; i < rows_here * (DP / 4); i += gridDim.y * kJoinThreads) {
     const int row = i / (DP / 4), d = i % (DP / 4) * 4;
     if (d >= p.c.head_dim) continue;
+    const int in_warp = row % Math::kRows;
+    const int at0 = Math::place(in_warp, d), at1 = Math::place(in_warp, d + 1), at2 = Math::place(in_warp, d + 2), at3 = Math::place(in_warp, d + 3);
     // (a run that the item begins in, but not with, has left it as its second part)
     const int later = run.all * first / run.parts != begins ? 1 : 0;
     float top = -CUDART_INF_F, sum = 0.0f;
@@ -287,10 +287,11 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attention_join_kernel(cons
 #pragma unroll
       for (int j = 0; j < kJoinAtOnce; ++j) {
         const int r = min(r0 + j, (int)blockIdx.x);
-        const float* const part = p.partial + (2 * (int64_t)r + (r == first ? later : 0)) * p.partial_floats;
-        m[j] = part[ROWS * DP + row];
-        l[j] = part[ROWS * DP + ROWS + row];
-        y[j] = *reinterpret_cast<const float4*>(part + (int64_t)row * DP + d);
+        const float* const part = p.partial + (2 * (int64_t)r + (r == first ? later : 0)) * p.partial_floats + row / Math::kRows * kPartOfWarp<Math>;
+        const float2 state = reinterpret_cast<const float2*>(part + Math::kOut * 32)[in_warp];
+        m[j] = state.x;
+        l[j] = state.y;
+        y[j] = make_float4(part[at0], part[at1], part[at2], part[at3]);
       }
 #pragma unroll
       for (int j = 0; j < kJoinAtOnce; ++j) {
@@ -329,18 +330,18 @@ struct Variant {
 template <typename Math, int RG>
 Variant variant() {
   using Z = Shape<Math, RG>;
-  return Variant{cache_attention_kernel<Math, RG>, cache_attention_join_kernel<typename Math::Type, Math::kDim, Z::kRows, Z::G::kKeys>, Z::kThreads, Z::kSmem,
-                 Z::kRows, Z::G::kKeys, Z::kGroups, part_floats(Math::kDim, Z::kRows)};
+  return Variant{cache_attention_kernel<Math, RG>, cache_attention_join_kernel<Math, RG>, Z::kThreads, Z::kSmem,
+                 Z::kRows, Z::G::kKeys, Z::kGroups, (int64_t)RG * kPartOfWarp<Math>};
 }
 
 // By the rows of an item, up to 64 to a row tile.
 template <typename T, int DP>
 Variant variant_of(int rows) {
   if constexpr (sizeof(T) == 4)
-    return rows <= 2 ? variant<FmaMath<DP, 2, 1>, 1>() : rows <= 4 ? variant<FmaMath<DP, 4, 1>, 1>() : rows <= 8 ? variant<FmaMath<DP, 8, 1>, 1>()
-           : rows <= 16 ? variant<FmaMath<DP, 16, 1>, 1>() : rows <= 32 ? variant<FmaMath<DP, 16, 2>, 2>() : variant<FmaMath<DP, 16, 4>, 4>();
+    return rows <= 2 ? variant<FmaMath<DP, 2>, 1>() : rows <= 4 ? variant<FmaMath<DP, 4>, 1>() : rows <= 8 ? variant<FmaMath<DP, 8>, 1>()
+           : rows <= 12 ? variant<FmaMath<DP, 12>, 1>() : rows <= 16 ? variant<FmaMath<DP, 16>, 1>() : rows <= 32 ? variant<FmaMath<DP, 16>, 2>() : variant<FmaMath<DP, 16>, 4>();
   else
-    return rows <= 16 ? variant<MmaMath<T, DP, 1>, 1>() : rows <= 32 ? variant<MmaMath<T, DP, 2>, 2>() : variant<MmaMath<T, DP, 4>, 4>();
+    return rows <= 16 ? variant<MmaMath<T, DP>, 1>() : rows <= 32 ? variant<MmaMath<T, DP>, 2>() : variant<MmaMath<T, DP>, 4>();
 }
 template <typename T>
 Variant variant_of(int head_dim, int rows) {
@@ -392,7 +393,7 @@ int cache_attention_prepare(Cache& c) {
   const CUresult r = encode(&c.map, type, 3, v.pool, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(KB200_ERR_UNSUPPORTED, "kb200_cache_create: the pool cannot be described to the copy engine (error %d)", (int)r);
-  for (int rows = 2; rows <= 64; rows *= 2) {
+  for (const int rows : {2, 4, 8, 12, 16, 32, 64}) {
     const Variant of = variant_for(c, rows);
     KB200_CUDA(cudaFuncSetAttribute(of.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, of.smem));
   }

@@ -67,12 +67,20 @@ __device__ __forceinline__ void store2(T* to, float a, float b) {
   if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(to) = make_float2(a, b);
   else *reinterpret_cast<uint32_t*>(to) = pack<T>(a, b);
 }
-// Does one of the elements in a 32-bit word hold an infinity or NaN?
+// Sets the top bit of every element of a 32-bit word that is infinite or NaN, and may set others below it: the exponent's ones and one more.
 template <typename T>
-__device__ __forceinline__ bool not_finite(uint32_t w) {
-  if constexpr (sizeof(T) == 4) return (w & 0x7f800000u) == 0x7f800000u;
-  else if constexpr (std::is_same<T, __half>::value) return (w & 0x7c000000u) == 0x7c000000u || (w & 0x7c00u) == 0x7c00u;
-  else return (w & 0x7f800000u) == 0x7f800000u || (w & 0x7f80u) == 0x7f80u;
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  if constexpr (sizeof(T) == 4) return (w & 0x7f800000u) + 0x00800000u;
+  else if constexpr (std::is_same<T, __half>::value) return (w & 0x7c007c00u) + 0x04000400u;
+  else return (w & 0x7f807f80u) + 0x00800080u;
+}
+// Two 16-bit elements with zeros in place of infinities and NaN.
+template <typename T>
+__device__ __forceinline__ uint32_t finite_pair(uint32_t w) {
+  constexpr uint32_t kExponent = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  if ((w & kExponent) == kExponent) w &= 0xffff0000u;
+  if ((w >> 16 & kExponent) == kExponent) w &= 0xffffu;
+  return w;
 }
 template <typename T>
 __device__ __forceinline__ float to_float(T x) {
@@ -89,82 +97,70 @@ struct Place {
   int warp, lane, row_group, key_group;
 };
 
-// The keys of a tile with drafted tokens that the warp's rows see, a word per 32, by all lanes: row i of the warp's in sees[i].  All
-// loads are in flight together (where there is nothing to look up they read the mask's first byte).
-template <int ROWS, int WARP_ROWS, int KEYS>
-__device__ __forceinline__ void look_at_mask(const CacheAttnParams& p, const CacheCursor& now, const Place& at, uint32_t (*sees)[2]) {
-  constexpr int W = (KEYS + 31) / 32;
-  uint8_t bytes[WARP_ROWS][W];
-  const int first = now.row_tile * ROWS + at.row0;
-  int token = first / p.group, in_group = first - token * p.group;
-  const uint8_t* const mask = p.mask + now.b * p.mask_stride[0];
-#pragma unroll
-  for (int i = 0; i < WARP_ROWS; ++i) {
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const int j = at.key0 + w * 32 + at.lane - now.it.length;
-      const bool looked_up = j >= 0 && j < now.it.count && at.row0 + i < at.rows_here;
-      bytes[i][w] = *(looked_up ? mask + token * p.mask_stride[1] + j * p.mask_stride[2] : p.mask);
-    }
-    if (++in_group == p.group) in_group = 0, ++token;
-  }
-#pragma unroll
-  for (int i = 0; i < WARP_ROWS; ++i)
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const int key = at.key0 + w * 32 + at.lane;
-      const bool visible = key < now.it.length || (bytes[i][w] != 0 && at.row0 + i < at.rows_here);
-      const uint32_t word = __ballot_sync(0xffffffffu, visible && key < now.it.end && w * 32 + at.lane < KEYS);
-      if (at.lane == 0) sees[i][w] = word;
-    }
-  __syncwarp();
-}
-// ... of a row where no mask is given: drafted tokens up to its own.
+// What a warp's rows see of the drafted tokens.  Lane i has row i % 16 of the warp's, and of its drafted tokens the 32 from `first` on.  Small code on purpose, here
+// and below: a launch meets it cold, once or twice, and its instructions come from L2 (unrolled over rows and keys this was 13000 cycles).
 template <int ROWS>
-__device__ __forceinline__ unsigned long long shown_by_order(const CacheAttnParams& p, const CacheCursor& now, const Place& at, int row) {
-  const int n = min(now.it.end, now.it.length + row_of<ROWS>(p, now, row).token + 1) - at.key0;
-  return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
+__device__ __forceinline__ uint32_t mask_word(const CacheAttnParams& p, const CacheCursor& now, const Place& at, int first) {
+  const int row = at.row0 + (at.lane & 15);
+  if (row >= at.rows_here) return 0u;
+  const CacheRow r = row_of<ROWS>(p, now, row);
+  const uint8_t* const mask = p.mask + now.b * p.mask_stride[0] + r.token * p.mask_stride[1];
+  const int lo = max(0, -first), hi = min(32, now.it.count - first);
+  uint32_t word = 0u;
+#pragma unroll 8
+  for (int j = lo; j < hi; ++j) word |= mask[(first + j) * p.mask_stride[2]] != 0 ? 1u << j : 0u;
+  return word;
+}
+// Of up to this many drafted tokens the words are fetched when an item begins, under the way of its first keys.
+constexpr int kMaskAhead = 64;
+
+// The keys of a tile with drafted tokens that the warp's rows see: row i of the warp's in sees[i].
+template <int ROWS, int WARP_ROWS, int KEYS>
+__device__ __forceinline__ void look_at_mask(const CacheAttnParams& p, const CacheCursor& now, const Place& at, uint32_t ahead, uint2* sees) {
+  const int row = at.lane & 15, off = now.it.length - at.key0;         // where the first drafted token is in the tile
+  unsigned long long shows = 0ull;
+  if (p.mask == nullptr) {
+    const int n = off + row_of<ROWS>(p, now, at.row0 + row).token + 1;
+    shows = n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
+  } else {
+    uint32_t low = ahead, high;
+    if (p.tokens > kMaskAhead) low = mask_word<ROWS>(p, now, at, (at.lane >> 4) * 32 - off);
+    high = __shfl_sync(0xffffffffu, low, row + 16);
+    low = __shfl_sync(0xffffffffu, low, row);
+    shows = (unsigned long long)high << 32 | low;
+    if (p.tokens <= kMaskAhead) shows = off >= 64 || off <= -64 ? 0ull : off >= 0 ? shows << off : shows >> -off;
+    if (off > 0) shows |= off >= 64 ? ~0ull : (1ull << off) - 1;
+  }
+  const int last = now.it.end - at.key0;
+  if (last < 64) shows &= last <= 0 ? 0ull : (1ull << last) - 1;
+  if (at.lane < WARP_ROWS) sees[row] = make_uint2((uint32_t)shows, (uint32_t)(shows >> 32));
+  __syncwarp();
 }
 
-// V behind the sequence's end is what an earlier tenant left, and V of a drafted token that some rows do not see may hold infinities or NaN; 0 times
-// those is NaN.  True: such elements are among the tile's keys.  (The former are made zeros where the warp has the tile for itself.)
-template <typename T, int DP, bool ALONE>
-__device__ __forceinline__ bool look_at_values(const CacheCursor& now, const Place& at) {
+// V behind the sequence's end is what an earlier tenant left, as far as its last page goes (pages that it has not come as zeros), and V of a drafted token that some
+// rows do not see may hold infinities or NaN; 0 times those is NaN.  The former become zeros (every warp that reads the tile writes them, and looks at none of
+// them).  True: the latter are there.
+template <typename T, int DP>
+__device__ __forceinline__ bool look_at_values(const CacheAttnParams& p, const CacheCursor& now, const Place& at) {
   using G = Tile<T, DP>;
-  const int last = now.it.end - at.key0;
-  bool odd = false;
-#pragma unroll 8
-  for (int i = at.lane; i < G::kKeys * G::kBlocks * 8; i += 32) {
-    const int key = i / (G::kBlocks * 8), chunk = i % (G::kBlocks * 8);
+  constexpr int kChunks = G::kBlocks * 8;
+  const int in_page = (1 << p.c.page_log2) - 1, last = now.it.end - at.key0;
+  const int from = max(0, at.sure - at.key0), to = min(G::kKeys, ((now.it.end + in_page) & ~in_page) - at.key0);
+  uint32_t odd = 0u;
+#pragma unroll 2
+  for (int i = from * kChunks + at.lane; i < to * kChunks; i += 32) {
+    const int key = i / kChunks, chunk = i % kChunks;
     uint4* const x = reinterpret_cast<uint4*>(G::at(at.v, key, chunk * (16 / (int)sizeof(T))));
-    if (ALONE && key >= last) *x = make_uint4(0, 0, 0, 0);
-    else if (key < last) odd = odd || not_finite<T>(x->x) || not_finite<T>(x->y) || not_finite<T>(x->z) || not_finite<T>(x->w);
+    if (key >= last) *x = make_uint4(0, 0, 0, 0);
+    else odd |= not_finite<T>(x->x) | not_finite<T>(x->y) | not_finite<T>(x->z) | not_finite<T>(x->w);
   }
-  odd = __any_sync(0xffffffffu, odd) != 0;
+  const bool any = __any_sync(0xffffffffu, (odd & (sizeof(T) == 4 ? 0x80000000u : 0x80008000u)) != 0u) != 0;
   __syncwarp();
-  return odd;
-}
-// The warps that read a tile meet, make what must not enter the product zero, and meet again.  (Warps of other rows: each waits for all to
-// have seen the tile as it was.)
-template <int RG>
-__device__ __forceinline__ void meet_rows(int key_group) {
-  if constexpr (RG > 1) asm volatile("bar.sync %0, %1;" ::"r"(2 + key_group), "n"(32 * RG) : "memory");
-  else __syncwarp();
-}
-template <typename T, int DP, int RG>
-__device__ __forceinline__ void clear_values(const CacheCursor& now, const Place& at) {
-  using G = Tile<T, DP>;
-  meet_rows<RG>(at.key_group);
-  const int last = now.it.end - at.key0;
-  for (int i = at.row_group * 32 + at.lane; i < G::kKeys * DP; i += 32 * RG) {
-    T* const x = G::at(at.v, i / DP, i % DP);
-    if (i / DP >= last || !(fabsf(to_float(*x)) < CUDART_INF_F)) *x = T(0.0f);
-  }
-  meet_rows<RG>(at.key_group);
+  return any;
 }
 
 // 16-bit caches: mma.sync m16n8k16, the scores' accumulators being the weights' operands.  A thread holds rows g and g + 8.
-template <typename T, int DP, int RG>
+template <typename T, int DP>
 struct MmaMath {
   using Type = T;
   static constexpr int kDim = DP, kRows = 16, kOut = DP / 2;             // rows of a warp; output registers of a thread
@@ -202,8 +198,30 @@ struct MmaMath {
     }
   }
 
+  // The weights times V; CLEAN: with zeros in place of infinities and NaN in V.
+  template <bool CLEAN>
+  __device__ __forceinline__ void times_values(const float (&s)[NT][4], uint32_t v_tile, int lane) {
+    const uint32_t v_row = v_tile + (((lane >> 3) & 1) * 8 + (lane & 7)) * 128;
+#pragma unroll
+    for (int k = 0; k < NT / 2; ++k) {
+      const uint32_t a[4] = {pack<T>(s[2 * k][0], s[2 * k][1]), pack<T>(s[2 * k][2], s[2 * k][3]), pack<T>(s[2 * k + 1][0], s[2 * k + 1][1]),
+                             pack<T>(s[2 * k + 1][2], s[2 * k + 1][3])};
+#pragma unroll
+      for (int d = 0; d < DT; d += 2) {
+        uint32_t b[4];
+        ldmatrix4_t(b, v_row + k * 16 * 128 + (d / 8) * G::kBlockBytes + (((d % 8 + (lane >> 4)) ^ (lane & 7)) << 4));
+        if constexpr (CLEAN) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) b[i] = finite_pair<T>(b[i]);
+        }
+        mma16<T>(o[d], a, b[0], b[1]);
+        mma16<T>(o[d + 1], a, b[2], b[3]);
+      }
+    }
+  }
+
   template <int ROWS>
-  __device__ __forceinline__ void tile(const CacheAttnParams& p, const CacheCursor& now, const Place& at, uint32_t (*sees)[2]) {
+  __device__ __forceinline__ void tile(const CacheAttnParams& p, const CacheCursor& now, const Place& at, uint32_t ahead, uint2* sees) {
     const int lane = at.lane, g = lane >> 2, t4 = lane & 3;
     const uint32_t k_tile = smem_u32(at.k), v_tile = smem_u32(at.v);
     float s[NT][4];
@@ -226,14 +244,12 @@ struct MmaMath {
 
     const bool drafted = at.key0 + G::kKeys > at.sure;
     bool infinite = false;
-    unsigned long long shows[2] = {~0ull, ~0ull};    // the tile's keys that rows g and g + 8 see
     if (drafted) {
-      if (p.mask != nullptr) look_at_mask<ROWS, 16, G::kKeys>(p, now, at, sees);
+      look_at_mask<ROWS, 16, G::kKeys>(p, now, at, ahead, sees);
+      infinite = look_at_values<T, DP>(p, now, at);
+      unsigned long long shows[2];                   // the tile's keys that rows g and g + 8 see
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        shows[h] = p.mask == nullptr ? shown_by_order<ROWS>(p, now, at, at.row0 + g + 8 * h)
-                                     : sees[g + 8 * h][0] | (G::kKeys > 32 ? (unsigned long long)sees[g + 8 * h][1] << 32 : 0ull);
-      infinite = look_at_values<T, DP, RG == 1>(now, at);
+      for (int h = 0; h < 2; ++h) shows[h] = sees[g + 8 * h].x | (unsigned long long)sees[g + 8 * h].y << 32;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -276,30 +292,25 @@ struct MmaMath {
         l[j >> 1] += s[n][j];
       }
 
-    if (infinite)                                    // such elements are added to the rows that see them one by one, and are zero in the product
-      for (int key = 0; key < G::kKeys; ++key)
+    if (infinite) {  // infinities and NaN: one by one, to the rows that give them any weight; they are zero in the product
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+      for (int n = 0; n < NT; ++n)
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float x = to_float(*G::at(at.v, key, d * 8 + t4 * 2 + (j & 1)));
-            if (!(fabsf(x) < CUDART_INF_F) && (shows[j >> 1] >> key & 1)) o[d][j] += x;
+          for (int e = 0; e < 2; ++e) {
+            const float w[2] = {__shfl_sync(0xffffffffu, s[n][e], (lane & ~3) | t), __shfl_sync(0xffffffffu, s[n][2 + e], (lane & ~3) | t)};
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float x = to_float(*G::at(at.v, n * 8 + t * 2 + e, d * 8 + t4 * 2 + (j & 1)));
+                if (!(fabsf(x) < CUDART_INF_F) && w[j >> 1] != 0.0f) o[d][j] += w[j >> 1] * x;
+              }
           }
-    if (drafted && (RG > 1 || infinite)) clear_values<T, DP, RG>(now, at);
-
-    const uint32_t v_row = v_tile + (((lane >> 3) & 1) * 8 + (lane & 7)) * 128;
-#pragma unroll
-    for (int k = 0; k < NT / 2; ++k) {
-      const uint32_t a[4] = {pack<T>(s[2 * k][0], s[2 * k][1]), pack<T>(s[2 * k][2], s[2 * k][3]), pack<T>(s[2 * k + 1][0], s[2 * k + 1][1]),
-                             pack<T>(s[2 * k + 1][2], s[2 * k + 1][3])};
-#pragma unroll
-      for (int d = 0; d < DT; d += 2) {
-        uint32_t b[4];
-        ldmatrix4_t(b, v_row + k * 16 * 128 + (d / 8) * G::kBlockBytes + (((d % 8 + (lane >> 4)) ^ (lane & 7)) << 4));
-        mma16<T>(o[d], a, b[0], b[1]);
-        mma16<T>(o[d + 1], a, b[2], b[3]);
-      }
     }
+
+    if (infinite) times_values<true>(s, v_tile, lane);
+    else times_values<false>(s, v_tile, lane);
     if (drafted) fence_async_smem();                 // (the zeros, in front of the next copy to this stage)
   }
 
@@ -311,57 +322,52 @@ struct MmaMath {
       if (l[h] != l[h]) m[h] = 0.0f;                 // (NaN, which a maximum passes over, reaches the result)
     }
   }
-  // Maxima and sums of the warp's rows out and in, f(row, maximum, sum) once per row ...
-  template <typename F>
-  __device__ __forceinline__ void states(int lane, F&& f) const {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if ((lane & 3) == 0) f((lane >> 2) + 8 * h, m[h], l[h]);
+  __device__ __forceinline__ void put_states(int lane, float2* states) const {
+    if ((lane & 3) == 0) states[lane >> 2] = make_float2(m[0], l[0]), states[(lane >> 2) + 8] = make_float2(m[1], l[1]);
   }
-  // ... to a new maximum, top(row), and with another warp's sums added, more(row).
-  template <typename F>
-  __device__ __forceinline__ void rescale(int lane, F&& top) {
+  __device__ __forceinline__ void rescale(int lane, const float* factors) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float t = top((lane >> 2) + 8 * h), mine = m[h] == -CUDART_INF_F ? 0.0f : ex2(m[h] - t);
-      l[h] *= mine;
-      m[h] = t;
+      const float f = factors[(lane >> 2) + 8 * h];
 #pragma unroll
-      for (int d = 0; d < DT; ++d) o[d][2 * h] *= mine, o[d][2 * h + 1] *= mine;
+      for (int d = 0; d < DT; ++d) o[d][2 * h] *= f, o[d][2 * h + 1] *= f;
     }
-  }
-  template <typename F>
-  __device__ __forceinline__ void add_sums(int lane, F&& more) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) l[h] += more((lane >> 2) + 8 * h);
   }
   template <typename F>
   __device__ __forceinline__ void each_out(F&& f) {
 #pragma unroll
     for (int i = 0; i < kOut; ++i) f(i, o[i / 4][i % 4]);
   }
-  // f(row, its sum, its maximum, a function that hands the row's columns over: f2(column, two values))
-  template <typename F>
-  __device__ __forceinline__ void each_row(int lane, F&& f) const {
+  // Where a row's column is among the 32 x kOut values of a warp.
+  static __device__ __forceinline__ int place(int row, int d) { return (d / 8 * 4 + (row >> 3) * 2 + (d & 1)) * 32 + (row & 7) * 4 + d % 8 / 2; }
+  // The rows, divided by their sums; states: of all the item's warps together.
+  template <int ROWS>
+  __device__ __forceinline__ void write(const CacheAttnParams& p, const CacheCursor& now, const Place& at, const float2* states, float*) const {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      f((lane >> 2) + 8 * h, l[h], m[h], (lane & 3) == 0, [&](auto&& f2) {
+    for (int h = 0; h < 2; ++h) {
+      const int in_warp = (at.lane >> 2) + 8 * h, row = at.row0 + in_warp;
+      if (row >= at.rows_here) continue;
+      const float sum = states[in_warp].y, inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const CacheRow r = row_of<ROWS>(p, now, row);
+      T* const to = static_cast<T*>(p.out) + now.b * p.out_stride[0] + r.token * p.out_stride[1] + r.head * p.out_stride[2] + (at.lane & 3) * 2;
 #pragma unroll
-        for (int d = 0; d < DT; ++d) f2(d * 8 + (lane & 3) * 2, o[d][2 * h], o[d][2 * h + 1]);
-      });
+      for (int d = 0; d < DT; ++d)
+        if (d * 8 < p.c.head_dim) store2<T>(to + d * 8, o[d][2 * h] * inv, o[d][2 * h + 1] * inv);
+    }
   }
 };
 
 // float32 caches: multiply-adds, two to an instruction.  (Three TF32 products of split operands by mma.sync took 9200 cycles for 64 keys of 64, whatever
 // the number of rows, and lost a bit: these take ~1000 for 4 rows and ~3300 for 16.)  For the scores a lane has keys (two lanes share one where a
 // tile has 16), for the output it has DP / 32 columns of all rows; weights go from one to the other through shared memory.
-template <int DP, int R, int RG>
+template <int DP, int R>
 struct FmaMath {
   using Type = float;
   static constexpr int kDim = DP, kRows = R, kOut = R * DP / 32;
   using G = Tile<float, DP>;
   static constexpr int KEYS = G::kKeys >= 32 ? G::kKeys / 32 : 1;        // of a lane
   static constexpr int SHARE = G::kKeys >= 32 ? 1 : 32 / G::kKeys;       // lanes to a key, each with part of the columns
+  static constexpr int kVec = R < 4 ? R : 4, kWeightRow = R < 4 ? R : R + 4;       // (the weights of a key: rows apart by banks that lanes do not share)
   static constexpr int C = DP / 32;                                      // output columns of a lane: C lane .. C lane + C - 1
   float2 o[C][R / 2];                                // rows 2i and 2i + 1
   float m[R], l[R];                                  // (l: of the lane's keys)
@@ -371,7 +377,7 @@ struct FmaMath {
   __device__ __forceinline__ void begin(const CacheAttnParams& p, const CacheCursor& now, const Place& at, float* q) {
 #pragma unroll
     for (int r = 0; r < R; ++r) m[r] = -CUDART_INF_F, l[r] = 0.0f;
-#pragma unroll 8
+#pragma unroll 2
     for (int i = at.lane; i < R * (DP / 4); i += 32) {
       const int r = i / (DP / 4), d = i % (DP / 4) * 4;
       const bool there = at.row0 + r < at.rows_here && d < p.c.head_dim;
@@ -386,8 +392,55 @@ struct FmaMath {
       for (int i = 0; i < R / 2; ++i) o[c][i] = make_float2(0.0f, 0.0f);
   }
 
+  template <bool CLEAN>
+  __device__ __forceinline__ void times_values(const Place& at, const float* weights) {
+    constexpr int kUnroll = CLEAN ? 1 : 4;
+#pragma unroll kUnroll
+    for (int k = 0; k < G::kKeys; ++k) {
+      float x[C];
+      constexpr int kAtOnce = C < 4 ? C : 4;
+#pragma unroll
+      for (int c = 0; c < C; c += kAtOnce) {
+        const float* const from = G::at(at.v, k, C * at.lane + c);
+        if constexpr (kAtOnce == 4) {
+          const float4 v = *reinterpret_cast<const float4*>(from);
+          x[c] = v.x, x[c + 1] = v.y, x[c + 2] = v.z, x[c + 3] = v.w;
+        } else {
+          const float2 v = *reinterpret_cast<const float2*>(from);
+          x[c] = v.x, x[c + 1] = v.y;
+        }
+      }
+      float w[R];
+#pragma unroll
+      for (int r = 0; r < R; r += kVec) {
+        const float* const from = weights + k * kWeightRow + r;
+        if constexpr (kVec == 4) {
+          const float4 v = *reinterpret_cast<const float4*>(from);
+          w[r] = v.x, w[r + 1] = v.y, w[r + 2] = v.z, w[r + 3] = v.w;
+        } else {
+          const float2 v = *reinterpret_cast<const float2*>(from);
+          w[r] = v.x, w[r + 1] = v.y;
+        }
+      }
+      if constexpr (CLEAN) {                         // infinities and NaN: to the rows that give them any weight; they are zero in the product
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          if (fabsf(x[c]) < CUDART_INF_F) continue;
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+            if (w[r] != 0.0f) (r & 1 ? o[c][r / 2].y : o[c][r / 2].x) += w[r] * x[c];
+          x[c] = 0.0f;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < R / 2; ++i) o[c][i] = ffma2(make_float2(w[2 * i], w[2 * i + 1]), make_float2(x[c], x[c]), o[c][i]);
+    }
+  }
+
   template <int ROWS>
-  __device__ __forceinline__ void tile(const CacheAttnParams& p, const CacheCursor& now, const Place& at, uint32_t (*sees)[2], const float* q, float* weights) {
+  __device__ __forceinline__ void tile(const CacheAttnParams& p, const CacheCursor& now, const Place& at, uint32_t ahead, uint2* sees, const float* q, float* weights) {
     const int lane = at.lane;
     float2 sum[KEYS][R];
 #pragma unroll
@@ -413,80 +466,76 @@ struct FmaMath {
         }
       }
     }
+    float s[KEYS][R], top[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int i = 0; i < KEYS; ++i) s[i][r] = (sum[i][r].x + sum[i][r].y) * p.scale_log2;
+    if constexpr (SHARE > 1) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int d = 32 / SHARE; d < 32; d *= 2) s[0][r] += __shfl_xor_sync(0xffffffffu, s[0][r], d);
+    }
     const bool drafted = at.key0 + G::kKeys > at.sure;
     bool infinite = false;
     if (drafted) {
-      if (p.mask != nullptr) look_at_mask<ROWS, R, G::kKeys>(p, now, at, sees);
-      infinite = look_at_values<float, DP, RG == 1>(now, at);
+      look_at_mask<ROWS, R, G::kKeys>(p, now, at, ahead, sees);
+      infinite = look_at_values<float, DP>(p, now, at);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const uint2 shows = sees[r];
+#pragma unroll
+        for (int i = 0; i < KEYS; ++i)
+          if (!((i == 0 ? shows.x : shows.y) >> (key & 31) & 1)) s[i][r] = -CUDART_INF_F;
+      }
     }
+    bool grown = false;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      float s[KEYS], top = -CUDART_INF_F;
-      unsigned long long shows = ~0ull;
-      if (drafted) shows = p.mask == nullptr ? shown_by_order<ROWS>(p, now, at, at.row0 + r) : sees[r][0] | (G::kKeys > 32 ? (unsigned long long)sees[r][1] << 32 : 0ull);
+      top[r] = s[0][r];
 #pragma unroll
-      for (int i = 0; i < KEYS; ++i) {
-        s[i] = sum[i][r].x + sum[i][r].y;
+      for (int i = 1; i < KEYS; ++i) top[r] = fmaxf(top[r], s[i][r]);
+    }
 #pragma unroll
-        for (int d = 32 / SHARE; d < 32; d *= 2) s[i] += __shfl_xor_sync(0xffffffffu, s[i], d);
-        s[i] = shows >> (key + 32 * i) & 1 ? s[i] * p.scale_log2 : -CUDART_INF_F;
-        top = fmaxf(top, s[i]);
-      }
+    for (int d = 16; d > 0; d /= 2)
 #pragma unroll
-      for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-      if (top > m[r]) {                              // (the same in all lanes)
-        const float alpha = ex2(m[r] - top);
-        m[r] = top;
+      for (int r = 0; r < R; ++r) top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], d));
+#pragma unroll
+    for (int r = 0; r < R; ++r) grown = grown || top[r] > m[r];          // (the same in all lanes)
+    if (grown) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        top[r] = fmaxf(top[r], m[r]);
+        const float alpha = top[r] == -CUDART_INF_F ? 1.0f : ex2(m[r] - top[r]);
+        m[r] = top[r];
         l[r] *= alpha;
 #pragma unroll
         for (int c = 0; c < C; ++c) (r & 1 ? o[c][r / 2].y : o[c][r / 2].x) *= alpha;
       }
-      const float shift = m[r] == -CUDART_INF_F ? 0.0f : m[r];
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float shift = m[r] == -CUDART_INF_F ? 0.0f : m[r];           // nothing seen so far: every weight is 2^-inf
 #pragma unroll
       for (int i = 0; i < KEYS; ++i) {
-        s[i] = ex2(s[i] - shift);
-        if (lane < 32 / SHARE) l[r] += s[i];
-        if (SHARE == 1 || lane < 32 / SHARE) weights[(key + 32 * i) * R + r] = s[i];
+        s[i][r] = ex2(s[i][r] - shift);
+        if (SHARE == 1 || lane < 32 / SHARE) l[r] += s[i][r];
       }
     }
-    __syncwarp();
-    if (infinite) {
-      for (int k = 0; k < G::kKeys; ++k)
+    if (SHARE == 1 || lane < 32 / SHARE) {
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-          const float x = *G::at(at.v, k, C * lane + c);
-          if (fabsf(x) < CUDART_INF_F) continue;
+      for (int i = 0; i < KEYS; ++i)
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            const unsigned long long shows = p.mask == nullptr ? shown_by_order<ROWS>(p, now, at, at.row0 + r)
-                                                               : sees[r][0] | (G::kKeys > 32 ? (unsigned long long)sees[r][1] << 32 : 0ull);
-            if (shows >> k & 1) (r & 1 ? o[c][r / 2].y : o[c][r / 2].x) += x;
-          }
+        for (int r = 0; r < R; r += kVec) {
+          float* const to = weights + (key + 32 * i) * kWeightRow + r;
+          if constexpr (kVec == 4) *reinterpret_cast<float4*>(to) = make_float4(s[i][r], s[i][r + 1], s[i][r + 2], s[i][r + 3]);
+          else *reinterpret_cast<float2*>(to) = make_float2(s[i][r], s[i][r + 1]);
         }
     }
-    if (drafted && (RG > 1 || infinite)) clear_values<float, DP, RG>(now, at);
-#pragma unroll 4
-    for (int k = 0; k < G::kKeys; ++k) {
-      float x[C];
-      constexpr int kVec = C < 4 ? C : 4;
-#pragma unroll
-      for (int c = 0; c < C; c += kVec) {
-        const float* const from = G::at(at.v, k, C * lane + c);
-        if constexpr (kVec == 4) *reinterpret_cast<float4*>(x + c) = *reinterpret_cast<const float4*>(from);
-        else *reinterpret_cast<float2*>(x + c) = *reinterpret_cast<const float2*>(from);
-      }
-      float w[R];
-      if constexpr (R >= 4) {
-#pragma unroll
-        for (int r = 0; r < R; r += 4) *reinterpret_cast<float4*>(w + r) = *reinterpret_cast<const float4*>(weights + k * R + r);
-      } else {
-        *reinterpret_cast<float2*>(w) = *reinterpret_cast<const float2*>(weights + k * R);
-      }
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int i = 0; i < R / 2; ++i) o[c][i] = ffma2(make_float2(w[2 * i], w[2 * i + 1]), make_float2(x[c], x[c]), o[c][i]);
-    }
+    __syncwarp();
+    if (infinite) times_values<true>(at, weights);
+    else times_values<false>(at, weights);
     if (drafted) fence_async_smem();
     __syncwarp();                                    // (the weights have been read)
   }
@@ -499,27 +548,18 @@ struct FmaMath {
       if (l[r] != l[r]) m[r] = 0.0f;
     }
   }
-  template <typename F>
-  __device__ __forceinline__ void states(int lane, F&& f) const {
+  __device__ __forceinline__ void put_states(int lane, float2* states) const {
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      if (lane == r) f(r, m[r], l[r]);
+      if (lane == r) states[r] = make_float2(m[r], l[r]);
   }
-  template <typename F>
-  __device__ __forceinline__ void rescale(int, F&& top) {
+  __device__ __forceinline__ void rescale(int, const float* factors) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const float t = top(r), mine = m[r] == -CUDART_INF_F ? 0.0f : ex2(m[r] - t);
-      l[r] *= mine;
-      m[r] = t;
+      const float f = factors[r];
 #pragma unroll
-      for (int c = 0; c < C; ++c) (r & 1 ? o[c][r / 2].y : o[c][r / 2].x) *= mine;
+      for (int c = 0; c < C; ++c) (r & 1 ? o[c][r / 2].y : o[c][r / 2].x) *= f;
     }
-  }
-  template <typename F>
-  __device__ __forceinline__ void add_sums(int, F&& more) {
-#pragma unroll
-    for (int r = 0; r < R; ++r) l[r] += more(r);
   }
   template <typename F>
   __device__ __forceinline__ void each_out(F&& f) {
@@ -528,15 +568,24 @@ struct FmaMath {
 #pragma unroll
       for (int i = 0; i < R / 2; ++i) f((c * (R / 2) + i) * 2, o[c][i].x), f((c * (R / 2) + i) * 2 + 1, o[c][i].y);
   }
-  template <typename F>
-  __device__ __forceinline__ void each_row(int lane, F&& f) const {
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-      f(r, l[r], m[r], lane == 0, [&](auto&& f2) {
-#pragma unroll
-        for (int c = 0; c < C; c += 2)
-          f2(C * lane + c, r & 1 ? o[c][r / 2].y : o[c][r / 2].x, r & 1 ? o[c + 1][r / 2].y : o[c + 1][r / 2].x);
-      });
+  static __device__ __forceinline__ int place(int row, int d) { return ((d % C * (R / 2) + row / 2) * 2 + (row & 1)) * 32 + d / C; }
+  // (by way of the query rows' place, so that a small loop does: a launch meets this code cold)
+  template <int ROWS>
+  __device__ __forceinline__ void write(const CacheAttnParams& p, const CacheCursor& now, const Place& at, const float2* states, float* query) {
+    const int lane = at.lane;
+    __syncwarp();
+    each_out([&](int i, float x) { query[i * 32 + lane] = x; });
+    __syncwarp();
+#pragma unroll 2
+    for (int i = lane; i < R * (DP / 2); i += 32) {
+      const int in_warp = i / (DP / 2), row = at.row0 + in_warp, d = i % (DP / 2) * 2;
+      if (row >= at.rows_here || d >= p.c.head_dim) continue;
+      const float sum = states[in_warp].y, inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const CacheRow r = row_of<ROWS>(p, now, row);
+      store2<float>(static_cast<float*>(p.out) + now.b * p.out_stride[0] + r.token * p.out_stride[1] + r.head * p.out_stride[2] + d,
+                    query[place(in_warp, d)] * inv, query[place(in_warp, d + 1)] * inv);
+    }
+    __syncwarp();
   }
 };
 
