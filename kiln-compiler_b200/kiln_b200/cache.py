@@ -48,7 +48,7 @@ class PagedCache:
         for name, n in sizes.items():
             if not isinstance(n, int) or isinstance(n, bool) or not 0 < n < 2**31:
                 raise ValueError(f"{name} must be a positive integer, got {n!r}")
-        self._cache = C.c_void_p()
+        self._cache, self._caller = C.c_void_p(), None
         self._lib = _cabi.load()
         # what the library would refuse is refused before anything is allocated
         desc = _cabi.CacheDesc(DTYPES[dtype], layers, sequences, max_pages, pages, kv_heads, page_tokens, head_dim, 16, 2**63, 16, 16, 16, 16)
@@ -70,138 +70,46 @@ class PagedCache:
         self.refs = torch.zeros(pages, dtype=torch.int32, device=self.device)
         desc.pool, desc.pool_bytes = self.pool.data_ptr(), pool_bytes
         desc.table, desc.held, desc.lengths, desc.refs = (t.data_ptr() for t in (self.table, self.held, self.lengths, self.refs))
+        self._call = _cabi.load_call()
         _cabi.check(self._lib.kb200_cache_create(C.byref(desc), self.device.index, C.byref(self._cache)), self._lib)
-
-    # -- arguments -------------------------------------------------------------------------------
-
-    def _stream(self):
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def _integers(self, name, t, shape):
-        """A call's integers as the library takes them."""
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a tensor")
-        if t.dtype not in (torch.int32, torch.int64):
-            raise TypeError(f"{name} must hold int32 or int64, got {t.dtype}")
-        if tuple(t.shape) != shape:
-            raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
-        if t.device != self.device:
-            raise ValueError(f"{name} is on {t.device}, the cache on {self.device}")
-        if t.dtype == torch.int64:
-            t = t.clamp(-2**31, 2**31 - 1).to(torch.int32)
-        return t.contiguous()
-
-    def _tokens(self, name, t, heads=None):
-        """Rows of new tokens: [rows, tokens, heads, head_dim], copied where the kernels cannot read them as they are."""
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a tensor")
-        if t.dim() != 4 or t.shape[3] != self.head_dim or (heads is not None and t.shape[2] != heads):
-            raise ValueError(f"{name} must be [rows, tokens, {heads or 'heads'}, {self.head_dim}], got {tuple(t.shape)}")
-        if t.dtype != self.dtype and t.dtype != torch.float32:
-            raise TypeError(f"{name} must be {self.dtype} or torch.float32, got {t.dtype}")
-        if t.device != self.device:
-            raise ValueError(f"{name} is on {t.device}, the cache on {self.device}")
-        t = t.detach()
-        unit = 16 // t.element_size()
-        strides = t.stride()
-        if strides[3] != 1 or t.data_ptr() % 16 or any(s % unit for s in strides[:3]) or t.is_neg() or t._is_zerotensor():
-            t = t.clone(memory_format=torch.contiguous_format)
-            strides = t.stride()
-        return t, _cabi.Rows(t.data_ptr(), DTYPES[t.dtype], t.shape[2], strides[:3])
-
-    def _batch(self, rows, counts, slots):
-        if slots is not None:
-            slots = self._integers("slots", slots, (rows,))
-        elif rows > self.sequences:
-            raise ValueError(f"{rows} rows, but the cache has {self.sequences} sequences")
-        if counts is not None:
-            counts = self._integers("counts", counts, (rows,))
-        return counts, slots
-
-    @staticmethod
-    def _at(t):
-        return None if t is None else t.data_ptr()
+        self._caller = self._call.cache_caller(self._cache.value, self.device.index, sequences, kv_heads, head_dim, DTYPES[dtype])
 
     # -- pages -----------------------------------------------------------------------------------
 
     def fork(self, sources):
         """Every sequence ``s`` becomes what ``sources[s]`` was before the call, sharing its pages (``s`` itself: unchanged, -1: empty)."""
-        sources = self._integers("sources", sources, (self.sequences,))
-        _cabi.check(self._lib.kb200_cache_fork(self._cache, sources.data_ptr(), self._stream()), self._lib)
+        self._call.cache_fork(self._caller, sources)
 
     def reserve(self, counts):
         """Pages of its own for the ``counts[s]`` tokens behind every sequence; all of them or, short of free pages, none."""
-        counts = self._integers("counts", counts, (self.sequences,))
-        _cabi.check(self._lib.kb200_cache_reserve(self._cache, counts.data_ptr(), self._stream()), self._lib)
+        self._call.cache_reserve(self._caller, counts)
 
     def truncate(self, lengths):
         """Keeps the first ``lengths[s]`` tokens of every sequence (0: none, the sequence is free; negative: all as it is)."""
-        lengths = self._integers("lengths", lengths, (self.sequences,))
-        _cabi.check(self._lib.kb200_cache_truncate(self._cache, lengths.data_ptr(), self._stream()), self._lib)
+        self._call.cache_truncate(self._caller, lengths)
 
     def compact(self):
         """Moves the pages in use to the front of the pool."""
-        _cabi.check(self._lib.kb200_cache_compact(self._cache, self._stream()), self._lib)
+        self._call.cache_compact(self._caller)
 
     # -- tokens ----------------------------------------------------------------------------------
 
     def append(self, layer, k, v, counts=None, slots=None):
         """Writes K and V of the first ``counts[b]`` tokens of every row of ``k`` and ``v`` [rows, tokens, kv_heads, head_dim] behind
         the committed tokens of sequence ``slots[b]`` (default: ``b``), in the cache's type."""
-        k, k_rows = self._tokens("k", k, self.kv_heads)
-        v, v_rows = self._tokens("v", v, self.kv_heads)
-        if k.shape != v.shape or k.dtype != v.dtype:
-            raise ValueError(f"k and v must be alike, got {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
-        counts, slots = self._batch(k.shape[0], counts, slots)
-        _cabi.check(self._lib.kb200_cache_append(self._cache, layer, k_rows, v_rows, k.shape[0], k.shape[1], self._at(counts), self._at(slots),
-                                                 self._stream()), self._lib)
+        self._call.cache_append(self._caller, layer, k, v, counts, slots)
 
     def accept(self, counts, kept=None):
         """Commits ``counts[s]`` tokens of those appended behind every sequence: the ones with the ascending indexes ``kept[s, :counts[s]]``,
         or the first ones; the rest is dropped and its pages are free."""
-        counts = self._integers("counts", counts, (self.sequences,))
-        width = 0
-        if kept is not None:
-            if not isinstance(kept, torch.Tensor) or kept.dim() != 2:
-                raise ValueError("kept must be a tensor [sequences, width]")
-            width = kept.shape[1]
-            kept = self._integers("kept", kept, (self.sequences, width))
-        _cabi.check(self._lib.kb200_cache_accept(self._cache, counts.data_ptr(), kept.data_ptr() or 16 if kept is not None else None, width, self._stream()),
-                    self._lib)
+        self._call.cache_accept(self._caller, counts, kept)
 
     def attend(self, layer, q, mask=None, counts=None, slots=None, scale=None, out=None):
         """Attention of the first ``counts[b]`` tokens of every row of ``q`` [rows, tokens, heads, head_dim] over the committed tokens of
         sequence ``slots[b]`` (default: ``b``) and, of the ``counts[b]`` tokens appended behind them, those that ``mask`` ([tokens, tokens]
         or [rows, tokens, tokens], bool; default: itself and those before it) shows.  ``heads`` is a multiple of the cache's; scale defaults to
         ``head_dim ** -0.5``.  Returns ``out``, of the cache's type, with zeros in rows of no token and in rows that see nothing."""
-        q, q_rows = self._tokens("q", q)
-        rows, tokens, heads = q.shape[:3]
-        if heads == 0 or heads % self.kv_heads:
-            raise ValueError(f"{heads} heads are no multiple of the cache's {self.kv_heads}")
-        counts, slots = self._batch(rows, counts, slots)
-        strides = None
-        if mask is not None:
-            if not isinstance(mask, torch.Tensor) or mask.dtype != torch.bool:
-                raise TypeError("mask must be a bool tensor")
-            if mask.device != self.device:
-                raise ValueError(f"mask is on {mask.device}, the cache on {self.device}")
-            if tuple(mask.shape) not in ((tokens, tokens), (rows, tokens, tokens)):
-                raise ValueError(f"mask must be [{tokens}, {tokens}] or [{rows}, {tokens}, {tokens}], got {tuple(mask.shape)}")
-            strides = (C.c_int64 * 3)(*((0,) if mask.dim() == 2 else ()), *mask.stride())
-        if out is None:
-            out = torch.empty((rows, tokens, heads, self.head_dim), dtype=self.dtype, device=self.device)
-        elif not isinstance(out, torch.Tensor) or out.shape != q.shape or out.dtype != self.dtype or out.device != self.device:
-            raise ValueError(f"out must be {tuple(q.shape)} of {self.dtype} on {self.device}")
-        elif out.requires_grad:
-            raise ValueError("out requires a gradient")
-        direct, out_rows = self._tokens("out", out)
-        n_bytes = self._lib.kb200_cache_attend_workspace(self._cache, rows, tokens, heads)
-        workspace = torch.empty(n_bytes, dtype=torch.uint8, device=self.device) if n_bytes else None
-        _cabi.check(self._lib.kb200_cache_attend(self._cache, layer, q_rows, out_rows, rows, tokens, self._at(mask), strides, self._at(counts), self._at(slots),
-                                                 self.head_dim ** -0.5 if scale is None else scale, self._at(workspace), n_bytes, self._stream()), self._lib)
-        if direct.data_ptr() != out.data_ptr():
-            out.copy_(direct)
-        return out
+        return self._call.cache_attend(self._caller, layer, q, mask, counts, slots, scale, out)
 
     # -- the rest --------------------------------------------------------------------------------
 
@@ -212,6 +120,7 @@ class PagedCache:
         _cabi.check(self._lib.kb200_cache_status(self._cache), self._lib)
 
     def close(self):
+        self._caller = None
         if getattr(self, "_cache", None) is not None and self._cache:
             self._lib.kb200_cache_destroy(self._cache)
             self._cache = C.c_void_p()

@@ -556,11 +556,10 @@ def test_c_entry_refuses_short_workspaces():
     q = q.to(BF16)
     lib = _cabi.load()
     n = lib.kb200_cache_attend_workspace(cache._cache, 1, 2, 2)
-    rows = cache._tokens("q", q)[1]
+    rows, out = _cabi.Rows(q.data_ptr(), 1, 2, q.stride()[:3]), torch.empty_like(q)
+    out_rows = _cabi.Rows(out.data_ptr(), 1, 2, out.stride()[:3])
     assert n > 0
     space = torch.empty(n + 16, dtype=torch.uint8, device="cuda")
-    out = torch.empty_like(q)
-    out_rows = cache._tokens("out", out)[1]
     call = lambda at, size, a=rows, b=out_rows: lib.kb200_cache_attend(cache._cache, 0, C.byref(a), C.byref(b), 1, 2, None, None, None, None, 0.125, at, size, None)  # noqa: E731
     assert call(space.data_ptr(), n - 1) == -1 and call(None, n) == -1 and call(space.data_ptr() + 8, n) == -1
     assert call(space.data_ptr(), n) == 0
