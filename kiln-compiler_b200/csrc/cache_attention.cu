@@ -17,7 +17,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "cache_attention_math.cuh"
+#include "cache_attention_common.cuh"
 
 #define KB200_EXPORT extern "C" __attribute__((visibility("default")))
 
@@ -45,29 +45,6 @@ struct Shape {
   static constexpr int kSmem = kStages * G::kBytes + kBeside;
   static constexpr int kRows = Math::kRows * RG;                         // of a row tile
 };
-
-// A wait of 2^31 cycles at most, about a second (a poll may suspend the thread, so a number of polls says little).
-__device__ __forceinline__ bool wait_a_second(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  const long long t0 = clock64();
-  while (true) {
-    for (int i = 0; i < 16; ++i) {
-      uint32_t ok;
-      asm volatile(
-          "{\n\t.reg .pred p;\n\t"
-          "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-          "selp.u32 %0, 1, 0, p;\n\t}"
-          : "=r"(ok)
-          : "r"(bar), "r"(parity)
-          : "memory");
-      if (ok != 0) return true;
-    }
-    if (*abort_flag || clock64() - t0 > (1ll << 31)) return false;
-  }
-}
-
-// A part, by groups of rows: a warp's output registers, not divided by their sums, then its rows' maxima and sums.
-template <typename Math>
-constexpr int kPartOfWarp = Math::kOut * 32 + 2 * Math::kRows;
 
 template <typename Math, int RG>
 __global__ void __launch_bounds__(Shape<Math, RG>::kThreads, 1)
@@ -108,46 +85,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
   };
 
   if (warp == Z::kWarps) {
-    // ---------------- producer ----------------
-    if (any) {
-      const int box = min(TILE, 1 << p.c.page_log2), boxes = TILE / box;       // rows of a box; of a tile
-      const int none = p.c.layers * 2 * p.c.pages;                             // beyond the map: zeros
-      int64_t left = run.hi - run.lo;
-      uint32_t u = 0;
-      int page_base = -1, page_slot = -1, my_page = -1;                        // 32 entries of a sequence's table row, one per lane
-      while (left > 0) {
-        const int first = now.tile * TILE >> p.c.page_log2;
-        const int wanted = first & ~31;
-        if (page_slot != now.it.slot || wanted != page_base) {
-          page_slot = now.it.slot;
-          page_base = wanted;
-          const int k = wanted + lane;
-          my_page = k << p.c.page_log2 < now.it.end ? p.c.table[(int64_t)now.it.slot * p.c.max_pages + k] : -1;
-          if (my_page >= p.c.pages || (my_page < 0 && k << p.c.page_log2 < now.it.end)) {
-            cache_fault(p.c, KB200_CACHE_BAD_INDEX);
-            my_page = -1;
-          }
-        }
-        const int stage = u % Z::kStages;
-        if (!wait(empty + 8 * stage, ((u / Z::kStages) & 1) ^ 1)) break;
-        const uint32_t to = stage0 + stage * G::kBytes, bar = full + 8 * stage;
-        if (lane == 0) mbar_expect_tx(bar, G::kBytes);
-        __syncwarp();
-        // K and V of every box, block by block: as many loads as there are, spread over the lanes
-        const int in_page = now.tile * TILE & ((1 << p.c.page_log2) - 1);
-        for (int i0 = 0; i0 < boxes * G::kBlocks * 2; i0 += 32) {
-          const int i = i0 + lane, which = i & 1, block = (i >> 1) % G::kBlocks, j = (i >> 1) / G::kBlocks;
-          const int page = __shfl_sync(0xffffffffu, my_page, (first + j) & 31);
-          if (i < boxes * G::kBlocks * 2)
-            tma_load_3d(to + which * G::kHalf + block * G::kBlockBytes + j * box * 128, &map, bar, block * (128 / (int)sizeof(T)),
-                        (now.head << p.c.page_log2) + in_page, page < 0 ? none : (p.layer * 2 + which) * p.c.pages + page);
-        }
-        ++u;
-        const bool ends = ++now.tile == now.it.key_tiles;
-        if (ends || !p.whole) --left;
-        if (ends && left > 0) next_item<ROWS, TILE>(p, now);
-      }
-    }
+    if (any) bring_tiles<T, Math::kDim, ROWS, Z::kStages>(map, p, run, stage0, full, empty, wait);
   } else {
     // ---------------- consumers ----------------
     const int row_group = warp % RG, key_group = warp / RG;
@@ -155,17 +93,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
     float* const query = slots + Z::kSlots * Z::kSlotFloats + warp * (Z::kQuery + Z::kWeights);
     auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(32 * Z::kWarps) : "memory"); };
 
-    // rows behind a sequence's drafted tokens
-    if (p.counts != nullptr || p.slots != nullptr) {
-      const int width = p.heads * p.c.head_dim;
-      for (int64_t r = blockIdx.x + (int64_t)warp * gridDim.x; r < (int64_t)p.rows * p.tokens; r += (int64_t)gridDim.x * Z::kWarps) {
-        const int b = (int)(r / p.tokens), i = (int)(r % p.tokens);
-        if ((p.counts == nullptr || i < p.counts[b]) && (p.slots == nullptr || (unsigned)p.slots[b] < (unsigned)p.c.sequences)) continue;
-        for (int x = lane; x < width; x += 32)
-          static_cast<T*>(p.out)[b * p.out_stride[0] + i * p.out_stride[1] + (x / p.c.head_dim) * p.out_stride[2] + x % p.c.head_dim] = T(0.0f);
-      }
-    }
-
+    clear_rows_behind<T>(p, warp, Z::kWarps, lane);
     Math math;
     Place at{nullptr, nullptr, 0, 0, row_group * Math::kRows, 0, warp, lane, row_group, key_group};
 
@@ -255,77 +183,9 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
   __syncthreads();
 }
 
-// Joins the parts of an item.  CTA x sees to the item that ends in the run of CTA x of the first launch and began before it.
-constexpr int kJoinThreads = 128, kJoinAtOnce = 8;      // parts whose loads are in flight together
-
-template <typename Math, int RG>
-__global__ void __launch_bounds__(kJoinThreads) cache_attention_join_kernel(const __grid_constant__ CacheAttnParams p) {
-  using T = typename Math::Type;
-  constexpr int DP = Math::kDim, ROWS = Math::kRows * RG, TILE = Tile<T, DP>::kKeys;
-  __shared__ CacheRunShared found;
-  pdl_wait();
-  pdl_launch_dependents();
-  CacheRun run;
-  if (!find_run<ROWS, TILE, kJoinThreads>(p, blockIdx.x, found, &run)) return;
-  const CacheCursor& at = run.at;
-  if (at.tile == 0 || at.it.key_tiles - at.tile > run.hi - run.lo) return;
-  const int64_t begins = run.lo - at.tile;         // the item's first unit
-  const int first = (int)(((begins + 1) * run.parts - 1) / run.all);       // the run that it is in
-  const int rows_here = min(ROWS, at.it.count * p.group - at.row_tile * ROWS);
-  for (int i = blockIdx.y * kJoinThreads + threadIdx.x; i < rows_here * (DP / 4); i += gridDim.y * kJoinThreads) {
-    const int row = i / (DP / 4), d = i % (DP / 4) * 4;
-    if (d >= p.c.head_dim) continue;
-    const int in_warp = row % Math::kRows;
-    const int at0 = Math::place(in_warp, d), at1 = Math::place(in_warp, d + 1), at2 = Math::place(in_warp, d + 2), at3 = Math::place(in_warp, d + 3);
-    // (a run that the item begins in, but not with, has left it as its second part)
-    const int later = run.all * first / run.parts != begins ? 1 : 0;
-    float top = -CUDART_INF_F, sum = 0.0f;
-    float4 x = make_float4(0, 0, 0, 0);
-    for (int r0 = first; r0 <= (int)blockIdx.x; r0 += kJoinAtOnce) {
-      float m[kJoinAtOnce], l[kJoinAtOnce], next = top;
-      float4 y[kJoinAtOnce];
-#pragma unroll
-      for (int j = 0; j < kJoinAtOnce; ++j) {
-        const int r = min(r0 + j, (int)blockIdx.x);
-        const float* const part = p.partial + (2 * (int64_t)r + (r == first ? later : 0)) * p.partial_floats + row / Math::kRows * kPartOfWarp<Math>;
-        const float2 state = reinterpret_cast<const float2*>(part + Math::kOut * 32)[in_warp];
-        m[j] = state.x;
-        l[j] = state.y;
-        y[j] = make_float4(part[at0], part[at1], part[at2], part[at3]);
-      }
-#pragma unroll
-      for (int j = 0; j < kJoinAtOnce; ++j) {
-        if (r0 + j > (int)blockIdx.x) m[j] = -CUDART_INF_F;
-        next = fmaxf(next, m[j]);
-      }
-      if (next == -CUDART_INF_F) continue;           // nothing seen so far
-      const float a = ex2(top - next);
-      sum *= a, x.x *= a, x.y *= a, x.z *= a, x.w *= a;
-#pragma unroll
-      for (int j = 0; j < kJoinAtOnce; ++j) {
-        if (m[j] == -CUDART_INF_F) continue;
-        const float b = ex2(m[j] - next);
-        sum += l[j] * b, x.x += y[j].x * b, x.y += y[j].y * b, x.z += y[j].z * b, x.w += y[j].w * b;
-      }
-      top = next;
-    }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const CacheRow r = row_of<ROWS>(p, at, row);
-    T* const to = static_cast<T*>(p.out) + at.b * p.out_stride[0] + r.token * p.out_stride[1] + r.head * p.out_stride[2] + d;
-    store2<T>(to, x.x * inv, x.y * inv);
-    store2<T>(to + 2, x.z * inv, x.w * inv);
-  }
-}
-
 // ---- host --------------------------------------------------------------------------------------
 
-struct Variant {
-  void (*kernel)(CUtensorMap, CacheAttnParams);
-  void (*join)(CacheAttnParams);
-  int threads, smem, rows, tile;   // rows and keys of a tile
-  int groups;                      // tiles at work at once
-  int64_t part_floats;
-};
+using Variant = CacheAttnVariant;
 
 template <typename Math, int RG>
 Variant variant() {
@@ -333,6 +193,9 @@ Variant variant() {
   return Variant{cache_attention_kernel<Math, RG>, cache_attention_join_kernel<Math, RG>, Z::kThreads, Z::kSmem,
                  Z::kRows, Z::G::kKeys, Z::kGroups, (int64_t)RG * kPartOfWarp<Math>};
 }
+
+// Rows of an item from which 16-bit caches go to tiles of 128 rows on tcgen05.
+constexpr int kFewRows = 16;
 
 // By the rows of an item, up to 64 to a row tile.
 template <typename T, int DP>
@@ -348,6 +211,7 @@ Variant variant_of(int head_dim, int rows) {
   return head_dim <= 64 ? variant_of<T, 64>(rows) : head_dim <= 128 ? variant_of<T, 128>(rows) : variant_of<T, 256>(rows);
 }
 Variant variant_for(const Cache& c, int rows) {
+  if (c.dtype != KB200_DTYPE_FP32 && c.view.head_dim <= 128 && rows > kFewRows) return cache_attention_tc_variant(c.dtype, c.view.head_dim);
   return c.dtype == KB200_DTYPE_FP32 ? variant_of<float>(c.view.head_dim, rows)
          : c.dtype == KB200_DTYPE_BF16 ? variant_of<__nv_bfloat16>(c.view.head_dim, rows) : variant_of<__half>(c.view.head_dim, rows);
 }

@@ -1,0 +1,383 @@
+// Attention of drafted tokens over a paged K/V cache with many query rows to a key head (wide trees, pieces of a prompt, many heads per key head):
+// 128-row tiles on tcgen05, 16-bit caches with heads up to 128.  Work, ring and parts as in cache_attention.cu.
+//
+// What bounds it: the cache's bytes up to about 128 rows (a tile of 64 keys of 128 is 32 KB, 1365 cycles of an SM's share of the memory; its products are 512
+// cycles of the tensor core, its exponentials 512 of the special-function unit), beyond that the exponentials.
+//
+// 192 threads: warp 0 brings tiles, warp 1 issues the products, warps 2..5 have a query row to a thread (tensor-memory lane = row of the tile).  256 columns of
+// tensor memory: the output rows, and scores of two tiles, so that a tile's Q K^T runs under the exponentials of the one before.  A tile's weights
+// (two to a column) are written over its scores, which are in registers by then: the tensor core runs in order, so the scores of the tile after the next
+// one, which go there, come behind the product that reads the weights.  Output rows stay in tensor memory over an item and are rescaled
+// only when a row's maximum has grown.  Q is put into shared memory by the threads that own its rows, from any strides, rounded on the way where it is float32.
+#include <algorithm>
+
+#include "cache_attention_common.cuh"
+
+namespace kb200 {
+namespace {
+
+constexpr int kRows = 128, kThreads = 64 + kRows;
+constexpr uint32_t kColumns = 256, kColS = 128;      // output rows, then two tiles' scores of 64 columns
+
+template <typename T, int DP>
+struct TcShape {
+  using G = Tile<T, DP>;
+  static constexpr int kQBlock = kRows * 128, kQBytes = DP / 64 * kQBlock;
+  static constexpr int kStages = (224 * 1024 - kQBytes) / G::kBytes;
+  static constexpr int kSmem = kQBytes + kStages * G::kBytes;
+};
+
+// Where a part's values are, for the join: a thread's row, column by column.
+template <typename T, int DP>
+struct TcMath {
+  using Type = T;
+  static constexpr int kDim = DP, kRows = kb200::kRows, kOut = DP * kb200::kRows / 32;
+  static __device__ __forceinline__ int place(int row, int d) { return d * kb200::kRows + row; }
+};
+
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+
+// V of a drafted token holds infinities or NaN: they are zero in the product, and this adds them to the output row of a thread that gives the token weight w.
+template <typename T, int DP>
+__device__ __noinline__ void add_infinite(const CacheAttnParams& p, const CacheItems& it, int head, int at, float w, uint32_t out_addr) {
+  const int page = p.c.table[(int64_t)it.slot * p.c.max_pages + (at >> p.c.page_log2)];
+  if (!cache_page_ok(p.c, page)) return;
+  const T* const v = static_cast<const T*>(p.c.pool) + (cache_row(p.c, p.layer, 1, page, head) + (at & ((1 << p.c.page_log2) - 1))) * p.c.head_dim;
+  for (int c = 0; c < DP; c += 32) {
+    float o[32];
+    tmem_ld32(out_addr + c, o);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const float x = c + j < p.c.head_dim ? to_float(v[c + j]) : 0.0f;
+      if (!(fabsf(x) < CUDART_INF_F) && w != 0.0f) o[j] += w * x;
+    }
+    tmem_st32(out_addr + c, o);
+    tmem_st_wait();
+  }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1)
+cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CacheAttnParams p) {
+  using Z = TcShape<T, DP>;
+  using G = Tile<T, DP>;
+  constexpr int TILE = G::kKeys;
+  static_assert(TILE == 64, "64 columns of scores");
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ __align__(8) uint64_t bars[2 * Z::kStages + 7];
+  __shared__ CacheRunShared found;
+  __shared__ unsigned long long odd_keys;            // keys of a tile whose V is not finite
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+
+  const int lane = threadIdx.x & 31, warp = warp_index();
+  const uint32_t q_smem = smem_u32(smem), stage0 = q_smem + Z::kQBytes;
+  const uint32_t full = smem_u32(bars), empty = full + 8 * Z::kStages, q_full = empty + 8 * Z::kStages, s_full = q_full + 8, p_full = s_full + 16, o_full = p_full + 16;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    odd_keys = 0ull;
+    prefetch_tensormap(&map);
+    for (int i = 0; i < 2 * Z::kStages; ++i) mbar_init(full + 8 * i, 1);
+    mbar_init(q_full, kRows / 32);
+    for (int i = 0; i < 2; ++i) mbar_init(s_full + 8 * i, 1), mbar_init(p_full + 8 * i, kRows / 32), mbar_init(o_full + 8 * i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(kColumns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = tmem_slot;
+  pdl_wait();
+  pdl_launch_dependents();
+  CacheRun run;
+  const bool any = find_run<kRows, TILE, kThreads>(p, blockIdx.x, found, &run);
+  CacheCursor& now = run.at;
+  volatile int* const abort_ptr = &abort_flag;
+  // A wait that ends for all lanes of a warp or none.  Where it runs out the softmax warps do no more work, but meet each other as if they did.
+  auto wait = [&](uint32_t bar, uint32_t parity) {
+    const bool got = wait_a_second(bar, parity, abort_ptr);
+    if (!got) *abort_ptr = 1;
+    return __all_sync(0xffffffffu, got ? 1 : 0) != 0;
+  };
+
+  if (warp == 0) {
+    if (any) bring_tiles<T, DP, kRows, Z::kStages>(map, p, run, stage0, full, empty, wait);
+  } else if (warp == 1) {
+    // ---------------- products ----------------
+    // Tiles are numbered over all items; scores, weights and the output's barrier take turns of two.
+    constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u;
+    const uint32_t idesc_qk = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(TILE >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+    const uint32_t idesc_pv = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+    uint32_t items = 0;
+    auto issue_qk = [&](uint32_t t, bool first) {
+      const uint32_t stage = t % Z::kStages;
+      if (first && !wait(q_full, items++ & 1)) return false;
+      if (!wait(full + 8 * stage, (t / Z::kStages) & 1)) return false;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t k = stage0 + stage * G::kBytes, on = elect_one() ? 1u : 0u;
+#pragma unroll
+      for (int kd = 0; kd < DP / 16; ++kd)
+        umma_if(on, tmem + kColS + (t & 1) * TILE, make_desc(q_smem + kd / 4 * Z::kQBlock + kd % 4 * 32, 16, 1024),
+                make_desc(k + kd / 4 * G::kBlockBytes + kd % 4 * 32, 16, 1024), idesc_qk, kd != 0 ? 1u : 0u, true);
+      if (on) umma_commit(s_full + 8 * (t & 1));
+      __syncwarp();
+      return true;
+    };
+    auto issue_pv = [&](uint32_t t, bool first) {
+      const uint32_t stage = t % Z::kStages;
+      if (!wait(p_full + 8 * (t & 1), (t >> 1) & 1)) return false;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t v = stage0 + stage * G::kBytes + G::kHalf, on = elect_one() ? 1u : 0u;
+      // 16 keys = 8 columns of weights and 16 128-byte rows of V per instruction
+#pragma unroll
+      for (int kk = 0; kk < TILE / 16; ++kk)
+        umma_ts_if(on, tmem, tmem + kColS + (t & 1) * TILE + kk * 8, make_desc(v + kk * 2048, G::kBlockBytes, 1024), idesc_pv, !first || kk != 0 ? 1u : 0u, true);
+      if (on) {
+        umma_commit(o_full + 8 * (t & 1));
+        umma_commit(empty + 8 * stage);
+      }
+      __syncwarp();
+      return true;
+    };
+    int64_t left = any ? run.hi - run.lo : 0;
+    uint32_t t = 0;
+    bool ok = true;
+    while (left > 0 && ok) {
+      const int tiles = p.whole ? now.it.key_tiles : (int)min(left, (int64_t)now.it.key_tiles - now.tile);
+      ok = issue_qk(t, true);
+      for (int i = 0; i < tiles && ok; ++i, ++t) {
+        if (i + 1 < tiles) ok = issue_qk(t + 1, false);
+        ok = ok && issue_pv(t, i == 0);
+      }
+      left -= p.whole ? 1 : tiles;
+      if (left > 0) next_item<kRows, TILE>(p, now);
+    }
+  } else {
+    // ---------------- softmax: a thread per query row ----------------
+    clear_rows_behind<T>(p, warp - 2, kRows / 32, lane);
+    const int quad = warp & 3, row = quad * 32 + lane, worker = threadIdx.x - 64;
+    const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16);
+    auto arrive = [&](uint32_t bar) {                // after this warp's last tensor-memory access that the barrier speaks of
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(kRows) : "memory"); };
+    int64_t left = any ? run.hi - run.lo : 0;
+    uint32_t t = 0;
+    while (left > 0) {
+      const int tiles = p.whole ? now.it.key_tiles : (int)min(left, (int64_t)now.it.key_tiles - now.tile);
+      const int rows_here = min(kRows, now.it.count * p.group - now.row_tile * kRows), sure = min(now.it.length, now.it.end);
+      const bool there = row < rows_here, warp_there = quad * 32 < rows_here;
+      const CacheRow r = row_of<kRows>(p, now, there ? row : 0);
+      // the row of Q (the products that read the last item's have been executed: its output was read); zeros for rows that are not there
+      if (warp_there) {
+        const int64_t from = now.b * p.q_stride[0] + r.token * p.q_stride[1] + r.head * p.q_stride[2];
+#pragma unroll 4
+        for (int c = 0; c < DP / 8; ++c) {
+          uint4 x = make_uint4(0u, 0u, 0u, 0u);
+          if (there && c * 8 < p.c.head_dim) {
+            if (p.q_fp32) {
+              const float4* const q = reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + from) + c * 2;
+              const float4 a = q[0], b = q[1];
+              x = make_uint4(pack<T>(a.x, a.y), pack<T>(a.z, a.w), pack<T>(b.x, b.y), pack<T>(b.z, b.w));
+            } else {
+              x = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + from)[c];
+            }
+          }
+          *reinterpret_cast<uint4*>(smem + c / 8 * Z::kQBlock + row * 128 + (((c % 8) ^ (row & 7)) << 4)) = x;
+        }
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+      // what the row sees of up to 64 drafted tokens, under the way of the first keys
+      unsigned long long tree = 0ull;
+      const uint8_t* const mask = p.mask + now.b * p.mask_stride[0] + r.token * p.mask_stride[1];
+      if (p.mask != nullptr && p.tokens <= kMaskAhead && there && (now.tile + tiles) * TILE > sure) {
+#pragma unroll 8
+        for (int j = 0; j < now.it.count; ++j) tree |= mask[j * p.mask_stride[2]] != 0 ? 1ull << j : 0ull;
+      }
+      float m = -CUDART_INF_F, l = 0.0f;
+      for (int i = 0; i < tiles; ++i, ++t) {
+        const int key0 = (now.tile + i) * TILE;
+        const uint32_t scores = lane_addr + kColS + (t & 1) * TILE, stage = t % Z::kStages;
+        bool ok = wait(s_full + 8 * (t & 1), (t >> 1) & 1);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const bool drafted = key0 + TILE > sure, work = ok && warp_there;
+        float v[64];
+        uint32_t packed[32];
+        unsigned long long odd = 0ull;
+        if (drafted) {
+          // V behind the sequence's end becomes zeros, and so do infinities and NaN (see look_at_values), by all rows' threads together.
+          uint8_t* const values = smem + Z::kQBytes + stage * G::kBytes + G::kHalf;
+          constexpr int kChunks = G::kBlocks * 8;
+          const int in_page = (1 << p.c.page_log2) - 1, last = now.it.end - key0;
+          const int from = max(0, sure - key0) * kChunks, to = min(TILE, ((now.it.end + in_page) & ~in_page) - key0) * kChunks;
+          if (worker == 0) odd_keys = 0ull;
+          meet();
+          if (wait(full + 8 * stage, (t / Z::kStages) & 1))
+            for (int c = from + worker; c < to; c += kRows) {
+              uint4* const x = reinterpret_cast<uint4*>(G::at(values, c / kChunks, c % kChunks * 8));
+              if (c / kChunks >= last) *x = make_uint4(0u, 0u, 0u, 0u);
+              else if ((not_finite<T>(x->x) | not_finite<T>(x->y) | not_finite<T>(x->z) | not_finite<T>(x->w)) & 0x80008000u) {
+                atomicOr(&odd_keys, 1ull << (c / kChunks));
+                *x = make_uint4(finite_pair<T>(x->x), finite_pair<T>(x->y), finite_pair<T>(x->z), finite_pair<T>(x->w));
+              }
+            }
+          fence_async_smem();
+          meet();
+          odd = odd_keys;
+          meet();
+        }
+        if (work) {
+          {
+            float a[32], b[32];
+            tmem_ld32x2(scores, scores + 32, a, b);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = a[j], v[32 + j] = b[j];
+          }
+          if (drafted) {
+            const int off = now.it.length - key0, last = now.it.end - key0;      // where the first drafted token is in the tile; where the keys end
+            unsigned long long shows;
+            if (p.mask == nullptr) {
+              const int n = off + r.token + 1;
+              shows = n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
+            } else {
+              if (p.tokens <= kMaskAhead) {
+                shows = off >= 64 || off <= -64 ? 0ull : off >= 0 ? tree << off : tree >> -off;
+              } else {
+                shows = 0ull;
+                const int lo = max(0, off), hi = there ? min(64, off + now.it.count) : 0;
+#pragma unroll 8
+                for (int j = lo; j < hi; ++j) shows |= mask[(j - off) * p.mask_stride[2]] != 0 ? 1ull << j : 0ull;
+              }
+              if (off > 0) shows |= off >= 64 ? ~0ull : (1ull << off) - 1;
+            }
+            if (last < 64) shows &= last <= 0 ? 0ull : (1ull << last) - 1;
+#pragma unroll
+            for (int j = 0; j < 64; ++j)
+              if (!((j < 32 ? (uint32_t)shows : (uint32_t)(shows >> 32)) >> (j & 31) & 1u)) v[j] = -CUDART_INF_F;
+          }
+          float top[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) top[q] = fmaxf(v[2 * q], v[2 * q + 1]);
+#pragma unroll
+          for (int j = 8; j < 64; j += 8)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) top[q] = fmax3(top[q], v[j + 2 * q], v[j + 2 * q + 1]);
+          const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
+          if (i == 0) {
+            m = mx;
+          } else if (__any_sync(0xffffffffu, mx > m)) {
+            const float grown = fmaxf(m, mx), alpha = grown == -CUDART_INF_F ? 1.0f : ex2(m - grown);
+            m = grown;
+            l *= alpha;
+            // the output rows of the tiles so far are there
+            ok = wait(o_full + 8 * ((t - 1) & 1), ((t - 1) >> 1) & 1);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+            for (int c = 0; c < DP; c += 32) {
+              float o[32];
+              tmem_ld32(lane_addr + c, o);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] *= alpha;
+              tmem_st32(lane_addr + c, o);
+            }
+          }
+          const float shift = m == -CUDART_INF_F ? 0.0f : -m;          // nothing seen so far: every weight is 2^-inf
+          const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), shift2 = make_float2(shift, shift);
+          float2 sum2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+          for (int j = 0; j < 64; j += 2) {
+            const float2 e = ffma2(make_float2(v[j], v[j + 1]), scale2, shift2);
+            v[j] = ex2(e.x);
+            v[j + 1] = ex2(e.y);
+            sum2[j >> 1 & 1] = fadd2(sum2[j >> 1 & 1], make_float2(v[j], v[j + 1]));
+            packed[j / 2] = pack<T>(v[j], v[j + 1]);
+          }
+          l += (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
+          tmem_st16(scores, packed);
+          tmem_st16(scores + 16, packed + 16);
+          tmem_st_wait();
+        }
+        arrive(p_full + 8 * (t & 1));
+        if (odd != 0ull && work) {
+          ok = wait(o_full + 8 * (t & 1), (t >> 1) & 1);
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+          for (int j = 0; j < 64; ++j)
+            if (odd >> j & 1) add_infinite<T, DP>(p, now.it, now.head, key0 + j, v[j], lane_addr);
+        }
+      }
+      // ---- the end of the item, or of the run inside it ----
+      const bool ok = wait(o_full + 8 * ((t - 1) & 1), ((t - 1) >> 1) & 1);
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (l != l) m = 0.0f;                          // (NaN, which a maximum passes over, reaches the result)
+      if (ok && warp_there) {
+        const bool whole = now.tile == 0 && tiles == now.it.key_tiles;
+        // a part that begins with the run is the run's first, else its second
+        float* const part = p.partial + (2 * (int64_t)blockIdx.x + (t == (uint32_t)tiles ? 0 : 1)) * p.partial_floats;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        T* const to = static_cast<T*>(p.out) + now.b * p.out_stride[0] + r.token * p.out_stride[1] + r.head * p.out_stride[2];
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 32) {
+          float o[32];
+          tmem_ld32(lane_addr + c, o);
+          if (there && whole) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 8)
+              if (c + j < p.c.head_dim)
+                *reinterpret_cast<uint4*>(to + c + j) = make_uint4(pack<T>(o[j] * inv, o[j + 1] * inv), pack<T>(o[j + 2] * inv, o[j + 3] * inv),
+                                                                   pack<T>(o[j + 4] * inv, o[j + 5] * inv), pack<T>(o[j + 6] * inv, o[j + 7] * inv));
+          } else if (there) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) part[TcMath<T, DP>::place(row, c + j)] = o[j];
+          }
+          __syncwarp();
+        }
+        if (!whole && there) reinterpret_cast<float2*>(part + TcMath<T, DP>::kOut * 32)[row] = make_float2(m, l);
+      }
+      // (the next item's first product writes the output rows behind this thread's next weights)
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      left -= p.whole ? 1 : tiles;
+      if (left > 0) next_item<kRows, TILE>(p, now);
+    }
+  }
+
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (abort_flag && threadIdx.x == 0) {
+    cache_fault(p.c, kCacheWaitFault);
+    let_copies_land();
+  }
+  __syncthreads();
+  if (warp == 2) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns) : "memory");
+  }
+}
+
+template <typename T, int DP>
+CacheAttnVariant tc_variant() {
+  using Z = TcShape<T, DP>;
+  return CacheAttnVariant{cache_attention_tc_kernel<T, DP>, cache_attention_join_kernel<TcMath<T, DP>, 1>, kThreads, Z::kSmem, kRows, Z::G::kKeys, 4,
+                          kPartOfWarp<TcMath<T, DP>>};
+}
+
+}  // namespace
+
+CacheAttnVariant cache_attention_tc_variant(int dtype, int head_dim) {
+  if (dtype == KB200_DTYPE_BF16) return head_dim <= 64 ? tc_variant<__nv_bfloat16, 64>() : tc_variant<__nv_bfloat16, 128>();
+  return head_dim <= 64 ? tc_variant<__half, 64>() : tc_variant<__half, 128>();
+}
+
+}  // namespace kb200

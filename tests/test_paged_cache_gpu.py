@@ -314,6 +314,9 @@ SHAPES = [
     (F32, [1900, 1200, 1, 1777], [2, 1, 2, 3], 32, 1, 64, 32),
     (F16, [1500, 1600, 1700], [9, 9, 3], 16, 3, 128, 64),
     (BF16, [1000, 2000], [40, 33], 16, 1, 64, 16),
+    (F16, [2000, 900, 0, 1900], [20, 33, 17, 1], 8, 4, 128, 16),        # 128 rows and more to a key head
+    (BF16, [700, 64, 3000], [64, 65, 5], 3, 5, 80, 64),
+    (BF16, [0, 1, 130], [130, 100, 17], 2, 2, 48, 8),
 ]
 
 
