@@ -86,6 +86,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
 
   if (warp == Z::kWarps) {
     if (any) bring_tiles<T, Math::kDim, ROWS, Z::kStages>(map, p, run, stage0, full, empty, wait);
+    clear_rows_behind<T>(p);
   } else {
     // ---------------- consumers ----------------
     const int row_group = warp % RG, key_group = warp / RG;
@@ -93,7 +94,6 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
     float* const query = slots + Z::kSlots * Z::kSlotFloats + warp * (Z::kQuery + Z::kWeights);
     auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(32 * Z::kWarps) : "memory"); };
 
-    clear_rows_behind<T>(p, warp, Z::kWarps, lane);
     Math math;
     Place at{nullptr, nullptr, 0, 0, row_group * Math::kRows, 0, warp, lane, row_group, key_group};
 

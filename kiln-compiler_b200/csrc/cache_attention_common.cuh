@@ -74,16 +74,17 @@ __device__ __forceinline__ void bring_tiles(const CUtensorMap& map, const CacheA
   }
 }
 
-// Rows behind a sequence's drafted tokens, and those of no sequence: zeros.  By all CTAs, a warp to a row.
+// Rows behind a sequence's drafted tokens, and those of no sequence: zeros.  By the producer warps, when they have asked for all of their tiles.
 template <typename T>
-__device__ __forceinline__ void clear_rows_behind(const CacheAttnParams& p, int warp, int warps, int lane) {
+__device__ __forceinline__ void clear_rows_behind(const CacheAttnParams& p) {
   if (p.counts == nullptr && p.slots == nullptr) return;
-  const int width = p.heads * p.c.head_dim;
-  for (int64_t r = blockIdx.x + (int64_t)warp * gridDim.x; r < (int64_t)p.rows * p.tokens; r += (int64_t)gridDim.x * warps) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t r = blockIdx.x; r < (int64_t)p.rows * p.tokens; r += gridDim.x) {
     const int b = (int)(r / p.tokens), i = (int)(r % p.tokens);
     if ((p.counts == nullptr || i < p.counts[b]) && (p.slots == nullptr || (unsigned)p.slots[b] < (unsigned)p.c.sequences)) continue;
-    for (int x = lane; x < width; x += 32)
-      static_cast<T*>(p.out)[b * p.out_stride[0] + i * p.out_stride[1] + (x / p.c.head_dim) * p.out_stride[2] + x % p.c.head_dim] = T(0.0f);
+    T* const row = static_cast<T*>(p.out) + b * p.out_stride[0] + i * p.out_stride[1];
+    for (int x = lane; x < p.heads * p.c.row_chunks; x += 32)
+      *reinterpret_cast<uint4*>(row + x / p.c.row_chunks * p.out_stride[2] + x % p.c.row_chunks * (16 / (int)sizeof(T))) = make_uint4(0u, 0u, 0u, 0u);
   }
 }
 
@@ -109,7 +110,8 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attention_join_kernel(cons
   const int first = (int)(((begins + 1) * run.parts - 1) / run.all);       // the run that it is in
   const int rows_here = min(ROWS, at.it.count * p.group - at.row_tile * ROWS);
   for (int i = blockIdx.y * kJoinThreads + threadIdx.x; i < rows_here * (DP / 4); i += gridDim.y * kJoinThreads) {
-    const int row = i / (DP / 4), d = i % (DP / 4) * 4;
+    // (neighbours in a part to neighbouring lanes)
+    const int row = Math::kByRows ? i % rows_here : i / (DP / 4), d = (Math::kByRows ? i / rows_here : i % (DP / 4)) * 4;
     if (d >= p.c.head_dim) continue;
     const int in_warp = row % Math::kRows;
     const int at0 = Math::place(in_warp, d), at1 = Math::place(in_warp, d + 1), at2 = Math::place(in_warp, d + 2), at3 = Math::place(in_warp, d + 3);

@@ -163,6 +163,7 @@ __device__ __forceinline__ bool look_at_values(const CacheAttnParams& p, const C
 template <typename T, int DP>
 struct MmaMath {
   using Type = T;
+  static constexpr bool kByRows = false;
   static constexpr int kDim = DP, kRows = 16, kOut = DP / 2;             // rows of a warp; output registers of a thread
   using G = Tile<T, DP>;
   static constexpr int NT = G::kKeys / 8, DT = DP / 8;                   // 8-wide column tiles of the scores, of the output rows
@@ -363,6 +364,7 @@ struct MmaMath {
 template <int DP, int R>
 struct FmaMath {
   using Type = float;
+  static constexpr bool kByRows = false;
   static constexpr int kDim = DP, kRows = R, kOut = R * DP / 32;
   using G = Tile<float, DP>;
   static constexpr int KEYS = G::kKeys >= 32 ? G::kKeys / 32 : 1;        // of a lane

@@ -4,8 +4,10 @@
 // What bounds it: the cache's bytes up to about 128 rows (a tile of 64 keys of 128 is 32 KB, 1365 cycles of an SM's share of the memory; its products are 512
 // cycles of the tensor core, its exponentials 512 of the special-function unit), beyond that the exponentials.
 //
-// 192 threads: warp 0 brings tiles, warp 1 issues the products, warps 2..5 have a query row to a thread (tensor-memory lane = row of the tile).  256 columns of
-// tensor memory: the output rows, and scores of two tiles, so that a tile's Q K^T runs under the exponentials of the one before.  A tile's weights
+// 320 threads: warp 0 brings tiles, warp 1 issues the products, and two groups of four warps take turns at the tiles, a query row to a thread of each
+// (tensor-memory lane = row of the tile): from a tile's scores to its weights a warp needs ~1500 cycles, of which the exponentials are 512, so that one group
+// alone holds the memory up (304 us for 32 sequences of up to 16384 tokens and 32 drafted ones).  Each group has maxima, sums and output rows of its own,
+// joined at the end of an item.  384 columns of tensor memory: two sets of output rows, and scores of two tiles.  A tile's weights
 // (two to a column) are written over its scores, which are in registers by then: the tensor core runs in order, so the scores of the tile after the next
 // one, which go there, come behind the product that reads the weights.  Output rows stay in tensor memory over an item and are rescaled
 // only when a row's maximum has grown.  Q is put into shared memory by the threads that own its rows, from any strides, rounded on the way where it is float32.
@@ -16,8 +18,8 @@
 namespace kb200 {
 namespace {
 
-constexpr int kRows = 128, kThreads = 64 + kRows;
-constexpr uint32_t kColumns = 256, kColS = 128;      // output rows, then two tiles' scores of 64 columns
+constexpr int kRows = 128, kThreads = 64 + 2 * kRows;
+constexpr uint32_t kColumns = 512, kColS = 256;      // a group's output rows, the other's, then two tiles' scores of 64 columns
 
 template <typename T, int DP>
 struct TcShape {
@@ -31,6 +33,7 @@ struct TcShape {
 template <typename T, int DP>
 struct TcMath {
   using Type = T;
+  static constexpr bool kByRows = true;
   static constexpr int kDim = DP, kRows = kb200::kRows, kOut = DP * kb200::kRows / 32;
   static __device__ __forceinline__ int place(int row, int d) { return d * kb200::kRows + row; }
 };
@@ -71,7 +74,8 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[2 * Z::kStages + 7];
   __shared__ CacheRunShared found;
-  __shared__ unsigned long long odd_keys;            // keys of a tile whose V is not finite
+  __shared__ unsigned long long odd_keys[2];         // keys of a group's tile whose V is not finite
+  __shared__ float2 states[2][kRows];                // the groups' maxima and sums at the end of an item
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
 
@@ -80,10 +84,9 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
   const uint32_t full = smem_u32(bars), empty = full + 8 * Z::kStages, q_full = empty + 8 * Z::kStages, s_full = q_full + 8, p_full = s_full + 16, o_full = p_full + 16;
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    odd_keys = 0ull;
     prefetch_tensormap(&map);
     for (int i = 0; i < 2 * Z::kStages; ++i) mbar_init(full + 8 * i, 1);
-    mbar_init(q_full, kRows / 32);
+    mbar_init(q_full, 2 * kRows / 32);
     for (int i = 0; i < 2; ++i) mbar_init(s_full + 8 * i, 1), mbar_init(p_full + 8 * i, kRows / 32), mbar_init(o_full + 8 * i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -110,6 +113,7 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
 
   if (warp == 0) {
     if (any) bring_tiles<T, DP, kRows, Z::kStages>(map, p, run, stage0, full, empty, wait);
+    clear_rows_behind<T>(p);
   } else if (warp == 1) {
     // ---------------- products ----------------
     // Tiles are numbered over all items; scores, weights and the output's barrier take turns of two.
@@ -139,7 +143,7 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
       // 16 keys = 8 columns of weights and 16 128-byte rows of V per instruction
 #pragma unroll
       for (int kk = 0; kk < TILE / 16; ++kk)
-        umma_ts_if(on, tmem, tmem + kColS + (t & 1) * TILE + kk * 8, make_desc(v + kk * 2048, G::kBlockBytes, 1024), idesc_pv, !first || kk != 0 ? 1u : 0u, true);
+        umma_ts_if(on, tmem + (t & 1) * DP, tmem + kColS + (t & 1) * TILE + kk * 8, make_desc(v + kk * 2048, G::kBlockBytes, 1024), idesc_pv, !first || kk != 0 ? 1u : 0u, true);
       if (on) {
         umma_commit(o_full + 8 * (t & 1));
         umma_commit(empty + 8 * stage);
@@ -155,34 +159,34 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
       ok = issue_qk(t, true);
       for (int i = 0; i < tiles && ok; ++i, ++t) {
         if (i + 1 < tiles) ok = issue_qk(t + 1, false);
-        ok = ok && issue_pv(t, i == 0);
+        ok = ok && issue_pv(t, i < 2);
       }
       left -= p.whole ? 1 : tiles;
       if (left > 0) next_item<kRows, TILE>(p, now);
     }
   } else {
-    // ---------------- softmax: a thread per query row ----------------
-    clear_rows_behind<T>(p, warp - 2, kRows / 32, lane);
-    const int quad = warp & 3, row = quad * 32 + lane, worker = threadIdx.x - 64;
-    const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16);
+    // ---------------- softmax: a thread per query row and group ----------------
+    const int group = (warp - 2) >> 2, quad = warp & 3, row = quad * 32 + lane, worker = (threadIdx.x - 64) & (kRows - 1);
+    const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16), out_addr = lane_addr + group * DP, scores = lane_addr + kColS + group * TILE;
     auto arrive = [&](uint32_t bar) {                // after this warp's last tensor-memory access that the barrier speaks of
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
-    auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(kRows) : "memory"); };
+    auto meet_group = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(kRows) : "memory"); };
+    auto meet_both = [&]() { asm volatile("bar.sync 3, %0;" ::"n"(2 * kRows) : "memory"); };
     int64_t left = any ? run.hi - run.lo : 0;
-    uint32_t t = 0;
+    uint32_t t0 = 0;                                 // the item's first tile
     while (left > 0) {
       const int tiles = p.whole ? now.it.key_tiles : (int)min(left, (int64_t)now.it.key_tiles - now.tile);
       const int rows_here = min(kRows, now.it.count * p.group - now.row_tile * kRows), sure = min(now.it.length, now.it.end);
       const bool there = row < rows_here, warp_there = quad * 32 < rows_here;
       const CacheRow r = row_of<kRows>(p, now, there ? row : 0);
-      // the row of Q (the products that read the last item's have been executed: its output was read); zeros for rows that are not there
+      // half a row of Q (the products that read the last item's have been executed: its output was read); zeros for rows that are not there
       if (warp_there) {
         const int64_t from = now.b * p.q_stride[0] + r.token * p.q_stride[1] + r.head * p.q_stride[2];
 #pragma unroll 4
-        for (int c = 0; c < DP / 8; ++c) {
+        for (int c = group * (DP / 16); c < (group + 1) * (DP / 16); ++c) {
           uint4 x = make_uint4(0u, 0u, 0u, 0u);
           if (there && c * 8 < p.c.head_dim) {
             if (p.q_fp32) {
@@ -207,37 +211,37 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
         for (int j = 0; j < now.it.count; ++j) tree |= mask[j * p.mask_stride[2]] != 0 ? 1ull << j : 0ull;
       }
       float m = -CUDART_INF_F, l = 0.0f;
-      for (int i = 0; i < tiles; ++i, ++t) {
+      uint32_t done = 0;                             // the group's last tile, plus one
+      for (int i = (int)((group + t0) & 1); i < tiles; i += 2) {
+        const uint32_t t = t0 + i, stage = t % Z::kStages;
         const int key0 = (now.tile + i) * TILE;
-        const uint32_t scores = lane_addr + kColS + (t & 1) * TILE, stage = t % Z::kStages;
-        bool ok = wait(s_full + 8 * (t & 1), (t >> 1) & 1);
+        const bool ok = wait(s_full + 8 * group, (t >> 1) & 1);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const bool drafted = key0 + TILE > sure, work = ok && warp_there;
-        float v[64];
-        uint32_t packed[32];
         unsigned long long odd = 0ull;
         if (drafted) {
-          // V behind the sequence's end becomes zeros, and so do infinities and NaN (see look_at_values), by all rows' threads together.
+          // V behind the sequence's end becomes zeros, and so do infinities and NaN (see look_at_values), by all rows' threads of the group together.
           uint8_t* const values = smem + Z::kQBytes + stage * G::kBytes + G::kHalf;
           constexpr int kChunks = G::kBlocks * 8;
           const int in_page = (1 << p.c.page_log2) - 1, last = now.it.end - key0;
           const int from = max(0, sure - key0) * kChunks, to = min(TILE, ((now.it.end + in_page) & ~in_page) - key0) * kChunks;
-          if (worker == 0) odd_keys = 0ull;
-          meet();
+          if (worker == 0) odd_keys[group] = 0ull;
+          meet_group();
           if (wait(full + 8 * stage, (t / Z::kStages) & 1))
             for (int c = from + worker; c < to; c += kRows) {
               uint4* const x = reinterpret_cast<uint4*>(G::at(values, c / kChunks, c % kChunks * 8));
               if (c / kChunks >= last) *x = make_uint4(0u, 0u, 0u, 0u);
               else if ((not_finite<T>(x->x) | not_finite<T>(x->y) | not_finite<T>(x->z) | not_finite<T>(x->w)) & 0x80008000u) {
-                atomicOr(&odd_keys, 1ull << (c / kChunks));
+                atomicOr(&odd_keys[group], 1ull << (c / kChunks));
                 *x = make_uint4(finite_pair<T>(x->x), finite_pair<T>(x->y), finite_pair<T>(x->z), finite_pair<T>(x->w));
               }
             }
           fence_async_smem();
-          meet();
-          odd = odd_keys;
-          meet();
+          meet_group();
+          odd = odd_keys[group];
+          meet_group();
         }
+        float v[64];
         if (work) {
           {
             float a[32], b[32];
@@ -275,79 +279,98 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
 #pragma unroll
             for (int q = 0; q < 4; ++q) top[q] = fmax3(top[q], v[j + 2 * q], v[j + 2 * q + 1]);
           const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
-          if (i == 0) {
+          if (done == 0) {
             m = mx;
           } else if (__any_sync(0xffffffffu, mx > m)) {
             const float grown = fmaxf(m, mx), alpha = grown == -CUDART_INF_F ? 1.0f : ex2(m - grown);
             m = grown;
             l *= alpha;
-            // the output rows of the tiles so far are there
-            ok = wait(o_full + 8 * ((t - 1) & 1), ((t - 1) >> 1) & 1);
+            wait(o_full + 8 * group, ((t - 2) >> 1) & 1);      // the output rows of the group's tiles so far are there
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
             for (int c = 0; c < DP; c += 32) {
               float o[32];
-              tmem_ld32(lane_addr + c, o);
+              tmem_ld32(out_addr + c, o);
 #pragma unroll
               for (int j = 0; j < 32; ++j) o[j] *= alpha;
-              tmem_st32(lane_addr + c, o);
+              tmem_st32(out_addr + c, o);
             }
           }
           const float shift = m == -CUDART_INF_F ? 0.0f : -m;          // nothing seen so far: every weight is 2^-inf
           const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), shift2 = make_float2(shift, shift);
           float2 sum2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-          for (int j = 0; j < 64; j += 2) {
-            const float2 e = ffma2(make_float2(v[j], v[j + 1]), scale2, shift2);
-            v[j] = ex2(e.x);
-            v[j + 1] = ex2(e.y);
-            sum2[j >> 1 & 1] = fadd2(sum2[j >> 1 & 1], make_float2(v[j], v[j + 1]));
-            packed[j / 2] = pack<T>(v[j], v[j + 1]);
+          for (int h = 0; h < 64; h += 32) {
+            uint32_t packed[16];
+#pragma unroll
+            for (int j = h; j < h + 32; j += 2) {
+              const float2 e = ffma2(make_float2(v[j], v[j + 1]), scale2, shift2);
+              v[j] = ex2(e.x);
+              v[j + 1] = ex2(e.y);
+              sum2[j >> 1 & 1] = fadd2(sum2[j >> 1 & 1], make_float2(v[j], v[j + 1]));
+              packed[(j - h) / 2] = pack<T>(v[j], v[j + 1]);
+            }
+            tmem_st16(scores + h / 2, packed);
           }
           l += (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
-          tmem_st16(scores, packed);
-          tmem_st16(scores + 16, packed + 16);
           tmem_st_wait();
         }
-        arrive(p_full + 8 * (t & 1));
+        arrive(p_full + 8 * group);
+        done = t + 1;
         if (odd != 0ull && work) {
-          ok = wait(o_full + 8 * (t & 1), (t >> 1) & 1);
+          wait(o_full + 8 * group, (t >> 1) & 1);
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
           for (int j = 0; j < 64; ++j)
-            if (odd >> j & 1) add_infinite<T, DP>(p, now.it, now.head, key0 + j, v[j], lane_addr);
+            if (odd >> j & 1) add_infinite<T, DP>(p, now.it, now.head, key0 + j, v[j], out_addr);
         }
       }
-      // ---- the end of the item, or of the run inside it ----
-      const bool ok = wait(o_full + 8 * ((t - 1) & 1), ((t - 1) >> 1) & 1);
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      // ---- the end of the item, or of the run inside it: both groups' rows, half of the columns each ----
+      bool ok = true;
+      if (done != 0) ok = wait(o_full + 8 * group, ((done - 1) >> 1) & 1);
       if (l != l) m = 0.0f;                          // (NaN, which a maximum passes over, reaches the result)
+      states[group][row] = make_float2(m, l);
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      meet_both();
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (ok && warp_there) {
         const bool whole = now.tile == 0 && tiles == now.it.key_tiles;
+        const float2 a = states[0][row], b = states[1][row];
+        const float top = fmaxf(a.x, b.x);
+        float fa = a.x == -CUDART_INF_F ? 0.0f : ex2(a.x - top), fb = b.x == -CUDART_INF_F ? 0.0f : ex2(b.x - top);
+        const float sum = a.y * fa + b.y * fb;
+        if (whole) {
+          const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+          fa *= inv, fb *= inv;
+        }
+        const bool first = t0 % 2 == 0 || tiles > 1, second = t0 % 2 == 1 || tiles > 1;       // which groups had a tile
         // a part that begins with the run is the run's first, else its second
-        float* const part = p.partial + (2 * (int64_t)blockIdx.x + (t == (uint32_t)tiles ? 0 : 1)) * p.partial_floats;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        float* const part = p.partial + (2 * (int64_t)blockIdx.x + (t0 == 0 ? 0 : 1)) * p.partial_floats;
         T* const to = static_cast<T*>(p.out) + now.b * p.out_stride[0] + r.token * p.out_stride[1] + r.head * p.out_stride[2];
 #pragma unroll 1
-        for (int c = 0; c < DP; c += 32) {
-          float o[32];
-          tmem_ld32(lane_addr + c, o);
+        for (int c = group * (DP / 2); c < (group + 1) * (DP / 2); c += 32) {
+          float o[32], o2[32];
+          tmem_ld32x2(lane_addr + c, lane_addr + DP + c, o, o2);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = (first ? o[j] * fa : 0.0f) + (second ? o2[j] * fb : 0.0f);
           if (there && whole) {
 #pragma unroll
             for (int j = 0; j < 32; j += 8)
               if (c + j < p.c.head_dim)
-                *reinterpret_cast<uint4*>(to + c + j) = make_uint4(pack<T>(o[j] * inv, o[j + 1] * inv), pack<T>(o[j + 2] * inv, o[j + 3] * inv),
-                                                                   pack<T>(o[j + 4] * inv, o[j + 5] * inv), pack<T>(o[j + 6] * inv, o[j + 7] * inv));
+                *reinterpret_cast<uint4*>(to + c + j) = make_uint4(pack<T>(o[j], o[j + 1]), pack<T>(o[j + 2], o[j + 3]), pack<T>(o[j + 4], o[j + 5]),
+                                                                   pack<T>(o[j + 6], o[j + 7]));
           } else if (there) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) part[TcMath<T, DP>::place(row, c + j)] = o[j];
           }
           __syncwarp();
         }
-        if (!whole && there) reinterpret_cast<float2*>(part + TcMath<T, DP>::kOut * 32)[row] = make_float2(m, l);
+        if (!whole && there && group == 0) reinterpret_cast<float2*>(part + TcMath<T, DP>::kOut * 32)[row] = make_float2(top, sum);
       }
-      // (the next item's first product writes the output rows behind this thread's next weights)
+      // the next item's products write the output rows behind both groups' next weights
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      meet_both();
+      t0 += tiles;
       left -= p.whole ? 1 : tiles;
       if (left > 0) next_item<kRows, TILE>(p, now);
     }
