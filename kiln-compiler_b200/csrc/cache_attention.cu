@@ -85,6 +85,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
   };
 
   if (warp == Z::kWarps) {
+    if (lane == 0) leave_join<ROWS>(p, any, run);
     if (any) bring_tiles<T, Math::kDim, ROWS, Z::kStages>(map, p, run, stage0, full, empty, wait);
     clear_rows_behind<T>(p);
   } else {
@@ -231,7 +232,9 @@ Division division_of(const Cache& c, const Variant& v, int rows, int tokens, int
   d.parts = (int)std::min<double>(std::ceil(units / d.min_units), (double)c.sm_count);
   return d;
 }
-uint64_t workspace_of(const Variant& v, const Division& d) { return d.whole ? 0 : (uint64_t)d.parts * 2 * v.part_floats * sizeof(float); }
+uint64_t workspace_of(const Variant& v, const Division& d) {
+  return d.whole ? 0 : (uint64_t)d.parts * (2 * v.part_floats * sizeof(float) + sizeof(CacheJoin));
+}
 
 Cache* cache_of(const kb200_cache* c) { return reinterpret_cast<Cache*>(const_cast<kb200_cache*>(c)); }
 
@@ -310,7 +313,8 @@ KB200_EXPORT int kb200_cache_attend(kb200_cache* handle, int layer, const kb200_
   p.mask = mask;
   p.counts = counts;
   p.slots = slots;
-  p.partial = static_cast<float*>(workspace);
+  p.joins = d.whole ? nullptr : static_cast<CacheJoin*>(workspace);
+  p.partial = reinterpret_cast<float*>(static_cast<CacheJoin*>(workspace) + d.parts);
   p.partial_floats = v.part_floats;
   p.layer = layer;
   p.rows = rows;

@@ -13,7 +13,8 @@ struct CacheAttnParams {
   const uint8_t* mask;                     // null: token t is seen by t and those behind it
   int64_t mask_stride[3];
   const int32_t *counts, *slots;
-  float* partial;                          // see below
+  struct CacheJoin* joins;                 // see below, as are these
+  float* partial;
   int64_t partial_floats;                  // of one part
   int layer, rows, tokens, heads, group;
   int parts;                               // CTAs that share the work at most
@@ -29,6 +30,13 @@ struct CacheAttnParams {
 // row tile of a head of a sequence) leaves its part of the softmax in the workspace, at most two parts per CTA; the
 // second launch joins them in the order of the keys.  Where no sequence can have more tiles than a CTA works on at once the units are whole items, and there is
 // nothing to join.
+
+// What CTA x leaves for CTA x of the second launch: the item that ends in its run and began before it.
+struct CacheJoin {
+  int b, head, row_tile, rows;             // rows 0: there is none
+  int first, later;                        // the run that the item begins in; 1: but not with, so that its part is that run's second
+  int pad[2];
+};
 
 struct CacheItems {                        // of one batch row
   int slot, length, count;                 // committed and drafted tokens
@@ -150,15 +158,33 @@ __device__ __forceinline__ bool find_run(const CacheAttnParams& p, int part, Cac
   return true;
 }
 
+// By one thread of every CTA of the first launch.
+template <int ROWS>
+__device__ __forceinline__ void leave_join(const CacheAttnParams& p, bool any, const CacheRun& run) {
+  if (p.joins == nullptr) return;
+  CacheJoin j{};
+  const CacheCursor& at = run.at;
+  if (any && at.tile != 0 && at.it.key_tiles - at.tile <= run.hi - run.lo) {
+    const int64_t begins = run.lo - at.tile;               // the item's first unit
+    j.b = at.b, j.head = at.head, j.row_tile = at.row_tile;
+    j.rows = min(ROWS, at.it.count * p.group - at.row_tile * ROWS);
+    j.first = (int)(((begins + 1) * run.parts - 1) / run.all);
+    j.later = run.all * j.first / run.parts != begins ? 1 : 0;
+  }
+  p.joins[blockIdx.x] = j;
+}
+
 // An item's row: the token and, of the heads that share its key head, the one.
 struct CacheRow {
   int token, head;
 };
 template <int ROWS>
-__device__ __forceinline__ CacheRow row_of(const CacheAttnParams& p, const CacheCursor& at, int row) {
-  const int r = at.row_tile * ROWS + row, token = r / p.group;
-  return CacheRow{token, at.head * p.group + r - token * p.group};
+__device__ __forceinline__ CacheRow row_of(const CacheAttnParams& p, int row_tile, int head, int row) {
+  const int r = row_tile * ROWS + row, token = r / p.group;
+  return CacheRow{token, head * p.group + r - token * p.group};
 }
+template <int ROWS>
+__device__ __forceinline__ CacheRow row_of(const CacheAttnParams& p, const CacheCursor& at, int row) { return row_of<ROWS>(p, at.row_tile, at.head, row); }
 #endif
 
 }  // namespace kb200

@@ -92,40 +92,32 @@ __device__ __forceinline__ void clear_rows_behind(const CacheAttnParams& p) {
 template <typename Math>
 constexpr int kPartOfWarp = Math::kOut * 32 + 2 * Math::kRows;
 
-// Joins the parts of an item.  CTA x sees to the item that ends in the run of CTA x of the first launch and began before it.
+// Joins the parts of the item that CTA x of the first launch has left (CacheJoin).
 constexpr int kJoinThreads = 128, kJoinAtOnce = 8;      // parts whose loads are in flight together
 
 template <typename Math, int RG>
 __global__ void __launch_bounds__(kJoinThreads) cache_attention_join_kernel(const __grid_constant__ CacheAttnParams p) {
   using T = typename Math::Type;
-  constexpr int DP = Math::kDim, ROWS = Math::kRows * RG, TILE = Tile<T, DP>::kKeys;
-  __shared__ CacheRunShared found;
+  constexpr int DP = Math::kDim, ROWS = Math::kRows * RG;
   pdl_wait();
   pdl_launch_dependents();
-  CacheRun run;
-  if (!find_run<ROWS, TILE, kJoinThreads>(p, blockIdx.x, found, &run)) return;
-  const CacheCursor& at = run.at;
-  if (at.tile == 0 || at.it.key_tiles - at.tile > run.hi - run.lo) return;
-  const int64_t begins = run.lo - at.tile;         // the item's first unit
-  const int first = (int)(((begins + 1) * run.parts - 1) / run.all);       // the run that it is in
-  const int rows_here = min(ROWS, at.it.count * p.group - at.row_tile * ROWS);
+  const CacheJoin at = p.joins[blockIdx.x];
+  const int rows_here = at.rows;
   for (int i = blockIdx.y * kJoinThreads + threadIdx.x; i < rows_here * (DP / 4); i += gridDim.y * kJoinThreads) {
     // (neighbours in a part to neighbouring lanes)
     const int row = Math::kByRows ? i % rows_here : i / (DP / 4), d = (Math::kByRows ? i / rows_here : i % (DP / 4)) * 4;
     if (d >= p.c.head_dim) continue;
     const int in_warp = row % Math::kRows;
     const int at0 = Math::place(in_warp, d), at1 = Math::place(in_warp, d + 1), at2 = Math::place(in_warp, d + 2), at3 = Math::place(in_warp, d + 3);
-    // (a run that the item begins in, but not with, has left it as its second part)
-    const int later = run.all * first / run.parts != begins ? 1 : 0;
     float top = -CUDART_INF_F, sum = 0.0f;
     float4 x = make_float4(0, 0, 0, 0);
-    for (int r0 = first; r0 <= (int)blockIdx.x; r0 += kJoinAtOnce) {
+    for (int r0 = at.first; r0 <= (int)blockIdx.x; r0 += kJoinAtOnce) {
       float m[kJoinAtOnce], l[kJoinAtOnce], next = top;
       float4 y[kJoinAtOnce];
 #pragma unroll
       for (int j = 0; j < kJoinAtOnce; ++j) {
         const int r = min(r0 + j, (int)blockIdx.x);
-        const float* const part = p.partial + (2 * (int64_t)r + (r == first ? later : 0)) * p.partial_floats + row / Math::kRows * kPartOfWarp<Math>;
+        const float* const part = p.partial + (2 * (int64_t)r + (r == at.first ? at.later : 0)) * p.partial_floats + row / Math::kRows * kPartOfWarp<Math>;
         const float2 state = reinterpret_cast<const float2*>(part + Math::kOut * 32)[in_warp];
         m[j] = state.x;
         l[j] = state.y;
@@ -148,7 +140,7 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attention_join_kernel(cons
       top = next;
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const CacheRow r = row_of<ROWS>(p, at, row);
+    const CacheRow r = row_of<ROWS>(p, at.row_tile, at.head, row);
     T* const to = static_cast<T*>(p.out) + at.b * p.out_stride[0] + r.token * p.out_stride[1] + r.head * p.out_stride[2] + d;
     store2<T>(to, x.x * inv, x.y * inv);
     store2<T>(to + 2, x.z * inv, x.w * inv);

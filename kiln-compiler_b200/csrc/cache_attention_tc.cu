@@ -45,6 +45,21 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
       : "memory");
 }
 
+// Two 8-column loads in flight at once.
+__device__ __forceinline__ void tmem_ld8x2(uint32_t addr_a, uint32_t addr_b, float (&va)[8], float (&vb)[8]) {
+  uint32_t a[8], b[8];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%16];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%17];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]), "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3]), "=r"(b[4]),
+        "=r"(b[5]), "=r"(b[6]), "=r"(b[7])
+      : "r"(addr_a), "r"(addr_b)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) va[i] = __uint_as_float(a[i]), vb[i] = __uint_as_float(b[i]);
+}
+
 // V of a drafted token holds infinities or NaN: they are zero in the product, and this adds them to the output row of a thread that gives the token weight w.
 template <typename T, int DP>
 __device__ __noinline__ void add_infinite(const CacheAttnParams& p, const CacheItems& it, int head, int at, float w, uint32_t out_addr) {
@@ -112,6 +127,7 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
   };
 
   if (warp == 0) {
+    if (lane == 0) leave_join<kRows>(p, any, run);
     if (any) bring_tiles<T, DP, kRows, Z::kStages>(map, p, run, stage0, full, empty, wait);
     clear_rows_behind<T>(p);
   } else if (warp == 1) {
@@ -203,12 +219,22 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
-      // what the row sees of up to 64 drafted tokens, under the way of the first keys
+      // what the row sees of up to 64 drafted tokens, under the way of the first keys: a ballot per token and 32 of them
       unsigned long long tree = 0ull;
-      const uint8_t* const mask = p.mask + now.b * p.mask_stride[0] + r.token * p.mask_stride[1];
-      if (p.mask != nullptr && p.tokens <= kMaskAhead && there && (now.tile + tiles) * TILE > sure) {
-#pragma unroll 8
-        for (int j = 0; j < now.it.count; ++j) tree |= mask[j * p.mask_stride[2]] != 0 ? 1ull << j : 0ull;
+      const uint8_t* const mask = p.mask + now.b * p.mask_stride[0];
+      if (p.mask != nullptr && p.tokens <= kMaskAhead && (now.tile + tiles) * TILE > sure) {
+        const int first = now.row_tile * kRows / p.group, last = (now.row_tile * kRows + rows_here - 1) / p.group;
+        uint32_t* const words = reinterpret_cast<uint32_t*>(states);       // (free between items)
+#pragma unroll 4
+        for (int w = warp - 2; w < 2 * (last - first + 1); w += 8) {
+          const int j = (w & 1) * 32 + lane;
+          const bool sees = j < now.it.count && mask[(first + w / 2) * p.mask_stride[1] + (j < now.it.count ? j : 0) * p.mask_stride[2]] != 0;
+          const uint32_t word = __ballot_sync(0xffffffffu, sees);
+          if (lane == 0) words[w] = word;
+        }
+        meet_both();
+        if (there) tree = words[2 * (r.token - first)] | (unsigned long long)words[2 * (r.token - first) + 1] << 32;
+        meet_both();
       }
       float m = -CUDART_INF_F, l = 0.0f;
       uint32_t done = 0;                             // the group's last tile, plus one
@@ -262,7 +288,7 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
                 shows = 0ull;
                 const int lo = max(0, off), hi = there ? min(64, off + now.it.count) : 0;
 #pragma unroll 8
-                for (int j = lo; j < hi; ++j) shows |= mask[(j - off) * p.mask_stride[2]] != 0 ? 1ull << j : 0ull;
+                for (int j = lo; j < hi; ++j) shows |= mask[r.token * p.mask_stride[1] + (j - off) * p.mask_stride[2]] != 0 ? 1ull << j : 0ull;
               }
               if (off > 0) shows |= off >= 64 ? ~0ull : (1ull << off) - 1;
             }
@@ -347,21 +373,18 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
         // a part that begins with the run is the run's first, else its second
         float* const part = p.partial + (2 * (int64_t)blockIdx.x + (t0 == 0 ? 0 : 1)) * p.partial_floats;
         T* const to = static_cast<T*>(p.out) + now.b * p.out_stride[0] + r.token * p.out_stride[1] + r.head * p.out_stride[2];
+        // (small code: a launch meets it cold)
 #pragma unroll 1
-        for (int c = group * (DP / 2); c < (group + 1) * (DP / 2); c += 32) {
-          float o[32], o2[32];
-          tmem_ld32x2(lane_addr + c, lane_addr + DP + c, o, o2);
+        for (int c = group * (DP / 2); c < (group + 1) * (DP / 2); c += 8) {
+          float o[8], o2[8];
+          tmem_ld8x2(lane_addr + c, lane_addr + DP + c, o, o2);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = (first ? o[j] * fa : 0.0f) + (second ? o2[j] * fb : 0.0f);
-          if (there && whole) {
+          for (int j = 0; j < 8; ++j) o[j] = (first ? o[j] * fa : 0.0f) + (second ? o2[j] * fb : 0.0f);
+          if (there && whole && c < p.c.head_dim) {
+            *reinterpret_cast<uint4*>(to + c) = make_uint4(pack<T>(o[0], o[1]), pack<T>(o[2], o[3]), pack<T>(o[4], o[5]), pack<T>(o[6], o[7]));
+          } else if (there && !whole) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 8)
-              if (c + j < p.c.head_dim)
-                *reinterpret_cast<uint4*>(to + c + j) = make_uint4(pack<T>(o[j], o[j + 1]), pack<T>(o[j + 2], o[j + 3]), pack<T>(o[j + 4], o[j + 5]),
-                                                                   pack<T>(o[j + 6], o[j + 7]));
-          } else if (there) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) part[TcMath<T, DP>::place(row, c + j)] = o[j];
+            for (int j = 0; j < 8; ++j) part[TcMath<T, DP>::place(row, c + j)] = o[j];
           }
           __syncwarp();
         }
