@@ -19,13 +19,14 @@ struct CacheAttnParams {
   int layer, rows, tokens, heads, group;
   int parts;                               // CTAs that share the work at most
   int min_units;                           // ... each this many units at least
+  int item_units;                          // what beginning and ending an item costs
   float scale_log2;
   bool whole;                              // items are not divided: no parts
   bool q_fp32;                             // q is float32 where the cache is not
 };
 
-// Work is counted in units: a tile of keys for a tile of query rows (the drafted tokens of a sequence times the heads that share a key head).  All units
-// of a call, sequence by sequence, key head by key head, row tile by row tile, are divided into equal runs of neighbours, one
+// Work is counted in units: a tile of keys for a tile of query rows (the drafted tokens of a sequence times the heads that share a key head), and in front of an
+// item's tiles a few for its beginning and end.  All units of a call, sequence by sequence, key head by key head, row tile by row tile, are divided into equal runs of neighbours, one
 // per CTA, whatever the sequences' lengths are: a ragged batch keeps all SMs busy to the end.  A run that starts or ends inside an item (a
 // row tile of a head of a sequence) leaves its part of the softmax in the workspace, at most two parts per CTA; the
 // second launch joins them in the order of the keys.  Where no sequence can have more tiles than a CTA works on at once the units are whole items, and there is
@@ -34,7 +35,7 @@ struct CacheAttnParams {
 // What CTA x leaves for CTA x of the second launch: the item that ends in its run and began before it.
 struct CacheJoin {
   int b, head, row_tile, rows;             // rows 0: there is none
-  int first, later;                        // the run that the item begins in; 1: but not with, so that its part is that run's second
+  int first, later;                        // the run that its first tile is in; 1: behind another item's, so that its part is that run's second
   int pad[2];
 };
 
@@ -66,7 +67,7 @@ __device__ __forceinline__ CacheItems cache_items(const CacheAttnParams& p, int 
   if (r.end < length + count) cache_fault(p.c, KB200_CACHE_NO_ROOM);
   r.row_tiles = (count * p.group + ROWS - 1) / ROWS;
   r.key_tiles = max(1, (r.end + TILE - 1) / TILE);
-  r.units = (int64_t)r.row_tiles * (p.whole ? 1 : r.key_tiles) * p.c.kv_heads;
+  r.units = (int64_t)r.row_tiles * (p.whole ? 1 : r.key_tiles + p.item_units) * p.c.kv_heads;
   return r;
 }
 
@@ -93,6 +94,19 @@ struct CacheRun {
   int64_t all, lo, hi;             // units of the call, of this CTA
   int parts;                       // CTAs that have any
   CacheCursor at;
+  int64_t left;                    // units from here on, the first `skip` of which are not tiles
+  int skip;
+  // The tiles of the item at hand that are in the run; 0: the run ends here.
+  __device__ __forceinline__ int tiles(const CacheAttnParams& p) const {
+    if (left <= skip) return 0;
+    return p.whole ? at.it.key_tiles : (int)min(left - skip, (int64_t)at.it.key_tiles - at.tile);
+  }
+  template <int ROWS, int TILE>
+  __device__ __forceinline__ void pass(const CacheAttnParams& p, int tiles) {
+    left -= p.whole ? 1 : skip + tiles;
+    skip = p.item_units;
+    if (left > 0) next_item<ROWS, TILE>(p, at);
+  }
 };
 struct CacheRunShared {
   int64_t sums[32], rest;
@@ -149,12 +163,15 @@ __device__ __forceinline__ bool find_run(const CacheAttnParams& p, int part, Cac
   at.b = shared.b;
   at.it = shared.it;
   int64_t rest = shared.rest;
-  const int item = p.whole ? 1 : at.it.key_tiles;
+  const int item = p.whole ? 1 : at.it.key_tiles + p.item_units;
   const int64_t per_head = (int64_t)at.it.row_tiles * item;
   at.head = (int)(rest / per_head);
   rest -= at.head * per_head;
   at.row_tile = (int)(rest / item);
-  at.tile = (int)(rest - (int64_t)at.row_tile * item);
+  const int in_item = (int)(rest - (int64_t)at.row_tile * item);
+  at.tile = max(0, in_item - p.item_units);
+  run->skip = max(0, p.item_units - in_item);
+  run->left = run->hi - run->lo;
   return true;
 }
 
@@ -165,11 +182,11 @@ __device__ __forceinline__ void leave_join(const CacheAttnParams& p, bool any, c
   CacheJoin j{};
   const CacheCursor& at = run.at;
   if (any && at.tile != 0 && at.it.key_tiles - at.tile <= run.hi - run.lo) {
-    const int64_t begins = run.lo - at.tile;               // the item's first unit
+    const int64_t first_tile = run.lo - at.tile;
     j.b = at.b, j.head = at.head, j.row_tile = at.row_tile;
     j.rows = min(ROWS, at.it.count * p.group - at.row_tile * ROWS);
-    j.first = (int)(((begins + 1) * run.parts - 1) / run.all);
-    j.later = run.all * j.first / run.parts != begins ? 1 : 0;
+    j.first = (int)(((first_tile + 1) * run.parts - 1) / run.all);
+    j.later = run.all * j.first / run.parts < first_tile - p.item_units ? 1 : 0;
   }
   p.joins[blockIdx.x] = j;
 }

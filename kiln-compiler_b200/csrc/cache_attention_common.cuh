@@ -37,9 +37,9 @@ __device__ __forceinline__ void bring_tiles(const CUtensorMap& map, const CacheA
   CacheCursor& now = run.at;
   const int box = min(TILE, 1 << p.c.page_log2), boxes = TILE / box;       // rows of a box; of a tile
   const int none = p.c.layers * 2 * p.c.pages;                             // beyond the map: zeros
-  int64_t left = run.hi - run.lo;
   uint32_t u = 0;
   int page_base = -1, page_slot = -1, my_page = -1;                        // 32 entries of a sequence's table row, one per lane
+  int left = run.tiles(p), tiles = left;
   while (left > 0) {
     const int first = now.tile * TILE >> p.c.page_log2;
     const int wanted = first & ~31;
@@ -68,9 +68,11 @@ __device__ __forceinline__ void bring_tiles(const CUtensorMap& map, const CacheA
                     (now.head << p.c.page_log2) + in_page, page < 0 ? none : (p.layer * 2 + which) * p.c.pages + page);
     }
     ++u;
-    const bool ends = ++now.tile == now.it.key_tiles;
-    if (ends || !p.whole) --left;
-    if (ends && left > 0) next_item<ROWS, TILE>(p, now);
+    ++now.tile;
+    if (--left == 0) {
+      run.pass<ROWS, TILE>(p, tiles);
+      left = tiles = run.tiles(p);
+    }
   }
 }
 
@@ -93,7 +95,7 @@ template <typename Math>
 constexpr int kPartOfWarp = Math::kOut * 32 + 2 * Math::kRows;
 
 // Joins the parts of the item that CTA x of the first launch has left (CacheJoin).
-constexpr int kJoinThreads = 128, kJoinAtOnce = 8;      // parts whose loads are in flight together
+constexpr int kJoinThreads = 128, kJoinAtOnce = 4;      // parts whose loads are in flight together
 
 template <typename Math, int RG>
 __global__ void __launch_bounds__(kJoinThreads) cache_attention_join_kernel(const __grid_constant__ CacheAttnParams p) {
@@ -155,6 +157,7 @@ struct CacheAttnVariant {
   void (*join)(CacheAttnParams);
   int threads, smem, rows, tile;   // rows and keys of a tile
   int groups;                      // tiles at work at once
+  int item_units;                  // see cache_attention.h
   int64_t part_floats;
 };
 CacheAttnVariant cache_attention_tc_variant(int dtype, int head_dim);      // (cache_attention_tc.cu) tiles of 128 query rows; 16-bit types, heads up to 128

@@ -7,9 +7,9 @@
 // 320 threads: warp 0 brings tiles, warp 1 issues the products, and two groups of four warps take turns at the tiles, a query row to a thread of each
 // (tensor-memory lane = row of the tile): from a tile's scores to its weights a warp needs ~1500 cycles, of which the exponentials are 512, so that one group
 // alone holds the memory up (304 us for 32 sequences of up to 16384 tokens and 32 drafted ones).  Each group has maxima, sums and output rows of its own,
-// joined at the end of an item.  384 columns of tensor memory: two sets of output rows, and scores of two tiles.  A tile's weights
-// (two to a column) are written over its scores, which are in registers by then: the tensor core runs in order, so the scores of the tile after the next
-// one, which go there, come behind the product that reads the weights.  Output rows stay in tensor memory over an item and are rescaled
+// joined at the end of an item.  448 columns of tensor memory: two sets of output rows, scores and weights (two to a column) of two tiles.  An instruction costs
+// the issuing warp ~60 cycles, a commit ~100, a tile ~1000: so a group's next scores are asked for as soon as it has read the last ones, under its exponentials.
+// (With the weights over the scores they had to wait for them: 3400 cycles for two tiles.)  Output rows stay in tensor memory over an item and are rescaled
 // only when a row's maximum has grown.  Q is put into shared memory by the threads that own its rows, from any strides, rounded on the way where it is float32.
 #include <algorithm>
 
@@ -19,7 +19,7 @@ namespace kb200 {
 namespace {
 
 constexpr int kRows = 128, kThreads = 64 + 2 * kRows;
-constexpr uint32_t kColumns = 512, kColS = 256;      // a group's output rows, the other's, then two tiles' scores of 64 columns
+constexpr uint32_t kColumns = 512, kColS = 256, kColP = 384;      // a group's output rows, the other's, two tiles' scores of 64 columns, their weights
 
 template <typename T, int DP>
 struct TcShape {
@@ -87,7 +87,7 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
   constexpr int TILE = G::kKeys;
   static_assert(TILE == 64, "64 columns of scores");
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ __align__(8) uint64_t bars[2 * Z::kStages + 7];
+  __shared__ __align__(8) uint64_t bars[2 * Z::kStages + 9];
   __shared__ CacheRunShared found;
   __shared__ unsigned long long odd_keys[2];         // keys of a group's tile whose V is not finite
   __shared__ float2 states[2][kRows];                // the groups' maxima and sums at the end of an item
@@ -96,13 +96,13 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
 
   const int lane = threadIdx.x & 31, warp = warp_index();
   const uint32_t q_smem = smem_u32(smem), stage0 = q_smem + Z::kQBytes;
-  const uint32_t full = smem_u32(bars), empty = full + 8 * Z::kStages, q_full = empty + 8 * Z::kStages, s_full = q_full + 8, p_full = s_full + 16, o_full = p_full + 16;
+  const uint32_t full = smem_u32(bars), empty = full + 8 * Z::kStages, q_full = empty + 8 * Z::kStages, s_full = q_full + 8, p_full = s_full + 16, o_full = p_full + 16, s_free = o_full + 16;
   if (threadIdx.x == 0) {
     abort_flag = 0;
     prefetch_tensormap(&map);
     for (int i = 0; i < 2 * Z::kStages; ++i) mbar_init(full + 8 * i, 1);
     mbar_init(q_full, 2 * kRows / 32);
-    for (int i = 0; i < 2; ++i) mbar_init(s_full + 8 * i, 1), mbar_init(p_full + 8 * i, kRows / 32), mbar_init(o_full + 8 * i, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(s_full + 8 * i, 1), mbar_init(p_full + 8 * i, kRows / 32), mbar_init(o_full + 8 * i, 1), mbar_init(s_free + 8 * i, kRows / 32);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 2) {
@@ -137,9 +137,10 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
     const uint32_t idesc_qk = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(TILE >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
     const uint32_t idesc_pv = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
     uint32_t items = 0;
-    auto issue_qk = [&](uint32_t t, bool first) {
+    auto issue_qk = [&](uint32_t t, bool first, bool behind) {       // `behind`: the scores of the tile before the last one, in the same place, are of this item
       const uint32_t stage = t % Z::kStages;
       if (first && !wait(q_full, items++ & 1)) return false;
+      if (behind && !wait(s_free + 8 * (t & 1), ((t - 2) >> 1) & 1)) return false;
       if (!wait(full + 8 * stage, (t / Z::kStages) & 1)) return false;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t k = stage0 + stage * G::kBytes, on = elect_one() ? 1u : 0u;
@@ -159,7 +160,7 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
       // 16 keys = 8 columns of weights and 16 128-byte rows of V per instruction
 #pragma unroll
       for (int kk = 0; kk < TILE / 16; ++kk)
-        umma_ts_if(on, tmem + (t & 1) * DP, tmem + kColS + (t & 1) * TILE + kk * 8, make_desc(v + kk * 2048, G::kBlockBytes, 1024), idesc_pv, !first || kk != 0 ? 1u : 0u, true);
+        umma_ts_if(on, tmem + (t & 1) * DP, tmem + kColP + (t & 1) * (TILE / 2) + kk * 8, make_desc(v + kk * 2048, G::kBlockBytes, 1024), idesc_pv, !first || kk != 0 ? 1u : 0u, true);
       if (on) {
         umma_commit(o_full + 8 * (t & 1));
         umma_commit(empty + 8 * stage);
@@ -167,23 +168,19 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
       __syncwarp();
       return true;
     };
-    int64_t left = any ? run.hi - run.lo : 0;
     uint32_t t = 0;
-    bool ok = true;
-    while (left > 0 && ok) {
-      const int tiles = p.whole ? now.it.key_tiles : (int)min(left, (int64_t)now.it.key_tiles - now.tile);
-      ok = issue_qk(t, true);
+    bool ok = any;
+    for (int tiles; ok && (tiles = run.tiles(p)) > 0; run.pass<kRows, TILE>(p, tiles)) {
+      ok = issue_qk(t, true, false) && (tiles == 1 || issue_qk(t + 1, false, false));
       for (int i = 0; i < tiles && ok; ++i, ++t) {
-        if (i + 1 < tiles) ok = issue_qk(t + 1, false);
+        if (i + 2 < tiles) ok = issue_qk(t + 2, false, true);
         ok = ok && issue_pv(t, i < 2);
       }
-      left -= p.whole ? 1 : tiles;
-      if (left > 0) next_item<kRows, TILE>(p, now);
     }
   } else {
     // ---------------- softmax: a thread per query row and group ----------------
     const int group = (warp - 2) >> 2, quad = warp & 3, row = quad * 32 + lane, worker = (threadIdx.x - 64) & (kRows - 1);
-    const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16), out_addr = lane_addr + group * DP, scores = lane_addr + kColS + group * TILE;
+    const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16), out_addr = lane_addr + group * DP, scores = lane_addr + kColS + group * TILE, weights = lane_addr + kColP + group * (TILE / 2);
     auto arrive = [&](uint32_t bar) {                // after this warp's last tensor-memory access that the barrier speaks of
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
@@ -191,10 +188,8 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
     };
     auto meet_group = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(kRows) : "memory"); };
     auto meet_both = [&]() { asm volatile("bar.sync 3, %0;" ::"n"(2 * kRows) : "memory"); };
-    int64_t left = any ? run.hi - run.lo : 0;
     uint32_t t0 = 0;                                 // the item's first tile
-    while (left > 0) {
-      const int tiles = p.whole ? now.it.key_tiles : (int)min(left, (int64_t)now.it.key_tiles - now.tile);
+    for (int tiles; any && (tiles = run.tiles(p)) > 0; run.pass<kRows, TILE>(p, tiles)) {
       const int rows_here = min(kRows, now.it.count * p.group - now.row_tile * kRows), sure = min(now.it.length, now.it.end);
       const bool there = row < rows_here, warp_there = quad * 32 < rows_here;
       const CacheRow r = row_of<kRows>(p, now, there ? row : 0);
@@ -275,6 +270,10 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = a[j], v[32 + j] = b[j];
           }
+          arrive(s_free + 8 * group);
+          // the product of the group's last tile has read its weights, and the output rows so far are there
+          if (done != 0) wait(o_full + 8 * group, ((t - 2) >> 1) & 1);
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           if (drafted) {
             const int off = now.it.length - key0, last = now.it.end - key0;      // where the first drafted token is in the tile; where the keys end
             unsigned long long shows;
@@ -311,8 +310,6 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
             const float grown = fmaxf(m, mx), alpha = grown == -CUDART_INF_F ? 1.0f : ex2(m - grown);
             m = grown;
             l *= alpha;
-            wait(o_full + 8 * group, ((t - 2) >> 1) & 1);      // the output rows of the group's tiles so far are there
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
             for (int c = 0; c < DP; c += 32) {
               float o[32];
@@ -336,10 +333,13 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
               sum2[j >> 1 & 1] = fadd2(sum2[j >> 1 & 1], make_float2(v[j], v[j + 1]));
               packed[(j - h) / 2] = pack<T>(v[j], v[j + 1]);
             }
-            tmem_st16(scores + h / 2, packed);
+            tmem_st16(weights + h / 2, packed);
           }
           l += (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
           tmem_st_wait();
+        } else {
+          arrive(s_free + 8 * group);
+          if (done != 0) wait(o_full + 8 * group, ((t - 2) >> 1) & 1);       // (no warp arrives for a tile's weights before all have for the last one's)
         }
         arrive(p_full + 8 * group);
         done = t + 1;
@@ -394,8 +394,6 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       meet_both();
       t0 += tiles;
-      left -= p.whole ? 1 : tiles;
-      if (left > 0) next_item<kRows, TILE>(p, now);
     }
   }
 
@@ -412,10 +410,14 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
   }
 }
 
+// What beginning and ending an item costs, in tiles: 32 sequences of 2000 to 16384 tokens, trees of 32: 269.8 us without, 263.9 with four, 258.9 with eight; five row
+// tiles of 20 tiles and more: 101.7, 86.8, 82.0.
+constexpr int kItemUnits = 8;
+
 template <typename T, int DP>
 CacheAttnVariant tc_variant() {
   using Z = TcShape<T, DP>;
-  return CacheAttnVariant{cache_attention_tc_kernel<T, DP>, cache_attention_join_kernel<TcMath<T, DP>, 1>, kThreads, Z::kSmem, kRows, Z::G::kKeys, 4,
+  return CacheAttnVariant{cache_attention_tc_kernel<T, DP>, cache_attention_join_kernel<TcMath<T, DP>, 1>, kThreads, Z::kSmem, kRows, Z::G::kKeys, 4, kItemUnits,
                           kPartOfWarp<TcMath<T, DP>>};
 }
 
