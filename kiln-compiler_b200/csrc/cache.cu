@@ -6,8 +6,8 @@
 // Nothing here depends on the order in which threads arrive: free pages are handed out by rank (a prefix sum), holders
 // are counted with integer atomics, and the list of copies is the only thing in any order.
 //
-// Tables that belong together change in one launch of a single cluster, whose CTAs meet at the hardware barrier (all of them are resident
-// by definition, so nothing can wait for a CTA that has not started); the tokens then move in a launch over the whole GPU.
+// Tables that belong together change in one launch: of one CTA where they are small, else of a single cluster, whose CTAs meet at the hardware barrier (all of them
+// are resident by definition, so nothing can wait for a CTA that has not started); the tokens then move in a launch over the whole GPU.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <limits.h>
@@ -25,6 +25,9 @@ namespace {
 
 constexpr int kCluster = 8;              // CTAs of a launch on the tables, the largest cluster that every GPU of the kind takes
 constexpr int kTableThreads = 1024;
+// One CTA up to here, whose barrier costs less than a cluster's: four beams of two prompts, forked and reserved, 17.4 us by clusters, 10.6 so; 96 pages compacted 21.4
+// and 14.7; a step of 64 drafting sequences 53.3 and 49.9.  But 128 sequences, eight beams each, 73.4 and 81.4.  (16384 pages are 16 to a thread.)
+constexpr int kFewPages = 16384, kFewSequences = 64;
 
 // counters: how many copies, pages in use, new pages of all sequences, and per CTA of the cluster three counts of its pages
 enum { kCopies = 0, kUsed, kWanted, kPerCta, kCounters = kPerCta + 3 * kCluster };
@@ -35,9 +38,15 @@ struct Scratch {
   int* counters;
 };
 
-__device__ __forceinline__ void cluster_sync() {
-  tc::cluster_arrive();
-  tc::cluster_wait();
+// All threads of the launch meet; what they wrote is there.
+template <bool ONE>
+__device__ __forceinline__ void meet() {
+  if constexpr (ONE) {
+    __syncthreads();
+  } else {
+    tc::cluster_arrive();
+    tc::cluster_wait();
+  }
 }
 
 // Exclusive prefix sum over the block's threads; `total` for all.  Shared memory for a value per warp.
@@ -115,6 +124,39 @@ __global__ void fork_commit_kernel(const CacheView c, const Scratch from) {
   }
 }
 
+// Both in one launch of one CTA, a warp to a sequence.
+__global__ void __launch_bounds__(kTableThreads) fork_small_kernel(const CacheView c, const int32_t* sources, const Scratch to) {
+  __shared__ int source_of[kFewSequences], held_of[kFewSequences], length_of[kFewSequences];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  for (int s = threadIdx.x >> 5; s < c.sequences; s += kTableThreads / 32) {
+    int source = sources[s];
+    if (source < -1 || source >= c.sequences) {
+      if (lane == 0) cache_fault(c, KB200_CACHE_BAD_INDEX);
+      source = s;
+    }
+    const int held = source < 0 ? 0 : min(max(c.held[source], 0), c.max_pages), old = min(max(c.held[s], 0), c.max_pages);
+    if (lane == 0) source_of[s] = source, held_of[s] = held, length_of[s] = source < 0 ? 0 : c.lengths[source];
+    if (source == s) continue;
+    for (int k = lane; k < max(held, old); k += 32) {
+      const int page = k < held ? c.table[(int64_t)source * c.max_pages + k] : -1, gone = k < old ? c.table[(int64_t)s * c.max_pages + k] : -1;
+      if (k < held) to.rows[(int64_t)s * c.max_pages + k] = page;
+      if (page == gone) continue;
+      if (cache_page_ok(c, page)) atomicAdd(c.refs + page, 1);
+      if (cache_page_ok(c, gone)) atomicSub(c.refs + gone, 1);
+    }
+  }
+  __syncthreads();
+  for (int s = threadIdx.x >> 5; s < c.sequences; s += kTableThreads / 32) {
+    if (source_of[s] == s) continue;
+    const int held = held_of[s], old = min(max(c.held[s], 0), c.max_pages);
+    for (int k = lane; k < max(held, old); k += 32) c.table[(int64_t)s * c.max_pages + k] = k < held ? to.rows[(int64_t)s * c.max_pages + k] : -1;
+    __syncwarp();
+    if (lane == 0) c.held[s] = held, c.lengths[s] = length_of[s];
+  }
+}
+
 // ---- room for new tokens -----------------------------------------------------------------------
 
 struct Span {
@@ -135,16 +177,19 @@ __device__ __forceinline__ Span span_of(const CacheView& c, const int32_t* count
   return r;
 }
 
-// One cluster.  A warp takes a sequence and its lanes the pages, so that both many sequences of a page each and a long prompt's hundreds of
-// pages are a few rounds.
+// A warp takes a sequence and its lanes the pages, so that both many sequences of a page each and a long prompt's hundreds of
+// pages are a few rounds; a thread takes neighbouring pages where free ones are counted.
+template <bool ONE>
 __global__ void __launch_bounds__(kTableThreads) reserve_kernel(const CacheView c, const int32_t* counts, const Scratch w) {
   __shared__ int shared[32];
   pdl_wait();
   pdl_launch_dependents();
-  const int rank = blockIdx.x, ranks = gridDim.x, lane = threadIdx.x & 31;
+  const int rank = ONE ? 0 : blockIdx.x, ranks = ONE ? 1 : gridDim.x, lane = threadIdx.x & 31;
   const int warp = rank * (kTableThreads / 32) + (threadIdx.x >> 5), warps = ranks * (kTableThreads / 32);
   int32_t* const wanted = w.slot;                          // [sequences]: new pages, then where the sequence's begin
   int32_t *const writers = w.page_a, *const lowest = w.page_b;
+  const int part = (c.pages + ranks * kTableThreads - 1) / (ranks * kTableThreads);
+  const int lo = min((rank * kTableThreads + (int)threadIdx.x) * part, c.pages), hi = min(lo + part, c.pages);
 
   // Everybody looks at all counts: nothing is done unless all are good.
   int faults = 0;
@@ -152,27 +197,41 @@ __global__ void __launch_bounds__(kTableThreads) reserve_kernel(const CacheView 
     const Span r = span_of(c, counts, s);
     faults |= (r.bad ? KB200_CACHE_BAD_INDEX : 0) | (r.too_long ? KB200_CACHE_TOO_LONG : 0);
   }
+  int free_mine = 0;
+  for (int page = lo; page < hi; ++page) free_mine += c.refs[page] == 0;
   const int bad = __syncthreads_or(faults & KB200_CACHE_BAD_INDEX), too_long = __syncthreads_or(faults & KB200_CACHE_TOO_LONG);
   if (rank == 0 && threadIdx.x == 0) w.counters[kCopies] = 0;
   if (bad || too_long) {
     if (rank == 0 && threadIdx.x == 0) cache_fault(c, (bad ? KB200_CACHE_BAD_INDEX : 0) | (too_long ? KB200_CACHE_TOO_LONG : 0));
     return;
   }
+  int free_here;
+  const int free_below = block_scan(free_mine, shared, &free_here);
+  if (threadIdx.x == 0) w.counters[kPerCta + rank] = free_here;
 
   // Shared pages that are going to be written: by how many, and by whom first.
   auto each_shared = [&](auto&& f) {
+    bool any = false;
     for (int s = warp; s < c.sequences; s += warps) {
       const Span r = span_of(c, counts, s);
       for (int k = r.first + lane; k < min(r.need, r.held); k += 32) {
         const int page = c.table[(int64_t)s * c.max_pages + k];
-        if (cache_page_ok(c, page) && c.refs[page] > 1) f(page, s);
+        if (cache_page_ok(c, page) && c.refs[page] > 1) {
+          f(page, s);
+          any = true;
+        }
       }
     }
+    return any;
   };
-  each_shared([&](int page, int) { writers[page] = 0, lowest[page] = INT_MAX; });
-  cluster_sync();
-  each_shared([&](int page, int s) { atomicAdd(writers + page, 1), atomicMin(lowest + page, s); });
-  cluster_sync();
+  bool any = each_shared([&](int page, int) { writers[page] = 0, lowest[page] = INT_MAX; });
+  if constexpr (ONE) any = __syncthreads_or(any);          // (a cluster meets in any case)
+  else any = true;
+  if (any) {
+    if constexpr (!ONE) meet<ONE>();
+    each_shared([&](int page, int s) { atomicAdd(writers + page, 1), atomicMin(lowest + page, s); });
+    meet<ONE>();
+  }
   // Which pages have to be new.
   for (int s = warp; s < c.sequences; s += warps) {
     const Span r = span_of(c, counts, s);
@@ -192,14 +251,7 @@ __global__ void __launch_bounds__(kTableThreads) reserve_kernel(const CacheView 
     n = __reduce_add_sync(0xffffffffu, n);
     if (lane == 0) wanted[s] = n;
   }
-  // How many pages of this CTA's part are free.
-  const int part = (c.pages + ranks - 1) / ranks, lo = min(rank * part, c.pages), hi = min(lo + part, c.pages);
-  int free_here = 0;
-  for (int page = lo + (int)threadIdx.x; page < hi; page += blockDim.x) free_here += c.refs[page] == 0;
-  int total_here;
-  block_scan(free_here, shared, &total_here);
-  if (threadIdx.x == 0) w.counters[kPerCta + rank] = total_here;
-  cluster_sync();
+  meet<ONE>();
   // The first CTA says where every sequence's new pages begin.
   if (rank == 0) {
     int base = 0;
@@ -213,9 +265,9 @@ __global__ void __launch_bounds__(kTableThreads) reserve_kernel(const CacheView 
     }
     if (threadIdx.x == 0) w.counters[kWanted] = base;
   }
-  cluster_sync();
+  meet<ONE>();
   const int all = __ldcg(w.counters + kWanted);
-  int free_before = 0, free_all = 0;
+  int free_before = free_below, free_all = 0;
   for (int r = 0; r < ranks; ++r) {
     const int n = __ldcg(w.counters + kPerCta + r);
     free_before += r < rank ? n : 0;
@@ -227,15 +279,9 @@ __global__ void __launch_bounds__(kTableThreads) reserve_kernel(const CacheView 
   }
   // The free pages by rank (over the list of writers, which has been read).
   int32_t* const free_pages = w.page_a;
-  for (int p0 = lo; p0 < hi && free_before < all; p0 += blockDim.x) {
-    const int page = p0 + threadIdx.x;
-    const bool is_free = page < hi && c.refs[page] == 0;
-    int total;
-    const int at = free_before + block_scan(is_free, shared, &total);
-    if (is_free && at < all) free_pages[at] = page;
-    free_before += total;
-  }
-  cluster_sync();
+  for (int page = lo; page < hi && free_before < all; ++page)
+    if (c.refs[page] == 0) free_pages[free_before++] = page;
+  meet<ONE>();
   for (int s = warp; s < c.sequences; s += warps) {
     const Span r = span_of(c, counts, s);
     int next = __ldcg(wanted + s);
@@ -408,48 +454,49 @@ __global__ void __launch_bounds__(kSlotThreads) accept_commit_kernel(const Cache
 
 // ---- compacting --------------------------------------------------------------------------------
 
+template <bool ONE>
 __global__ void __launch_bounds__(kTableThreads) compact_kernel(const CacheView c, const Scratch w) {
   __shared__ int shared[32];
   pdl_wait();
   pdl_launch_dependents();
-  const int rank = blockIdx.x, ranks = gridDim.x;
-  const int part = (c.pages + ranks - 1) / ranks, lo = min(rank * part, c.pages), hi = min(lo + part, c.pages);
-  int n = 0, total;
-  for (int page = lo + (int)threadIdx.x; page < hi; page += blockDim.x) n += c.refs[page] != 0;
-  block_scan(n, shared, &total);
-  if (threadIdx.x == 0) w.counters[kPerCta + rank] = total;
-  cluster_sync();
-  int used = 0;
-  for (int r = 0; r < ranks; ++r) used += __ldcg(w.counters + kPerCta + r);
+  const int rank = ONE ? 0 : blockIdx.x, ranks = ONE ? 1 : gridDim.x;
+  const int part = (c.pages + ranks * kTableThreads - 1) / (ranks * kTableThreads);
+  const int lo = min((rank * kTableThreads + (int)threadIdx.x) * part, c.pages), hi = min(lo + part, c.pages);
+  int n = 0, used;
+  for (int page = lo; page < hi; ++page) n += c.refs[page] != 0;
+  block_scan(n, shared, &used);
+  if constexpr (!ONE) {
+    if (threadIdx.x == 0) w.counters[kPerCta + rank] = used;
+    meet<ONE>();
+    used = 0;
+    for (int r = 0; r < ranks; ++r) used += __ldcg(w.counters + kPerCta + r);
+  }
   // Pages in use behind the first `used`, and free ones among those: as many of one as of the other.
-  int leave = 0, enter = 0, leave_here, enter_here;
-  for (int page = lo + (int)threadIdx.x; page < hi; page += blockDim.x) {
+  int leave = 0, enter = 0, moves, enter_here;
+  for (int page = lo; page < hi; ++page) {
     const bool in_use = c.refs[page] != 0;
     leave += in_use && page >= used;
     enter += !in_use && page < used;
   }
-  block_scan(leave, shared, &leave_here);
-  block_scan(enter, shared, &enter_here);
-  if (threadIdx.x == 0) w.counters[kPerCta + kCluster + rank] = leave_here, w.counters[kPerCta + 2 * kCluster + rank] = enter_here;
-  cluster_sync();
-  int leave_at = 0, enter_at = 0, moves = 0;
-  for (int r = 0; r < ranks; ++r) {
-    const int l = __ldcg(w.counters + kPerCta + kCluster + r), e = __ldcg(w.counters + kPerCta + 2 * kCluster + r);
-    leave_at += r < rank ? l : 0;
-    enter_at += r < rank ? e : 0;
-    moves += l;
+  int leave_at = block_scan(leave, shared, &moves), enter_at = block_scan(enter, shared, &enter_here);
+  if constexpr (!ONE) {
+    if (threadIdx.x == 0) w.counters[kPerCta + kCluster + rank] = moves, w.counters[kPerCta + 2 * kCluster + rank] = enter_here;
+    meet<ONE>();
+    moves = 0;
+    for (int r = 0; r < ranks; ++r) {
+      const int l = __ldcg(w.counters + kPerCta + kCluster + r), e = __ldcg(w.counters + kPerCta + 2 * kCluster + r);
+      leave_at += r < rank ? l : 0;
+      enter_at += r < rank ? e : 0;
+      moves += l;
+    }
   }
   int32_t *const leaving = w.page_a, *const entering = w.page_b;
-  for (int p0 = lo; p0 < hi; p0 += blockDim.x) {
-    const int page = p0 + threadIdx.x;
-    const bool in_use = page < hi && c.refs[page] != 0, leaves = in_use && page >= used, enters = page < hi && !in_use && page < used;
-    const int l = leave_at + block_scan(leaves, shared, &leave_here), e = enter_at + block_scan(enters, shared, &enter_here);
-    if (leaves) leaving[l] = page;
-    if (enters) entering[e] = page;
-    leave_at += leave_here;
-    enter_at += enter_here;
+  for (int page = lo; page < hi; ++page) {
+    const bool in_use = c.refs[page] != 0;
+    if (in_use && page >= used) leaving[leave_at++] = page;
+    if (!in_use && page < used) entering[enter_at++] = page;
   }
-  cluster_sync();
+  meet<ONE>();
   for (int i = rank * kTableThreads + threadIdx.x; i < moves; i += ranks * kTableThreads) {
     const int from = __ldcg(leaving + i), to = __ldcg(entering + i);
     w.copies[i] = make_int4(from, to, 1 << c.page_log2, 0);
@@ -561,9 +608,11 @@ __global__ void __launch_bounds__(kCopyThreads) append_kernel(const CacheView c,
 
 Scratch scratch_of(const Cache& c) { return Scratch{c.stage_rows, c.stage_slot, c.page_a, c.page_b, c.copies, c.counters}; }
 
-// One cluster.
+// One CTA or one cluster.
+bool few(const Cache& c) { return c.view.pages <= kFewPages && c.view.sequences <= kFewSequences; }
 template <typename... KArgs, typename... Args>
-cudaError_t launch_cluster(void (*kernel)(KArgs...), cudaStream_t s, Args&&... args) {
+cudaError_t launch_tables(const Cache& c, void (*one)(KArgs...), void (*cluster)(KArgs...), cudaStream_t s, Args&&... args) {
+  if (few(c)) return launch_kernel(true, one, dim3(1), dim3(kTableThreads), 0, s, static_cast<KArgs>(args)...);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(kCluster);
   cfg.blockDim = dim3(kTableThreads);
@@ -576,7 +625,7 @@ cudaError_t launch_cluster(void (*kernel)(KArgs...), cudaStream_t s, Args&&... a
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+  return cudaLaunchKernelEx(&cfg, cluster, static_cast<KArgs>(args)...);
 }
 
 int copy_grid(const Cache& c) { return c.sm_count * 8; }
@@ -684,6 +733,10 @@ KB200_EXPORT int kb200_cache_create(const kb200_cache_desc* d, int device, kb200
 KB200_EXPORT int kb200_cache_fork(kb200_cache* handle, const int32_t* sources, void* stream) {
   KB200_CACHE_ENTER("kb200_cache_fork");
   if (sources == nullptr) return fail(KB200_ERR_ARGUMENT, "kb200_cache_fork: sources is null");
+  if (few(c)) {
+    KB200_CUDA(launch_kernel(true, fork_small_kernel, dim3(1), dim3(kTableThreads), 0, s, c.view, sources, scratch_of(c)));
+    return KB200_OK;
+  }
   const dim3 grid(std::min(c.view.sequences, 4 * c.sm_count));
   KB200_CUDA(launch_kernel(true, fork_stage_kernel, grid, dim3(kSlotThreads), 0, s, c.view, sources, scratch_of(c)));
   KB200_CUDA(launch_kernel(true, fork_commit_kernel, grid, dim3(kSlotThreads), 0, s, c.view, scratch_of(c)));
@@ -693,7 +746,7 @@ KB200_EXPORT int kb200_cache_fork(kb200_cache* handle, const int32_t* sources, v
 KB200_EXPORT int kb200_cache_reserve(kb200_cache* handle, const int32_t* counts, void* stream) {
   KB200_CACHE_ENTER("kb200_cache_reserve");
   if (counts == nullptr) return fail(KB200_ERR_ARGUMENT, "kb200_cache_reserve: counts is null");
-  KB200_CUDA(launch_cluster(reserve_kernel, s, c.view, counts, scratch_of(c)));
+  KB200_CUDA(launch_tables(c, reserve_kernel<true>, reserve_kernel<false>, s, c.view, counts, scratch_of(c)));
   KB200_CUDA(launch_kernel(true, copy_pages_kernel, dim3(copy_grid(c)), dim3(kCopyThreads), 0, s, c.view, scratch_of(c)));
   return KB200_OK;
 }
@@ -708,7 +761,7 @@ KB200_EXPORT int kb200_cache_truncate(kb200_cache* handle, const int32_t* length
 
 KB200_EXPORT int kb200_cache_compact(kb200_cache* handle, void* stream) {
   KB200_CACHE_ENTER("kb200_cache_compact");
-  KB200_CUDA(launch_cluster(compact_kernel, s, c.view, scratch_of(c)));
+  KB200_CUDA(launch_tables(c, compact_kernel<true>, compact_kernel<false>, s, c.view, scratch_of(c)));
   KB200_CUDA(launch_kernel(true, compact_move_kernel, dim3(copy_grid(c)), dim3(kCopyThreads), 0, s, c.view, scratch_of(c)));
   return KB200_OK;
 }

@@ -78,11 +78,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
   CacheCursor& now = run.at;
   volatile int* const abort_ptr = &abort_flag;
   // A wait that ends for all lanes of a warp or none.  Where it runs out the warps do no more work, but meet each other as if they did.
-  auto wait = [&](uint32_t bar, uint32_t parity) {
-    const bool got = wait_a_second(bar, parity, abort_ptr);
-    if (!got) *abort_ptr = 1;
-    return __all_sync(0xffffffffu, got ? 1 : 0) != 0;
-  };
+  auto wait = [&](uint32_t bar, uint32_t parity) { return warp_waits(bar, parity, abort_ptr); };
 
   if (warp == Z::kWarps) {
     if (lane == 0) leave_join<ROWS>(p, any, run);
@@ -196,8 +192,10 @@ Variant variant() {
                  Z::kRows, Z::G::kKeys, Z::kGroups, kItemUnits<Math>, (int64_t)RG * kPartOfWarp<Math>};
 }
 
-// Rows of an item from which 16-bit caches go to tiles of 128 rows on tcgen05.
-constexpr int kFewRows = 16;
+// 16-bit caches go to tiles of 128 rows on tcgen05 above this many rows of an item, above half of it where the items are fewer than half of the SMs.  (BF16, heads
+// of 128, four to a key head, up to 8192 tokens.  32 sequences of 20, 32, 48 and 64 rows: 110, 121, 164, 151 us by warps; 127, 137, 127, 119 on tcgen05.  One sequence of
+// 20, 32 and 64 rows: 28.2, 29.1, 34.2 us and 21.9, 22.3, 24.7.)
+constexpr int kFewRows = 32;
 
 // By the rows of an item, up to 64 to a row tile.
 template <typename T, int DP>
@@ -212,12 +210,14 @@ template <typename T>
 Variant variant_of(int head_dim, int rows) {
   return head_dim <= 64 ? variant_of<T, 64>(rows) : head_dim <= 128 ? variant_of<T, 128>(rows) : variant_of<T, 256>(rows);
 }
-Variant variant_for(const Cache& c, int rows) {
-  if (c.dtype != KB200_DTYPE_FP32 && c.view.head_dim <= 128 && rows > kFewRows) return cache_attention_tc_variant(c.dtype, c.view.head_dim);
+Variant variant_for(const Cache& c, int rows, bool many_items) {
+  if (c.dtype != KB200_DTYPE_FP32 && c.view.head_dim <= 128 && rows > (many_items ? kFewRows : kFewRows / 2)) return cache_attention_tc_variant(c.dtype, c.view.head_dim);
   return c.dtype == KB200_DTYPE_FP32 ? variant_of<float>(c.view.head_dim, rows)
          : c.dtype == KB200_DTYPE_BF16 ? variant_of<__nv_bfloat16>(c.view.head_dim, rows) : variant_of<__half>(c.view.head_dim, rows);
 }
-Variant variant_for(const Cache& c, int tokens, int heads) { return variant_for(c, tokens * (heads / c.view.kv_heads)); }
+Variant variant_for(const Cache& c, int rows, int tokens, int heads) {
+  return variant_for(c, tokens * (heads / c.view.kv_heads), 2 * (int64_t)rows * c.view.kv_heads >= c.sm_count);
+}
 
 // How a call is divided: a CTA per SM, but no more than have a tile for each of their warps.
 struct Division {
@@ -250,7 +250,7 @@ int cache_attention_prepare(Cache& c) {
   const EncodeFn encode = encode_fn();
   if (encode == nullptr) return fail(KB200_ERR_CUDA, "kb200_cache_create: the driver has no cuTensorMapEncodeTiled");
   const CacheView& v = c.view;
-  const int page = 1 << v.page_log2, columns = 128 / c.element, tile = variant_for(c, 1).tile;
+  const int page = 1 << v.page_log2, columns = 128 / c.element, tile = variant_for(c, 1, true).tile;
   const cuuint64_t dims[3] = {(cuuint64_t)v.head_dim, (cuuint64_t)v.kv_heads * page, (cuuint64_t)v.layers * 2 * v.pages};
   const cuuint64_t strides[2] = {(cuuint64_t)v.head_dim * c.element, dims[1] * v.head_dim * c.element};
   const cuuint32_t box[3] = {(cuuint32_t)columns, (cuuint32_t)std::min(page, tile), 1}, steps[3] = {1, 1, 1};
@@ -262,7 +262,7 @@ int cache_attention_prepare(Cache& c) {
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(KB200_ERR_UNSUPPORTED, "kb200_cache_create: the pool cannot be described to the copy engine (error %d)", (int)r);
   for (const int rows : {2, 4, 8, 12, 16, 32, 64}) {
-    const Variant of = variant_for(c, rows);
+    const Variant of = variant_for(c, rows, true);
     KB200_CUDA(cudaFuncSetAttribute(of.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, of.smem));
   }
   return KB200_OK;
@@ -276,7 +276,7 @@ KB200_EXPORT uint64_t kb200_cache_attend_workspace(const kb200_cache* handle, in
   if (handle == nullptr) return 0;
   const Cache& c = *cache_of(handle);
   if (!call_ok(c, rows, tokens, heads) || rows == 0 || tokens == 0) return 0;
-  const Variant v = variant_for(c, tokens, heads);
+  const Variant v = variant_for(c, rows, tokens, heads);
   return workspace_of(v, division_of(c, v, rows, tokens, heads));
 }
 
@@ -298,7 +298,7 @@ KB200_EXPORT int kb200_cache_attend(kb200_cache* handle, int layer, const kb200_
   }
   if (mask != nullptr && mask_stride == nullptr) return fail(KB200_ERR_ARGUMENT, "kb200_cache_attend: a mask without strides");
   if (!(scale > 0.0f) || !(scale < 1e30f)) return fail(KB200_ERR_ARGUMENT, "kb200_cache_attend: scale must be positive and finite");
-  const Variant v = variant_for(c, tokens, q->heads);
+  const Variant v = variant_for(c, rows, tokens, q->heads);
   const Division d = division_of(c, v, rows, tokens, q->heads);
   const uint64_t need = workspace_of(v, d);
   if (need > 0 && (workspace == nullptr || !tc::aligned16(workspace) || workspace_bytes < need))

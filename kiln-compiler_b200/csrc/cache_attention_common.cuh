@@ -9,23 +9,33 @@ namespace {
 
 using namespace cache_math;
 
-// A wait of 2^31 cycles at most, about a second (a poll may suspend the thread, so a number of polls says little).
-__device__ __forceinline__ bool wait_a_second(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+// A wait of 2^31 cycles at most, about a second (a poll may suspend the thread, so a number of polls says little).  Where the barrier is ready it is one poll and
+// nothing else: the warp that issues the tensor core's instructions waits twice a tile.
+__device__ __forceinline__ bool polled(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __noinline__ bool wait_a_second(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   const long long t0 = clock64();
   while (true) {
-    for (int i = 0; i < 16; ++i) {
-      uint32_t ok;
-      asm volatile(
-          "{\n\t.reg .pred p;\n\t"
-          "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-          "selp.u32 %0, 1, 0, p;\n\t}"
-          : "=r"(ok)
-          : "r"(bar), "r"(parity)
-          : "memory");
-      if (ok != 0) return true;
-    }
+    for (int i = 0; i < 16; ++i)
+      if (polled(bar, parity)) return true;
     if (*abort_flag || clock64() - t0 > (1ll << 31)) return false;
   }
+}
+// By a converged warp: ends for all lanes or none (a lane may have a barrier of its own).  Where it runs out the CTA's other waits do too.
+__device__ __forceinline__ bool warp_waits(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  if (__all_sync(0xffffffffu, polled(bar, parity))) return true;
+  const bool got = wait_a_second(bar, parity, abort_flag);
+  if (!got) *abort_flag = 1;
+  return __all_sync(0xffffffffu, got) != 0;
 }
 
 // The producer warp: brings the run's tiles, page by page, as the ring's stages become free.

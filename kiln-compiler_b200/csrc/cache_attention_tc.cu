@@ -120,11 +120,7 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
   CacheCursor& now = run.at;
   volatile int* const abort_ptr = &abort_flag;
   // A wait that ends for all lanes of a warp or none.  Where it runs out the softmax warps do no more work, but meet each other as if they did.
-  auto wait = [&](uint32_t bar, uint32_t parity) {
-    const bool got = wait_a_second(bar, parity, abort_ptr);
-    if (!got) *abort_ptr = 1;
-    return __all_sync(0xffffffffu, got ? 1 : 0) != 0;
-  };
+  auto wait = [&](uint32_t bar, uint32_t parity) { return warp_waits(bar, parity, abort_ptr); };
 
   if (warp == 0) {
     if (lane == 0) leave_join<kRows>(p, any, run);
@@ -140,8 +136,9 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
     auto issue_qk = [&](uint32_t t, bool first, bool behind) {       // `behind`: the scores of the tile before the last one, in the same place, are of this item
       const uint32_t stage = t % Z::kStages;
       if (first && !wait(q_full, items++ & 1)) return false;
-      if (behind && !wait(s_free + 8 * (t & 1), ((t - 2) >> 1) & 1)) return false;
-      if (!wait(full + 8 * stage, (t / Z::kStages) & 1)) return false;
+      // (both at once, half of the lanes each)
+      const bool scores = behind && (lane & 1) != 0;
+      if (!wait(scores ? s_free + 8 * (t & 1) : full + 8 * stage, scores ? ((t - 2) >> 1) & 1 : (t / Z::kStages) & 1)) return false;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t k = stage0 + stage * G::kBytes, on = elect_one() ? 1u : 0u;
 #pragma unroll
