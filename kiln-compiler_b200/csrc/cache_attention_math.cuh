@@ -358,9 +358,10 @@ struct MmaMath {
   }
 };
 
-// float32 caches: multiply-adds, two to an instruction.  (Three TF32 products of split operands by mma.sync took 9200 cycles for 64 keys of 64, whatever
-// the number of rows, and lost a bit: these take ~1000 for 4 rows and ~3300 for 16.)  For the scores a lane has keys (two lanes share one where a
-// tile has 16), for the output it has DP / 32 columns of all rows; weights go from one to the other through shared memory.
+// float32 caches: multiply-adds, two to an instruction.  (Three TF32 products of split operands by mma.sync took 9200 cycles for 64 keys of 64 whatever the
+// number of rows was, and were off by twice as much.  A tile's multiply-adds take the SM 64 cycles a row; with five warps at it a warp needs 5000 to 7000 for 16 rows.)
+// For the scores a lane has keys (two lanes share one where a tile has 16), for the output it has DP / 32 columns of all rows; weights go from one to the
+// other through shared memory.
 template <int DP, int R>
 struct FmaMath {
   using Type = float;

@@ -317,6 +317,9 @@ SHAPES = [
     (F16, [2000, 900, 0, 1900], [20, 33, 17, 1], 8, 4, 128, 16),        # 128 rows and more to a key head
     (BF16, [700, 64, 3000], [64, 65, 5], 3, 5, 80, 64),
     (BF16, [0, 1, 130], [130, 100, 17], 2, 2, 48, 8),
+    (F32, [300, 45], [3, 9], 2, 1, 144, 32),
+    (BF16, [300, 45, 1000], [3, 9, 1], 2, 3, 144, 16),
+    (F32, [600, 2], [1, 1], 1, 5, 112, 128),
 ]
 
 
@@ -418,6 +421,8 @@ def test_strides_types_and_outputs():
     wide = torch.full((2, 5, 6, 64), 7.0, dtype=BF16, device="cuda")
     out = cache.attend(0, q, out=wide[:, :, :4])
     assert out.data_ptr() == wide.data_ptr() and torch.equal(out, plain) and (wide[:, :, 4:] == 7).all()
+    own = q.to(BF16)
+    assert torch.equal(plain, cache.attend(0, own, out=own)) and torch.equal(plain, own)       # in place
     odd.zero_()
     assert cache.attend(0, q, out=odd) is odd and torch.equal(odd, plain)
     sees = torch.ones(5, 5, dtype=torch.bool, device="cuda").tril()
@@ -495,18 +500,20 @@ def test_calls_on_other_streams_and_two_at_once():
     assert all(torch.equal(x, plain[i]) for i in range(2) for x in outs[i])
 
 
-def test_a_captured_step_follows_the_tables():
-    """Reserve, append, attend and accept as one graph: replays go on where the cache is, and two graphs do not share a workspace."""
-    sizes = dict(sequences=3, max_pages=40, pages=120, kv_heads=2, head_dim=64, dtype=BF16, layers=2, fill=0.0)
+@pytest.mark.parametrize("sequences", [3, 90])                         # (tables on one CTA, on a cluster)
+def test_a_captured_step_follows_the_tables(sequences):
+    """Fork, reserve, append, attend and accept as one graph: replays go on where the cache is, and two graphs do not share a workspace."""
+    sizes = dict(sequences=sequences, max_pages=40, pages=40 * sequences, kv_heads=2, head_dim=64, dtype=BF16, layers=2, fill=0.0)
     cache, eager = make(**sizes), make(**sizes)
     tokens = 4
-    x = torch.zeros(3, 2, 3, tokens, 2, 64, device="cuda")              # q, k, v by layer
-    counts, n = ints([4, 3, 1]), ints([2, 3, 1])
-    kept = ints([[0, 2], [0, 1], [0, 0]])
-    kept = torch.cat([kept, ints([[0], [2], [0]])], 1).contiguous()
+    x = torch.zeros(3, 2, sequences, tokens, 2, 64, device="cuda")      # q, k, v by layer
+    counts, n = ints([4, 3, 1] * (sequences // 3)), ints([2, 3, 1] * (sequences // 3))
+    kept = ints([[0, 2, 0], [0, 1, 2], [0, 0, 0]] * (sequences // 3))
+    sources = torch.arange(sequences, device="cuda", dtype=torch.int32)
     mask = torch.from_numpy(tree(random.Random(2), tokens)).cuda()
 
     def step(c, data):
+        c.fork(sources)
         c.reserve(counts)
         outs = []
         for layer in range(2):
@@ -520,22 +527,25 @@ def test_a_captured_step_follows_the_tables():
     with torch.cuda.stream(side):
         step(cache, x)                                                  # loads the kernels
     torch.cuda.current_stream().wait_stream(side)
-    cache.truncate(ints([0, 0, 0]))
+    cache.truncate(torch.zeros_like(counts))
     graphs, outs = [], []
     for _ in range(2):
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             outs.append(step(cache, x))
         graphs.append(graph)
-    assert cache.lengths.tolist() == [0, 0, 0]
+    assert cache.lengths.tolist() == [0] * sequences
     generator = torch.Generator("cuda").manual_seed(4)
     for i in range(20):
         x.copy_(torch.randn(x.shape, generator=generator, device="cuda"))
+        sources.copy_(torch.arange(sequences, device="cuda"))
+        if i == 10:
+            sources[0] = 1                                              # a beam, then writes into what it shares
         graphs[i % 2].replay()
         want = step(eager, x)
         for got, w in zip(outs[i % 2], want):
             assert torch.equal(got, w)
-    assert cache.lengths.tolist() == eager.lengths.tolist() == [40, 60, 20]
+    assert cache.lengths.tolist() == eager.lengths.tolist() and cache.lengths.tolist()[:3] == [50, 60, 20]
     assert torch.equal(cache.table, eager.table) and torch.equal(cache.refs, eager.refs)
     assert faults_of(cache) == faults_of(eager) == 0
 
