@@ -190,42 +190,58 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
       const int rows_here = min(kRows, now.it.count * p.group - now.row_tile * kRows), sure = min(now.it.length, now.it.end);
       const bool there = row < rows_here, warp_there = quad * 32 < rows_here;
       const CacheRow r = row_of<kRows>(p, now, there ? row : 0);
+      // What the rows see of up to 64 drafted tokens: a lane has a drafted token and a warp a word in eight of two per token.  All of these loads and those of Q are
+      // under way before any is waited for, and they are under the way of the first keys.
+      const uint8_t* const mask = p.mask + now.b * p.mask_stride[0];
+      const bool masked = p.mask != nullptr && p.tokens <= kMaskAhead && (now.tile + tiles) * TILE > sure;
+      const int first_token = now.row_tile * kRows / p.group, words = 2 * ((now.row_tile * kRows + rows_here - 1) / p.group - first_token + 1);
+      uint32_t seen = 0u;
+      if (masked) {
+        const int j = (warp & 1) * 32 + lane;                // (the words of a warp are all even or all odd)
+        const uint8_t* const column = mask + (j < now.it.count ? j : 0) * p.mask_stride[2];
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+          const int w = warp - 2 + 8 * n;
+          if (w < words && column[(first_token + w / 2) * p.mask_stride[1]] != 0 && j < now.it.count) seen |= 1u << n;
+        }
+      }
       // half a row of Q (the products that read the last item's have been executed: its output was read); zeros for rows that are not there
       if (warp_there) {
         const int64_t from = now.b * p.q_stride[0] + r.token * p.q_stride[1] + r.head * p.q_stride[2];
-#pragma unroll 4
-        for (int c = group * (DP / 16); c < (group + 1) * (DP / 16); ++c) {
-          uint4 x = make_uint4(0u, 0u, 0u, 0u);
-          if (there && c * 8 < p.c.head_dim) {
+        uint4 x[DP / 16];
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) {
+          const int at = group * (DP / 16) + c;
+          x[c] = make_uint4(0u, 0u, 0u, 0u);
+          if (there && at * 8 < p.c.head_dim) {
             if (p.q_fp32) {
-              const float4* const q = reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + from) + c * 2;
+              const float4* const q = reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + from) + at * 2;
               const float4 a = q[0], b = q[1];
-              x = make_uint4(pack<T>(a.x, a.y), pack<T>(a.z, a.w), pack<T>(b.x, b.y), pack<T>(b.z, b.w));
+              x[c] = make_uint4(pack<T>(a.x, a.y), pack<T>(a.z, a.w), pack<T>(b.x, b.y), pack<T>(b.z, b.w));
             } else {
-              x = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + from)[c];
+              x[c] = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + from)[at];
             }
           }
-          *reinterpret_cast<uint4*>(smem + c / 8 * Z::kQBlock + row * 128 + (((c % 8) ^ (row & 7)) << 4)) = x;
+        }
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) {
+          const int at = group * (DP / 16) + c;
+          *reinterpret_cast<uint4*>(smem + at / 8 * Z::kQBlock + row * 128 + (((at % 8) ^ (row & 7)) << 4)) = x[c];
         }
       }
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
-      // what the row sees of up to 64 drafted tokens, under the way of the first keys: a ballot per token and 32 of them
       unsigned long long tree = 0ull;
-      const uint8_t* const mask = p.mask + now.b * p.mask_stride[0];
-      if (p.mask != nullptr && p.tokens <= kMaskAhead && (now.tile + tiles) * TILE > sure) {
-        const int first = now.row_tile * kRows / p.group, last = (now.row_tile * kRows + rows_here - 1) / p.group;
-        uint32_t* const words = reinterpret_cast<uint32_t*>(states);       // (free between items)
-#pragma unroll 4
-        for (int w = warp - 2; w < 2 * (last - first + 1); w += 8) {
-          const int j = (w & 1) * 32 + lane;
-          const bool sees = j < now.it.count && mask[(first + w / 2) * p.mask_stride[1] + (j < now.it.count ? j : 0) * p.mask_stride[2]] != 0;
-          const uint32_t word = __ballot_sync(0xffffffffu, sees);
-          if (lane == 0) words[w] = word;
+      if (masked) {
+        uint32_t* const to = reinterpret_cast<uint32_t*>(states);        // (free between items)
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+          const uint32_t word = __ballot_sync(0xffffffffu, (seen >> n & 1u) != 0u);
+          if (lane == 0 && warp - 2 + 8 * n < words) to[warp - 2 + 8 * n] = word;
         }
         meet_both();
-        if (there) tree = words[2 * (r.token - first)] | (unsigned long long)words[2 * (r.token - first) + 1] << 32;
+        if (there) tree = to[2 * (r.token - first_token)] | (unsigned long long)to[2 * (r.token - first_token) + 1] << 32;
         meet_both();
       }
       float m = -CUDART_INF_F, l = 0.0f;
