@@ -4,13 +4,14 @@
 // What bounds it: the cache's bytes.  A key head's K and V are read once for all query rows that share them (drafted tokens x heads per key head).
 // Products run by warp (cache_attention_math.cuh): the rows of a decoding step do not fill larger units.
 //
-// A CTA has one producer warp and up to six consumer warps (from the eighth on a scheduler holds three warps and a thread 168 registers) and walks its run of key tiles (cache_attention.h).  The producer brings
-// tiles of K and V through a tensor map of the pool, page by page, as far ahead as the ring of stages goes, across the borders of sequences and
+// A CTA has one producer warp and up to six consumer warps (from the eighth on a scheduler holds three warps and a thread 168 registers) and walks
+// its run of key tiles (cache_attention.h).  The producer brings tiles of K and V through a tensor map of the pool, page by page, as far ahead as the ring of stages goes, across the borders of sequences and
 // heads.  A consumer warp takes a WHOLE tile for up to 16 query rows and keeps maxima, sums and output rows in registers; the
-// warps' sums are joined at the end of an item only.  Every stage of the ring belongs to one warp (or the group of warps with the other rows of the row
-// tile), which therefore sees each of its fillings: a barrier's parity tells no more than the last one.  (With the tile's keys divided among the warps, and copies issued by them, a warp
-// paid the rescaling, the shuffles and the addresses for 16 keys instead of 64: 985 instructions per warp and tile at 5.8 cycles each, two warps to
-// a scheduler, 187 us for 32 sequences of up to 8192 tokens, 52 % of the bandwidth.)
+// warps' sums are joined at the end of an item only.  Every stage of the ring belongs to one warp (or the group of warps with the other rows
+// of the row tile), which therefore sees each of its fillings: a barrier's parity tells no more than the last one.  (With the tile's keys divided among the
+// warps, and copies issued by them, a warp paid the rescaling, the shuffles and the addresses for 16 keys instead of 64: 985 instructions per warp and tile at 5.8 cycles each, two warps to
+// a scheduler, 187 us for 32 sequences of up to 8192 tokens in BF16, 52 % of the bandwidth; now 108, 0.89 of the
+// measured copy bandwidth.)
 //
 // Scores, maxima, sums and output rows are float32.  16-bit caches: the weights of a tile are rounded to the cache's type for the product with V
 // (half a step, 2^-9 for bfloat16, of every summand; the sum of the weights is kept of the unrounded ones).  float32 caches are not rounded anywhere.
@@ -203,6 +204,8 @@ Variant variant_of(int rows) {
   if constexpr (sizeof(T) == 4)
     return rows <= 2 ? variant<FmaMath<DP, 2>, 1>() : rows <= 4 ? variant<FmaMath<DP, 4>, 1>() : rows <= 8 ? variant<FmaMath<DP, 8>, 1>()
            : rows <= 12 ? variant<FmaMath<DP, 12>, 1>() : rows <= 16 ? variant<FmaMath<DP, 16>, 1>() : rows <= 32 ? variant<FmaMath<DP, 16>, 2>() : variant<FmaMath<DP, 16>, 4>();
+  else if constexpr (DP <= 128)
+    return rows <= 16 ? variant<MmaMath<T, DP>, 1>() : variant<MmaMath<T, DP>, 2>();       // (more: tcgen05)
   else
     return rows <= 16 ? variant<MmaMath<T, DP>, 1>() : rows <= 32 ? variant<MmaMath<T, DP>, 2>() : variant<MmaMath<T, DP>, 4>();
 }
