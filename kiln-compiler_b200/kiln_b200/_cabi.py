@@ -126,7 +126,7 @@ def sources():
 
 def nvcc_command(out=LIB_PATH, verbose=False):
     cmd = ["nvcc", "-std=c++17", "-O3", "-lineinfo", "-gencode", "arch=compute_100a,code=sm_100a",
-           "-shared", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
+           "-shared", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "--threads", str(min(8, os.cpu_count() or 1)),
            f"-I{INCLUDE_DIR}", f"-I{CSRC_DIR}"]
     if verbose:
         cmd += ["-Xptxas", "-v"]
