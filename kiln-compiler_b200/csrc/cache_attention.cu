@@ -62,12 +62,12 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
   __shared__ float2 states[Z::kWarps][Math::kRows];       // maxima and sums, by place in an item that several groups had a tile of
   __shared__ float2 own_states[Z::kWarps][Math::kRows];   // ... of all of them, or of a warp that had it alone: others may be at other items
   __shared__ float factors[Z::kWarps][Math::kRows];
-  __shared__ int abort_flag;
+  __shared__ int gave_up;
 
   const int lane = threadIdx.x & 31, warp = warp_index();
   const uint32_t stage0 = smem_u32(smem), full = smem_u32(bars), empty = full + 8 * Z::kStages;
   if (threadIdx.x == 0) {
-    abort_flag = 0;
+    gave_up = 0;
     prefetch_tensormap(&map);
     for (int i = 0; i < Z::kStages; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, RG);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -77,7 +77,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
   CacheRun run;
   const bool any = find_run<ROWS, TILE, Z::kThreads>(p, blockIdx.x, found, &run);       // (a barrier for all that is above, too)
   CacheCursor& now = run.at;
-  volatile int* const abort_ptr = &abort_flag;
+  volatile int* const abort_ptr = &gave_up;
   // A wait that ends for all lanes of a warp or none.  Where it runs out the warps do no more work, but meet each other as if they did.
   auto wait = [&](uint32_t bar, uint32_t parity) { return warp_waits(bar, parity, abort_ptr); };
 
@@ -170,7 +170,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
     }
   }
   __syncthreads();
-  if (abort_flag && threadIdx.x == 0) {
+  if (gave_up && threadIdx.x == 0) {
     cache_fault(p.c, kCacheWaitFault);
     let_copies_land();
   }

@@ -92,13 +92,13 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
   __shared__ unsigned long long odd_keys[2];         // keys of a group's tile whose V is not finite
   __shared__ float2 states[2][kRows];                // the groups' maxima and sums at the end of an item
   __shared__ uint32_t tmem_slot;
-  __shared__ int abort_flag;
+  __shared__ int gave_up;
 
   const int lane = threadIdx.x & 31, warp = warp_index();
   const uint32_t q_smem = smem_u32(smem), stage0 = q_smem + Z::kQBytes;
   const uint32_t full = smem_u32(bars), empty = full + 8 * Z::kStages, q_full = empty + 8 * Z::kStages, s_full = q_full + 8, p_full = s_full + 16, o_full = p_full + 16, s_free = o_full + 16;
   if (threadIdx.x == 0) {
-    abort_flag = 0;
+    gave_up = 0;
     prefetch_tensormap(&map);
     for (int i = 0; i < 2 * Z::kStages; ++i) mbar_init(full + 8 * i, 1);
     mbar_init(q_full, 2 * kRows / 32);
@@ -118,7 +118,7 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
   CacheRun run;
   const bool any = find_run<kRows, TILE, kThreads>(p, blockIdx.x, found, &run);
   CacheCursor& now = run.at;
-  volatile int* const abort_ptr = &abort_flag;
+  volatile int* const abort_ptr = &gave_up;
   // A wait that ends for all lanes of a warp or none.  Where it runs out the softmax warps do no more work, but meet each other as if they did.
   auto wait = [&](uint32_t bar, uint32_t parity) { return warp_waits(bar, parity, abort_ptr); };
 
@@ -412,7 +412,7 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
 
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  if (abort_flag && threadIdx.x == 0) {
+  if (gave_up && threadIdx.x == 0) {
     cache_fault(p.c, kCacheWaitFault);
     let_copies_land();
   }

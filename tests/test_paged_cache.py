@@ -134,3 +134,18 @@ def test_oracle_attention_against_attention_over_a_plain_sequence():
     again, *_ = o.attend(0, q[:, 13:], torch.from_numpy(some))
     assert np.abs(again - want.numpy()[:, 13:]).max() < 1e-13
     assert cache_oracle.rounded(torch.tensor([1.0 + 2**-9]), torch.bfloat16)[0] == 1.0
+
+
+@pytest.mark.parametrize("name", ["cache_attention.cu", "cache_attention_tc.cu"])
+def test_copies_in_flight_land_before_shared_memory_is_released(name):
+    """What a CTA does when one of its bounded waits has run out, read from the source (no kernel is made to fail for it): it meets, lets copies that are
+    under way land, and only then frees tensor memory and ends."""
+    from kiln_b200._cabi import CSRC_DIR
+
+    text = (CSRC_DIR / name).read_text()
+    way_out = text.index("if (gave_up && threadIdx.x == 0) {")
+    assert text.rindex("__syncthreads();", 0, way_out) > 0
+    assert text.index("let_copies_land();", way_out) < text.index("__syncthreads();", way_out)
+    if "tcgen05.alloc" in text:
+        assert text.index("tcgen05.dealloc") > text.index("__syncthreads();", way_out)
+    assert "mbar_wait(" not in text and "mbar_try_wait(" not in text       # only waits that end
