@@ -423,7 +423,8 @@ int kb200_cache_reserve(kb200_cache* cache, const int32_t* counts, void* cuda_st
 int kb200_cache_truncate(kb200_cache* cache, const int32_t* lengths, void* cuda_stream);
 
 /* Moves pages so that those in use come first: the used pages behind their own number fill the free ones before it, both in
- * ascending order.  Sequences see the same tokens; the pages behind are free and keep what they held. */
+ * ascending order.  Sequences see the same tokens; the pages behind are free and keep what they held.  Pages that the caller counts for itself move
+ * like the others. */
 int kb200_cache_compact(kb200_cache* cache, void* cuda_stream);
 
 /* Writes K and V of new tokens of one layer: token i < counts[b] of batch row b goes to position lengths[slots[b]] + i.
@@ -440,6 +441,7 @@ int kb200_cache_accept(kb200_cache* cache, const int32_t* counts, const int32_t*
  * the committed tokens j of sequence slots[b] and over the drafted ones t < counts[b] behind them with
  * mask[b * mask_stride[0] + i * mask_stride[1] + t * mask_stride[2]] != 0 (bytes; mask NULL: t <= i).  Tokens that a row does not see
  * contribute nothing, whatever they hold.  A row that sees nothing, and rows i >= counts[b], are 0.  One token per sequence is ordinary decoding.
+ * scale: from 1e-30 to 1e30.
  * q and out: [rows, tokens, heads, head_dim]; out has the cache's type, q that or float32 (rounded to it); they may be the same tensor.  Products of 16-bit types
  * are summed in float32, the weights rounded to that type in front of V; with a float32 cache all of it is float32.  Results depend on how the call is divided among
  * the SMs (the order of sums), not on what ran before or beside it.

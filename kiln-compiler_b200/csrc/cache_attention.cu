@@ -84,7 +84,6 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
   if (warp == Z::kWarps) {
     if (lane == 0) leave_join<ROWS>(p, any, run);
     if (any) bring_tiles<T, Math::kDim, ROWS, Z::kStages>(map, p, run, stage0, full, empty, wait);
-    clear_rows_behind<T>(p);
   } else {
     // ---------------- consumers ----------------
     const int row_group = warp % RG, key_group = warp / RG;
@@ -169,6 +168,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
       u0 += tiles;
     }
   }
+  clear_rows_behind<T>(p, warp, Z::kWarps + 1);
   __syncthreads();
   if (gave_up && threadIdx.x == 0) {
     cache_fault(p.c, kCacheWaitFault);
@@ -213,13 +213,13 @@ template <typename T>
 Variant variant_of(int head_dim, int rows) {
   return head_dim <= 64 ? variant_of<T, 64>(rows) : head_dim <= 128 ? variant_of<T, 128>(rows) : variant_of<T, 256>(rows);
 }
-Variant variant_for(const Cache& c, int rows, bool many_items) {
-  if (c.dtype != KB200_DTYPE_FP32 && c.view.head_dim <= 128 && rows > (many_items ? kFewRows : kFewRows / 2)) return cache_attention_tc_variant(c.dtype, c.view.head_dim);
+Variant variant_for(const Cache& c, int rows, int tokens, bool many_items) {
+  if (c.dtype != KB200_DTYPE_FP32 && c.view.head_dim <= 128 && rows > (many_items ? kFewRows : kFewRows / 2)) return cache_attention_tc_variant(c.dtype, c.view.head_dim, tokens);
   return c.dtype == KB200_DTYPE_FP32 ? variant_of<float>(c.view.head_dim, rows)
          : c.dtype == KB200_DTYPE_BF16 ? variant_of<__nv_bfloat16>(c.view.head_dim, rows) : variant_of<__half>(c.view.head_dim, rows);
 }
 Variant variant_for(const Cache& c, int rows, int tokens, int heads) {
-  return variant_for(c, tokens * (heads / c.view.kv_heads), 2 * (int64_t)rows * c.view.kv_heads >= c.sm_count);
+  return variant_for(c, tokens * (heads / c.view.kv_heads), tokens, 2 * (int64_t)rows * c.view.kv_heads >= c.sm_count);
 }
 
 // How a call is divided: a CTA per SM, but no more than have a tile for each of their warps.
@@ -253,7 +253,7 @@ int cache_attention_prepare(Cache& c) {
   const EncodeFn encode = encode_fn();
   if (encode == nullptr) return fail(KB200_ERR_CUDA, "kb200_cache_create: the driver has no cuTensorMapEncodeTiled");
   const CacheView& v = c.view;
-  const int page = 1 << v.page_log2, columns = 128 / c.element, tile = variant_for(c, 1, true).tile;
+  const int page = 1 << v.page_log2, columns = 128 / c.element, tile = variant_for(c, 1, 1, true).tile;
   const cuuint64_t dims[3] = {(cuuint64_t)v.head_dim, (cuuint64_t)v.kv_heads * page, (cuuint64_t)v.layers * 2 * v.pages};
   const cuuint64_t strides[2] = {(cuuint64_t)v.head_dim * c.element, dims[1] * v.head_dim * c.element};
   const cuuint32_t box[3] = {(cuuint32_t)columns, (cuuint32_t)std::min(page, tile), 1}, steps[3] = {1, 1, 1};
@@ -264,10 +264,11 @@ int cache_attention_prepare(Cache& c) {
   const CUresult r = encode(&c.map, type, 3, v.pool, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(KB200_ERR_UNSUPPORTED, "kb200_cache_create: the pool cannot be described to the copy engine (error %d)", (int)r);
-  for (const int rows : {2, 4, 8, 12, 16, 32, 64}) {
-    const Variant of = variant_for(c, rows, true);
-    KB200_CUDA(cudaFuncSetAttribute(of.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, of.smem));
-  }
+  for (const int tokens : {1, kMaskAhead + 1})
+    for (const int rows : {2, 4, 8, 12, 16, 32, 64}) {
+      const Variant of = variant_for(c, rows, tokens, true);
+      KB200_CUDA(cudaFuncSetAttribute(of.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, of.smem));
+    }
   return KB200_OK;
 }
 
@@ -300,7 +301,7 @@ KB200_EXPORT int kb200_cache_attend(kb200_cache* handle, int layer, const kb200_
       if (s % (wide ? 4 : 8) != 0) return fail(KB200_ERR_ARGUMENT, "kb200_cache_attend: strides of q and out must be multiples of 16 bytes");
   }
   if (mask != nullptr && mask_stride == nullptr) return fail(KB200_ERR_ARGUMENT, "kb200_cache_attend: a mask without strides");
-  if (!(scale > 0.0f) || !(scale < 1e30f)) return fail(KB200_ERR_ARGUMENT, "kb200_cache_attend: scale must be positive and finite");
+  if (!(scale >= 1e-30f) || !(scale <= 1e30f)) return fail(KB200_ERR_ARGUMENT, "kb200_cache_attend: scale must be from 1e-30 to 1e30");
   const Variant v = variant_for(c, rows, tokens, q->heads);
   const Division d = division_of(c, v, rows, tokens, q->heads);
   const uint64_t need = workspace_of(v, d);

@@ -60,6 +60,23 @@ __device__ __forceinline__ void tmem_ld8x2(uint32_t addr_a, uint32_t addr_b, flo
   for (int i = 0; i < 8; ++i) va[i] = __uint_as_float(a[i]), vb[i] = __uint_as_float(b[i]);
 }
 
+// More drafted tokens than are looked up ahead: what the rows see of those in one tile, two words per token, a warp a word in four.  (64 sequences, trees of 300 tokens behind
+// 100, four heads to a key head: 222 us; 285 when each row's thread read its own bytes.)
+template <int ROWS>
+__device__ __forceinline__ void look_at_tile(const CacheAttnParams& p, int b, int row_tile, int length, int count, int key0, uint32_t* to) {
+  const int quarter = ((threadIdx.x >> 5) - 2) & 3, lane = threadIdx.x & 31;
+  const int first_token = row_tile * ROWS / p.group, words = 2 * ((min((row_tile + 1) * ROWS, count * p.group) - 1) / p.group - first_token + 1);
+  const int j = key0 + (quarter & 1) * 32 + lane - length;
+  const bool is_drafted = j >= 0 && j < count;
+  const uint8_t* const column = p.mask + b * p.mask_stride[0] + (is_drafted ? j : 0) * p.mask_stride[2];
+  const int64_t step = p.mask_stride[1];
+#pragma unroll 8
+  for (int w = quarter; w < words; w += 4) {
+    const uint32_t word = __ballot_sync(0xffffffffu, column[(first_token + w / 2) * step] != 0 && is_drafted);
+    if (lane == 0) to[w] = word;
+  }
+}
+
 // V of a drafted token holds infinities or NaN: they are zero in the product, and this adds them to the output row of a thread that gives the token weight w.
 template <typename T, int DP>
 __device__ __noinline__ void add_infinite(const CacheAttnParams& p, const CacheItems& it, int head, int at, float w, uint32_t out_addr) {
@@ -79,7 +96,8 @@ __device__ __noinline__ void add_infinite(const CacheAttnParams& p, const CacheI
   }
 }
 
-template <typename T, int DP>
+// MANY: more than kMaskAhead drafted tokens.  (Two kernels: with both ways in one, its registers cost a call of few tokens up to 9%: 109 us where 100 are.)
+template <typename T, int DP, bool MANY>
 __global__ void __launch_bounds__(kThreads, 1)
 cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CacheAttnParams p) {
   using Z = TcShape<T, DP>;
@@ -125,7 +143,6 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
   if (warp == 0) {
     if (lane == 0) leave_join<kRows>(p, any, run);
     if (any) bring_tiles<T, DP, kRows, Z::kStages>(map, p, run, stage0, full, empty, wait);
-    clear_rows_behind<T>(p);
   } else if (warp == 1) {
     // ---------------- products ----------------
     // Tiles are numbered over all items; scores, weights and the output's barrier take turns of two.
@@ -193,7 +210,7 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
       // What the rows see of up to 64 drafted tokens: a lane has a drafted token and a warp a word in eight of two per token.  All of these loads and those of Q are
       // under way before any is waited for, and they are under the way of the first keys.
       const uint8_t* const mask = p.mask + now.b * p.mask_stride[0];
-      const bool masked = p.mask != nullptr && p.tokens <= kMaskAhead && (now.tile + tiles) * TILE > sure;
+      const bool masked = !MANY && p.mask != nullptr && (now.tile + tiles) * TILE > sure;
       const int first_token = now.row_tile * kRows / p.group, words = 2 * ((now.row_tile * kRows + rows_here - 1) / p.group - first_token + 1);
       uint32_t seen = 0u;
       if (masked) {
@@ -271,8 +288,13 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
               }
             }
           fence_async_smem();
+          // more drafted tokens than are looked up ahead: those of this tile, the same way
+          uint32_t* const to_see = reinterpret_cast<uint32_t*>(states[group]);
+          const bool look = MANY && p.mask != nullptr;
+          if (look) look_at_tile<kRows>(p, now.b, now.row_tile, now.it.length, now.it.count, key0, to_see);
           meet_group();
           odd = odd_keys[group];
+          if (look && there) tree = to_see[2 * (r.token - first_token)] | (unsigned long long)to_see[2 * (r.token - first_token) + 1] << 32;
           meet_group();
         }
         float v[64];
@@ -294,14 +316,7 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
               const int n = off + r.token + 1;
               shows = n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
             } else {
-              if (p.tokens <= kMaskAhead) {
-                shows = off >= 64 || off <= -64 ? 0ull : off >= 0 ? tree << off : tree >> -off;
-              } else {
-                shows = 0ull;
-                const int lo = max(0, off), hi = there ? min(64, off + now.it.count) : 0;
-#pragma unroll 8
-                for (int j = lo; j < hi; ++j) shows |= mask[r.token * p.mask_stride[1] + (j - off) * p.mask_stride[2]] != 0 ? 1ull << j : 0ull;
-              }
+              shows = MANY ? tree : off >= 64 || off <= -64 ? 0ull : off >= 0 ? tree << off : tree >> -off;
               if (off > 0) shows |= off >= 64 ? ~0ull : (1ull << off) - 1;
             }
             if (last < 64) shows &= last <= 0 ? 0ull : (1ull << last) - 1;
@@ -410,6 +425,7 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
     }
   }
 
+  clear_rows_behind<T>(p, warp, kThreads / 32);
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (gave_up && threadIdx.x == 0) {
@@ -427,18 +443,23 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
 // tiles of 20 tiles and more: 101.7, 86.8, 82.0.
 constexpr int kItemUnits = 8;
 
-template <typename T, int DP>
+template <typename T, int DP, bool MANY>
 CacheAttnVariant tc_variant() {
   using Z = TcShape<T, DP>;
-  return CacheAttnVariant{cache_attention_tc_kernel<T, DP>, cache_attention_join_kernel<TcMath<T, DP>, 1>, kThreads, Z::kSmem, kRows, Z::G::kKeys, 4, kItemUnits,
+  return CacheAttnVariant{cache_attention_tc_kernel<T, DP, MANY>, cache_attention_join_kernel<TcMath<T, DP>, 1>, kThreads, Z::kSmem, kRows, Z::G::kKeys, 4, kItemUnits,
                           kPartOfWarp<TcMath<T, DP>>};
+}
+template <typename T, bool MANY>
+CacheAttnVariant tc_variant(int head_dim) {
+  return head_dim <= 64 ? tc_variant<T, 64, MANY>() : tc_variant<T, 128, MANY>();
 }
 
 }  // namespace
 
-CacheAttnVariant cache_attention_tc_variant(int dtype, int head_dim) {
-  if (dtype == KB200_DTYPE_BF16) return head_dim <= 64 ? tc_variant<__nv_bfloat16, 64>() : tc_variant<__nv_bfloat16, 128>();
-  return head_dim <= 64 ? tc_variant<__half, 64>() : tc_variant<__half, 128>();
+CacheAttnVariant cache_attention_tc_variant(int dtype, int head_dim, int tokens) {
+  const bool many = tokens > kMaskAhead;
+  if (dtype == KB200_DTYPE_BF16) return many ? tc_variant<__nv_bfloat16, true>(head_dim) : tc_variant<__nv_bfloat16, false>(head_dim);
+  return many ? tc_variant<__half, true>(head_dim) : tc_variant<__half, false>(head_dim);
 }
 
 }  // namespace kb200

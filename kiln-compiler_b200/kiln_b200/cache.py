@@ -68,6 +68,7 @@ class PagedCache:
         self.table = torch.full((sequences, max_pages), -1, dtype=torch.int32, device=self.device)
         self.held, self.lengths = (torch.zeros(sequences, dtype=torch.int32, device=self.device) for _ in range(2))
         self.refs = torch.zeros(pages, dtype=torch.int32, device=self.device)
+        self._buffers = (self.pool, self.table, self.held, self.lengths, self.refs)      # (what the library's pointers are of)
         desc.pool, desc.pool_bytes = self.pool.data_ptr(), pool_bytes
         desc.table, desc.held, desc.lengths, desc.refs = (t.data_ptr() for t in (self.table, self.held, self.lengths, self.refs))
         self._call = _cabi.load_call()

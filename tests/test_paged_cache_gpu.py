@@ -216,7 +216,8 @@ def test_arguments_that_are_refused():
             (lambda: cache.attend(0, good[:, :, :1]), ValueError), (lambda: cache.attend(2, good), ValueError), (lambda: cache.attend(0, good.double()), TypeError),
             (lambda: cache.attend(0, good, mask=torch.ones(3, 3, device="cuda")), TypeError), (lambda: cache.attend(0, good, mask=torch.ones(2, 3, dtype=torch.bool, device="cuda")), ValueError),
             (lambda: cache.attend(0, good, mask=torch.ones(3, 3, dtype=torch.bool)), ValueError), (lambda: cache.attend(0, good, scale=0.0), ValueError),
-            (lambda: cache.attend(0, good, scale=float("nan")), ValueError), (lambda: cache.attend(0, good, out=good), ValueError),
+            (lambda: cache.attend(0, good, scale=float("nan")), ValueError), (lambda: cache.attend(0, good, scale=1e-40), ValueError),
+            (lambda: cache.attend(0, good, scale=-1.0), ValueError), (lambda: cache.attend(0, good, scale=float("inf")), ValueError), (lambda: cache.attend(0, good, out=good), ValueError),
             (lambda: cache.attend(0, good, out=good[:1].to(BF16)), ValueError), (lambda: cache.attend(0, good, counts=three), ValueError)]:
         with pytest.raises(error):
             call()
@@ -434,6 +435,22 @@ def test_strides_types_and_outputs():
     cache.append(0, k[:, :, :, 0], k[:, :, :, 1])
     before.append(0, k[:, :, :, 0], k[:, :, :, 1])
     same(cache, before)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_many_empty_rows_are_zero(dtype):
+    """A padded batch of which most rows hold no token, in an output that held something else."""
+    counts = [0, 200, 1, 0, 77, 3]
+    cache, q = filled([0, 5, 300, 40, 9, 0], counts, dtype=dtype, kv_heads=2, head_dim=64)
+    q = q.to(dtype)
+    out = torch.full_like(q, 3.0)
+    cache.attend(0, q, counts=ints(counts), out=out)
+    check(cache, q, None, counts)
+    for s, n in enumerate(counts):
+        assert (out[s, n:] == 0).all() and (out[s, :n] != 0).any() == (n > 0)
+    out.fill_(3.0)
+    cache.attend(0, q[:2], counts=ints([200, 0]), slots=ints([1, 1]), out=out[:2])
+    assert (out[1] == 0).all() and (out[2:] == 3).all() and faults_of(cache) == 0
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
