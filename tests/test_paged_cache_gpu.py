@@ -437,6 +437,25 @@ def test_strides_types_and_outputs():
     same(cache, before)
 
 
+@pytest.mark.parametrize("dtype, heads, head_dim", [(BF16, 1, 128), (F16, 3, 64), (F32, 2, 64), (BF16, 2, 160)])
+def test_masks_of_hundreds_of_tokens(dtype, heads, head_dim):
+    """Their columns and rows in any order of memory, hidden tokens that hold NaN in every tile, tokens that see none of the drafted ones."""
+    counts = [300, 65, 0, 129]
+    cache, _ = filled([40, 0, 7, 64], counts, dtype=dtype, kv_heads=1, head_dim=head_dim)
+    q = torch.randn(4, 300, heads, head_dim, device="cuda", generator=torch.Generator("cuda").manual_seed(7)).to(dtype)
+    dice = np.random.default_rng(5)
+    mask = np.tril(dice.random((4, 300, 300)) < 0.3)
+    mask[:, ::7] = False
+    mask[:, :, 3::31] = False
+    clean = check(cache, q, mask, counts)
+    for s, length in ((0, 40), (1, 0), (3, 64)):
+        for at in range(length + 3, length + counts[s], 31):
+            cache.pool[0, :, cache.table[s, at // 16].item(), :, at % 16] = float("nan")
+    device = torch.from_numpy(mask).cuda()
+    for same_mask in (device, device.permute(2, 0, 1).contiguous().permute(1, 2, 0), torch.stack((~device, device), 3)[..., 1]):
+        assert torch.equal(clean, cache.attend(0, q, mask=same_mask, counts=ints(counts)))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_many_empty_rows_are_zero(dtype):
     """A padded batch of which most rows hold no token, in an output that held something else."""
