@@ -14,7 +14,7 @@ prompt, and the attention of new tokens over them.  One step of a server that dr
 Ordinary decoding drafts one token and accepts it; a prompt is a chain of tokens (no mask) that are all accepted.
 
 All arguments and all of the cache's state are tensors on the GPU, every call is enqueued on the current stream, and none waits for the GPU: a step can be
-captured into a CUDA graph whose replays follow what the tensors hold then.  Calls that change the cache are
+captured into a CUDA graph whose replays follow what the tensors hold then; the cache has to live until the last of them has run.  Calls that change the cache are
 ordered by the caller (one stream, or events), like calls of one ``GPUExecutable``.  What cannot be done on the way, such as a
 reservation beyond the free pages, is left out and told by ``status()``.
 
