@@ -65,14 +65,16 @@ __device__ __forceinline__ void bring_tiles(const CUtensorMap& map, const CacheA
   const int box = min(TILE, 1 << p.c.page_log2), boxes = TILE / box;       // rows of a box; of a tile
   const int none = p.c.layers * 2 * p.c.pages;                             // beyond the map: zeros
   uint32_t u = 0;
-  int page_base = -1, page_slot = -1, my_page = -1;                        // 32 entries of a sequence's table row, one per lane
+  // 32 entries of a sequence's table row as far as a batch row's keys go, one per lane (rows that name the same sequence may end apart)
+  int page_base = -1, page_slot = -1, page_end = -1, my_page = -1;
   int left = run.tiles(p), tiles = left;
   if (left > 0) ask_for_rows<T, ROWS>(p, now, lane);
   while (left > 0) {
     const int first = now.tile * TILE >> p.c.page_log2;
     const int wanted = first & ~31;
-    if (page_slot != now.it.slot || wanted != page_base) {
+    if (page_slot != now.it.slot || page_end != now.it.end || wanted != page_base) {
       page_slot = now.it.slot;
+      page_end = now.it.end;
       page_base = wanted;
       const int k = wanted + lane;
       my_page = k << p.c.page_log2 < now.it.end ? p.c.table[(int64_t)now.it.slot * p.c.max_pages + k] : -1;
