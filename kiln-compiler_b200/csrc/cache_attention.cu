@@ -110,9 +110,9 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
         for (int w = 0; w < n; ++w) all.x = fmaxf(all.x, states[w * RG + row_group][row].x);
         for (int w = 0; w < n; ++w) {
           const float2 state = states[w * RG + row_group][row];
-          if (state.x != -CUDART_INF_F) all.y += state.y * ex2(state.x - all.x);
+          if (state.x != -CUDART_INF_F) all.y += state.y * ex2(Math::exponent(state.x - all.x, p.scale_log2));
         }
-        if (top != -CUDART_INF_F) factor = ex2(top - all.x);
+        if (top != -CUDART_INF_F) factor = ex2(Math::exponent(top - all.x, p.scale_log2));
         if (lane < Math::kRows) factors[warp][lane] = factor;
         meet();                                      // (which also says that the states have been read)
         math.rescale(lane, factors[warp]);

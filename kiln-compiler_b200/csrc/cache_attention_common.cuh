@@ -170,12 +170,12 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attention_join_kernel(cons
         next = fmaxf(next, m[j]);
       }
       if (next == -CUDART_INF_F) continue;           // nothing seen so far
-      const float a = ex2(top - next);
+      const float a = ex2(Math::exponent(top - next, p.scale_log2));
       sum *= a, x.x *= a, x.y *= a, x.z *= a, x.w *= a;
 #pragma unroll
       for (int j = 0; j < kJoinAtOnce; ++j) {
         if (m[j] == -CUDART_INF_F) continue;
-        const float b = ex2(m[j] - next);
+        const float b = ex2(Math::exponent(m[j] - next, p.scale_log2));
         sum += l[j] * b, x.x += y[j].x * b, x.y += y[j].y * b, x.z += y[j].z * b, x.w += y[j].w * b;
       }
       top = next;

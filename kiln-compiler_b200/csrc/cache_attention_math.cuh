@@ -169,6 +169,8 @@ struct MmaMath {
   static constexpr int NT = G::kKeys / 8, DT = DP / 8;                   // 8-wide column tiles of the scores, of the output rows
   uint32_t q[DP / 16][4];
   float o[DT][4], m[2], l[2];
+  // Maxima are powers of two's exponents: the scale and the maximum go into one multiply-add per score, and a rounding of the maximum cancels.
+  static __device__ __forceinline__ float exponent(float behind, float) { return behind; }
 
   template <int ROWS>
   __device__ __forceinline__ void begin(const CacheAttnParams& p, const CacheCursor& now, const Place& at) {
@@ -374,6 +376,9 @@ struct FmaMath {
   static constexpr int C = DP / 32;                                      // output columns of a lane: C lane .. C lane + C - 1
   float2 o[C][R / 2];                                // rows 2i and 2i + 1
   float m[R], l[R];                                  // (l: of the lane's keys)
+  // Scores and maxima are kept as they were summed, and the scale is applied to differences: a rounding then goes with the distance from the maximum, not with
+  // the score's size.  (Scores of 8000 that were scaled and rounded first gave errors of 1e-4.)
+  static __device__ __forceinline__ float exponent(float behind, float scale) { return behind * scale; }
 
   // The query rows go to shared memory, [R][DP] of the warp's own.
   template <int ROWS>
@@ -473,7 +478,7 @@ struct FmaMath {
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int i = 0; i < KEYS; ++i) s[i][r] = (sum[i][r].x + sum[i][r].y) * p.scale_log2;
+      for (int i = 0; i < KEYS; ++i) s[i][r] = sum[i][r].x + sum[i][r].y;
     if constexpr (SHARE > 1) {
 #pragma unroll
       for (int r = 0; r < R; ++r)
@@ -510,7 +515,7 @@ struct FmaMath {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         top[r] = fmaxf(top[r], m[r]);
-        const float alpha = top[r] == -CUDART_INF_F ? 1.0f : ex2(m[r] - top[r]);
+        const float alpha = top[r] == -CUDART_INF_F ? 1.0f : ex2(exponent(m[r] - top[r], p.scale_log2));
         m[r] = top[r];
         l[r] *= alpha;
 #pragma unroll
@@ -522,7 +527,7 @@ struct FmaMath {
       const float shift = m[r] == -CUDART_INF_F ? 0.0f : m[r];           // nothing seen so far: every weight is 2^-inf
 #pragma unroll
       for (int i = 0; i < KEYS; ++i) {
-        s[i][r] = ex2(s[i][r] - shift);
+        s[i][r] = ex2(exponent(s[i][r] - shift, p.scale_log2));
         if (SHARE == 1 || lane < 32 / SHARE) l[r] += s[i][r];
       }
     }

@@ -36,6 +36,7 @@ struct TcMath {
   static constexpr bool kByRows = true;
   static constexpr int kDim = DP, kRows = kb200::kRows, kOut = DP * kb200::kRows / 32;
   static __device__ __forceinline__ int place(int row, int d) { return d * kb200::kRows + row; }
+  static __device__ __forceinline__ float exponent(float behind, float) { return behind; }       // (maxima are exponents, as MmaMath's)
 };
 
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {

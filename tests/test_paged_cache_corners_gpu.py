@@ -1,8 +1,10 @@
 """The paged K/V cache on the GPU: calls at the corners of what its interface allows."""
 
+import numpy as np
 import pytest
 import torch
 
+from oracle.cache_oracle import Oracle
 from test_paged_cache_gpu import BF16, F16, F32, check, filled, ints
 
 pytestmark = pytest.mark.gpu
@@ -22,3 +24,22 @@ def test_neighbouring_rows_of_one_sequence_that_end_apart(dtype, tokens, rows, k
     again = cache.attend(0, q, counts=ints(counts), slots=ints([0] * rows))
     few = torch.tensor(counts, device="cuda") == 1
     assert behind.numel() > 0 and torch.equal(clean[few], again[few])
+
+
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+@pytest.mark.parametrize("length, tokens, group", [(100, 1, 1), (100, 1, 4), (100, 9, 1), (3000, 1, 2), (3000, 12, 1), (700, 33, 1)])
+def test_float32_scores_far_from_zero_that_lie_close_together(length, tokens, group, head_dim):
+    """Queries of ones and keys of whole numbers: every score is exact in float32 in any order of its sum, 8000 and more after the scale, and a few apart.
+
+    What is left: the scale times log2 e is off by three roundings at most (2^-22), and so is an exponent of at most 5 / ln 2 = 7.3 by 7.3 x 2^-22 and its own
+    rounding of 2^-22, a weight by ln 2 times that, 2^-20 with the 2^-22 of the exponential; once for itself and once for their sum.  Rescaling adds as much again; the
+    sums add (N / 8 + 64) 2^-23."""
+    cache, _ = filled([length], [tokens], dtype=F32, kv_heads=2, head_dim=head_dim)
+    generator = torch.Generator("cuda").manual_seed(6)
+    keys = torch.full(cache.pool[0, 0].shape, 1000.0, device="cuda")
+    keys[..., 0] += torch.randint(0, int(5 * head_dim ** 0.5), keys.shape[:-1], device="cuda", generator=generator)
+    cache.pool[0, 0] = keys
+    got = cache.attend(0, torch.ones(1, tokens, 2 * group, head_dim, device="cuda"))
+    want, weight, _ = Oracle.of(cache).attend(0, torch.ones(1, tokens, 2 * group, head_dim))
+    allowed = weight * (4 * 2.0**-20 + ((length + tokens) / 8 + 64) * 2.0**-23)
+    assert (np.abs(got.cpu().double().numpy() - want) <= allowed).all()
