@@ -89,6 +89,14 @@ __device__ __forceinline__ float to_float(T x) {
   else return __bfloat162float(x);
 }
 
+// 16-bit caches: a maximum of this size is a power of two's exponent that its rounding has moved by up to a half, which all weights of a row share and the division by
+// their sum takes back.  Larger ones (float16 reaches 2^36) could be off by hundreds, and weights overflow; there an exponent is cut at zero, its value at the maximum.
+constexpr float kFarScore = 4194304.0f;
+__device__ __forceinline__ float behind_top(float score, float scale, float shift) {
+  const float e = fmaf(score, scale, shift);
+  return e > 0.0f ? 0.0f : e;                      // (NaN stays)
+}
+
 // Where a warp is: its tile and rows.
 struct Place {
   uint8_t *k, *v;              // the stage
@@ -169,7 +177,8 @@ struct MmaMath {
   static constexpr int NT = G::kKeys / 8, DT = DP / 8;                   // 8-wide column tiles of the scores, of the output rows
   uint32_t q[DP / 16][4];
   float o[DT][4], m[2], l[2];
-  // Maxima are powers of two's exponents: the scale and the maximum go into one multiply-add per score, and a rounding of the maximum cancels.
+  // Maxima are powers of two's exponents: the scale and the maximum go into one multiply-add per score, and a rounding of the maximum cancels.  It is rounded
+  // down, so that the largest weight is not below 1; see kFarScore for where it would be far above.
   static __device__ __forceinline__ float exponent(float behind, float) { return behind; }
 
   template <int ROWS>
@@ -269,7 +278,7 @@ struct MmaMath {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2)) * p.scale_log2;
+      top[h] = __fmul_rd(fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2)), p.scale_log2);
     }
     if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
       float alpha[2];
@@ -287,11 +296,19 @@ struct MmaMath {
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) shift[h] = m[h] == -CUDART_INF_F ? 0.0f : -m[h];          // nothing seen so far: every weight is 2^-inf
+    float scale = p.scale_log2;
+    if (fabsf(shift[0]) > kFarScore || fabsf(shift[1]) > kFarScore) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][j] = behind_top(s[n][j], scale, shift[j >> 1]);
+      scale = 1.0f, shift[0] = shift[1] = 0.0f;
+    }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        s[n][j] = ex2(fmaf(s[n][j], p.scale_log2, shift[j >> 1]));
+        s[n][j] = ex2(fmaf(s[n][j], scale, shift[j >> 1]));
         l[j >> 1] += s[n][j];
       }
 

@@ -43,3 +43,23 @@ def test_float32_scores_far_from_zero_that_lie_close_together(length, tokens, gr
     want, weight, _ = Oracle.of(cache).attend(0, torch.ones(1, tokens, 2 * group, head_dim))
     allowed = weight * (4 * 2.0**-20 + ((length + tokens) / 8 + 64) * 2.0**-23)
     assert (np.abs(got.cpu().double().numpy() - want) <= allowed).all()
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("dtype, tokens, head_dim", [(BF16, 1, 64), (F16, 1, 64), (BF16, 40, 128), (F16, 40, 64), (BF16, 90, 64), (F32, 3, 64), (BF16, 3, 160)])
+def test_scores_beyond_float32_steps_of_one(dtype, tokens, head_dim, sign):
+    """Scores of 2^28 to 2^36, exact and far apart: every row is the value of its largest key, to the bit."""
+    cache, _ = filled([500], [tokens], dtype=dtype, kv_heads=2, head_dim=head_dim)
+    dice = np.random.default_rng(3)
+    ones = torch.from_numpy(dice.choice([1.0, 3.0], head_dim)).cuda()
+    low, high = (2.0**6, 2.0**13) if dtype == F16 else (2.0**16, 2.0**18)
+    at = torch.arange(500 + tokens, device="cuda")
+    pages, rows = cache.table[0, at // 16].long(), at % 16
+    want = []
+    for head in range(2):
+        sizes, top = dice.integers(2, 60, 500 + tokens), int(dice.integers(0, 500))
+        sizes[top] = 64 if sign > 0 else 1
+        cache.pool[0, 0, pages, head, rows] = (torch.from_numpy(sizes).cuda()[:, None] * low * ones).to(dtype)
+        want.append(cache.pool[0, 1, pages[top], head, rows[top]])
+    q = (sign * high * ones).expand(1, tokens, 2, head_dim).to(dtype)
+    assert torch.equal(cache.attend(0, q), torch.stack(want).expand(1, tokens, 2, head_dim))
