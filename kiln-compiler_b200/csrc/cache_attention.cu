@@ -14,7 +14,8 @@
 // measured copy bandwidth.)
 //
 // Scores, maxima, sums and output rows are float32.  16-bit caches: the weights of a tile are rounded to the cache's type for the product with V
-// (half a step, 2^-9 for bfloat16, of every summand; the sum of the weights is kept of the unrounded ones).  float32 caches are not rounded anywhere.
+// (half a step, 2^-9 for bfloat16, of every summand; the largest is 2^12 in float16, so that smaller ones keep their bits too; the sum of the weights is kept of the
+// unrounded ones).  float32 caches are not rounded anywhere.
 #include <algorithm>
 #include <cmath>
 

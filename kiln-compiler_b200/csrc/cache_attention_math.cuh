@@ -90,11 +90,23 @@ __device__ __forceinline__ float to_float(T x) {
 }
 
 // 16-bit caches: a maximum of this size is a power of two's exponent that its rounding has moved by up to a half, which all weights of a row share and the division by
-// their sum takes back.  Larger ones (float16 reaches 2^36) could be off by hundreds, and weights overflow; there an exponent is cut at zero, its value at the maximum.
+// their sum takes back.  Larger ones (float16 reaches 2^36) could be off by hundreds, and weights overflow; there an exponent is cut at its value at the maximum.
 constexpr float kFarScore = 4194304.0f;
+// The exponent of the largest weight.  float16 has 14 powers of two below 1 and 15 above: with a largest weight of 1, weights below 2^-14 would lose bits and those
+// below 2^-25 vanish, and where a first token draws nearly all of the weight and its V is small the result is such weights' (3000 tokens whose scores are 17 behind its:
+// off by 28 times what a rounding to float16 gives).  From 2^12 on it is 2^-26 and 2^-37 of the largest; sums and rows have the same factor, and their division takes it out.
+template <typename T>
+constexpr float kTopExponent = std::is_same<T, __half>::value ? 12.0f : 0.0f;
+template <typename T>
+__device__ __forceinline__ float exponent_of_top(float top, float scale) {
+  const float e = __fmul_rd(top, scale);
+  if constexpr (kTopExponent<T> != 0.0f) return __fadd_rd(e, -kTopExponent<T>);
+  else return e;
+}
+template <typename T>
 __device__ __forceinline__ float behind_top(float score, float scale, float shift) {
   const float e = fmaf(score, scale, shift);
-  return e > 0.0f ? 0.0f : e;                      // (NaN stays)
+  return e > kTopExponent<T> ? kTopExponent<T> : e;        // (NaN stays)
 }
 
 // Where a warp is: its tile and rows.
@@ -178,7 +190,7 @@ struct MmaMath {
   uint32_t q[DP / 16][4];
   float o[DT][4], m[2], l[2];
   // Maxima are powers of two's exponents: the scale and the maximum go into one multiply-add per score, and a rounding of the maximum cancels.  It is rounded
-  // down, so that the largest weight is not below 1; see kFarScore for where it would be far above.
+  // down, so that the largest weight is not below 2^kTopExponent; see kFarScore for where it would be far above.
   static __device__ __forceinline__ float exponent(float behind, float) { return behind; }
 
   template <int ROWS>
@@ -278,7 +290,7 @@ struct MmaMath {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-      top[h] = __fmul_rd(fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2)), p.scale_log2);
+      top[h] = exponent_of_top<T>(fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2)), p.scale_log2);
     }
     if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
       float alpha[2];
@@ -301,7 +313,7 @@ struct MmaMath {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[n][j] = behind_top(s[n][j], scale, shift[j >> 1]);
+        for (int j = 0; j < 4; ++j) s[n][j] = behind_top<T>(s[n][j], scale, shift[j >> 1]);
       scale = 1.0f, shift[0] = shift[1] = 0.0f;
     }
 #pragma unroll

@@ -332,7 +332,7 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
           for (int j = 8; j < 64; j += 8)
 #pragma unroll
             for (int q = 0; q < 4; ++q) top[q] = fmax3(top[q], v[j + 2 * q], v[j + 2 * q + 1]);
-          const float mx = __fmul_rd(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), p.scale_log2);       // (down: see kFarScore)
+          const float mx = exponent_of_top<T>(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), p.scale_log2);
           if (done == 0) {
             m = mx;
           } else if (__any_sync(0xffffffffu, mx > m)) {
@@ -351,7 +351,7 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
           float shift = m == -CUDART_INF_F ? 0.0f : -m, scale = p.scale_log2;          // nothing seen so far: every weight is 2^-inf
           if (fabsf(shift) > kFarScore) {
 #pragma unroll
-            for (int j = 0; j < 64; ++j) v[j] = behind_top(v[j], scale, shift);
+            for (int j = 0; j < 64; ++j) v[j] = behind_top<T>(v[j], scale, shift);
             scale = 1.0f, shift = 0.0f;
           }
           const float2 scale2 = make_float2(scale, scale), shift2 = make_float2(shift, shift);

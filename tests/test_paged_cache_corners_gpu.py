@@ -63,3 +63,18 @@ def test_scores_beyond_float32_steps_of_one(dtype, tokens, head_dim, sign):
         want.append(cache.pool[0, 1, pages[top], head, rows[top]])
     q = (sign * high * ones).expand(1, tokens, 2, head_dim).to(dtype)
     assert torch.equal(cache.attend(0, q), torch.stack(want).expand(1, tokens, 2, head_dim))
+
+
+@pytest.mark.parametrize("gap", [9, 12, 15, 17])
+@pytest.mark.parametrize("dtype, tokens, head_dim", [(F16, 1, 64), (F16, 40, 128), (F16, 90, 64), (F16, 3, 160), (BF16, 1, 64)])
+def test_a_first_token_that_draws_nearly_all_of_the_weight(dtype, tokens, head_dim, gap):
+    """Its V is zero, so that the result is the other tokens', whose weights are e^-gap of its: off by half a step of the type as any (`check`)."""
+    cache, q = filled([3000], [tokens], dtype=dtype, kv_heads=2, head_dim=head_dim)
+    page = cache.table[0, 0].item()
+    q = (q * 0.1).to(dtype)
+    q[..., 0] = 8.0
+    cache.pool[0, 0, :, :, :, 0] = 0.0
+    cache.pool[0, 1] = cache.pool[0, 1].abs()
+    cache.pool[0, 0, page, :, 0, 0] = gap * head_dim**0.5 / 8
+    cache.pool[0, 1, page, :, 0] = 0.0
+    check(cache, q)
