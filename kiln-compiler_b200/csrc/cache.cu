@@ -50,22 +50,23 @@ __device__ __forceinline__ void meet() {
 }
 
 // Exclusive prefix sum over the block's threads; `total` for all.  Shared memory for a value per warp.
-__device__ __forceinline__ int block_scan(int value, int* shared, int* total) {
+template <typename S>
+__device__ __forceinline__ S block_scan(S value, S* shared, S* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  int sum = value;
+  S sum = value;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
-    const int below = __shfl_up_sync(0xffffffffu, sum, d);
+    const S below = __shfl_up_sync(0xffffffffu, sum, d);
     if (lane >= d) sum += below;
   }
   __syncthreads();                       // (the last call's values have been read)
   if (lane == 31) shared[warp] = sum;
   __syncthreads();
   if (warp == 0) {
-    int of_warp = lane < warps ? shared[lane] : 0;
+    S of_warp = lane < warps ? shared[lane] : 0;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
-      const int below = __shfl_up_sync(0xffffffffu, of_warp, d);
+      const S below = __shfl_up_sync(0xffffffffu, of_warp, d);
       if (lane >= d) of_warp += below;
     }
     if (lane < warps) shared[lane] = of_warp;
@@ -182,6 +183,7 @@ __device__ __forceinline__ Span span_of(const CacheView& c, const int32_t* count
 template <bool ONE>
 __global__ void __launch_bounds__(kTableThreads) reserve_kernel(const CacheView c, const int32_t* counts, const Scratch w) {
   __shared__ int shared[32];
+  __shared__ int64_t shared_wide[32];
   pdl_wait();
   pdl_launch_dependents();
   const int rank = ONE ? 0 : blockIdx.x, ranks = ONE ? 1 : gridDim.x, lane = threadIdx.x & 31;
@@ -252,18 +254,19 @@ __global__ void __launch_bounds__(kTableThreads) reserve_kernel(const CacheView 
     if (lane == 0) wanted[s] = n;
   }
   meet<ONE>();
-  // The first CTA says where every sequence's new pages begin.
+  // The first CTA says where every sequence's new pages begin.  (A table of 2^31 entries and more may ask for as many: summed in 64 bits.  Where a sum does not fit in
+  // 32 it is beyond the free pages, and nobody uses it.)
   if (rank == 0) {
-    int base = 0;
+    int64_t base = 0;
     for (int s0 = 0; s0 < c.sequences; s0 += blockDim.x) {
       const int s = s0 + threadIdx.x;
-      const int n = s < c.sequences ? __ldcg(wanted + s) : 0;
-      int total;
-      const int before = block_scan(n, shared, &total);
-      if (s < c.sequences) wanted[s] = base + before;
+      const int64_t n = s < c.sequences ? __ldcg(wanted + s) : 0;
+      int64_t total;
+      const int64_t before = block_scan(n, shared_wide, &total);
+      if (s < c.sequences) wanted[s] = (int)min(base + before, (int64_t)INT_MAX);
       base += total;
     }
-    if (threadIdx.x == 0) w.counters[kWanted] = base;
+    if (threadIdx.x == 0) w.counters[kWanted] = (int)min(base, (int64_t)INT_MAX);
   }
   meet<ONE>();
   const int all = __ldcg(w.counters + kWanted);

@@ -4,8 +4,8 @@ import numpy as np
 import pytest
 import torch
 
-from oracle.cache_oracle import Oracle
-from test_paged_cache_gpu import BF16, F16, F32, check, filled, ints
+from oracle.cache_oracle import NO_PAGES, Oracle
+from test_paged_cache_gpu import BF16, F16, F32, check, faults_of, filled, ints, make
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +78,18 @@ def test_a_first_token_that_draws_nearly_all_of_the_weight(dtype, tokens, head_d
     cache.pool[0, 0, page, :, 0, 0] = gap * head_dim**0.5 / 8
     cache.pool[0, 1, page, :, 0] = 0.0
     check(cache, q)
+
+
+def test_a_reservation_of_two_to_the_31_pages_is_refused():
+    """Every sequence asks for all of its table: 2^31 pages where there are eight."""
+    cache = make(sequences=1 << 15, max_pages=1 << 16, pages=8, head_dim=16, page_tokens=8, fill=0.0)         # 8.6 GB of table, as much of scratch
+    cache.reserve(torch.full((1 << 15,), 1 << 19, dtype=torch.int32, device="cuda"))
+    assert faults_of(cache) == NO_PAGES
+    assert cache.refs.tolist() == [0] * 8 and cache.held.max().item() == 0 and cache.table.max().item() == -1
+    few = torch.zeros(1 << 15, dtype=torch.int32, device="cuda")
+    few[5], few[30000] = 20, 40
+    cache.reserve(few)
+    assert faults_of(cache) == 0 and cache.table[5, :4].tolist() == [0, 1, 2, -1] and cache.table[30000, :6].tolist() == [3, 4, 5, 6, 7, -1]
+    cache.close()
+    del cache
+    torch.cuda.empty_cache()
