@@ -384,10 +384,10 @@ __device__ __forceinline__ int accept_faults(const CacheView& c, const int32_t* 
   const int32_t* const mine = kept + (int64_t)s * width;
   int faults = 0;
   bool moves = false;
-  for (int i = lane; i < n; i += 32) {
+  for (unsigned i = lane; i < (unsigned)n; i += 32) {
     const int at = mine[i], before = i > 0 ? mine[i - 1] : -1;
     faults |= at <= before ? KB200_CACHE_BAD_INDEX : at >= room ? KB200_CACHE_NO_ROOM : 0;
-    moves = moves || at != i;
+    moves = moves || at != (int)i;
   }
   if (__any_sync(0xffffffffu, moves))                                      // what is written has to be the sequence's own
     for (int k = (length >> c.page_log2) + lane; k < held && k <= (int)(((int64_t)length + n - 1) >> c.page_log2); k += 32) {
@@ -417,27 +417,30 @@ __global__ void __launch_bounds__(kCopyThreads) accept_move_kernel(const CacheVi
       if (!cache_page_ok(c, page)) return nullptr;
       return pool + ((((of + page) * c.kv_heads + head) << c.page_log2) + (at & in_page)) * c.row_chunks + chunk;
     };
-    const int chunks = n * c.row_chunks;
-    for (int i0 = 0; i0 < chunks; i0 += 32 * 4) {
-      uint4 v[4];
-      uint4* to[4];
+    // (by 2^20 tokens, whose chunks are a number of 32 bits; those of 2^25 are not)
+    for (int first = 0; first < n; first += 1 << 20) {
+      const int chunks = min(n - first, 1 << 20) * c.row_chunks;
+      for (int i0 = 0; i0 < chunks; i0 += 32 * 4) {
+        uint4 v[4];
+        uint4* to[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = i0 + 32 * j + lane, token = i / c.row_chunks;
-        to[j] = nullptr;
-        if (i < chunks && mine[token] != token) {
-          const uint4* const from = place(mine[token], i - token * c.row_chunks);
-          if (from != nullptr) {
-            v[j] = *from;
-            to[j] = place(token, i - token * c.row_chunks);
+        for (int j = 0; j < 4; ++j) {
+          const int i = i0 + 32 * j + lane, chunk = i % c.row_chunks, token = first + i / c.row_chunks;
+          to[j] = nullptr;
+          if (i < chunks && mine[token] != token) {
+            const uint4* const from = place(mine[token], chunk);
+            if (from != nullptr) {
+              v[j] = *from;
+              to[j] = place(token, chunk);
+            }
           }
         }
-      }
-      __syncwarp();
+        __syncwarp();
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (to[j] != nullptr) *to[j] = v[j];
-      __syncwarp();
+        for (int j = 0; j < 4; ++j)
+          if (to[j] != nullptr) *to[j] = v[j];
+        __syncwarp();
+      }
     }
   }
 }

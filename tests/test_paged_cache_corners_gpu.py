@@ -93,3 +93,24 @@ def test_a_reservation_of_two_to_the_31_pages_is_refused():
     cache.close()
     del cache
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("n, dtype, head_dim", [((1 << 20) + 40, BF16, 16), ((1 << 25) + 8, F32, 256)])
+def test_accepting_millions_of_tokens(n, dtype, head_dim):
+    """The last few of a prompt move; their bytes, 16 at a time, are 2^31 and more in the second case (K and V of 64 GB)."""
+    cache = make(layers=1, max_pages=n // 256 + 2, pages=n // 256 + 2, head_dim=head_dim, page_tokens=256, dtype=dtype, fill=0.0)
+    cache.reserve(ints([n + 3]))
+    at = torch.arange(n - 10, n + 3, device="cuda")
+    pages, rows = cache.table[0, at // 256].long(), at % 256
+    assert faults_of(cache) == 0 and pages.min().item() >= 0
+    cache.pool[0, :, pages, 0, rows] = torch.arange(1.0, 14.0, device="cuda")[None, :, None].expand(2, 13, head_dim).to(dtype)
+    kept = torch.arange(n, dtype=torch.int32, device="cuda")
+    kept[-4:] += 3
+    cache.accept(ints([n]), kept[None])
+    got = cache.pool[0, :, pages[:10], 0, rows[:10]]
+    assert faults_of(cache) == 0 and cache.lengths.tolist() == [n]
+    want = torch.tensor([1.0, 2, 3, 4, 5, 6, 10, 11, 12, 13], device="cuda")[None, :, None].expand(2, 10, head_dim)
+    assert torch.equal(got.float(), want)
+    cache.close()
+    del cache, kept
+    torch.cuda.empty_cache()
