@@ -452,7 +452,8 @@ int kb200_cache_attend(kb200_cache* cache, int layer, const kb200_rows* q, const
                        void* workspace, uint64_t workspace_bytes, void* cuda_stream);
 
 /* After the caller synchronised: 0, or what the operations since the last call left out (KB200_ERR_PAGES where pages
- * were short, else KB200_ERR_BOUNDS; the text names the bits).  A blocking 4-byte copy; clears the status word. */
+ * were short, else KB200_ERR_BOUNDS; the text names the bits).  A blocking 4-byte copy; what it tells is cleared when it
+ * returns. */
 int kb200_cache_status(kb200_cache* cache);
 
 void kb200_cache_destroy(kb200_cache* cache);

@@ -610,6 +610,8 @@ __global__ void __launch_bounds__(kCopyThreads) append_kernel(const CacheView c,
   }
 }
 
+__global__ void told_kernel(int* status, int bits) { atomicAnd(status, ~bits); }
+
 // ---- host --------------------------------------------------------------------------------------
 
 Scratch scratch_of(const Cache& c) { return Scratch{c.stage_rows, c.stage_slot, c.page_a, c.page_b, c.copies, c.counters}; }
@@ -815,7 +817,10 @@ KB200_EXPORT int kb200_cache_status(kb200_cache* handle) {
   int word = 0;
   KB200_CUDA(cudaMemcpy(&word, c.view.status, sizeof(int), cudaMemcpyDeviceToHost));
   if (word == 0) return KB200_OK;
-  KB200_CUDA(cudaMemset(c.view.status, 0, sizeof(int)));
+  // What has been read is cleared and nothing else (calls may be under way), and that is done before this returns: no stream of the caller's waits for this one.
+  told_kernel<<<1, 1, 0, cudaStreamLegacy>>>(c.view.status, word);
+  KB200_CUDA(cudaGetLastError());
+  KB200_CUDA(cudaStreamSynchronize(cudaStreamLegacy));
   if (word & kCacheWaitFault) return fail(KB200_ERR_DEVICE_WAIT, "a bounded device-side wait of kb200_cache_attend ran out");
   return fail(word & KB200_CACHE_NO_PAGES ? KB200_ERR_PAGES : KB200_ERR_BOUNDS, "cache:%s%s%s%s%s",
               word & KB200_CACHE_NO_PAGES ? " fewer free pages than were to be reserved;" : "",

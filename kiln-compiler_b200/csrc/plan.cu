@@ -1515,9 +1515,11 @@ KB200_EXPORT int kb200_plan_status(kb200_plan* p) {
   int word = 0;
   KB200_CUDA(cudaMemcpy(&word, plan.d_status, sizeof(int), cudaMemcpyDeviceToHost));
   if (word != 0) {
-    cudaMemset(plan.d_status, 0, sizeof(int));
+    KB200_CUDA(cudaMemset(plan.d_status, 0, sizeof(int)));
     // a fused attention that gave up may have counted one half of a shared query tile and not the other
     for (PlanKernel& k : plan.kernels) attention_reset_arrivals(k);
+    // (a memset does not wait, and streams that do not wait for the legacy one may launch the plan next)
+    KB200_CUDA(cudaStreamSynchronize(cudaStreamLegacy));
     return fail(KB200_ERR_DEVICE_WAIT, "a bounded device-side wait ran out (code 0x%x: kernel %d, site %d)", word,
                 (word >> 8) & 0xffff, word & 0xff);
   }

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from oracle.cache_oracle import NO_PAGES, Oracle
+from oracle.cache_oracle import BAD_INDEX, NO_PAGES, Oracle
 from test_paged_cache_gpu import BF16, F16, F32, check, faults_of, filled, ints, make
 
 pytestmark = pytest.mark.gpu
@@ -114,3 +114,17 @@ def test_accepting_millions_of_tokens(n, dtype, head_dim):
     cache.close()
     del cache, kept
     torch.cuda.empty_cache()
+
+
+def test_what_calls_on_other_streams_left_out_is_told_once():
+    cache = make(sequences=2, pages=4, fill=0.0)
+    side, wrong, many, fine = torch.cuda.Stream(), ints([5, 0]), ints([128, 0]), ints([0, 0])
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(300):
+            cache.fork(wrong)
+            assert faults_of(cache) == BAD_INDEX
+            cache.reserve(many)
+            assert faults_of(cache) == NO_PAGES
+            cache.reserve(fine)
+            assert faults_of(cache) == 0
