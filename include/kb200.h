@@ -442,7 +442,7 @@ int kb200_cache_accept(kb200_cache* cache, const int32_t* counts, const int32_t*
  * mask[b * mask_stride[0] + i * mask_stride[1] + t * mask_stride[2]] != 0 (bytes; mask NULL: t <= i).  Tokens that a row does not see
  * contribute nothing, whatever they hold.  A row that sees nothing, and rows i >= counts[b], are 0.  One token per sequence is ordinary decoding.
  * scale: from 1e-30 to 1e30.
- * q and out: [rows, tokens, heads, head_dim]; out has the cache's type, q that or float32 (rounded to it); they may be the same tensor.  Products of 16-bit types
+ * q and out: [rows, tokens, heads, head_dim]; out has the cache's type, q that or float32 (rounded to it); they may be the same tensor, or else share no memory.  Products of 16-bit types
  * are summed in float32, the weights rounded to that type in front of V; with a float32 cache all of it is float32.  Results depend on how the call is divided among
  * the SMs (the order of sums), not on what ran before or beside it.
  * workspace: kb200_cache_attend_workspace bytes, 16-byte aligned, used by this call alone until it has run. */

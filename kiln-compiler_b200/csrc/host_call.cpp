@@ -9,6 +9,7 @@
 // launch per kernel.
 #include <Python.h>
 
+#include <ATen/MemoryOverlap.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/clamp.h>
 #include <ATen/cuda/EmptyTensor.h>
@@ -396,6 +397,9 @@ PyObject* cache_attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
       if (out.sizes() != q.t.sizes() || out.scalar_type() != c.type || out.device() != c.device || out.layout() != c10::kStrided || !has_memory(out))
         REFUSE(PyExc_ValueError, "out must be %s of the cache's type on its device", text(q.t.sizes()).c_str());
       if (out.requires_grad()) REFUSE(PyExc_ValueError, "out requires a gradient");
+      // rows are written while others of q are still read: the same tensor is fine, part of it is not
+      if (at::has_internal_overlap(out) == at::MemOverlap::Yes) REFUSE(PyExc_ValueError, "elements of out share memory");
+      if (at::get_overlap_status(out, q.t) == at::MemOverlapStatus::Partial) REFUSE(PyExc_ValueError, "out shares part of q's memory");
     }
     const TokenRows to(out);
     if (rows > 0 && tokens > 0) {

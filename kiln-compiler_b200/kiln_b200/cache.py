@@ -109,7 +109,8 @@ class PagedCache:
         """Attention of the first ``counts[b]`` tokens of every row of ``q`` [rows, tokens, heads, head_dim] over the committed tokens of
         sequence ``slots[b]`` (default: ``b``) and, of the ``counts[b]`` tokens appended behind them, those that ``mask`` ([tokens, tokens]
         or [rows, tokens, tokens], bool; default: itself and those before it) shows.  ``heads`` is a multiple of the cache's; scale defaults to
-        ``head_dim ** -0.5``.  Returns ``out``, of the cache's type, with zeros in rows of no token and in rows that see nothing."""
+        ``head_dim ** -0.5``.  Returns ``out``, of the cache's type, with zeros in rows of no token and in rows that see nothing; it may be ``q``
+        itself, but not share part of its memory."""
         return self._call.cache_attend(self._caller, layer, q, mask, counts, slots, scale, out)
 
     # -- the rest --------------------------------------------------------------------------------

@@ -128,3 +128,19 @@ def test_what_calls_on_other_streams_left_out_is_told_once():
             assert faults_of(cache) == NO_PAGES
             cache.reserve(fine)
             assert faults_of(cache) == 0
+
+
+def test_outputs_that_share_memory_are_refused():
+    cache, q = filled([20, 30], [3, 3], dtype=BF16, kv_heads=2, head_dim=64)
+    one = torch.full((1, 3, 2, 64), 7.0, dtype=BF16, device="cuda")
+    with pytest.raises(ValueError, match="share memory"):
+        cache.attend(0, q, out=one.expand(2, 3, 2, 64))
+    three = torch.full((3, 3, 2, 64), 7.0, dtype=BF16, device="cuda")
+    with pytest.raises(ValueError, match="part of q"):
+        cache.attend(0, three[:2], out=three[1:])
+    assert (one == 7).all() and (three == 7).all()
+    cache.attend(0, three[:2], out=three[:2])                          # the same
+    fused = torch.zeros(2, 3, 6, 64, dtype=BF16, device="cuda")
+    fused[:, :, :2] = q
+    cache.attend(0, fused[:, :, :2], out=fused[:, :, 4:])              # beside each other
+    assert torch.equal(fused[:, :, 4:], cache.attend(0, q)) and (fused[:, :, 2:4] == 0).all() and (three[2] == 7).all()
