@@ -404,6 +404,8 @@ PyObject* cache_attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const TokenRows to(out);
     if (rows > 0 && tokens > 0) {
       const uint64_t bytes = kb200_cache_attend_workspace(c.cache, (int)rows, (int)tokens, (int)heads);
+      // the kernels write into it (said first: it raises for a tensor that may not change)
+      if (args[7] != Py_None && to.t.is_same(out)) out.unsafeGetTensorImpl()->bump_version();
       at::Tensor workspace;                            // (of this call alone; its memory is used again behind the kernels, on their stream)
       if (bytes > 0) workspace = at::detail::empty_cuda({(int64_t)bytes}, c10::kByte, c.device, std::nullopt);
       PyObject* const done = enqueue(c, [&](cudaStream_t s) {
@@ -412,10 +414,9 @@ PyObject* cache_attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
       });
       if (done == nullptr) return nullptr;
       Py_DECREF(done);
-      if (args[7] != Py_None) {
+      if (args[7] != Py_None && !to.t.is_same(out)) {
         const c10::NoGradGuard no_grad;
-        if (!to.t.is_same(out)) out.copy_(to.t);
-        else out.unsafeGetTensorImpl()->bump_version();      // the kernels wrote into it
+        out.copy_(to.t);
       }
     }
     if (args[7] != Py_None) {

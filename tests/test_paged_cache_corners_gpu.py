@@ -144,3 +144,19 @@ def test_outputs_that_share_memory_are_refused():
     fused[:, :, :2] = q
     cache.attend(0, fused[:, :, :2], out=fused[:, :, 4:])              # beside each other
     assert torch.equal(fused[:, :, 4:], cache.attend(0, q)) and (fused[:, :, 2:4] == 0).all() and (three[2] == 7).all()
+
+
+def test_inference_mode():
+    """Calls inside it are as any; a tensor from there is not written to outside of it."""
+    cache, q = filled([20, 30], [3, 3], dtype=BF16, kv_heads=2, head_dim=64)
+    plain = cache.attend(0, q)
+    with torch.inference_mode():
+        out = torch.full((2, 3, 2, 64), 7.0, dtype=BF16, device="cuda")
+        assert torch.equal(cache.attend(0, q), plain) and torch.equal(cache.attend(0, q, out=out.clone()), plain)
+    with pytest.raises(RuntimeError, match="InferenceMode"):
+        cache.attend(0, q, out=out)
+    assert (out == 7).all()
+    mine = torch.zeros(2, 3, 2, 64, dtype=BF16, device="cuda")
+    before = mine._version
+    cache.attend(0, q, out=mine)
+    assert torch.equal(mine, plain) and mine._version == before + 1
