@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from oracle.cache_oracle import BAD_INDEX, NO_PAGES, Oracle
+from oracle.cache_oracle import BAD_INDEX, NO_PAGES, NO_ROOM, Oracle
 from test_paged_cache_gpu import BF16, F16, F32, check, faults_of, filled, ints, make
 
 pytestmark = pytest.mark.gpu
@@ -160,3 +160,33 @@ def test_inference_mode():
     before = mine._version
     cache.attend(0, q, out=mine)
     assert torch.equal(mine, plain) and mine._version == before + 1
+
+
+def test_attention_tells_exactly_what_it_left_out():
+    cache, _ = filled([8, 8, 8], [1, 1, 1], dtype=BF16, kv_heads=1, head_dim=64)
+    q = torch.randn(3, 1, 1, 64, device="cuda")
+    plain = cache.attend(0, q)
+    assert faults_of(cache) == 0
+    for slots in ([0, 7, 2], [0, -1, 2], [0, 2**31 - 1, 2]):
+        out = cache.attend(0, q, slots=ints(slots))
+        assert faults_of(cache) == BAD_INDEX and (out[1] == 0).all() and torch.equal(out[::2], plain[::2])
+    for counts in ([1, -1, 1], [1, 2, 1]):
+        cache.attend(0, q, counts=ints(counts))
+        assert faults_of(cache) == BAD_INDEX
+    cache.lengths[1] = 16                                              # a page's end
+    cache.attend(0, q)
+    assert faults_of(cache) == NO_ROOM
+    cache.lengths[1] = 8
+    cache.table[0, 0] = 10**6
+    cache.attend(0, q[:1])
+    assert faults_of(cache) == BAD_INDEX
+    cache.fork(ints([0, 0, 2]))
+    cache.truncate(ints([4, 4, 4]))
+    cache.compact()
+    assert faults_of(cache) == 0
+
+
+@pytest.mark.parametrize("dtype, head_dim, page_tokens", [(F32, 64, 256), (BF16, 64, 16), (F16, 128, 256), (F32, 256, 256), (BF16, 256, 128)])
+def test_prompts_in_pieces_of_hundreds_of_tokens(dtype, head_dim, page_tokens):
+    cache, q = filled([0, 33, 5], [700, 513, 1], dtype=dtype, kv_heads=1, head_dim=head_dim, page_tokens=page_tokens)
+    check(cache, q.to(dtype), None, [700, 513, 1])
