@@ -434,7 +434,7 @@ int kb200_cache_append(kb200_cache* cache, int layer, const kb200_rows* k, const
 
 /* Commits counts[s] of the tokens drafted behind each sequence: those with the ascending indexes kept[s * kept_width + i], which
  * are moved together in all layers (kept NULL: the first ones, which stay where they are), and frees the pages behind them.
- * A sequence whose entries are not ascending, or have no pages, or would move within shared pages, stays as it is. */
+ * A sequence whose entries are not ascending, or have no pages, or would move within pages that were shared before the call, stays as it is. */
 int kb200_cache_accept(kb200_cache* cache, const int32_t* counts, const int32_t* kept, int kept_width, void* cuda_stream);
 
 /* Attention of drafted tokens: out[b, i, h] = sum_j softmax_j(scale * q[b, i, h] . k[j, g]) v[j, g], g = h * kv_heads / heads, over

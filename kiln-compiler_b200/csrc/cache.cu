@@ -373,7 +373,8 @@ __global__ void __launch_bounds__(kSlotThreads) truncate_kernel(const CacheView 
 
 // ---- accepted tokens ---------------------------------------------------------------------------
 
-// Can a sequence's entries be followed?  By a warp; says the same in the kernel that moves and the one that commits.
+// Can a sequence's entries be followed?  By a warp, while nobody changes how many hold a page: what moves is committed by the answer that the moving launch got, since
+// in the committing one other sequences give their pages back.
 __device__ __forceinline__ int accept_faults(const CacheView& c, const int32_t* counts, const int32_t* kept, int width, int s) {
   const int lane = threadIdx.x & 31, n = counts[s];
   if (n < 0 || (kept != nullptr && n > width)) return KB200_CACHE_BAD_INDEX;
@@ -399,7 +400,7 @@ __device__ __forceinline__ int accept_faults(const CacheView& c, const int32_t* 
 
 // A warp moves one sequence's tokens in one layer, head and of K or V.  Row i comes from row kept[i] >= i: batches ascend, and a batch is
 // read before any of it is written, so nothing is overwritten that is still to be read.
-__global__ void __launch_bounds__(kCopyThreads) accept_move_kernel(const CacheView c, const int32_t* counts, const int32_t* kept, int width) {
+__global__ void __launch_bounds__(kCopyThreads) accept_move_kernel(const CacheView c, const int32_t* counts, const int32_t* kept, int width, int32_t* answers) {
   pdl_wait();
   pdl_launch_dependents();
   const int64_t planes = (int64_t)c.layers * 2 * c.kv_heads, units = planes * c.sequences;
@@ -407,8 +408,9 @@ __global__ void __launch_bounds__(kCopyThreads) accept_move_kernel(const CacheVi
   uint4* const pool = static_cast<uint4*>(c.pool);
   for (int64_t u = (int64_t)blockIdx.x * (kCopyThreads / 32) + (threadIdx.x >> 5); u < units; u += (int64_t)gridDim.x * (kCopyThreads / 32)) {
     const int s = (int)(u / planes);
-    const int n = counts[s];
-    if (n <= 0 || accept_faults(c, counts, kept, width, s) != 0) continue;
+    const int n = counts[s], faults = accept_faults(c, counts, kept, width, s);
+    if (lane == 0 && u % planes == 0) answers[s] = faults;
+    if (n <= 0 || faults != 0) continue;
     const int64_t plane = u % planes, of = plane / c.kv_heads * c.pages;
     const int head = (int)(plane % c.kv_heads), length = max(c.lengths[s], 0);
     const int32_t *const mine = kept + (int64_t)s * width, *const row = c.table + (int64_t)s * c.max_pages;
@@ -445,12 +447,13 @@ __global__ void __launch_bounds__(kCopyThreads) accept_move_kernel(const CacheVi
   }
 }
 
-__global__ void __launch_bounds__(kSlotThreads) accept_commit_kernel(const CacheView c, const int32_t* counts, const int32_t* kept, int width) {
+// answers: of the moving launch; null: nothing moves, and a sequence's own numbers say all.
+__global__ void __launch_bounds__(kSlotThreads) accept_commit_kernel(const CacheView c, const int32_t* counts, const int32_t* kept, int width, const int32_t* answers) {
   pdl_wait();
   pdl_launch_dependents();
   const int s = blockIdx.x * (kSlotThreads / 32) + (threadIdx.x >> 5);
   if (s >= c.sequences) return;
-  const int faults = accept_faults(c, counts, kept, width, s);
+  const int faults = answers != nullptr ? answers[s] : accept_faults(c, counts, kept, width, s);
   if (faults != 0) {
     if ((threadIdx.x & 31) == 0) cache_fault(c, faults);
     return;
@@ -799,13 +802,14 @@ KB200_EXPORT int kb200_cache_accept(kb200_cache* handle, const int32_t* counts, 
   KB200_CACHE_ENTER("kb200_cache_accept");
   if (counts == nullptr) return fail(KB200_ERR_ARGUMENT, "kb200_cache_accept: counts is null");
   if (kept != nullptr && width < 0) return fail(KB200_ERR_ARGUMENT, "kb200_cache_accept: kept is %d wide", width);
-  if (kept != nullptr && width > 0) {
+  int32_t* const answers = kept != nullptr && width > 0 ? c.stage_slot : nullptr;
+  if (answers != nullptr) {
     const int64_t units = c.planes() * c.view.sequences;
     const int grid = (int)std::min<int64_t>((units + kCopyThreads / 32 - 1) / (kCopyThreads / 32), copy_grid(c));
-    KB200_CUDA(launch_kernel(true, accept_move_kernel, dim3(grid), dim3(kCopyThreads), 0, s, c.view, counts, kept, width));
+    KB200_CUDA(launch_kernel(true, accept_move_kernel, dim3(grid), dim3(kCopyThreads), 0, s, c.view, counts, kept, width, answers));
   }
   const int per = kSlotThreads / 32;
-  KB200_CUDA(launch_kernel(true, accept_commit_kernel, dim3((c.view.sequences + per - 1) / per), dim3(kSlotThreads), 0, s, c.view, counts, kept, width));
+  KB200_CUDA(launch_kernel(true, accept_commit_kernel, dim3((c.view.sequences + per - 1) / per), dim3(kSlotThreads), 0, s, c.view, counts, kept, width, answers));
   return KB200_OK;
 }
 

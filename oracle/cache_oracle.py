@@ -121,13 +121,14 @@ class Oracle:
                 self.pool[layer, 0, page, :, row], self.pool[layer, 1, page, :, row] = k[b, i], v[b, i]
 
     def accept(self, counts, kept=None):
+        refs = list(self.refs)                 # pages are shared or not as they were before the call
         for s, n in enumerate(counts):
             mine = list(range(max(n, 0))) if kept is None else list(kept[s])[:max(n, 0)]
             room = len(self.rows[s]) * self.P - self.lengths[s]
             fault = BAD_INDEX if n < 0 or len(mine) < n or any(b <= a for a, b in zip([-1] + mine, mine)) else 0
             fault |= NO_ROOM if any(x >= room for x in mine) else 0
             if not fault and any(i != x for i, x in enumerate(mine)):
-                fault = SHARED if any(self.refs[self._place(s, self.lengths[s] + i)[0]] > 1 for i in range(n)) else 0
+                fault = SHARED if any(refs[self._place(s, self.lengths[s] + i)[0]] > 1 for i in range(n)) else 0
             if fault:
                 self.faults |= fault
                 continue

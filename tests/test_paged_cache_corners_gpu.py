@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from oracle.cache_oracle import BAD_INDEX, NO_PAGES, NO_ROOM, Oracle
+from oracle.cache_oracle import BAD_INDEX, NO_PAGES, NO_ROOM, SHARED, Oracle
 from test_paged_cache_gpu import BF16, F16, F32, check, faults_of, filled, ints, make
 
 pytestmark = pytest.mark.gpu
@@ -190,3 +190,27 @@ def test_attention_tells_exactly_what_it_left_out():
 def test_prompts_in_pieces_of_hundreds_of_tokens(dtype, head_dim, page_tokens):
     cache, q = filled([0, 33, 5], [700, 513, 1], dtype=dtype, kv_heads=1, head_dim=head_dim, page_tokens=page_tokens)
     check(cache, q.to(dtype), None, [700, 513, 1])
+
+
+@pytest.mark.parametrize("sequences", [64, 256])
+@pytest.mark.parametrize("first", [0, 1])
+def test_tokens_in_shared_pages_stay_while_the_other_holder_leaves(sequences, first):
+    """Pairs share a page of drafted tokens; one of each accepts a token that would move, the other gives the page back in the same call."""
+    cache = make(sequences=sequences, pages=sequences, max_pages=2, fill=0.0)
+    one = torch.arange(sequences, device="cuda", dtype=torch.int32) % 2 == first
+    cache.reserve(5 * one.int())
+    k = torch.randn(sequences, 5, 1, 64, device="cuda")
+    cache.append(0, k, k, 5 * one.int())
+    both = torch.arange(sequences, device="cuda", dtype=torch.int32) // 2 * 2 + first
+    kept = torch.full((sequences, 1), 3, dtype=torch.int32, device="cuda")
+    table, pool = cache.table.clone(), cache.pool.clone()
+    for _ in range(20):
+        cache.fork(both)
+        assert faults_of(cache) == 0 and cache.refs.max().item() == 2
+        cache.accept(one.int(), kept)
+        assert faults_of(cache) == SHARED
+        assert cache.lengths.max().item() == 0 and torch.equal(cache.table, table) and torch.equal(cache.pool, pool)
+    cache.accept(one.int(), kept)                                      # now they are alone
+    assert faults_of(cache) == 0 and torch.equal(cache.lengths, one.int())
+    page = cache.table[one, 0].long()
+    assert torch.equal(cache.pool[0, 0, page, 0, 0], k[one, 3, 0].to(BF16))
