@@ -428,7 +428,8 @@ int kb200_cache_truncate(kb200_cache* cache, const int32_t* lengths, void* cuda_
 int kb200_cache_compact(kb200_cache* cache, void* cuda_stream);
 
 /* Writes K and V of new tokens of one layer: token i < counts[b] of batch row b goes to position lengths[slots[b]] + i.
- * counts NULL: all `tokens`; slots NULL: row b is sequence b.  Needs room (kb200_cache_reserve). */
+ * counts NULL: all `tokens`; slots NULL: row b is sequence b.  Needs room (kb200_cache_reserve).  No sequence twice, rows of no token
+ * included; 2^30 rows at most. */
 int kb200_cache_append(kb200_cache* cache, int layer, const kb200_rows* k, const kb200_rows* v, int rows, int tokens,
                        const int32_t* counts, const int32_t* slots, void* cuda_stream);
 
@@ -441,7 +442,7 @@ int kb200_cache_accept(kb200_cache* cache, const int32_t* counts, const int32_t*
  * the committed tokens j of sequence slots[b] and over the drafted ones t < counts[b] behind them with
  * mask[b * mask_stride[0] + i * mask_stride[1] + t * mask_stride[2]] != 0 (bytes; mask NULL: t <= i).  Tokens that a row does not see
  * contribute nothing, whatever they hold.  A row that sees nothing, and rows i >= counts[b], are 0.  One token per sequence is ordinary decoding.
- * scale: from 1e-30 to 1e30.
+ * scale: from 1e-30 to 1e30.  rows * tokens and 16-byte chunks of a token's heads: 2^30 each at most; tokens * heads / kv_heads: below 2^24.
  * q and out: [rows, tokens, heads, head_dim]; out has the cache's type, q that or float32 (rounded to it); they may be the same tensor, or else share no memory.  Products of 16-bit types
  * are summed in float32, the weights rounded to that type in front of V; with a float32 cache all of it is float32.  Results depend on how the call is divided among
  * the SMs (the order of sums), not on what ran before or beside it.

@@ -781,7 +781,7 @@ KB200_EXPORT int kb200_cache_append(kb200_cache* handle, int layer, const kb200_
                                     const int32_t* counts, const int32_t* slots, void* stream) {
   KB200_CACHE_ENTER("kb200_cache_append");
   if (layer < 0 || layer >= c.view.layers) return fail(KB200_ERR_ARGUMENT, "kb200_cache_append: layer %d of %d", layer, c.view.layers);
-  if (rows < 0 || tokens < 0 || (slots == nullptr && rows > c.view.sequences))
+  if (rows < 0 || rows > (1 << 30) || tokens < 0 || (slots == nullptr && rows > c.view.sequences))
     return fail(KB200_ERR_ARGUMENT, "kb200_cache_append: %d rows of %d tokens for %d sequences", rows, tokens, c.view.sequences);
   if (rows == 0 || tokens == 0) return KB200_OK;
   if (!rows_ok(c, k, c.view.kv_heads) || !rows_ok(c, v, c.view.kv_heads) || k->dtype != v->dtype)

@@ -243,9 +243,10 @@ uint64_t workspace_of(const Variant& v, const Division& d) {
 
 Cache* cache_of(const kb200_cache* c) { return reinterpret_cast<Cache*>(const_cast<kb200_cache*>(c)); }
 
+// (The kernels count batch rows, and 16-byte chunks of a row's heads, in 32 bits, and go beyond the last by a step.)
 bool call_ok(const Cache& c, int rows, int tokens, int heads) {
   return rows >= 0 && tokens >= 0 && heads >= 1 && heads % c.view.kv_heads == 0 && (int64_t)tokens * (heads / c.view.kv_heads) < (1 << 24) &&
-         (int64_t)rows * std::max(tokens, 1) < ((int64_t)1 << 31);
+         (int64_t)rows * std::max(tokens, 1) <= (1 << 30) && (int64_t)heads * c.view.row_chunks <= (1 << 30);
 }
 
 }  // namespace

@@ -97,7 +97,7 @@ class PagedCache:
 
     def append(self, layer, k, v, counts=None, slots=None):
         """Writes K and V of the first ``counts[b]`` tokens of every row of ``k`` and ``v`` [rows, tokens, kv_heads, head_dim] behind
-        the committed tokens of sequence ``slots[b]`` (default: ``b``), in the cache's type."""
+        the committed tokens of sequence ``slots[b]`` (default: ``b``; none twice, rows of no token included), in the cache's type."""
         self._call.cache_append(self._caller, layer, k, v, counts, slots)
 
     def accept(self, counts, kept=None):

@@ -1,9 +1,12 @@
 """The paged K/V cache on the GPU: calls at the corners of what its interface allows."""
 
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
 
+from kiln_b200 import _cabi
 from oracle.cache_oracle import BAD_INDEX, NO_PAGES, NO_ROOM, SHARED, Oracle
 from test_paged_cache_gpu import BF16, F16, F32, check, faults_of, filled, ints, make
 
@@ -214,3 +217,19 @@ def test_tokens_in_shared_pages_stay_while_the_other_holder_leaves(sequences, fi
     assert faults_of(cache) == 0 and torch.equal(cache.lengths, one.int())
     page = cache.table[one, 0].long()
     assert torch.equal(cache.pool[0, 0, page, 0, 0], k[one, 3, 0].to(BF16))
+
+
+def test_calls_of_more_rows_than_are_counted_are_refused():
+    """Nothing is launched for them: tensors of stride 0 would describe such rows in a few bytes."""
+    cache = make(sequences=2, pages=4, fill=0.0)
+    lib, x = _cabi.load(), torch.zeros(64, dtype=BF16, device="cuda")
+    rows = lambda heads: C.byref(_cabi.Rows(x.data_ptr(), 1, heads, (0, 0, 0)))  # noqa: E731
+    slots = ints([0, 1]).data_ptr()
+    for n in ((1 << 30) + 1, (1 << 31) - 1):
+        assert lib.kb200_cache_append(cache._cache, 0, rows(1), rows(1), n, 1, None, slots, None) == -1
+        assert lib.kb200_cache_attend(cache._cache, 0, rows(1), rows(1), n, 1, None, None, None, slots, 1.0, None, 0, None) == -1
+        assert lib.kb200_cache_attend_workspace(cache._cache, n, 1, 1) == 0
+    assert lib.kb200_cache_attend(cache._cache, 0, rows(1), rows(1), 1 << 20, 1025, None, None, None, slots, 1.0, None, 0, None) == -1
+    many = make(kv_heads=128, pages=1, fill=0.0)                       # 2^31 chunks to a token
+    assert lib.kb200_cache_attend(many._cache, 0, rows(1 << 28), rows(1 << 28), 1, 1, None, None, None, slots, 1.0, None, 0, None) == -1
+    assert faults_of(cache) == 0
