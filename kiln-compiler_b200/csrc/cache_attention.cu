@@ -10,7 +10,7 @@
 // warps' sums are joined at the end of an item only.  Every stage of the ring belongs to one warp (or the group of warps with the other rows
 // of the row tile), which therefore sees each of its fillings: a barrier's parity tells no more than the last one.  (With the tile's keys divided among the
 // warps, and copies issued by them, a warp paid the rescaling, the shuffles and the addresses for 16 keys instead of 64: 985 instructions per warp and tile at 5.8 cycles each, two warps to
-// a scheduler, 187 us for 32 sequences of up to 8192 tokens in BF16, 52 % of the bandwidth; now 108, 0.89 of the
+// a scheduler, 187 us for 32 sequences of up to 8192 tokens in BF16, 52 % of the bandwidth; now 110, 0.88 of the
 // measured copy bandwidth.)
 //
 // Scores, maxima, sums and output rows are float32.  16-bit caches: the weights of a tile are rounded to the cache's type for the product with V
