@@ -35,7 +35,7 @@
 extern "C" {
 #endif
 
-#define KB200_ABI_VERSION 6
+#define KB200_ABI_VERSION 7
 
 #define KB200_MAX_RANK 6      /* iteration dims after the host collapsed contiguous ones */
 #define KB200_MAX_OPERANDS 12 /* distinct tensors one fused kernel touches */
@@ -397,9 +397,11 @@ typedef struct kb200_rows {
 typedef enum kb200_cache_fault {
   KB200_CACHE_NO_PAGES = 1,   /* kb200_cache_reserve: fewer free pages than needed; nothing was reserved */
   KB200_CACHE_TOO_LONG = 2,   /* ... a sequence would need more than max_pages; nothing was reserved */
-  KB200_CACHE_BAD_INDEX = 4,  /* a sequence, count, kept token or page out of range, a sequence given twice to kb200_cache_append */
+  KB200_CACHE_BAD_INDEX = 4,  /* a sequence, count, kept token or page out of range, a sequence given twice to kb200_cache_append,
+                                 kb200_cache_weigh or kb200_cache_verify, a temperature that is negative or not finite */
   KB200_CACHE_NO_ROOM = 8,    /* a token's position has no page (see kb200_cache_reserve) */
-  KB200_CACHE_SHARED = 16     /* a write into a page that another sequence holds as well */
+  KB200_CACHE_SHARED = 16,    /* a write into a page that another sequence holds as well */
+  KB200_CACHE_BAD_VALUE = 32  /* kb200_cache_verify: logits of an accepted token that are no distribution (NaN, +inf, all -inf) */
 } kb200_cache_fault;
 
 /* Whether kb200_cache_create takes the description; needs no GPU. */
@@ -451,6 +453,66 @@ uint64_t kb200_cache_attend_workspace(const kb200_cache* cache, int rows, int to
 int kb200_cache_attend(kb200_cache* cache, int layer, const kb200_rows* q, const kb200_rows* out, int rows, int tokens,
                        const uint8_t* mask, const int64_t* mask_stride, const int32_t* counts, const int32_t* slots, float scale,
                        void* workspace, uint64_t workspace_bytes, void* cuda_stream);
+
+/* kb200_cache_attend to a sliding window and a few first tokens, with the logarithms of the rows' sums.  Token i of a batch row stands `place` behind the committed
+ * ones: places[b * tokens + i], or i where places is NULL (the depth in a tree, for masks of trees).  Of the committed tokens j it sees those with
+ * j < sinks or j > lengths + place - window.  Of the drafted ones it sees what `mask` shows, whatever the window is; with mask NULL those t <= i that are
+ * in the window or among the first `sinks` tokens in the same way.  window: 1 or more, 0: all tokens (sinks and places then change nothing).
+ * Pages of which no row sees a token may be missing from the table (kb200_cache_release).
+ * lse: NULL, or [rows, tokens, heads] by strides: log sum_j exp(scale * q k[j]) over the tokens that the row sees, -inf for rows that see nothing and rows i >= counts[b]. */
+uint64_t kb200_cache_attend_window_workspace(const kb200_cache* cache, int rows, int tokens, int heads, int window, int sinks);
+int kb200_cache_attend_window(kb200_cache* cache, int layer, const kb200_rows* q, const kb200_rows* out, int rows, int tokens,
+                              const uint8_t* mask, const int64_t* mask_stride, const int32_t* counts, const int32_t* slots, float scale,
+                              int window, int sinks, const int32_t* places, float* lse, const int64_t* lse_stride,
+                              void* workspace, uint64_t workspace_bytes, void* cuda_stream);
+
+/* Gives back the pages that a window has left: those of which every token j has j >= sinks and j <= lengths[s] - window, so that no token to come sees it (places of 0
+ * and more).  Their entries become -1; held and lengths stay.  What reads them afterwards (a larger window, kb200_cache_attend) is told KB200_CACHE_BAD_INDEX. */
+int kb200_cache_release(kb200_cache* cache, int window, int sinks, void* cuda_stream);
+
+/* The weight that the tokens of a sequence draw: out[s, j] = weights[s, j] + sum over i < counts[b] and heads h of exp(scale * q[b, i, h] . k[j, g] - lse[b, i, h]) for the tokens
+ * j that token i of batch row b (s = slots[b]) sees, as in kb200_cache_attend, whose lse makes them its weights.  Rows whose lse is -inf add nothing.  All other entries of out
+ * are weights'.  weights and out: float32 [sequences, max_pages * page_tokens], a row `stride` elements behind the last; weights NULL: zeros; out may be weights.
+ * No sequence twice.  Sums are float32; every key's are taken in the same order in every call. */
+int kb200_cache_weigh(kb200_cache* cache, int layer, const kb200_rows* q, const float* lse, const int64_t* lse_stride, int rows, int tokens,
+                      const uint8_t* mask, const int64_t* mask_stride, const int32_t* counts, const int32_t* slots, float scale,
+                      const float* weights, int64_t weights_stride, float* out, int64_t out_stride, void* cuda_stream);
+
+/* Keeps keep[s] of every sequence's committed tokens and drops the others, in all layers: the first `sinks`, of the rest the last `recent`, and of what then lacks the heaviest
+ * by weights[s] (of equal ones the first; NaN is heaviest); fewer than the first and last ones where keep[s] is less.  They keep their order and become the sequence's first keep[s]
+ * tokens; the pages behind them are free, what was reserved too.  A negative entry, or one of lengths[s] and more, leaves the sequence as it is.
+ * out[s]: the weights of the tokens that the sequence then has, zeros behind them.  weights and out: as in kb200_cache_weigh; out may be weights.
+ * A sequence whose tokens would move within pages that were shared before the call, or from pages that it does not have, stays as it is.
+ * workspace: kb200_cache_evict_workspace bytes, 16-byte aligned, used by this call alone until it has run. */
+uint64_t kb200_cache_evict_workspace(const kb200_cache* cache);
+int kb200_cache_evict(kb200_cache* cache, const float* weights, int64_t weights_stride, const int32_t* keep, int recent, int sinks,
+                      float* out, int64_t out_stride, void* workspace, uint64_t workspace_bytes, void* cuda_stream);
+
+/* Rows over a vocabulary, [batch, tokens, vocabulary] with the last contiguous; strides in elements. */
+typedef struct kb200_scores {
+  const void* data;
+  int32_t dtype;        /* kb200_dtype */
+  int32_t pad;
+  int64_t stride[2];
+} kb200_scores;
+
+/* Which drafted tokens the model accepts, and the token that follows them, by given random numbers: what is returned is distributed as the model's own samples.
+ *   drafted [rows, tokens]: token i < counts[b] of a batch row, as appended behind sequence slots[b].  Token 0 is not in question (it followed the last step).
+ *   parents [rows, tokens] by parents_stride: the token i that each one follows, smaller than itself (NULL: a chain); -1: none, it is never asked for.
+ *   logits: the model's of what follows each token.  p_i = softmax(logits[b, i] / temperature[b]); temperature 0: all of it on the largest logit (the first of equal ones);
+ *     NULL: 1.
+ *   draft: the probabilities by which the tokens that follow token i were drawn, each for itself; NULL (and for temperature 0): they were chosen without chance.
+ *   uniform [rows, tokens]: numbers from [0, 1), one for each drafted token and, in place 0, one for the token that follows.
+ * From a = 0 on, with r = p_a and R = 1, the tokens c that follow a are asked for in their order.  With x = drafted[b, c], c is accepted if
+ * uniform[b, c] * draft[b, a, x] * R < r(x) (without draft: uniform[b, c] * R < r(x)); then it takes a's place.  If not, r becomes max(r / R - draft[b, a], 0) (without: r(x)
+ * becomes 0) and R its sum, unless that is 0.  In the end following[s] is the first v at which r, summed up, exceeds uniform[b, 0] times its sum.
+ * n_accepted [sequences], accepted [sequences, tokens] (-1 behind): as kb200_cache_accept takes them; sequences without a row, or with counts[b] 0: 0, and -1 in following.
+ * Numbers are compared as if computed in float64.  If the logits of an accepted token are no distribution the row ends there, with -1 in following.  tokens: 512 at most.
+ * workspace: kb200_cache_verify_workspace bytes, 16-byte aligned, used by this call alone until it has run. */
+uint64_t kb200_cache_verify_workspace(const kb200_cache* cache, int rows, int tokens, int vocab);
+int kb200_cache_verify(kb200_cache* cache, const kb200_scores* logits, const kb200_scores* draft, int rows, int tokens, int vocab, const int32_t* drafted,
+                       const int32_t* parents, int64_t parents_stride, const float* uniform, const float* temperature, const int32_t* counts, const int32_t* slots,
+                       int32_t* n_accepted, int32_t* accepted, int32_t* following, void* workspace, uint64_t workspace_bytes, void* cuda_stream);
 
 /* After the caller synchronised: 0, or what the operations since the last call left out (KB200_ERR_PAGES where pages
  * were short, else KB200_ERR_BOUNDS; the text names the bits).  A blocking 4-byte copy; what it tells is cleared when it

@@ -345,22 +345,6 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const CacheVie
 
 // ---- freeing -----------------------------------------------------------------------------------
 
-// Sets a sequence's length and gives back the pages behind it.  By a warp.
-__device__ __forceinline__ void cut(const CacheView& c, int s, int length) {
-  const int lane = threadIdx.x & 31, held = min(max(c.held[s], 0), c.max_pages);
-  const int keep = (int)(((int64_t)length + (1 << c.page_log2) - 1) >> c.page_log2);
-  for (int k = keep + lane; k < held; k += 32) {
-    int32_t* const entry = c.table + (int64_t)s * c.max_pages + k;
-    if (cache_page_ok(c, *entry)) atomicSub(c.refs + *entry, 1);
-    *entry = -1;
-  }
-  __syncwarp();
-  if (lane == 0) {
-    c.lengths[s] = length;
-    c.held[s] = min(held, keep);
-  }
-}
-
 constexpr int kSlotThreads = 128;
 
 __global__ void __launch_bounds__(kSlotThreads) truncate_kernel(const CacheView c, const int32_t* lengths) {
@@ -641,8 +625,6 @@ cudaError_t launch_tables(const Cache& c, void (*one)(KArgs...), void (*cluster)
 
 int copy_grid(const Cache& c) { return c.sm_count * 8; }
 
-Cache* cache_of(kb200_cache* c) { return reinterpret_cast<Cache*>(c); }
-
 bool rows_ok(const Cache& c, const kb200_rows* r, int heads) {
   if (r == nullptr || r->data == nullptr || !tc::aligned16(r->data) || r->heads != heads || (r->dtype != c.dtype && r->dtype != KB200_DTYPE_FP32)) return false;
   const int per16 = r->dtype == KB200_DTYPE_FP32 ? 4 : 8;
@@ -734,13 +716,6 @@ KB200_EXPORT int kb200_cache_create(const kb200_cache_desc* d, int device, kb200
   return KB200_OK;
 }
 
-#define KB200_CACHE_ENTER(name)                                                       \
-  if (handle == nullptr) return fail(KB200_ERR_ARGUMENT, name ": cache is null");     \
-  Cache& c = *cache_of(handle);                                                       \
-  const DeviceGuard guard(c.device);                                                  \
-  if (guard.error != cudaSuccess) return cuda_fail(guard.error, name);                \
-  const cudaStream_t s = static_cast<cudaStream_t>(stream)
-
 KB200_EXPORT int kb200_cache_fork(kb200_cache* handle, const int32_t* sources, void* stream) {
   KB200_CACHE_ENTER("kb200_cache_fork");
   if (sources == nullptr) return fail(KB200_ERR_ARGUMENT, "kb200_cache_fork: sources is null");
@@ -826,12 +801,12 @@ KB200_EXPORT int kb200_cache_status(kb200_cache* handle) {
   KB200_CUDA(cudaGetLastError());
   KB200_CUDA(cudaStreamSynchronize(cudaStreamLegacy));
   if (word & kCacheWaitFault) return fail(KB200_ERR_DEVICE_WAIT, "a bounded device-side wait of kb200_cache_attend ran out");
-  return fail(word & KB200_CACHE_NO_PAGES ? KB200_ERR_PAGES : KB200_ERR_BOUNDS, "cache:%s%s%s%s%s",
+  return fail(word & KB200_CACHE_NO_PAGES ? KB200_ERR_PAGES : KB200_ERR_BOUNDS, "cache:%s%s%s%s%s%s",
               word & KB200_CACHE_NO_PAGES ? " fewer free pages than were to be reserved;" : "",
               word & KB200_CACHE_TOO_LONG ? " a sequence would need more than max_pages;" : "",
               word & KB200_CACHE_BAD_INDEX ? " an index or a count out of range;" : "",
               word & KB200_CACHE_NO_ROOM ? " tokens without a page;" : "",
-              word & KB200_CACHE_SHARED ? " a write into a shared page;" : "");
+              word & KB200_CACHE_SHARED ? " a write into a shared page;" : "", word & KB200_CACHE_BAD_VALUE ? " logits that are no distribution;" : "");
 }
 
 KB200_EXPORT void kb200_cache_destroy(kb200_cache* handle) {

@@ -16,6 +16,10 @@
 // Scores, maxima, sums and output rows are float32.  16-bit caches: the weights of a tile are rounded to the cache's type for the product with V
 // (half a step, 2^-9 for bfloat16, of every summand; the largest is 2^12 in float16, so that smaller ones keep their bits too; the sum of the weights is kept of the
 // unrounded ones).  float32 caches are not rounded anywhere.
+//
+// WINDOW: the kernels with a window (kb200_cache_attend_window), which cache_attention_window.cu compiles from the same text.
+#include <limits.h>
+
 #include <algorithm>
 #include <cmath>
 
@@ -48,7 +52,7 @@ struct Shape {
   static constexpr int kRows = Math::kRows * RG;                         // of a row tile
 };
 
-template <typename Math, int RG>
+template <typename Math, int RG, bool WINDOW>
 __global__ void __launch_bounds__(Shape<Math, RG>::kThreads, 1)
 cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CacheAttnParams p) {
   using Z = Shape<Math, RG>;
@@ -76,7 +80,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
   pdl_wait();
   pdl_launch_dependents();
   CacheRun run;
-  const bool any = find_run<ROWS, TILE, Z::kThreads>(p, blockIdx.x, found, &run);       // (a barrier for all that is above, too)
+  const bool any = find_run<ROWS, TILE, Z::kThreads, WINDOW>(p, blockIdx.x, found, &run);       // (a barrier for all that is above, too)
   CacheCursor& now = run.at;
   volatile int* const abort_ptr = &gave_up;
   // A wait that ends for all lanes of a warp or none.  Where it runs out the warps do no more work, but meet each other as if they did.
@@ -84,7 +88,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
 
   if (warp == Z::kWarps) {
     if (lane == 0) leave_join<ROWS>(p, any, run);
-    if (any) bring_tiles<T, Math::kDim, ROWS, Z::kStages>(map, p, run, stage0, full, empty, wait);
+    if (any) bring_tiles<T, Math::kDim, ROWS, Z::kStages, WINDOW>(map, p, run, stage0, full, empty, wait);
   } else {
     // ---------------- consumers ----------------
     const int row_group = warp % RG, key_group = warp / RG;
@@ -93,7 +97,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
     auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(32 * Z::kWarps) : "memory"); };
 
     Math math;
-    Place at{nullptr, nullptr, 0, 0, row_group * Math::kRows, 0, warp, lane, row_group, key_group};
+    Place at{nullptr, nullptr, 0, 0, row_group * Math::kRows, 0, 0, warp, lane, row_group, key_group};
 
     // The end of an item, or of the run inside one: the warps' sums, then the rows or a part.  `order`: this warp's place among those that had a tile of
     // it, in the order of the keys.
@@ -134,7 +138,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
       __syncwarp();
       if (order != 0) return;
       if (whole) {
-        math.template write<ROWS>(p, now, at, own_states[warp], query);
+        math.template write<ROWS, WINDOW>(p, now, at, own_states[warp], query);
       } else {
         float* const to = p.partial + part * p.partial_floats + row_group * kPartOfWarp<Math>;
         math.each_out([&](int i, float x) { to[i * 32 + lane] = x; });
@@ -143,23 +147,29 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
     };
 
     uint32_t u0 = 0;
-    for (int tiles; any && (tiles = run.tiles(p)) > 0; run.pass<ROWS, TILE>(p, tiles)) {
+    for (int tiles; any && (tiles = run.tiles(p)) > 0; run.pass<ROWS, TILE, WINDOW>(p, tiles)) {
       at.rows_here = min(ROWS, now.it.count * p.group - now.row_tile * ROWS);
       at.sure = min(now.it.length, now.it.end);
+      CacheGap gap{0, 0};
+      if constexpr (WINDOW) {
+        gap = gap_of<ROWS, TILE>(p, now);
+        at.hidden = now.it.length + last_place<ROWS>(p, now.row_tile, at.rows_here) - p.window + 1;
+      }
+      auto key_of = [&](int tile) { return (WINDOW ? gap.tile(tile) : tile) * TILE; };
       if constexpr (Z::kWide) math.template begin<ROWS>(p, now, at, query);
       else math.template begin<ROWS>(p, now, at);
       const int order = (int)((key_group + KG - u0 % KG) % KG);
       uint32_t ahead = 0u;
-      if (p.mask != nullptr && p.tokens <= kMaskAhead && order < tiles && (now.tile + tiles) * TILE > at.sure)
+      if (p.mask != nullptr && p.tokens <= kMaskAhead && order < tiles && key_of(now.tile + tiles - 1) + TILE > at.sure)
         ahead = mask_word<ROWS>(p, now, at, (lane >> 4) * 32);
       for (int i = order; i < tiles; i += KG) {
         const uint32_t u = u0 + i, stage = u % Z::kStages;
-        at.key0 = (now.tile + i) * TILE;
+        at.key0 = key_of(now.tile + i);
         if (wait(full + 8 * stage, (u / Z::kStages) & 1)) {
           at.k = smem + stage * G::kBytes;
           at.v = at.k + G::kHalf;
-          if constexpr (Z::kWide) math.template tile<ROWS>(p, now, at, ahead, sees[warp], query, query + Z::kQuery);
-          else math.template tile<ROWS>(p, now, at, ahead, sees[warp]);
+          if constexpr (Z::kWide) math.template tile<ROWS, WINDOW>(p, now, at, ahead, sees[warp], query, query + Z::kQuery);
+          else math.template tile<ROWS, WINDOW>(p, now, at, ahead, sees[warp]);
           __syncwarp();
           if (lane == 0) mbar_arrive(empty + 8 * stage);
         }
@@ -169,7 +179,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
       u0 += tiles;
     }
   }
-  clear_rows_behind<T>(p, warp, Z::kWarps + 1);
+  clear_rows_behind<T, WINDOW>(p, warp, Z::kWarps + 1);
   __syncthreads();
   if (gave_up && threadIdx.x == 0) {
     cache_fault(p.c, kCacheWaitFault);
@@ -178,8 +188,6 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
   __syncthreads();
 }
 
-// ---- host --------------------------------------------------------------------------------------
-
 using Variant = CacheAttnVariant;
 
 // What beginning and ending an item costs, in tiles.  32 sequences of 1000 to 8192 tokens, BF16: 128.5 us without, 119.9 with two tiles, 115.2 with four, 111.2 with
@@ -187,40 +195,56 @@ using Variant = CacheAttnVariant;
 template <typename Math>
 constexpr int kItemUnits = sizeof(typename Math::Type) == 4 ? 4 : 6;
 
-template <typename Math, int RG>
+template <typename Math, int RG, bool WINDOW>
 Variant variant() {
   using Z = Shape<Math, RG>;
-  return Variant{cache_attention_kernel<Math, RG>, cache_attention_join_kernel<Math, RG>, Z::kThreads, Z::kSmem,
+  return Variant{cache_attention_kernel<Math, RG, WINDOW>, cache_attention_join_kernel<Math, RG, WINDOW>, Z::kThreads, Z::kSmem,
                  Z::kRows, Z::G::kKeys, Z::kGroups, kItemUnits<Math>, (int64_t)RG * kPartOfWarp<Math>};
 }
+
+// By the rows of an item, up to 64 to a row tile.
+template <typename T, int DP, bool WINDOW>
+Variant variant_of(int rows) {
+  if constexpr (sizeof(T) == 4)
+    return rows <= 2 ? variant<FmaMath<DP, 2>, 1, WINDOW>() : rows <= 4 ? variant<FmaMath<DP, 4>, 1, WINDOW>() : rows <= 8 ? variant<FmaMath<DP, 8>, 1, WINDOW>()
+           : rows <= 12 ? variant<FmaMath<DP, 12>, 1, WINDOW>() : rows <= 16 ? variant<FmaMath<DP, 16>, 1, WINDOW>() : rows <= 32 ? variant<FmaMath<DP, 16>, 2, WINDOW>() : variant<FmaMath<DP, 16>, 4, WINDOW>();
+  else if constexpr (DP <= 128)
+    return rows <= 16 ? variant<MmaMath<T, DP>, 1, WINDOW>() : variant<MmaMath<T, DP>, 2, WINDOW>();       // (more: tcgen05)
+  else
+    return rows <= 16 ? variant<MmaMath<T, DP>, 1, WINDOW>() : rows <= 32 ? variant<MmaMath<T, DP>, 2, WINDOW>() : variant<MmaMath<T, DP>, 4, WINDOW>();
+}
+template <typename T, bool WINDOW>
+Variant variant_of(int head_dim, int rows) {
+  return head_dim <= 64 ? variant_of<T, 64, WINDOW>(rows) : head_dim <= 128 ? variant_of<T, 128, WINDOW>(rows) : variant_of<T, 256, WINDOW>(rows);
+}
+template <bool WINDOW>
+Variant variant_of(int dtype, int head_dim, int rows) {
+  return dtype == KB200_DTYPE_FP32 ? variant_of<float, WINDOW>(head_dim, rows)
+         : dtype == KB200_DTYPE_BF16 ? variant_of<__nv_bfloat16, WINDOW>(head_dim, rows) : variant_of<__half, WINDOW>(head_dim, rows);
+}
+
+}  // namespace
+
+#ifdef KB200_WINDOW
+CacheAttnVariant cache_attention_warp_window_variant(int dtype, int head_dim, int rows) { return variant_of<true>(dtype, head_dim, rows); }
+}  // namespace kb200
+#else
+namespace {
+
+// ---- host --------------------------------------------------------------------------------------
 
 // 16-bit caches go to tiles of 128 rows on tcgen05 above this many rows of an item, above half of it where the items are fewer than half of the SMs.  (BF16, heads
 // of 128, four to a key head, up to 8192 tokens.  32 sequences of 20, 32, 48 and 64 rows: 110, 121, 164, 151 us by warps; 127, 137, 127, 119 on tcgen05.  One sequence of
 // 20, 32 and 64 rows: 28.2, 29.1, 34.2 us and 21.9, 22.3, 24.7.)
 constexpr int kFewRows = 32;
 
-// By the rows of an item, up to 64 to a row tile.
-template <typename T, int DP>
-Variant variant_of(int rows) {
-  if constexpr (sizeof(T) == 4)
-    return rows <= 2 ? variant<FmaMath<DP, 2>, 1>() : rows <= 4 ? variant<FmaMath<DP, 4>, 1>() : rows <= 8 ? variant<FmaMath<DP, 8>, 1>()
-           : rows <= 12 ? variant<FmaMath<DP, 12>, 1>() : rows <= 16 ? variant<FmaMath<DP, 16>, 1>() : rows <= 32 ? variant<FmaMath<DP, 16>, 2>() : variant<FmaMath<DP, 16>, 4>();
-  else if constexpr (DP <= 128)
-    return rows <= 16 ? variant<MmaMath<T, DP>, 1>() : variant<MmaMath<T, DP>, 2>();       // (more: tcgen05)
-  else
-    return rows <= 16 ? variant<MmaMath<T, DP>, 1>() : rows <= 32 ? variant<MmaMath<T, DP>, 2>() : variant<MmaMath<T, DP>, 4>();
+Variant variant_for(const Cache& c, int rows, int tokens, bool many_items, bool window) {
+  if (c.dtype != KB200_DTYPE_FP32 && c.view.head_dim <= 128 && rows > (many_items ? kFewRows : kFewRows / 2))
+    return window ? cache_attention_tc_window_variant(c.dtype, c.view.head_dim, tokens) : cache_attention_tc_variant(c.dtype, c.view.head_dim, tokens);
+  return window ? cache_attention_warp_window_variant(c.dtype, c.view.head_dim, rows) : variant_of<false>(c.dtype, c.view.head_dim, rows);
 }
-template <typename T>
-Variant variant_of(int head_dim, int rows) {
-  return head_dim <= 64 ? variant_of<T, 64>(rows) : head_dim <= 128 ? variant_of<T, 128>(rows) : variant_of<T, 256>(rows);
-}
-Variant variant_for(const Cache& c, int rows, int tokens, bool many_items) {
-  if (c.dtype != KB200_DTYPE_FP32 && c.view.head_dim <= 128 && rows > (many_items ? kFewRows : kFewRows / 2)) return cache_attention_tc_variant(c.dtype, c.view.head_dim, tokens);
-  return c.dtype == KB200_DTYPE_FP32 ? variant_of<float>(c.view.head_dim, rows)
-         : c.dtype == KB200_DTYPE_BF16 ? variant_of<__nv_bfloat16>(c.view.head_dim, rows) : variant_of<__half>(c.view.head_dim, rows);
-}
-Variant variant_for(const Cache& c, int rows, int tokens, int heads) {
-  return variant_for(c, tokens * (heads / c.view.kv_heads), tokens, 2 * (int64_t)rows * c.view.kv_heads >= c.sm_count);
+Variant variant_for(const Cache& c, int rows, int tokens, int heads, bool window) {
+  return variant_for(c, tokens * (heads / c.view.kv_heads), tokens, 2 * (int64_t)rows * c.view.kv_heads >= c.sm_count, window);
 }
 
 // How a call is divided: a CTA per SM, but no more than have a tile for each of their warps.
@@ -228,9 +252,9 @@ struct Division {
   int parts, min_units, item_units;
   bool whole;
 };
-Division division_of(const Cache& c, const Variant& v, int rows, int tokens, int heads) {
+Division division_of(const Cache& c, const Variant& v, int rows, int tokens, int heads, int64_t most_keys) {
   const int64_t row_tiles = ((int64_t)tokens * (heads / c.view.kv_heads) + v.rows - 1) / v.rows;
-  const int64_t tiles = (((int64_t)c.view.max_pages << c.view.page_log2) + v.tile - 1) / v.tile;
+  const int64_t tiles = std::min(most_keys, ((int64_t)c.view.max_pages << c.view.page_log2) + v.tile - 1) / v.tile;
   Division d{0, 1, 0, tiles <= v.groups};
   if (!d.whole) d.min_units = v.groups, d.item_units = v.item_units;
   const double units = (double)rows * c.view.kv_heads * row_tiles * (d.whole ? 1 : tiles + d.item_units);
@@ -241,13 +265,20 @@ uint64_t workspace_of(const Variant& v, const Division& d) {
   return d.whole ? 0 : (uint64_t)d.parts * (2 * v.part_floats * sizeof(float) + sizeof(CacheJoin));
 }
 
-Cache* cache_of(const kb200_cache* c) { return reinterpret_cast<Cache*>(const_cast<kb200_cache*>(c)); }
-
-// (The kernels count batch rows, and 16-byte chunks of a row's heads, in 32 bits, and go beyond the last by a step.)
-bool call_ok(const Cache& c, int rows, int tokens, int heads) {
-  return rows >= 0 && tokens >= 0 && heads >= 1 && heads % c.view.kv_heads == 0 && (int64_t)tokens * (heads / c.view.kv_heads) < (1 << 24) &&
-         (int64_t)rows * std::max(tokens, 1) <= (1 << 30) && (int64_t)heads * c.view.row_chunks <= (1 << 30);
+constexpr int64_t kAllKeys = INT64_MAX;
+// Keys of the tiles that an item may have (cache_items): those with the first keys, and a window's wherever it lies.
+int64_t window_keys(const Variant& v, int tokens, int window, int sinks) {
+  const int64_t front = ((int64_t)sinks + v.tile - 1) / v.tile, near = ((int64_t)window + tokens - 1 + v.tile - 2) / v.tile + 1;
+  return (front + near) * v.tile;
 }
+
+// What a call with a window or with the logarithms of sums asks for beside (window 0: neither).
+struct Beside {
+  int window = 0, sinks = 0;
+  const int32_t* places = nullptr;
+  float* lse = nullptr;
+  int64_t lse_stride[3] = {0, 0, 0};
+};
 
 }  // namespace
 
@@ -255,7 +286,7 @@ int cache_attention_prepare(Cache& c) {
   const EncodeFn encode = encode_fn();
   if (encode == nullptr) return fail(KB200_ERR_CUDA, "kb200_cache_create: the driver has no cuTensorMapEncodeTiled");
   const CacheView& v = c.view;
-  const int page = 1 << v.page_log2, columns = 128 / c.element, tile = variant_for(c, 1, 1, true).tile;
+  const int page = 1 << v.page_log2, columns = 128 / c.element, tile = variant_for(c, 1, 1, true, false).tile;
   const cuuint64_t dims[3] = {(cuuint64_t)v.head_dim, (cuuint64_t)v.kv_heads * page, (cuuint64_t)v.layers * 2 * v.pages};
   const cuuint64_t strides[2] = {(cuuint64_t)v.head_dim * c.element, dims[1] * v.head_dim * c.element};
   const cuuint32_t box[3] = {(cuuint32_t)columns, (cuuint32_t)std::min(page, tile), 1}, steps[3] = {1, 1, 1};
@@ -267,32 +298,23 @@ int cache_attention_prepare(Cache& c) {
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(KB200_ERR_UNSUPPORTED, "kb200_cache_create: the pool cannot be described to the copy engine (error %d)", (int)r);
   for (const int tokens : {1, kMaskAhead + 1})
-    for (const int rows : {2, 4, 8, 12, 16, 32, 64}) {
-      const Variant of = variant_for(c, rows, tokens, true);
-      KB200_CUDA(cudaFuncSetAttribute(of.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, of.smem));
-    }
+    for (const int rows : {2, 4, 8, 12, 16, 32, 64})
+      for (const bool window : {false, true}) {
+        const Variant of = variant_for(c, rows, tokens, true, window);
+        KB200_CUDA(cudaFuncSetAttribute(of.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, of.smem));
+      }
   return KB200_OK;
 }
 
-}  // namespace kb200
+namespace {
 
-using namespace kb200;
-
-KB200_EXPORT uint64_t kb200_cache_attend_workspace(const kb200_cache* handle, int rows, int tokens, int heads) {
-  if (handle == nullptr) return 0;
-  const Cache& c = *cache_of(handle);
-  if (!call_ok(c, rows, tokens, heads) || rows == 0 || tokens == 0) return 0;
-  const Variant v = variant_for(c, rows, tokens, heads);
-  return workspace_of(v, division_of(c, v, rows, tokens, heads));
-}
-
-KB200_EXPORT int kb200_cache_attend(kb200_cache* handle, int layer, const kb200_rows* q, const kb200_rows* out, int rows, int tokens,
-                                    const uint8_t* mask, const int64_t* mask_stride, const int32_t* counts, const int32_t* slots, float scale,
-                                    void* workspace, uint64_t workspace_bytes, void* stream) {
+int attend(kb200_cache* handle, int layer, const kb200_rows* q, const kb200_rows* out, int rows, int tokens, const uint8_t* mask, const int64_t* mask_stride,
+           const int32_t* counts, const int32_t* slots, float scale, const Beside& beside, void* workspace, uint64_t workspace_bytes, void* stream) {
+  const bool window = beside.window > 0;
   if (handle == nullptr) return fail(KB200_ERR_ARGUMENT, "kb200_cache_attend: cache is null");
   const Cache& c = *cache_of(handle);
   if (layer < 0 || layer >= c.view.layers) return fail(KB200_ERR_ARGUMENT, "kb200_cache_attend: layer %d of %d", layer, c.view.layers);
-  if (q == nullptr || out == nullptr || q->heads != out->heads || !call_ok(c, rows, tokens, q->heads) || (slots == nullptr && rows > c.view.sequences))
+  if (q == nullptr || out == nullptr || q->heads != out->heads || !cache_attention_call_ok(c, rows, tokens, q->heads) || (slots == nullptr && rows > c.view.sequences))
     return fail(KB200_ERR_ARGUMENT, "kb200_cache_attend: rows and tokens do not suit the cache, or heads are no multiple of its %d", c.view.kv_heads);
   if (rows == 0 || tokens == 0) return KB200_OK;
   for (const kb200_rows* r : {q, out}) {
@@ -304,8 +326,8 @@ KB200_EXPORT int kb200_cache_attend(kb200_cache* handle, int layer, const kb200_
   }
   if (mask != nullptr && mask_stride == nullptr) return fail(KB200_ERR_ARGUMENT, "kb200_cache_attend: a mask without strides");
   if (!(scale >= 1e-30f) || !(scale <= 1e30f)) return fail(KB200_ERR_ARGUMENT, "kb200_cache_attend: scale must be from 1e-30 to 1e30");
-  const Variant v = variant_for(c, rows, tokens, q->heads);
-  const Division d = division_of(c, v, rows, tokens, q->heads);
+  const Variant v = variant_for(c, rows, tokens, q->heads, window);
+  const Division d = division_of(c, v, rows, tokens, q->heads, window ? window_keys(v, tokens, beside.window, beside.sinks) : kAllKeys);
   const uint64_t need = workspace_of(v, d);
   if (need > 0 && (workspace == nullptr || !tc::aligned16(workspace) || workspace_bytes < need))
     return fail(KB200_ERR_ARGUMENT, "kb200_cache_attend: a workspace of %llu bytes on 16 bytes is needed", (unsigned long long)need);
@@ -334,7 +356,55 @@ KB200_EXPORT int kb200_cache_attend(kb200_cache* handle, int layer, const kb200_
   p.whole = d.whole;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.q_fp32 = q->dtype != c.dtype;
+  p.window = beside.window;
+  p.sinks = beside.sinks;
+  p.places = beside.places;
+  p.lse = beside.lse;
+  for (int i = 0; i < 3; ++i) p.lse_stride[i] = beside.lse_stride[i];
   KB200_CUDA(launch_kernel(true, v.kernel, dim3(d.parts), dim3(v.threads), v.smem, s, c.map, p));
   if (!d.whole) KB200_CUDA(launch_kernel(true, v.join, dim3(d.parts, std::max(1, v.rows / 8)), dim3(kJoinThreads), 0, s, p));
   return KB200_OK;
 }
+
+uint64_t workspace_for(const kb200_cache* handle, int rows, int tokens, int heads, int window, int sinks) {
+  if (handle == nullptr) return 0;
+  const Cache& c = *cache_of(handle);
+  if (!cache_attention_call_ok(c, rows, tokens, heads) || rows == 0 || tokens == 0) return 0;
+  const Variant v = variant_for(c, rows, tokens, heads, window > 0);
+  return workspace_of(v, division_of(c, v, rows, tokens, heads, window > 0 ? window_keys(v, tokens, window, sinks) : kAllKeys));
+}
+
+}  // namespace
+}  // namespace kb200
+
+using namespace kb200;
+
+KB200_EXPORT uint64_t kb200_cache_attend_workspace(const kb200_cache* handle, int rows, int tokens, int heads) { return workspace_for(handle, rows, tokens, heads, 0, 0); }
+
+KB200_EXPORT int kb200_cache_attend(kb200_cache* handle, int layer, const kb200_rows* q, const kb200_rows* out, int rows, int tokens,
+                                    const uint8_t* mask, const int64_t* mask_stride, const int32_t* counts, const int32_t* slots, float scale,
+                                    void* workspace, uint64_t workspace_bytes, void* stream) {
+  return attend(handle, layer, q, out, rows, tokens, mask, mask_stride, counts, slots, scale, Beside(), workspace, workspace_bytes, stream);
+}
+
+// (No window: one that all tokens are in.)
+KB200_EXPORT uint64_t kb200_cache_attend_window_workspace(const kb200_cache* handle, int rows, int tokens, int heads, int window, int sinks) {
+  if (window < 0 || sinks < 0) return 0;
+  return workspace_for(handle, rows, tokens, heads, window == 0 ? INT_MAX : window, sinks);
+}
+
+KB200_EXPORT int kb200_cache_attend_window(kb200_cache* handle, int layer, const kb200_rows* q, const kb200_rows* out, int rows, int tokens,
+                                           const uint8_t* mask, const int64_t* mask_stride, const int32_t* counts, const int32_t* slots, float scale,
+                                           int window, int sinks, const int32_t* places, float* lse, const int64_t* lse_stride,
+                                           void* workspace, uint64_t workspace_bytes, void* stream) {
+  if (window < 0 || sinks < 0) return fail(KB200_ERR_ARGUMENT, "kb200_cache_attend_window: a window of %d tokens behind %d", window, sinks);
+  if (lse != nullptr && lse_stride == nullptr) return fail(KB200_ERR_ARGUMENT, "kb200_cache_attend_window: lse without strides");
+  Beside beside;
+  beside.window = window == 0 ? INT_MAX : window;
+  beside.sinks = sinks;
+  beside.places = places;
+  beside.lse = lse;
+  for (int i = 0; i < 3; ++i) beside.lse_stride[i] = lse != nullptr ? lse_stride[i] : 0;
+  return attend(handle, layer, q, out, rows, tokens, mask, mask_stride, counts, slots, scale, beside, workspace, workspace_bytes, stream);
+}
+#endif

@@ -23,6 +23,11 @@ struct CacheAttnParams {
   float scale_log2;
   bool whole;                              // items are not divided: no parts
   bool q_fp32;                             // q is float32 where the cache is not
+  // of kernels with a window (WINDOW below)
+  int window, sinks;
+  const int32_t* places;                   // null: token t stands t behind the committed ones
+  float* lse;                              // or null
+  int64_t lse_stride[3];
 };
 
 // Work is counted in units: a tile of keys for a tile of query rows (the drafted tokens of a sequence times the heads that share a key head), and in front of an
@@ -47,7 +52,36 @@ struct CacheItems {                        // of one batch row
 };
 
 #ifdef __CUDACC__
-template <int ROWS, int TILE>
+// A window: a row at position P sees the keys from P - window + 1 on, and the first `sinks`.  The tiles of an item are those with the first keys that it sees, and, behind
+// a gap, those from the first key that its first row sees in its window.  (WINDOW is a parameter of the kernels, so that calls without one keep their registers.)
+struct CacheGap {
+  int front, gap;                          // tiles in front of it; tiles that are left out
+  __device__ __forceinline__ int tile(int i) const { return i < front ? i : i + gap; }
+};
+// Of the rows from place `place` on.
+template <int TILE>
+__device__ __forceinline__ CacheGap gap_of(const CacheAttnParams& p, int length, int place) {
+  const int begin = max(0, length + place - p.window + 1), front = (min(p.sinks, begin) + TILE - 1) / TILE;
+  return CacheGap{front, max(0, begin / TILE - front)};
+}
+// Tokens that a tile of query rows has at most.
+template <int ROWS>
+__host__ __device__ __forceinline__ int tokens_of_tile(int group) { return ROWS % group == 0 ? ROWS / group : (ROWS + group - 2) / group + 1; }
+// Tiles from the window's first key to the rows' last, wherever they lie.
+template <int TILE>
+__host__ __device__ __forceinline__ int64_t window_tiles(int window, int tokens) { return ((int64_t)window + tokens - 1 + TILE - 2) / TILE + 1; }
+
+// The last place of an item's rows.
+template <int ROWS>
+__device__ __forceinline__ int last_place(const CacheAttnParams& p, int row_tile, int rows_here) {
+  return p.mask != nullptr || p.places != nullptr ? p.tokens - 1 : (row_tile * ROWS + rows_here - 1) / p.group;
+}
+__device__ __forceinline__ int place_of(const CacheAttnParams& p, int b, int token) {
+  return p.places == nullptr ? token : min(max(p.places[(int64_t)b * p.tokens + token], 0), p.tokens - 1);
+}
+__device__ __forceinline__ bool own_places(const CacheAttnParams& p) { return p.mask == nullptr && p.places == nullptr; }
+
+template <int ROWS, int TILE, bool WINDOW>
 __device__ __forceinline__ CacheItems cache_items(const CacheAttnParams& p, int b) {
   CacheItems r{};
   const int slot = p.slots != nullptr ? p.slots[b] : b;
@@ -67,6 +101,14 @@ __device__ __forceinline__ CacheItems cache_items(const CacheAttnParams& p, int 
   if (r.end < length + count) cache_fault(p.c, KB200_CACHE_NO_ROOM);
   r.row_tiles = (count * p.group + ROWS - 1) / ROWS;
   r.key_tiles = max(1, (r.end + TILE - 1) / TILE);
+  if constexpr (WINDOW) {
+    if (r.row_tiles > 1 && own_places(p)) {          // row tiles begin at keys of their own; all have as many tiles as any may have
+      const int begin = max(0, length + count - p.window), front = (min(p.sinks, begin) + TILE - 1) / TILE;
+      r.key_tiles = (int)min((int64_t)r.key_tiles, front + window_tiles<TILE>(p.window, tokens_of_tile<ROWS>(p.group)));
+    } else {
+      r.key_tiles = max(1, r.key_tiles - gap_of<TILE>(p, length, 0).gap);
+    }
+  }
   r.units = (int64_t)r.row_tiles * (p.whole ? 1 : r.key_tiles + p.item_units) * p.c.kv_heads;
   return r;
 }
@@ -76,8 +118,13 @@ struct CacheCursor {
   int b, head, row_tile, tile;
   CacheItems it;
 };
-// To the next item.
+// The gap of the item at hand.
 template <int ROWS, int TILE>
+__device__ __forceinline__ CacheGap gap_of(const CacheAttnParams& p, const CacheCursor& u) {
+  return gap_of<TILE>(p, u.it.length, u.it.row_tiles > 1 && own_places(p) ? u.row_tile * ROWS / p.group : 0);
+}
+// To the next item.
+template <int ROWS, int TILE, bool WINDOW>
 __device__ __forceinline__ void next_item(const CacheAttnParams& p, CacheCursor& u) {
   u.tile = 0;
   if (++u.row_tile < u.it.row_tiles) return;
@@ -85,7 +132,7 @@ __device__ __forceinline__ void next_item(const CacheAttnParams& p, CacheCursor&
   if (++u.head < p.c.kv_heads) return;
   u.head = 0;
   while (++u.b < p.rows) {
-    u.it = cache_items<ROWS, TILE>(p, u.b);
+    u.it = cache_items<ROWS, TILE, WINDOW>(p, u.b);
     if (u.it.units > 0) return;
   }
 }
@@ -101,11 +148,11 @@ struct CacheRun {
     if (left <= skip) return 0;
     return p.whole ? at.it.key_tiles : (int)min(left - skip, (int64_t)at.it.key_tiles - at.tile);
   }
-  template <int ROWS, int TILE>
+  template <int ROWS, int TILE, bool WINDOW = false>
   __device__ __forceinline__ void pass(const CacheAttnParams& p, int tiles) {
     left -= p.whole ? 1 : skip + tiles;
     skip = p.item_units;
-    if (left > 0) next_item<ROWS, TILE>(p, at);
+    if (left > 0) next_item<ROWS, TILE, WINDOW>(p, at);
   }
 };
 struct CacheRunShared {
@@ -115,7 +162,7 @@ struct CacheRunShared {
 };
 
 // The run of CTA `part`, by all threads of a CTA of THREADS; false: it has none.
-template <int ROWS, int TILE, int THREADS>
+template <int ROWS, int TILE, int THREADS, bool WINDOW = false>
 __device__ __forceinline__ bool find_run(const CacheAttnParams& p, int part, CacheRunShared& shared, CacheRun* run) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool one_round = p.rows <= THREADS;
@@ -126,7 +173,7 @@ __device__ __forceinline__ bool find_run(const CacheAttnParams& p, int part, Cac
       base = 0;
       for (int b0 = 0; b0 < p.rows; b0 += THREADS) {
         const int b = b0 + threadIdx.x;
-        if (b < p.rows) it = cache_items<ROWS, TILE>(p, b);
+        if (b < p.rows) it = cache_items<ROWS, TILE, WINDOW>(p, b);
         else it.units = 0;
         int64_t sum = it.units;
 #pragma unroll

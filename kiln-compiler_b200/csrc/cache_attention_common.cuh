@@ -56,7 +56,7 @@ __device__ __forceinline__ void ask_for_rows(const CacheAttnParams& p, const Cac
 }
 
 // The producer warp: brings the run's tiles, page by page, as the ring's stages become free.
-template <typename T, int DP, int ROWS, int STAGES, typename Wait>
+template <typename T, int DP, int ROWS, int STAGES, bool WINDOW, typename Wait>
 __device__ __forceinline__ void bring_tiles(const CUtensorMap& map, const CacheAttnParams& p, CacheRun& run, uint32_t stage0, uint32_t full, uint32_t empty, Wait&& wait) {
   using G = Tile<T, DP>;
   constexpr int TILE = G::kKeys;
@@ -69,8 +69,11 @@ __device__ __forceinline__ void bring_tiles(const CUtensorMap& map, const CacheA
   int page_base = -1, page_slot = -1, page_end = -1, my_page = -1;
   int left = run.tiles(p), tiles = left;
   if (left > 0) ask_for_rows<T, ROWS>(p, now, lane);
+  CacheGap gap{0, 0};
+  if constexpr (WINDOW) gap = gap_of<ROWS, TILE>(p, now);
   while (left > 0) {
-    const int first = now.tile * TILE >> p.c.page_log2;
+    const int tile = WINDOW ? gap.tile(now.tile) : now.tile;
+    const int first = tile * TILE >> p.c.page_log2;
     const int wanted = first & ~31;
     if (page_slot != now.it.slot || page_end != now.it.end || wanted != page_base) {
       page_slot = now.it.slot;
@@ -78,7 +81,10 @@ __device__ __forceinline__ void bring_tiles(const CUtensorMap& map, const CacheA
       page_base = wanted;
       const int k = wanted + lane;
       my_page = k << p.c.page_log2 < now.it.end ? p.c.table[(int64_t)now.it.slot * p.c.max_pages + k] : -1;
-      if (my_page >= p.c.pages || (my_page < 0 && k << p.c.page_log2 < now.it.end)) {
+      bool needed = true;                  // (pages that no row sees may be gone)
+      if constexpr (WINDOW)
+        needed = k << p.c.page_log2 < p.sinks || ((int64_t)k + 1) << p.c.page_log2 > (int64_t)now.it.length - p.window + 1;
+      if (my_page >= p.c.pages || (my_page < 0 && needed && k << p.c.page_log2 < now.it.end)) {
         cache_fault(p.c, KB200_CACHE_BAD_INDEX);
         my_page = -1;
       }
@@ -89,7 +95,7 @@ __device__ __forceinline__ void bring_tiles(const CUtensorMap& map, const CacheA
     if (lane == 0) mbar_expect_tx(bar, G::kBytes);
     __syncwarp();
     // K and V of every box, block by block: as many loads as there are, spread over the lanes
-    const int in_page = now.tile * TILE & ((1 << p.c.page_log2) - 1);
+    const int in_page = tile * TILE & ((1 << p.c.page_log2) - 1);
     for (int i0 = 0; i0 < boxes * G::kBlocks * 2; i0 += 32) {
       const int i = i0 + lane, which = i & 1, block = (i >> 1) % G::kBlocks, j = (i >> 1) / G::kBlocks;
       const int page = __shfl_sync(0xffffffffu, my_page, (first + j) & 31);
@@ -100,7 +106,8 @@ __device__ __forceinline__ void bring_tiles(const CUtensorMap& map, const CacheA
     ++u;
     ++now.tile;
     if (--left == 0) {
-      run.pass<ROWS, TILE>(p, tiles);
+      run.pass<ROWS, TILE, WINDOW>(p, tiles);
+      if constexpr (WINDOW) gap = gap_of<ROWS, TILE>(p, now);
       left = tiles = run.tiles(p);
       if (left > 0) ask_for_rows<T, ROWS>(p, now, lane);
     }
@@ -109,7 +116,7 @@ __device__ __forceinline__ void bring_tiles(const CUtensorMap& map, const CacheA
 
 // Rows behind a sequence's drafted tokens, and those of no sequence: zeros.  By every warp, when it has nothing else to do: 32 rows are looked at at a time, which lie
 // apart, so that neighbours go to other SMs (32 neighbours to a warp: 249 us where 231 are, a few warps cleared whole sequences).
-template <typename T>
+template <typename T, bool WINDOW>
 __device__ __forceinline__ void clear_rows_behind(const CacheAttnParams& p, int warp, int warps) {
   if (p.counts == nullptr && p.slots == nullptr) return;
   const int lane = threadIdx.x & 31, chunks = p.heads * p.c.row_chunks;
@@ -125,6 +132,8 @@ __device__ __forceinline__ void clear_rows_behind(const CacheAttnParams& p, int 
       T* const row = static_cast<T*>(p.out) + at / p.tokens * p.out_stride[0] + at % p.tokens * p.out_stride[1];
       for (int x = lane; x < chunks; x += 32)
         *reinterpret_cast<uint4*>(row + x / p.c.row_chunks * p.out_stride[2] + x % p.c.row_chunks * (16 / (int)sizeof(T))) = make_uint4(0u, 0u, 0u, 0u);
+      if constexpr (WINDOW)
+        for (int x = lane; p.lse != nullptr && x < p.heads; x += 32) p.lse[at / p.tokens * p.lse_stride[0] + at % p.tokens * p.lse_stride[1] + x * p.lse_stride[2]] = -CUDART_INF_F;
     }
   }
 }
@@ -136,7 +145,7 @@ constexpr int kPartOfWarp = Math::kOut * 32 + 2 * Math::kRows;
 // Joins the parts of the item that CTA x of the first launch has left (CacheJoin).
 constexpr int kJoinThreads = 128, kJoinAtOnce = 4;      // parts whose loads are in flight together
 
-template <typename Math, int RG>
+template <typename Math, int RG, bool WINDOW>
 __global__ void __launch_bounds__(kJoinThreads) cache_attention_join_kernel(const __grid_constant__ CacheAttnParams p) {
   using T = typename Math::Type;
   constexpr int DP = Math::kDim, ROWS = Math::kRows * RG;
@@ -185,6 +194,9 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attention_join_kernel(cons
     T* const to = static_cast<T*>(p.out) + at.b * p.out_stride[0] + r.token * p.out_stride[1] + r.head * p.out_stride[2] + d;
     store2<T>(to, x.x * inv, x.y * inv);
     store2<T>(to + 2, x.z * inv, x.w * inv);
+    if constexpr (WINDOW) {
+      if (d == 0) write_lse(p, at.b, r, Math::log_sum(top, sum, p.scale_log2));
+    }
   }
 }
 
@@ -199,6 +211,10 @@ struct CacheAttnVariant {
   int item_units;                  // see cache_attention.h
   int64_t part_floats;
 };
-CacheAttnVariant cache_attention_tc_variant(int dtype, int head_dim, int tokens);      // (cache_attention_tc.cu) tiles of 128 query rows; 16-bit types, heads up to 128
+// (cache_attention_tc.cu) tiles of 128 query rows; 16-bit types, heads up to 128
+CacheAttnVariant cache_attention_tc_variant(int dtype, int head_dim, int tokens);
+CacheAttnVariant cache_attention_tc_window_variant(int dtype, int head_dim, int tokens);
+// (cache_attention_window.cu) the warps' kernels with a window
+CacheAttnVariant cache_attention_warp_window_variant(int dtype, int head_dim, int rows);
 
 }  // namespace kb200

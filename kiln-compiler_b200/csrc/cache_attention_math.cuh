@@ -114,8 +114,22 @@ struct Place {
   uint8_t *k, *v;              // the stage
   int key0, sure;              // the tile's first key; keys that every row sees
   int row0, rows_here;         // the warp's first row of the item's row tile; rows of that
+  int hidden;                  // (a window) keys from here on are not hidden from any row
   int warp, lane, row_group, key_group;
 };
+
+// A window hides some of a tile's keys from some rows.
+__device__ __forceinline__ bool window_hides(const CacheAttnParams& p, int key0, int keys, int hidden) { return key0 < hidden && key0 + keys > p.sinks; }
+// ... the bits of those that are hidden from a row of place `place`; drafted tokens are the mask's matter where there is one.
+__device__ __forceinline__ unsigned long long hidden_keys(const CacheAttnParams& p, int length, int place, int key0) {
+  const int begin = length + place - p.window + 1;
+  const int from = max(0, p.sinks - key0), to = (p.mask != nullptr ? min(begin, length) : begin) - key0;
+  if (to <= from || from >= 64) return 0ull;
+  return (to >= 64 ? ~0ull : (1ull << to) - 1) & ~((1ull << from) - 1);
+}
+__device__ __forceinline__ void write_lse(const CacheAttnParams& p, int b, const CacheRow& r, float value) {
+  if (p.lse != nullptr) p.lse[b * p.lse_stride[0] + r.token * p.lse_stride[1] + r.head * p.lse_stride[2]] = value;
+}
 
 // What a warp's rows see of the drafted tokens.  Lane i has row i % 16 of the warp's, and of its drafted tokens the 32 from `first` on.  Small code on purpose, here
 // and below: a launch meets it cold, once or twice, and its instructions come from L2 (unrolled over rows and keys this was 13000 cycles).
@@ -135,7 +149,7 @@ __device__ __forceinline__ uint32_t mask_word(const CacheAttnParams& p, const Ca
 constexpr int kMaskAhead = 64;
 
 // The keys of a tile with drafted tokens that the warp's rows see: row i of the warp's in sees[i].
-template <int ROWS, int WARP_ROWS, int KEYS>
+template <int ROWS, int WARP_ROWS, int KEYS, bool WINDOW>
 __device__ __forceinline__ void look_at_mask(const CacheAttnParams& p, const CacheCursor& now, const Place& at, uint32_t ahead, uint2* sees) {
   const int row = at.lane & 15, off = now.it.length - at.key0;         // where the first drafted token is in the tile
   unsigned long long shows = 0ull;
@@ -153,6 +167,9 @@ __device__ __forceinline__ void look_at_mask(const CacheAttnParams& p, const Cac
   }
   const int last = now.it.end - at.key0;
   if (last < 64) shows &= last <= 0 ? 0ull : (1ull << last) - 1;
+  if constexpr (WINDOW) {
+    if (at.row0 + row < at.rows_here) shows &= ~hidden_keys(p, now.it.length, place_of(p, now.b, row_of<ROWS>(p, now, at.row0 + row).token), at.key0);
+  }
   if (at.lane < WARP_ROWS) sees[row] = make_uint2((uint32_t)shows, (uint32_t)(shows >> 32));
   __syncwarp();
 }
@@ -160,12 +177,12 @@ __device__ __forceinline__ void look_at_mask(const CacheAttnParams& p, const Cac
 // V behind the sequence's end is what an earlier tenant left, as far as its last page goes (pages that it has not come as zeros), and V of a drafted token that some
 // rows do not see may hold infinities or NaN; 0 times those is NaN.  The former become zeros (every warp that reads the tile writes them, and looks at none of
 // them).  True: the latter are there.
-template <typename T, int DP>
+template <typename T, int DP, bool WINDOW>
 __device__ __forceinline__ bool look_at_values(const CacheAttnParams& p, const CacheCursor& now, const Place& at) {
   using G = Tile<T, DP>;
   constexpr int kChunks = G::kBlocks * 8;
   const int in_page = (1 << p.c.page_log2) - 1, last = now.it.end - at.key0;
-  const int from = max(0, at.sure - at.key0), to = min(G::kKeys, ((now.it.end + in_page) & ~in_page) - at.key0);
+  const int from = WINDOW && window_hides(p, at.key0, G::kKeys, at.hidden) ? 0 : max(0, at.sure - at.key0), to = min(G::kKeys, ((now.it.end + in_page) & ~in_page) - at.key0);
   uint32_t odd = 0u;
 #pragma unroll 2
   for (int i = from * kChunks + at.lane; i < to * kChunks; i += 32) {
@@ -192,6 +209,8 @@ struct MmaMath {
   // Maxima are powers of two's exponents: the scale and the maximum go into one multiply-add per score, and a rounding of the maximum cancels.  It is rounded
   // down, so that the largest weight is not below 2^kTopExponent; see kFarScore for where it would be far above.
   static __device__ __forceinline__ float exponent(float behind, float) { return behind; }
+  // The logarithm of a row's sum.
+  static __device__ __forceinline__ float log_sum(float top, float sum, float) { return sum == 0.0f ? -CUDART_INF_F : fmaf(top, 0.69314718f, logf(sum)); }
 
   template <int ROWS>
   __device__ __forceinline__ void begin(const CacheAttnParams& p, const CacheCursor& now, const Place& at) {
@@ -244,7 +263,7 @@ struct MmaMath {
     }
   }
 
-  template <int ROWS>
+  template <int ROWS, bool WINDOW>
   __device__ __forceinline__ void tile(const CacheAttnParams& p, const CacheCursor& now, const Place& at, uint32_t ahead, uint2* sees) {
     const int lane = at.lane, g = lane >> 2, t4 = lane & 3;
     const uint32_t k_tile = smem_u32(at.k), v_tile = smem_u32(at.v);
@@ -266,11 +285,11 @@ struct MmaMath {
       }
     }
 
-    const bool drafted = at.key0 + G::kKeys > at.sure;
+    const bool drafted = at.key0 + G::kKeys > at.sure || (WINDOW && window_hides(p, at.key0, G::kKeys, at.hidden));
     bool infinite = false;
     if (drafted) {
-      look_at_mask<ROWS, 16, G::kKeys>(p, now, at, ahead, sees);
-      infinite = look_at_values<T, DP>(p, now, at);
+      look_at_mask<ROWS, 16, G::kKeys, WINDOW>(p, now, at, ahead, sees);
+      infinite = look_at_values<T, DP, WINDOW>(p, now, at);
       unsigned long long shows[2];                   // the tile's keys that rows g and g + 8 see
 #pragma unroll
       for (int h = 0; h < 2; ++h) shows[h] = sees[g + 8 * h].x | (unsigned long long)sees[g + 8 * h].y << 32;
@@ -373,7 +392,7 @@ struct MmaMath {
   // Where a row's column is among the 32 x kOut values of a warp.
   static __device__ __forceinline__ int place(int row, int d) { return (d / 8 * 4 + (row >> 3) * 2 + (d & 1)) * 32 + (row & 7) * 4 + d % 8 / 2; }
   // The rows, divided by their sums; states: of all the item's warps together.
-  template <int ROWS>
+  template <int ROWS, bool WINDOW>
   __device__ __forceinline__ void write(const CacheAttnParams& p, const CacheCursor& now, const Place& at, const float2* states, float*) const {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -385,6 +404,9 @@ struct MmaMath {
 #pragma unroll
       for (int d = 0; d < DT; ++d)
         if (d * 8 < p.c.head_dim) store2<T>(to + d * 8, o[d][2 * h] * inv, o[d][2 * h + 1] * inv);
+      if constexpr (WINDOW) {
+        if ((at.lane & 3) == 0) write_lse(p, now.b, r, log_sum(states[in_warp].x, sum, p.scale_log2));
+      }
     }
   }
 };
@@ -408,6 +430,7 @@ struct FmaMath {
   // Scores and maxima are kept as they were summed, and the scale is applied to differences: a rounding then goes with the distance from the maximum, not with
   // the score's size.  (Scores of 8000 that were scaled and rounded first gave errors of 1e-4.)
   static __device__ __forceinline__ float exponent(float behind, float scale) { return behind * scale; }
+  static __device__ __forceinline__ float log_sum(float top, float sum, float scale) { return sum == 0.0f ? -CUDART_INF_F : fmaf(top * scale, 0.69314718f, logf(sum)); }
 
   // The query rows go to shared memory, [R][DP] of the warp's own.
   template <int ROWS>
@@ -476,7 +499,7 @@ struct FmaMath {
     }
   }
 
-  template <int ROWS>
+  template <int ROWS, bool WINDOW>
   __device__ __forceinline__ void tile(const CacheAttnParams& p, const CacheCursor& now, const Place& at, uint32_t ahead, uint2* sees, const float* q, float* weights) {
     const int lane = at.lane;
     // Few rows: sums in two parts, so that half as many roundings follow each other (one token over 128 keys: 2.0e-7 to 3.3e-7 off, 2.9e-7 to 4.0e-7 in one part, in the
@@ -519,11 +542,11 @@ struct FmaMath {
 #pragma unroll
         for (int d = 32 / SHARE; d < 32; d *= 2) s[0][r] += __shfl_xor_sync(0xffffffffu, s[0][r], d);
     }
-    const bool drafted = at.key0 + G::kKeys > at.sure;
+    const bool drafted = at.key0 + G::kKeys > at.sure || (WINDOW && window_hides(p, at.key0, G::kKeys, at.hidden));
     bool infinite = false;
     if (drafted) {
-      look_at_mask<ROWS, R, G::kKeys>(p, now, at, ahead, sees);
-      infinite = look_at_values<float, DP>(p, now, at);
+      look_at_mask<ROWS, R, G::kKeys, WINDOW>(p, now, at, ahead, sees);
+      infinite = look_at_values<float, DP, WINDOW>(p, now, at);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const uint2 shows = sees[r];
@@ -612,7 +635,7 @@ struct FmaMath {
   }
   static __device__ __forceinline__ int place(int row, int d) { return ((d % C * (R / 2) + row / 2) * 2 + (row & 1)) * 32 + d / C; }
   // (by way of the query rows' place, so that a small loop does: a launch meets this code cold)
-  template <int ROWS>
+  template <int ROWS, bool WINDOW>
   __device__ __forceinline__ void write(const CacheAttnParams& p, const CacheCursor& now, const Place& at, const float2* states, float* query) {
     const int lane = at.lane;
     __syncwarp();
@@ -626,6 +649,9 @@ struct FmaMath {
       const CacheRow r = row_of<ROWS>(p, now, row);
       store2<float>(static_cast<float*>(p.out) + now.b * p.out_stride[0] + r.token * p.out_stride[1] + r.head * p.out_stride[2] + d,
                     query[place(in_warp, d)] * inv, query[place(in_warp, d + 1)] * inv);
+      if constexpr (WINDOW) {
+        if (d == 0) write_lse(p, now.b, r, log_sum(states[in_warp].x, sum, p.scale_log2));
+      }
     }
     __syncwarp();
   }

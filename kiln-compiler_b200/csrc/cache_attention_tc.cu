@@ -11,8 +11,8 @@
 // the issuing warp ~60 cycles, a commit ~100, a tile ~1000: so a group's next scores are asked for as soon as it has read the last ones, under its exponentials.
 // (With the weights over the scores they had to wait for them: 3400 cycles for two tiles.)  Output rows stay in tensor memory over an item and are rescaled
 // only when a row's maximum has grown.  Q is put into shared memory by the threads that own its rows, from any strides, rounded on the way where it is float32.
-#include <algorithm>
-
+//
+// WINDOW: the kernels with a window, which cache_attention_tc_window.cu compiles from the same text.
 #include "cache_attention_common.cuh"
 
 namespace kb200 {
@@ -37,6 +37,7 @@ struct TcMath {
   static constexpr int kDim = DP, kRows = kb200::kRows, kOut = DP * kb200::kRows / 32;
   static __device__ __forceinline__ int place(int row, int d) { return d * kb200::kRows + row; }
   static __device__ __forceinline__ float exponent(float behind, float) { return behind; }       // (maxima are exponents, as MmaMath's)
+  static __device__ __forceinline__ float log_sum(float top, float sum, float scale) { return MmaMath<T, DP>::log_sum(top, sum, scale); }
 };
 
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
@@ -98,7 +99,7 @@ __device__ __noinline__ void add_infinite(const CacheAttnParams& p, const CacheI
 }
 
 // MANY: more than kMaskAhead drafted tokens.  (Two kernels: with both ways in one, its registers cost a call of few tokens up to 9%: 109 us where 100 are.)
-template <typename T, int DP, bool MANY>
+template <typename T, int DP, bool MANY, bool WINDOW>
 __global__ void __launch_bounds__(kThreads, 1)
 cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CacheAttnParams p) {
   using Z = TcShape<T, DP>;
@@ -135,7 +136,7 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
   pdl_wait();
   pdl_launch_dependents();
   CacheRun run;
-  const bool any = find_run<kRows, TILE, kThreads>(p, blockIdx.x, found, &run);
+  const bool any = find_run<kRows, TILE, kThreads, WINDOW>(p, blockIdx.x, found, &run);
   CacheCursor& now = run.at;
   volatile int* const abort_ptr = &gave_up;
   // A wait that ends for all lanes of a warp or none.  Where it runs out the softmax warps do no more work, but meet each other as if they did.
@@ -143,7 +144,7 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
 
   if (warp == 0) {
     if (lane == 0) leave_join<kRows>(p, any, run);
-    if (any) bring_tiles<T, DP, kRows, Z::kStages>(map, p, run, stage0, full, empty, wait);
+    if (any) bring_tiles<T, DP, kRows, Z::kStages, WINDOW>(map, p, run, stage0, full, empty, wait);
   } else if (warp == 1) {
     // ---------------- products ----------------
     // Tiles are numbered over all items; scores, weights and the output's barrier take turns of two.
@@ -185,7 +186,7 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
     };
     uint32_t t = 0;
     bool ok = any;
-    for (int tiles; ok && (tiles = run.tiles(p)) > 0; run.pass<kRows, TILE>(p, tiles)) {
+    for (int tiles; ok && (tiles = run.tiles(p)) > 0; run.pass<kRows, TILE, WINDOW>(p, tiles)) {
       ok = issue_qk(t, true, false) && (tiles == 1 || issue_qk(t + 1, false, false));
       for (int i = 0; i < tiles && ok; ++i, ++t) {
         if (i + 2 < tiles) ok = issue_qk(t + 2, false, true);
@@ -204,14 +205,21 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
     auto meet_group = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(kRows) : "memory"); };
     auto meet_both = [&]() { asm volatile("bar.sync 3, %0;" ::"n"(2 * kRows) : "memory"); };
     uint32_t t0 = 0;                                 // the item's first tile
-    for (int tiles; any && (tiles = run.tiles(p)) > 0; run.pass<kRows, TILE>(p, tiles)) {
+    for (int tiles; any && (tiles = run.tiles(p)) > 0; run.pass<kRows, TILE, WINDOW>(p, tiles)) {
       const int rows_here = min(kRows, now.it.count * p.group - now.row_tile * kRows), sure = min(now.it.length, now.it.end);
       const bool there = row < rows_here, warp_there = quad * 32 < rows_here;
+      CacheGap gap{0, 0};
+      int hidden = 0;                                // (a window) keys from here on are not hidden from any row
+      if constexpr (WINDOW) {
+        gap = gap_of<kRows, TILE>(p, now);
+        hidden = now.it.length + last_place<kRows>(p, now.row_tile, rows_here) - p.window + 1;
+      }
+      auto key_of = [&](int tile) { return (WINDOW ? gap.tile(tile) : tile) * TILE; };
       const CacheRow r = row_of<kRows>(p, now, there ? row : 0);
       // What the rows see of up to 64 drafted tokens: a lane has a drafted token and a warp a word in eight of two per token.  All of these loads and those of Q are
       // under way before any is waited for, and they are under the way of the first keys.
       const uint8_t* const mask = p.mask + now.b * p.mask_stride[0];
-      const bool masked = !MANY && p.mask != nullptr && (now.tile + tiles) * TILE > sure;
+      const bool masked = !MANY && p.mask != nullptr && key_of(now.tile + tiles - 1) + TILE > sure;
       const int first_token = now.row_tile * kRows / p.group, words = 2 * ((now.row_tile * kRows + rows_here - 1) / p.group - first_token + 1);
       uint32_t seen = 0u;
       if (masked) {
@@ -262,21 +270,23 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
         if (there) tree = to[2 * (r.token - first_token)] | (unsigned long long)to[2 * (r.token - first_token) + 1] << 32;
         meet_both();
       }
+      int place = 0;
+      if constexpr (WINDOW) place = there ? place_of(p, now.b, r.token) : 0;
       float m = -CUDART_INF_F, l = 0.0f;
       uint32_t done = 0;                             // the group's last tile, plus one
       for (int i = (int)((group + t0) & 1); i < tiles; i += 2) {
         const uint32_t t = t0 + i, stage = t % Z::kStages;
-        const int key0 = (now.tile + i) * TILE;
+        const int key0 = key_of(now.tile + i);
         const bool ok = wait(s_full + 8 * group, (t >> 1) & 1);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const bool drafted = key0 + TILE > sure, work = ok && warp_there;
+        const bool hides = WINDOW && window_hides(p, key0, TILE, hidden), drafted = key0 + TILE > sure || hides, work = ok && warp_there;
         unsigned long long odd = 0ull;
         if (drafted) {
           // V behind the sequence's end becomes zeros, and so do infinities and NaN (see look_at_values), by all rows' threads of the group together.
           uint8_t* const values = smem + Z::kQBytes + stage * G::kBytes + G::kHalf;
           constexpr int kChunks = G::kBlocks * 8;
           const int in_page = (1 << p.c.page_log2) - 1, last = now.it.end - key0;
-          const int from = max(0, sure - key0) * kChunks, to = min(TILE, ((now.it.end + in_page) & ~in_page) - key0) * kChunks;
+          const int from = (hides ? 0 : max(0, sure - key0)) * kChunks, to = min(TILE, ((now.it.end + in_page) & ~in_page) - key0) * kChunks;
           if (worker == 0) odd_keys[group] = 0ull;
           meet_group();
           if (wait(full + 8 * stage, (t / Z::kStages) & 1))
@@ -321,6 +331,7 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
               if (off > 0) shows |= off >= 64 ? ~0ull : (1ull << off) - 1;
             }
             if (last < 64) shows &= last <= 0 ? 0ull : (1ull << last) - 1;
+            if constexpr (WINDOW) shows &= ~hidden_keys(p, now.it.length, place, key0);
 #pragma unroll
             for (int j = 0; j < 64; ++j)
               if (!((j < 32 ? (uint32_t)shows : (uint32_t)(shows >> 32)) >> (j & 31) & 1u)) v[j] = -CUDART_INF_F;
@@ -407,6 +418,9 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
         // a part that begins with the run is the run's first, else its second
         float* const part = p.partial + (2 * (int64_t)blockIdx.x + (t0 == 0 ? 0 : 1)) * p.partial_floats;
         T* const to = static_cast<T*>(p.out) + now.b * p.out_stride[0] + r.token * p.out_stride[1] + r.head * p.out_stride[2];
+        if constexpr (WINDOW) {
+          if (whole && there && group == 0) write_lse(p, now.b, r, TcMath<T, DP>::log_sum(top, sum, p.scale_log2));
+        }
         // (small code: a launch meets it cold)
 #pragma unroll 1
         for (int c = group * (DP / 2); c < (group + 1) * (DP / 2); c += 8) {
@@ -431,7 +445,7 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
     }
   }
 
-  clear_rows_behind<T>(p, warp, kThreads / 32);
+  clear_rows_behind<T, WINDOW>(p, warp, kThreads / 32);
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (gave_up && threadIdx.x == 0) {
@@ -449,23 +463,29 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
 // tiles of 20 tiles and more: 101.7, 86.8, 82.0.
 constexpr int kItemUnits = 8;
 
-template <typename T, int DP, bool MANY>
+template <typename T, int DP, bool MANY, bool WINDOW>
 CacheAttnVariant tc_variant() {
   using Z = TcShape<T, DP>;
-  return CacheAttnVariant{cache_attention_tc_kernel<T, DP, MANY>, cache_attention_join_kernel<TcMath<T, DP>, 1>, kThreads, Z::kSmem, kRows, Z::G::kKeys, 4, kItemUnits,
+  return CacheAttnVariant{cache_attention_tc_kernel<T, DP, MANY, WINDOW>, cache_attention_join_kernel<TcMath<T, DP>, 1, WINDOW>, kThreads, Z::kSmem, kRows, Z::G::kKeys, 4, kItemUnits,
                           kPartOfWarp<TcMath<T, DP>>};
 }
-template <typename T, bool MANY>
+template <typename T, bool MANY, bool WINDOW>
 CacheAttnVariant tc_variant(int head_dim) {
-  return head_dim <= 64 ? tc_variant<T, 64, MANY>() : tc_variant<T, 128, MANY>();
+  return head_dim <= 64 ? tc_variant<T, 64, MANY, WINDOW>() : tc_variant<T, 128, MANY, WINDOW>();
+}
+template <bool WINDOW>
+CacheAttnVariant tc_variant(int dtype, int head_dim, int tokens) {
+  const bool many = tokens > kMaskAhead;
+  if (dtype == KB200_DTYPE_BF16) return many ? tc_variant<__nv_bfloat16, true, WINDOW>(head_dim) : tc_variant<__nv_bfloat16, false, WINDOW>(head_dim);
+  return many ? tc_variant<__half, true, WINDOW>(head_dim) : tc_variant<__half, false, WINDOW>(head_dim);
 }
 
 }  // namespace
 
-CacheAttnVariant cache_attention_tc_variant(int dtype, int head_dim, int tokens) {
-  const bool many = tokens > kMaskAhead;
-  if (dtype == KB200_DTYPE_BF16) return many ? tc_variant<__nv_bfloat16, true>(head_dim) : tc_variant<__nv_bfloat16, false>(head_dim);
-  return many ? tc_variant<__half, true>(head_dim) : tc_variant<__half, false>(head_dim);
-}
+#ifdef KB200_WINDOW
+CacheAttnVariant cache_attention_tc_window_variant(int dtype, int head_dim, int tokens) { return tc_variant<true>(dtype, head_dim, tokens); }
+#else
+CacheAttnVariant cache_attention_tc_variant(int dtype, int head_dim, int tokens) { return tc_variant<false>(dtype, head_dim, tokens); }
+#endif
 
 }  // namespace kb200

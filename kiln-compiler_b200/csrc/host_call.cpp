@@ -21,6 +21,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
+#include <memory>
 #include <mutex>
 #include <string>
 #include <vector>
@@ -174,23 +175,23 @@ PyObject* run(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
 struct CacheCaller {
   kb200_cache* cache;
   c10::Device device{c10::kCUDA, 0};
-  int64_t sequences, kv_heads, head_dim;
+  int64_t sequences, kv_heads, head_dim, width;      // width: tokens that a sequence may have
   c10::ScalarType type;
 };
 constexpr const char* kCacheCapsule = "kb200.cache";
 void destroy_cache_caller(PyObject* capsule) { delete static_cast<CacheCaller*>(PyCapsule_GetPointer(capsule, kCacheCapsule)); }
 
-// cache_caller(cache address, device index, sequences, kv heads, head dim, dtype code)
+// cache_caller(cache address, device index, sequences, kv heads, head dim, dtype code, tokens of a sequence)
 PyObject* make_cache_caller(PyObject*, PyObject* args) {
   HANDLE_TH_ERRORS
   unsigned long long cache;
   int device, type;
-  long long sequences, kv_heads, head_dim;
-  if (!PyArg_ParseTuple(args, "KiLLLi", &cache, &device, &sequences, &kv_heads, &head_dim, &type)) return nullptr;
+  long long sequences, kv_heads, head_dim, width;
+  if (!PyArg_ParseTuple(args, "KiLLLiL", &cache, &device, &sequences, &kv_heads, &head_dim, &type, &width)) return nullptr;
   auto c = std::make_unique<CacheCaller>();
   c->cache = reinterpret_cast<kb200_cache*>(cache);
   c->device = c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(device));
-  c->sequences = sequences, c->kv_heads = kv_heads, c->head_dim = head_dim;
+  c->sequences = sequences, c->kv_heads = kv_heads, c->head_dim = head_dim, c->width = width;
   c->type = type == KB200_DTYPE_FP32 ? c10::kFloat : type == KB200_DTYPE_BF16 ? c10::kBFloat16 : c10::kHalf;
   return PyCapsule_New(c.release(), kCacheCapsule, destroy_cache_caller);
   END_HANDLE_TH_ERRORS
@@ -354,10 +355,59 @@ PyObject* cache_accept(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// cache_attend(cache, layer, q, mask, counts, slots, scale, out) -> out
+// A call's mask, and its strides by batch row, token and drafted token.
+at::Tensor mask_of(const CacheCaller& c, PyObject* o, int64_t rows, int64_t tokens, int64_t (&stride)[3]) {
+  at::Tensor mask;
+  if (o == Py_None) return mask;
+  if (!THPVariable_Check(o) || THPVariable_Unpack(o).scalar_type() != c10::kBool) REFUSE(PyExc_TypeError, "mask must be a bool tensor");
+  mask = THPVariable_Unpack(o);
+  on_device(c, mask, "mask");
+  const bool each = mask.dim() == 3;
+  if (mask.dim() < 2 || mask.dim() > 3 || mask.size(-1) != tokens || mask.size(-2) != tokens || (each && mask.size(0) != rows))
+    REFUSE(PyExc_ValueError, "mask must be [%lld, %lld] or [%lld, %lld, %lld], got %s", (long long)tokens, (long long)tokens, (long long)rows, (long long)tokens,
+           (long long)tokens, text(mask.sizes()).c_str());
+  if (!has_memory(mask)) mask = mask.clone();
+  for (int i = 0; i < (int)mask.dim(); ++i) stride[i + (each ? 0 : 1)] = mask.stride(i);
+  return mask;
+}
+double scale_of(const CacheCaller& c, PyObject* o) {
+  if (o == Py_None) return 1.0 / std::sqrt((double)c.head_dim);
+  const double scale = PyFloat_AsDouble(o);
+  if (scale == -1.0 && PyErr_Occurred()) throw Refused();
+  return scale;
+}
+// A number of tokens.
+int tokens_of(PyObject* o, const char* name, long least) {
+  const long long value = PyLong_Check(o) && !PyBool_Check(o) ? PyLong_AsLongLong(o) : -1;
+  PyErr_Clear();
+  if (value < least || value > 2147483647) REFUSE(PyExc_ValueError, "%s must be an integer from %ld on", name, least);
+  return (int)value;
+}
+// float32 numbers that a call reads.
+const at::Tensor& floats_of(const CacheCaller& c, PyObject* o, const char* name, c10::IntArrayRef shape) {
+  const at::Tensor& t = tensor_of(o, name);
+  if (t.scalar_type() != c10::kFloat) REFUSE(PyExc_TypeError, "%s must hold float32", name);
+  if (t.sizes() != shape) REFUSE(PyExc_ValueError, "%s must have shape %s, got %s", name, text(shape).c_str(), text(t.sizes()).c_str());
+  on_device(c, t, name);
+  return t;
+}
+// ... and that it writes.
+const at::Tensor& floats_to(const CacheCaller& c, PyObject* o, const char* name, c10::IntArrayRef shape) {
+  const at::Tensor& t = floats_of(c, o, name, shape);
+  if (!has_memory(t)) REFUSE(PyExc_ValueError, "%s has no memory of its own", name);
+  if (t.requires_grad()) REFUSE(PyExc_ValueError, "%s requires a gradient", name);
+  if (at::has_internal_overlap(t) == at::MemOverlap::Yes) REFUSE(PyExc_ValueError, "elements of %s share memory", name);
+  return t;
+}
+void apart(const at::Tensor& a, const at::Tensor& b, const char* name_a, const char* name_b) {
+  const at::MemOverlapStatus is = at::get_overlap_status(a, b);
+  if (is == at::MemOverlapStatus::Partial || is == at::MemOverlapStatus::Full) REFUSE(PyExc_ValueError, "%s shares memory with %s", name_a, name_b);
+}
+
+// cache_attend(cache, layer, q, mask, counts, slots, scale, out, window, sinks, places, lse) -> out
 PyObject* cache_attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (!n_args(n, 8)) return nullptr;
+  if (!n_args(n, 12)) return nullptr;
   try {
     CacheCaller& c = cache_of(args[0]);
     const c10::cuda::CUDAGuard guard(c.device);
@@ -367,27 +417,21 @@ PyObject* cache_attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (heads == 0 || heads % c.kv_heads != 0) REFUSE(PyExc_ValueError, "%lld heads are no multiple of the cache's %lld", (long long)heads, (long long)c.kv_heads);
     batch_ok(c, rows, args[5]);
     if (tokens >= 2147483647 || heads >= 2147483647) REFUSE(PyExc_ValueError, "too many tokens or heads");
-    at::Tensor mask;
     int64_t mask_stride[3] = {0, 0, 0};
-    if (args[3] != Py_None) {
-      if (!THPVariable_Check(args[3]) || THPVariable_Unpack(args[3]).scalar_type() != c10::kBool) REFUSE(PyExc_TypeError, "mask must be a bool tensor");
-      mask = THPVariable_Unpack(args[3]);
-      on_device(c, mask, "mask");
-      const bool each = mask.dim() == 3;
-      if (mask.dim() < 2 || mask.dim() > 3 || mask.size(-1) != tokens || mask.size(-2) != tokens || (each && mask.size(0) != rows))
-        REFUSE(PyExc_ValueError, "mask must be [%lld, %lld] or [%lld, %lld, %lld], got %s", (long long)tokens, (long long)tokens, (long long)rows, (long long)tokens,
-               (long long)tokens, text(mask.sizes()).c_str());
-      if (!has_memory(mask)) mask = mask.clone();
-      for (int i = 0; i < (int)mask.dim(); ++i) mask_stride[i + (each ? 0 : 1)] = mask.stride(i);
-    }
+    const at::Tensor mask = mask_of(c, args[3], rows, tokens, mask_stride);
     const at::Tensor counts = integers_or_none(c, args[4], "counts", rows), slots = integers_or_none(c, args[5], "slots", rows);
-    double scale = 0.0;
-    if (args[6] == Py_None) {
-      scale = 1.0 / std::sqrt((double)c.head_dim);
-    } else {
-      scale = PyFloat_AsDouble(args[6]);
-      if (scale == -1.0 && PyErr_Occurred()) return nullptr;
+    const double scale = scale_of(c, args[6]);
+    const int window = args[8] == Py_None ? 0 : tokens_of(args[8], "window", 1), sinks = tokens_of(args[9], "sinks", 0);
+    if (window == 0 && (sinks != 0 || args[10] != Py_None)) REFUSE(PyExc_ValueError, "sinks and places go with a window");
+    at::Tensor places, lse;
+    int64_t lse_stride[3] = {0, 0, 0};
+    if (args[10] != Py_None) places = integers(c, args[10], "places", {rows, tokens});
+    if (args[11] != Py_None) {
+      lse = floats_to(c, args[11], "lse", {rows, tokens, heads});
+      apart(lse, q.t, "lse", "q");
+      for (int i = 0; i < 3; ++i) lse_stride[i] = lse.stride(i);
     }
+    const bool beside = window > 0 || lse.defined();
     at::Tensor out;
     if (args[7] == Py_None) {
       out = at::detail::empty_cuda({rows, tokens, heads, c.head_dim}, c.type, c.device, std::nullopt);
@@ -401,14 +445,21 @@ PyObject* cache_attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
       if (at::has_internal_overlap(out) == at::MemOverlap::Yes) REFUSE(PyExc_ValueError, "elements of out share memory");
       if (at::get_overlap_status(out, q.t) == at::MemOverlapStatus::Partial) REFUSE(PyExc_ValueError, "out shares part of q's memory");
     }
+    if (lse.defined()) apart(lse, out, "lse", "out");
     const TokenRows to(out);
     if (rows > 0 && tokens > 0) {
-      const uint64_t bytes = kb200_cache_attend_workspace(c.cache, (int)rows, (int)tokens, (int)heads);
+      const uint64_t bytes = beside ? kb200_cache_attend_window_workspace(c.cache, (int)rows, (int)tokens, (int)heads, window, sinks)
+                                    : kb200_cache_attend_workspace(c.cache, (int)rows, (int)tokens, (int)heads);
       // the kernels write into it (said first: it raises for a tensor that may not change)
       if (args[7] != Py_None && to.t.is_same(out)) out.unsafeGetTensorImpl()->bump_version();
+      if (lse.defined()) lse.unsafeGetTensorImpl()->bump_version();
       at::Tensor workspace;                            // (of this call alone; its memory is used again behind the kernels, on their stream)
       if (bytes > 0) workspace = at::detail::empty_cuda({(int64_t)bytes}, c10::kByte, c.device, std::nullopt);
       PyObject* const done = enqueue(c, [&](cudaStream_t s) {
+        if (beside)
+          return kb200_cache_attend_window(c.cache, layer, &q.rows, &to.rows, (int)rows, (int)tokens, mask.defined() ? static_cast<const uint8_t*>(mask.const_data_ptr()) : nullptr,
+                                           mask_stride, at_of(counts), at_of(slots), (float)scale, window, sinks, at_of(places),
+                                           lse.defined() ? static_cast<float*>(lse.mutable_data_ptr()) : nullptr, lse_stride, bytes > 0 ? workspace.mutable_data_ptr() : nullptr, bytes, s);
         return kb200_cache_attend(c.cache, layer, &q.rows, &to.rows, (int)rows, (int)tokens, mask.defined() ? static_cast<const uint8_t*>(mask.const_data_ptr()) : nullptr,
                                   mask_stride, at_of(counts), at_of(slots), (float)scale, bytes > 0 ? workspace.mutable_data_ptr() : nullptr, bytes, s);
       });
@@ -430,18 +481,212 @@ PyObject* cache_attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// cache_release(cache, window, sinks)
+PyObject* cache_release(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!n_args(n, 3)) return nullptr;
+  try {
+    CacheCaller& c = cache_of(args[0]);
+    const int window = tokens_of(args[1], "window", 1), sinks = tokens_of(args[2], "sinks", 0);
+    return enqueue(c, [&](cudaStream_t s) { return kb200_cache_release(c.cache, window, sinks, s); });
+  } catch (const Refused&) {
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+// A number for each token of each sequence, [sequences, width] of float32: where a call reads and writes them.  What is not laid out row by row is copied.
+struct TokenWeights {
+  at::Tensor from, to, result;         // result: what the caller gets
+  TokenWeights(const CacheCaller& c, PyObject* weights, PyObject* out) {
+    const std::vector<int64_t> shape = {c.sequences, c.width};
+    if (weights != Py_None) {
+      from = floats_of(c, weights, "weights", shape);
+      if (!has_memory(from) || !by_rows(from)) {
+        const c10::NoGradGuard no_grad;
+        from = from.clone(at::MemoryFormat::Contiguous);
+      }
+    }
+    if (out == Py_None) {
+      to = result = at::detail::empty_cuda(shape, c10::kFloat, c.device, std::nullopt);
+      return;
+    }
+    to = result = floats_to(c, out, "out", shape);
+    if (from.defined() && at::get_overlap_status(to, from) == at::MemOverlapStatus::Partial) REFUSE(PyExc_ValueError, "out shares part of the weights' memory");
+    if (!by_rows(to)) to = at::detail::empty_cuda(shape, c10::kFloat, c.device, std::nullopt);
+  }
+  static bool by_rows(const at::Tensor& t) { return t.stride(1) == 1 && (t.size(0) == 1 || t.stride(0) >= t.size(1)); }
+  const float* read() const { return from.defined() ? static_cast<const float*>(from.const_data_ptr()) : nullptr; }
+  int64_t read_stride() const { return from.defined() ? from.stride(0) : 0; }
+  // (said first: it raises for a tensor that may not change)
+  float* write() const {
+    if (to.is_same(result)) to.unsafeGetTensorImpl()->bump_version();
+    return static_cast<float*>(to.mutable_data_ptr());
+  }
+  PyObject* done(PyObject* out) {
+    if (!to.is_same(result)) {
+      const c10::NoGradGuard no_grad;
+      result.copy_(to);
+    }
+    if (out == Py_None) return THPVariable_Wrap(std::move(result));
+    Py_INCREF(out);
+    return out;
+  }
+};
+
+// cache_weigh(cache, layer, q, lse, weights, mask, counts, slots, scale, out) -> out
+PyObject* cache_weigh(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!n_args(n, 10)) return nullptr;
+  try {
+    CacheCaller& c = cache_of(args[0]);
+    const c10::cuda::CUDAGuard guard(c.device);
+    const int layer = layer_of(args[1]);
+    const TokenRows q(c, args[2], "q", -1);
+    const int64_t rows = q.t.size(0), tokens = q.t.size(1), heads = q.t.size(2);
+    if (heads == 0 || heads % c.kv_heads != 0) REFUSE(PyExc_ValueError, "%lld heads are no multiple of the cache's %lld", (long long)heads, (long long)c.kv_heads);
+    batch_ok(c, rows, args[7]);
+    if (tokens >= 2147483647 || heads >= 2147483647) REFUSE(PyExc_ValueError, "too many tokens or heads");
+    at::Tensor lse = floats_of(c, args[3], "lse", {rows, tokens, heads});
+    if (!has_memory(lse)) lse = lse.clone();
+    int64_t mask_stride[3] = {0, 0, 0};
+    const at::Tensor mask = mask_of(c, args[5], rows, tokens, mask_stride);
+    const at::Tensor counts = integers_or_none(c, args[6], "counts", rows), slots = integers_or_none(c, args[7], "slots", rows);
+    const double scale = scale_of(c, args[8]);
+    TokenWeights w(c, args[4], args[9]);
+    apart(w.to, q.t, "out", "q");
+    apart(w.to, lse, "out", "lse");
+    const int64_t lse_stride[3] = {lse.stride(0), lse.stride(1), lse.stride(2)};
+    float* const to = w.write();
+    PyObject* const done = enqueue(c, [&](cudaStream_t s) {
+      return kb200_cache_weigh(c.cache, layer, &q.rows, static_cast<const float*>(lse.const_data_ptr()), lse_stride, (int)rows, (int)tokens,
+                               mask.defined() ? static_cast<const uint8_t*>(mask.const_data_ptr()) : nullptr, mask_stride, at_of(counts), at_of(slots), (float)scale, w.read(),
+                               w.read_stride(), to, w.to.stride(0), s);
+    });
+    if (done == nullptr) return nullptr;
+    Py_DECREF(done);
+    return w.done(args[9]);
+  } catch (const Refused&) {
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+// cache_evict(cache, weights, keep, recent, sinks, out) -> out
+PyObject* cache_evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!n_args(n, 6)) return nullptr;
+  try {
+    CacheCaller& c = cache_of(args[0]);
+    const c10::cuda::CUDAGuard guard(c.device);
+    if (args[1] == Py_None) REFUSE(PyExc_TypeError, "weights must be a tensor");
+    const at::Tensor keep = integers(c, args[2], "keep", {c.sequences});
+    const int recent = tokens_of(args[3], "recent", 0), sinks = tokens_of(args[4], "sinks", 0);
+    TokenWeights w(c, args[1], args[5]);
+    const uint64_t bytes = kb200_cache_evict_workspace(c.cache);
+    const at::Tensor workspace = at::detail::empty_cuda({(int64_t)bytes}, c10::kByte, c.device, std::nullopt);
+    float* const to = w.write();
+    PyObject* const done = enqueue(c, [&](cudaStream_t s) {
+      return kb200_cache_evict(c.cache, w.read(), w.read_stride(), at_of(keep), recent, sinks, to, w.to.stride(0), workspace.mutable_data_ptr(), bytes, s);
+    });
+    if (done == nullptr) return nullptr;
+    Py_DECREF(done);
+    return w.done(args[5]);
+  } catch (const Refused&) {
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+// Rows over a vocabulary, [rows, tokens, vocabulary]: copied where the kernels cannot read them as they are.
+struct VocabularyRows {
+  at::Tensor t;
+  kb200_scores scores;
+  VocabularyRows(const CacheCaller& c, PyObject* o, const char* name, c10::IntArrayRef shape) : t(tensor_of(o, name)) {
+    if (t.dim() != 3 || (!shape.empty() && t.sizes() != shape))
+      REFUSE(PyExc_ValueError, "%s must be %s, got %s", name, shape.empty() ? "[rows, tokens, vocabulary]" : text(shape).c_str(), text(t.sizes()).c_str());
+    const c10::ScalarType type = t.scalar_type();
+    if (type != c10::kFloat && type != c10::kBFloat16 && type != c10::kHalf) REFUSE(PyExc_TypeError, "%s must hold float32, bfloat16 or float16", name);
+    on_device(c, t, name);
+    if (!has_memory(t) || (t.stride(2) != 1 && t.size(2) != 1)) {
+      const c10::NoGradGuard no_grad;
+      t = t.clone(at::MemoryFormat::Contiguous);
+    }
+    scores = kb200_scores{t.const_data_ptr(), type == c10::kFloat ? KB200_DTYPE_FP32 : type == c10::kBFloat16 ? KB200_DTYPE_BF16 : KB200_DTYPE_FP16, 0, {t.stride(0), t.stride(1)}};
+  }
+};
+
+// cache_verify(cache, logits, tokens, uniform, draft, parents, counts, slots, temperature) -> (n_accepted, accepted, following)
+PyObject* cache_verify(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!n_args(n, 9)) return nullptr;
+  try {
+    CacheCaller& c = cache_of(args[0]);
+    const c10::cuda::CUDAGuard guard(c.device);
+    const VocabularyRows logits(c, args[1], "logits", {});
+    const int64_t rows = logits.t.size(0), tokens = logits.t.size(1), vocab = logits.t.size(2);
+    batch_ok(c, rows, args[7]);
+    if (rows > 1 << 20 || tokens > 512 || vocab < 1 || vocab >= 1 << 30)
+      REFUSE(PyExc_ValueError, "logits must be of at most 2^20 rows, 512 tokens and fewer than 2^30 numbers each, got %s", text(logits.t.sizes()).c_str());
+    const at::Tensor drafted = integers(c, args[2], "tokens", {rows, tokens});
+    auto contiguous = [&](PyObject* o, const char* name, c10::IntArrayRef shape) {
+      const at::Tensor& t = floats_of(c, o, name, shape);
+      return t.is_contiguous() && has_memory(t) ? t : t.clone(at::MemoryFormat::Contiguous);
+    };
+    const at::Tensor uniform = contiguous(args[3], "uniform", {rows, tokens});
+    std::unique_ptr<VocabularyRows> draft;
+    if (args[4] != Py_None) draft = std::make_unique<VocabularyRows>(c, args[4], "draft", logits.t.sizes());
+    at::Tensor parents, temperature;
+    int64_t parents_stride = tokens;
+    if (args[5] != Py_None) {
+      const bool each = tensor_of(args[5], "parents").dim() != 1;
+      parents = each ? integers(c, args[5], "parents", {rows, tokens}) : integers(c, args[5], "parents", {tokens});
+      parents_stride = each ? tokens : 0;
+    }
+    const at::Tensor counts = integers_or_none(c, args[6], "counts", rows), slots = integers_or_none(c, args[7], "slots", rows);
+    if (args[8] != Py_None) temperature = contiguous(args[8], "temperature", {rows});
+    auto whole = [&](c10::IntArrayRef shape) { return at::detail::empty_cuda(shape, c10::kInt, c.device, std::nullopt); };
+    at::Tensor n_accepted = whole({c.sequences}), accepted = whole({c.sequences, tokens}), following = whole({c.sequences});
+    const uint64_t bytes = kb200_cache_verify_workspace(c.cache, (int)rows, (int)tokens, (int)vocab);
+    at::Tensor workspace;
+    if (bytes > 0) workspace = at::detail::empty_cuda({(int64_t)bytes}, c10::kByte, c.device, std::nullopt);
+    PyObject* const done = enqueue(c, [&](cudaStream_t s) {
+      return kb200_cache_verify(c.cache, &logits.scores, draft ? &draft->scores : nullptr, (int)rows, (int)tokens, (int)vocab, at_of(drafted), at_of(parents), parents_stride,
+                                static_cast<const float*>(uniform.const_data_ptr()), temperature.defined() ? static_cast<const float*>(temperature.const_data_ptr()) : nullptr,
+                                at_of(counts), at_of(slots), static_cast<int32_t*>(n_accepted.mutable_data_ptr()), static_cast<int32_t*>(accepted.mutable_data_ptr()),
+                                static_cast<int32_t*>(following.mutable_data_ptr()), bytes > 0 ? workspace.mutable_data_ptr() : nullptr, bytes, s);
+    });
+    if (done == nullptr) return nullptr;
+    Py_DECREF(done);
+    PyObject* const a = THPVariable_Wrap(std::move(n_accepted));
+    PyObject* const b = THPVariable_Wrap(std::move(accepted));
+    PyObject* const f = THPVariable_Wrap(std::move(following));
+    PyObject* const all = a && b && f ? PyTuple_Pack(3, a, b, f) : nullptr;
+    Py_XDECREF(a), Py_XDECREF(b), Py_XDECREF(f);
+    return all;
+  } catch (const Refused&) {
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
 template <typename F>
 PyCFunction fast(F f) { return reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(f)); }
 
 PyMethodDef methods[] = {
-    {"cache_caller", make_cache_caller, METH_VARARGS, "cache_caller(cache, device, sequences, kv_heads, head_dim, dtype)"},
+    {"cache_caller", make_cache_caller, METH_VARARGS, "cache_caller(cache, device, sequences, kv_heads, head_dim, dtype, tokens)"},
     {"cache_fork", fast(cache_fork), METH_FASTCALL, "cache_fork(cache, sources)"},
     {"cache_reserve", fast(cache_reserve), METH_FASTCALL, "cache_reserve(cache, counts)"},
     {"cache_truncate", fast(cache_truncate), METH_FASTCALL, "cache_truncate(cache, lengths)"},
     {"cache_compact", fast(cache_compact), METH_FASTCALL, "cache_compact(cache)"},
     {"cache_append", fast(cache_append), METH_FASTCALL, "cache_append(cache, layer, k, v, counts, slots)"},
     {"cache_accept", fast(cache_accept), METH_FASTCALL, "cache_accept(cache, counts, kept)"},
-    {"cache_attend", fast(cache_attend), METH_FASTCALL, "cache_attend(cache, layer, q, mask, counts, slots, scale, out) -> out"},
+    {"cache_attend", fast(cache_attend), METH_FASTCALL, "cache_attend(cache, layer, q, mask, counts, slots, scale, out, window, sinks, places, lse) -> out"},
+    {"cache_release", fast(cache_release), METH_FASTCALL, "cache_release(cache, window, sinks)"},
+    {"cache_weigh", fast(cache_weigh), METH_FASTCALL, "cache_weigh(cache, layer, q, lse, weights, mask, counts, slots, scale, out) -> out"},
+    {"cache_evict", fast(cache_evict), METH_FASTCALL, "cache_evict(cache, weights, keep, recent, sinks, out) -> out"},
+    {"cache_verify", fast(cache_verify), METH_FASTCALL,
+     "cache_verify(cache, logits, tokens, uniform, draft, parents, counts, slots, temperature) -> (n_accepted, accepted, following)"},
     {"caller", make_caller, METH_VARARGS, "caller(plan, device, input_shapes, output_shapes, fixed_inputs)"},
     {"run", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(run)), METH_FASTCALL, "run(caller, *inputs) -> list of output tensors"},
     {nullptr, nullptr, 0, nullptr}};

@@ -16,7 +16,7 @@ import subprocess
 import sysconfig
 from pathlib import Path
 
-ABI_VERSION = 6
+ABI_VERSION = 7
 MAX_RANK, MAX_OPERANDS, MAX_TAPE = 6, 12, 96
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -77,6 +77,10 @@ class Rows(C.Structure):
     _fields_ = [("data", C.c_void_p), ("dtype", C.c_int32), ("heads", C.c_int32), ("stride", C.c_int64 * 3)]
 
 
+class Scores(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("dtype", C.c_int32), ("pad", C.c_int32), ("stride", C.c_int64 * 2)]
+
+
 EXPORTS = {
     "kb200_version": (C.c_int, []),
     "kb200_last_error": (C.c_char_p, []),
@@ -112,6 +116,21 @@ EXPORTS = {
     "kb200_cache_attend_workspace": (C.c_uint64, [C.c_void_p, C.c_int, C.c_int, C.c_int]),
     "kb200_cache_attend": (C.c_int, [C.c_void_p, C.c_int, C.POINTER(Rows), C.POINTER(Rows), C.c_int, C.c_int, C.c_void_p,
                                      C.POINTER(C.c_int64), C.c_void_p, C.c_void_p, C.c_float, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "kb200_cache_attend_window_workspace": (C.c_uint64, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "kb200_cache_attend_window": (C.c_int, [C.c_void_p, C.c_int, C.POINTER(Rows), C.POINTER(Rows), C.c_int, C.c_int, C.c_void_p,
+                                            C.POINTER(C.c_int64), C.c_void_p, C.c_void_p, C.c_float, C.c_int, C.c_int, C.c_void_p, C.c_void_p,
+                                            C.POINTER(C.c_int64), C.c_void_p, C.c_uint64, C.c_void_p]),
+    "kb200_cache_release": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
+    "kb200_cache_weigh": (C.c_int, [C.c_void_p, C.c_int, C.POINTER(Rows), C.c_void_p, C.POINTER(C.c_int64), C.c_int, C.c_int, C.c_void_p,
+                                    C.POINTER(C.c_int64), C.c_void_p, C.c_void_p, C.c_float, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                    C.c_void_p]),
+    "kb200_cache_evict_workspace": (C.c_uint64, [C.c_void_p]),
+    "kb200_cache_evict": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_int64, C.c_void_p,
+                                    C.c_uint64, C.c_void_p]),
+    "kb200_cache_verify_workspace": (C.c_uint64, [C.c_void_p, C.c_int, C.c_int, C.c_int]),
+    "kb200_cache_verify": (C.c_int, [C.c_void_p, C.POINTER(Scores), C.POINTER(Scores), C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p,
+                                     C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                     C.c_void_p, C.c_uint64, C.c_void_p]),
     "kb200_cache_status": (C.c_int, [C.c_void_p]),
     "kb200_cache_destroy": (None, [C.c_void_p]),
 }

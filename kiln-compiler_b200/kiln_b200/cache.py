@@ -9,9 +9,13 @@ prompt, and the attention of new tokens over them.  One step of a server that dr
         q, k, v = ...                                      # of the drafted tokens, from the compiled modules
         cache.append(layer, k, v, counts)
         out = cache.attend(layer, q, mask, counts)         # over the sequence and the drafted tokens each one follows
+    n_accepted, accepted, following = cache.verify(logits, tokens, uniform, draft, parents, counts)
     cache.accept(n_accepted, accepted)                     # the accepted ones become the sequence's
 
 Ordinary decoding drafts one token and accepts it; a prompt is a chain of tokens (no mask) that are all accepted.
+
+A sequence need not keep all of its tokens.  With a sliding window and a few first tokens (``attend(..., window=, sinks=)``) ``release`` gives the pages behind the window
+back; or ``weigh`` adds up what weight its tokens draw (from ``attend(..., lse=)``), and ``evict`` keeps the heaviest.
 
 All arguments and all of the cache's state are tensors on the GPU, every call is enqueued on the current stream, and none waits for the GPU: a step can be
 captured into a CUDA graph whose replays follow what the tensors hold then; the cache has to live until the last of them has run.  Calls that change the cache are
@@ -73,7 +77,7 @@ class PagedCache:
         desc.table, desc.held, desc.lengths, desc.refs = (t.data_ptr() for t in (self.table, self.held, self.lengths, self.refs))
         self._call = _cabi.load_call()
         _cabi.check(self._lib.kb200_cache_create(C.byref(desc), self.device.index, C.byref(self._cache)), self._lib)
-        self._caller = self._call.cache_caller(self._cache.value, self.device.index, sequences, kv_heads, head_dim, DTYPES[dtype])
+        self._caller = self._call.cache_caller(self._cache.value, self.device.index, sequences, kv_heads, head_dim, DTYPES[dtype], max_pages * page_tokens)
 
     # -- pages -----------------------------------------------------------------------------------
 
@@ -105,19 +109,53 @@ class PagedCache:
         or the first ones; the rest is dropped and its pages are free."""
         self._call.cache_accept(self._caller, counts, kept)
 
-    def attend(self, layer, q, mask=None, counts=None, slots=None, scale=None, out=None):
+    def attend(self, layer, q, mask=None, counts=None, slots=None, scale=None, out=None, window=None, sinks=0, places=None, lse=None):
         """Attention of the first ``counts[b]`` tokens of every row of ``q`` [rows, tokens, heads, head_dim] over the committed tokens of
         sequence ``slots[b]`` (default: ``b``) and, of the ``counts[b]`` tokens appended behind them, those that ``mask`` ([tokens, tokens]
         or [rows, tokens, tokens], bool; default: itself and those before it) shows.  ``heads`` is a multiple of the cache's; scale defaults to
         ``head_dim ** -0.5``.  Returns ``out``, of the cache's type, with zeros in rows of no token and in rows that see nothing; it may be ``q``
-        itself, but not share part of its memory."""
-        return self._call.cache_attend(self._caller, layer, q, mask, counts, slots, scale, out)
+        itself, but not share part of its memory.
+
+        ``window``: a token sees itself and the ``window - 1`` tokens before it, and the sequence's first ``sinks``.  Which of the drafted tokens a mask shows
+        is the mask's matter; a token of a tree stands ``places[b, i]`` (its depth, from 0 to ``tokens - 1``; default: ``i``) behind the committed ones.
+        ``lse``: a float32 tensor [rows, tokens, heads] that gets the logarithm of each row's sum of exponentials (-inf where a row sees nothing)."""
+        return self._call.cache_attend(self._caller, layer, q, mask, counts, slots, scale, out, window, sinks, places, lse)
+
+    def verify(self, logits, tokens, uniform, draft=None, parents=None, counts=None, slots=None, temperature=None):
+        """Which of the drafted ``tokens`` [rows, tokens] the model accepts, by its ``logits`` [rows, tokens, vocabulary] of what follows each of them and by given
+        random numbers ``uniform`` [rows, tokens] from [0, 1): ``(n_accepted, accepted, following)``, by sequence, the first two as ``accept`` takes them and the third the token
+        that comes next (-1: none).  What is returned is distributed as the model's own samples.
+
+        Token 0 of a row followed the last step and is not in question; token ``i`` was drafted behind token ``parents[i]`` or ``parents[b, i]`` (default: ``i - 1``), by the
+        probabilities ``draft[b, parent]`` or, without ``draft``, without chance.  Of several that follow the same token the first one that is accepted counts.
+        ``temperature`` [rows], float32 (default: 1); 0 stands for the largest logit."""
+        return self._call.cache_verify(self._caller, logits, tokens, uniform, draft, parents, counts, slots, temperature)
+
+    # -- what a sequence gives up before its end ---------------------------------------------------
+
+    def release(self, window, sinks=0):
+        """Gives back the pages of every sequence that no token to come will see through this ``window``, none of whose tokens are among the first ``sinks``.
+        The sequences keep their lengths; ``attend`` with that window (or a smaller one) goes on as before."""
+        self._call.cache_release(self._caller, window, sinks)
+
+    def weigh(self, layer, q, lse, weights=None, mask=None, counts=None, slots=None, scale=None, out=None):
+        """Adds up what weight the tokens of the sequences draw: ``weights`` [sequences, max_pages * page_tokens] (float32; default: zeros) plus the sum over heads and over the first
+        ``counts[b]`` rows of ``q`` of the weights that ``attend`` (without a window) gave them, whose ``lse`` this takes.  Returns ``out``, which may be ``weights``.
+        To be called before ``accept``, of tokens that are going to be accepted where they stand.  ``slots`` names no sequence twice."""
+        return self._call.cache_weigh(self._caller, layer, q, lse, weights, mask, counts, slots, scale, out)
+
+    def evict(self, weights, keep, recent=0, sinks=0, out=None):
+        """Keeps ``keep[s]`` committed tokens of every sequence, in all layers: the first ``sinks``, the last ``recent`` and, of the others, the heaviest (of equal ones the
+        first).  They become its first tokens, in their order, and its other pages are free.  A negative entry, or a sequence of no more tokens, changes nothing.
+        Returns ``out`` (which may be ``weights``): the weights of the tokens that are left, zeros behind them."""
+        return self._call.cache_evict(self._caller, weights, keep, recent, sinks, out)
 
     # -- the rest --------------------------------------------------------------------------------
 
     def status(self):
         """Waits for the current stream and raises if an operation since the last check left something out: MemoryError for a
-        reservation beyond the free pages, ValueError for indexes or counts out of range, tokens without a page, writes into shared pages."""
+        reservation beyond the free pages, ValueError for indexes or counts out of range, tokens without a page, writes into shared pages, logits that are no
+        distribution."""
         torch.cuda.current_stream(self.device).synchronize()
         _cabi.check(self._lib.kb200_cache_status(self._cache), self._lib)
 
