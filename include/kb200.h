@@ -467,7 +467,8 @@ int kb200_cache_attend_window(kb200_cache* cache, int layer, const kb200_rows* q
                               void* workspace, uint64_t workspace_bytes, void* cuda_stream);
 
 /* Gives back the pages that a window has left: those of which every token j has j >= sinks and j <= lengths[s] - window, so that no token to come sees it (places of 0
- * and more).  Their entries become -1; held and lengths stay.  What reads them afterwards (a larger window, kb200_cache_attend) is told KB200_CACHE_BAD_INDEX. */
+ * and more).  Their entries become -1; held and lengths stay.  What needs them afterwards (a larger window, kb200_cache_attend, room behind a sequence that was truncated into
+ * them) is told KB200_CACHE_BAD_INDEX. */
 int kb200_cache_release(kb200_cache* cache, int window, int sinks, void* cuda_stream);
 
 /* The weight that the tokens of a sequence draw: out[s, j] = weights[s, j] + sum over i < counts[b] and heads h of exp(scale * q[b, i, h] . k[j, g] - lse[b, i, h]) for the tokens
@@ -482,7 +483,8 @@ int kb200_cache_weigh(kb200_cache* cache, int layer, const kb200_rows* q, const 
  * by weights[s] (of equal ones the first; NaN is heaviest); fewer than the first and last ones where keep[s] is less.  They keep their order and become the sequence's first keep[s]
  * tokens; the pages behind them are free, what was reserved too.  A negative entry, or one of lengths[s] and more, leaves the sequence as it is.
  * out[s]: the weights of the tokens that the sequence then has, zeros behind them.  weights and out: as in kb200_cache_weigh; out may be weights.
- * A sequence whose tokens would move within pages that were shared before the call, or from pages that it does not have, stays as it is.
+ * A sequence whose tokens would move within pages that were shared before the call, or that would keep tokens of pages that it does not have (kb200_cache_release), stays
+ * as it is.
  * workspace: kb200_cache_evict_workspace bytes, 16-byte aligned, used by this call alone until it has run. */
 uint64_t kb200_cache_evict_workspace(const kb200_cache* cache);
 int kb200_cache_evict(kb200_cache* cache, const float* weights, int64_t weights_stride, const int32_t* keep, int recent, int sinks,

@@ -301,6 +301,8 @@ __global__ void __launch_bounds__(kTableThreads) reserve_kernel(const CacheView 
         if (cache_page_ok(c, old)) {
           atomicSub(c.refs + old, 1);
           if (k == r.first && r.rows > 0) w.copies[atomicAdd(w.counters + kCopies, 1)] = make_int4(old, page, r.rows, 0);
+        } else if (k == r.first && r.rows > 0) {
+          cache_fault(c, KB200_CACHE_BAD_INDEX);             // committed tokens whose page is gone (truncated into what was released)
         }
       }
       next += __popc(all_fresh);

@@ -150,10 +150,8 @@ __global__ void __launch_bounds__(kChooseThreads) evict_choose_kernel(const Cach
         const int at = places + __popc(all_stay & below), page = row[j >> c.page_log2];
         kept[at] = ((int64_t)page << c.page_log2) + (j & in_page);
         staged[at] = w;
-        if (at != j) {
-          moved = min(moved, at);
-          fault |= cache_page_ok(c, page) ? 0 : KB200_CACHE_NO_ROOM;
-        }
+        if (at != j) moved = min(moved, at);
+        fault |= cache_page_ok(c, page) ? 0 : KB200_CACHE_NO_ROOM;
       }
       places += __popc(all_stay);
       equal += __popc(all_tied);

@@ -81,20 +81,20 @@ struct RowOf {
   }
 };
 
-// A row's sequence, or -1 where the row is left out; drafted tokens.  By all threads of a CTA.
+// A row's sequence, or -1 where that is not the row's; drafted tokens, none where the row is left out.  By all threads of a CTA.
 __device__ __forceinline__ int row_slot(const VerifyParams& p, int b, int* count, float* temperature, bool tell) {
   const int slot = p.slots != nullptr ? p.slots[b] : b;
   int n = p.counts != nullptr ? p.counts[b] : p.width;
   const float t = p.temperature != nullptr ? p.temperature[b] : 1.0f;
-  bool bad = (unsigned)slot >= (unsigned)p.c.sequences || !(t >= 0.0f && t < CUDART_INF_F);
-  bool again = false;
+  bool bad = (unsigned)slot >= (unsigned)p.c.sequences, again = false;
+  const bool cold = !(t >= 0.0f && t < CUDART_INF_F);
   if (p.slots != nullptr) {              // a sequence that an earlier row names is that row's
     for (int i = threadIdx.x; i < b; i += blockDim.x) again = again || p.slots[i] == slot;
     again = __syncthreads_or(again);
   }
   bad = bad || again;
-  if ((bad || n < 0 || n > p.width) && tell && threadIdx.x == 0) cache_fault(p.c, KB200_CACHE_BAD_INDEX);
-  *count = min(max(n, 0), p.width);
+  if ((bad || cold || n < 0 || n > p.width) && tell && threadIdx.x == 0) cache_fault(p.c, KB200_CACHE_BAD_INDEX);
+  *count = cold ? 0 : min(max(n, 0), p.width);
   *temperature = t;
   return bad ? -1 : slot;
 }

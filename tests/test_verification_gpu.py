@@ -1,0 +1,327 @@
+"""Verification of drafted tokens on the GPU (``PagedCache.verify``): against the rules in float64, token for token."""
+
+import random
+
+import numpy as np
+import pytest
+import torch
+
+from kiln_b200 import _cabi
+from oracle.cache_oracle import BAD_INDEX
+from oracle.cache_steps_oracle import BAD_VALUE, verify as by_the_rules
+from test_paged_cache_gpu import BF16, F16, F32, ints
+
+pytestmark = pytest.mark.gpu
+
+
+def cache_of(sequences):
+    from kiln_b200.cache import PagedCache
+
+    return PagedCache(layers=1, sequences=sequences, max_pages=4, pages=4 * sequences, kv_heads=1, head_dim=16, page_tokens=16)
+
+
+def faults_of(cache):
+    torch.cuda.synchronize()
+    try:
+        cache.status()
+    except ValueError as e:
+        return (BAD_INDEX if "out of range" in str(e) else 0) | (BAD_VALUE if "no distribution" in str(e) else 0)
+    return 0
+
+
+def drafts(rows, tokens, vocab, dtype, draft_dtype, seed=0, trees=False, spread=2.5, noise=0.7, temperature=None):
+    """Logits, and tokens as a small model draws them that knows much of what the large one does."""
+    generator = torch.Generator("cuda").manual_seed(seed)
+    dice = random.Random(seed)
+    logits = (torch.randn(rows, tokens, vocab, device="cuda", generator=generator) * spread).to(dtype)
+    t = torch.ones(rows, device="cuda") if temperature is None else temperature.clamp_min(0.3)
+    q = torch.softmax(logits.float() / t[:, None, None] + noise * torch.randn(rows, tokens, vocab, device="cuda", generator=generator), -1)
+    parents = [[-1] + [dice.randint(max(0, i - 3), i - 1) if trees else i - 1 for i in range(1, tokens)] for _ in range(rows)]
+    of = torch.tensor(parents, device="cuda").clamp_min(0)
+    drawn = q[torch.arange(rows, device="cuda")[:, None], of].reshape(-1, vocab)
+    chosen = torch.multinomial(drawn, 1, generator=generator)[:, 0] if draft_dtype is not None else drawn.argmax(-1)
+    uniform = torch.rand(rows, tokens, device="cuda", generator=generator)
+    return dict(logits=logits, tokens=chosen.view(rows, tokens).int(), uniform=uniform, draft=None if draft_dtype is None else q.to(draft_dtype),
+                parents=torch.tensor(parents, device="cuda", dtype=torch.int32) if trees else None)
+
+
+def check(cache, counts=None, slots=None, **given):
+    got = cache.verify(**given, counts=None if counts is None else ints(counts), slots=None if slots is None else ints(slots))
+    *want, faults = by_the_rules(cache.sequences, counts=counts, slots=slots, **given)
+    assert [x.tolist() for x in got] == want
+    assert faults_of(cache) == faults
+    return want
+
+
+@pytest.mark.parametrize("trees", [False, True])
+@pytest.mark.parametrize("draft", [None, F32, "same"])
+@pytest.mark.parametrize("dtype, rows, tokens, vocab", [
+    (F32, 1, 1, 1), (F32, 3, 2, 5), (BF16, 2, 9, 7), (F16, 4, 5, 50257), (BF16, 20, 7, 1000), (F32, 5, 33, 2049), (F32, 1, 4, 131073), (BF16, 150, 3, 4001), (F16, 2, 200, 300)])
+def test_verification(dtype, rows, tokens, vocab, draft, trees):
+    cache = cache_of(rows)
+    dice = random.Random(vocab)
+    for seed in range(3):
+        counts = [dice.randint(0, tokens) if b else tokens for b in range(rows)]
+        temperature = torch.tensor([dice.choice([0.0, 0.5, 1.0, 1.7]) for _ in range(rows)], device="cuda")
+        given = drafts(rows, tokens, vocab, dtype, dtype if draft == "same" else draft, seed, trees, temperature=temperature)
+        check(cache, counts, temperature=temperature if seed else None, **given)
+
+
+def test_tokens_that_follow_the_same_one():
+    """Many drafts of one token: each refusal leaves less, down to nothing."""
+    rows, tokens, vocab = 40, 12, 6
+    cache = cache_of(rows)
+    for draft in (None, F32):
+        for seed in range(6):
+            given = drafts(rows, tokens, vocab, F32, draft, seed, spread=[0.5, 4.0][seed % 2], noise=[0.0, 0.5, 3.0][seed % 3])
+            given["parents"] = ints([-1] + [0] * (tokens - 2) + [1])
+            given["uniform"] = 1 - (1 - given["uniform"]) * 2.0**-(4 * (seed % 3))      # close to 1: more is refused
+            check(cache, **given)
+    # equal tokens: what was refused once is refused again
+    given["tokens"] = torch.full((rows, tokens), 2, dtype=torch.int32, device="cuda")
+    given["draft"] = None
+    n, _, following = check(cache, **given)
+    assert any(x == 1 and v != 2 for x, v in zip(n, following))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_numbers_next_to_a_border(dtype):
+    """Random numbers one step of float32 to either side of a token's chance and of the border between two tokens that may follow: float32's sums cannot tell them."""
+    rows, vocab = 64, 20011
+    cache = cache_of(rows)
+    given = drafts(rows, 2, vocab, dtype, None, 3, spread=1.0)
+    p = torch.softmax(given["logits"].double(), -1)
+    given["tokens"][:, 1] = p[:, 0].topk(40, -1).indices[:, 30].int()
+    chance = p[:, 0].gather(1, given["tokens"][:, 1:].long())[:, 0].float()
+    at = torch.arange(rows, device="cuda")
+    steps = torch.tensor([-1.0, 0.0, 1.0, 2.0], device="cuda")[at % 4]
+    given["uniform"][:, 1] = (chance.view(torch.int32) + steps.int()).view(F32)
+    n, *_ = check(cache, **given)
+    assert {1, 2} <= set(n)
+    sums = p[:, 0].cumsum(-1)[at, at * 300]
+    given["uniform"][:, 0] = (sums.float().view(torch.int32) + steps.int()).view(F32)
+    check(cache, **{**given, "logits": given["logits"][:, :1], "tokens": given["tokens"][:, :1], "uniform": given["uniform"][:, :1]})
+    # with a draft: the ratio of two chances
+    given["draft"] = torch.softmax(given["logits"].float() * 0.9, -1)
+    ratio = (p[:, 0] / given["draft"][:, 0].double()).gather(1, given["tokens"][:, 1:].long())[:, 0].float()
+    given["uniform"][:, 1] = (ratio.view(torch.int32) + steps.int()).view(F32)
+    n, *_ = check(cache, **given)
+    assert {1, 2} <= set(n)
+    given["uniform"][:, 0] = torch.where(at % 2 == 0, 0.0, 1 - 2.0**-24)              # the first token and the last one that may follow
+    check(cache, **given)
+
+
+def test_what_is_returned_is_distributed_as_the_models_samples():
+    """The first token that a step adds, over 32768 rows each: of a chain, of several drafts of one token, with probabilities of a draft and without.  A count is off by its standard
+    deviation sqrt(n p (1 - p)) five times at most (24 counts: one in 70000 would be)."""
+    vocab, rows = 6, 1 << 15
+    cache = cache_of(rows)
+    generator = torch.Generator("cuda").manual_seed(0)
+    p = torch.tensor([0.4, 0.05, 0.25, 0.02, 0.08, 0.2], dtype=torch.float64, device="cuda")
+    q = torch.tensor([0.1, 0.3, 0.2, 0.2, 0.15, 0.05], device="cuda")
+    for tokens, parents, with_draft in ((2, None, True), (2, None, False), (4, ints([-1, 0, 0, 0]), True), (4, ints([-1, 0, 0, 0]), False)):
+        drawn = torch.multinomial(q.expand(rows, vocab), tokens, replacement=True, generator=generator).int()
+        if not with_draft:
+            drawn[:] = ints([0, 1, 0, 5])[:tokens]
+        uniform = torch.rand(rows, tokens, device="cuda", generator=generator)
+        n, accepted, following = cache.verify(p.log().float().expand(rows, tokens, vocab), drawn, uniform, draft=q.expand(rows, tokens, vocab) if with_draft else None, parents=parents)
+        first = torch.where(n > 1, drawn.gather(1, accepted[:, 1:2].clamp_min(0).long())[:, 0], following)
+        assert (n > 1).any() and (n == 1).any()
+        counts = torch.bincount(first, minlength=vocab).double()
+        assert ((counts - rows * p).abs() <= 5 * (rows * p * (1 - p)).sqrt()).all()
+    assert faults_of(cache) == 0
+
+
+def test_rows_that_name_their_sequences():
+    cache = cache_of(7)
+    given = drafts(3, 4, 500, BF16, F32, 5)
+    check(cache, [4, 2, 0], [6, 0, 3], **given)
+    n, accepted, following = check(cache, [4, 2, 3], [5, 5, 9], **given)              # a sequence twice, and one that there is not
+    assert n[5] > 0 and sum(n) == n[5] and following[:5] == [-1] * 5
+    check(cache, [9, -2, 3], [1, 2, 3], **given)
+    check(cache, None, None, **given)
+    check(cache, [0, 0, 0], None, **given)
+
+
+def test_tokens_and_parents_out_of_range():
+    cache = cache_of(4)
+    given = drafts(4, 4, 50, F32, F32, 6, trees=True)
+    given["tokens"][:, 0] = -7                                              # (nobody asks for the first one's)
+    check(cache, **given)
+    for at, token in ((1, 50), (2, -1), (3, 2**31 - 1)):
+        check(cache, **{**given, "tokens": given["tokens"].index_fill(1, torch.tensor([at], device="cuda"), token)})
+    for at, parent in ((1, 1), (2, 3), (3, -2), (1, -1), (2, -1)):
+        check(cache, **{**given, "parents": given["parents"].index_fill(1, torch.tensor([at], device="cuda"), parent)})
+    check(cache, **{**given, "parents": ints([5, 0, 0, 0])})
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("temperature", [None, 0.0, 0.7])
+def test_logits_that_are_no_distribution(dtype, temperature):
+    """-inf is a token of no chance; NaN, +inf and nothing but -inf end a row where it reaches them, and nowhere else."""
+    rows, vocab = 8, 3001
+    cache = cache_of(rows)
+    given = drafts(rows, 3, vocab, dtype, F32, 7, noise=0.0)
+    given["uniform"] *= 0.5                                                 # most are accepted
+    x = given["logits"]
+    x[0, :, 1::2] = -float("inf")
+    x[1, 0, 5], x[2, 1, vocab - 1], x[3, 2, 0] = float("nan"), float("nan"), float("nan")
+    x[4, 1, 7] = float("inf")
+    x[5, 0] = -float("inf")
+    x[6, 2] = float("nan")
+    t = None if temperature is None else torch.full((rows,), temperature, device="cuda")
+    n, _, following = check(cache, temperature=t, **given)
+    assert n[1] == 1 and following[1] == -1 and following[5] == -1 and following[7] >= 0
+    given["draft"][7] = float("nan")
+    check(cache, temperature=t, **given)
+
+
+def test_temperatures():
+    cache = cache_of(9)
+    given = drafts(9, 3, 2000, F32, F32, 8)
+    t = torch.tensor([-1.0, float("nan"), float("inf"), 0.0, 1e-30, 1e-42, 1e30, 0.1, -0.0], device="cuda")
+    n, _, following = check(cache, temperature=t, **given)
+    assert n[:3] == [0, 0, 0] and following[:3] == [-1] * 3 and min(n[3:]) > 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_strides_and_alignment(dtype):
+    """Rows that begin anywhere, of any number of tokens, in tensors that hold more."""
+    cache = cache_of(3)
+    for vocab in (1, 7, 8, 15, 64, 1001):
+        plain = drafts(3, 4, vocab, dtype, dtype, vocab, trees=True)
+        want = [x.tolist() for x in cache.verify(**plain)]
+        assert check(cache, **plain) == want
+        for lead in (1, 3, 5):
+            wide = torch.full((4, 3, vocab + 9), float("nan"), dtype=dtype, device="cuda")
+            logits = wide.transpose(0, 1)[:, :, lead:lead + vocab]
+            logits.copy_(plain["logits"])
+            far = torch.full((3, 6, vocab + 2), float("nan"), dtype=dtype, device="cuda")[:, 1:5, 1:1 + vocab]
+            far.copy_(plain["draft"])
+            uniform = torch.zeros(4, 3, device="cuda").T.copy_(plain["uniform"])
+            got = cache.verify(logits, plain["tokens"].long(), uniform, draft=far, parents=plain["parents"].long())
+            assert [x.tolist() for x in got] == want
+        turned = plain["logits"].permute(2, 0, 1).contiguous().permute(1, 2, 0)
+        assert [x.tolist() for x in cache.verify(**{**plain, "logits": turned, "draft": turned.to(F32).softmax(-1)})] == \
+            [x.tolist() for x in cache.verify(**{**plain, "draft": turned.contiguous().to(F32).softmax(-1).contiguous()})]
+        one = plain["logits"][:, :1].expand(3, 4, vocab)                    # (rows that share memory)
+        check(cache, **{**plain, "logits": one})
+    assert faults_of(cache) == 0
+
+
+def test_offsets_beyond_32_bits():
+    rows, tokens, vocab = 18, 1000, 250007                                  # 4.5e9 elements, of which each row takes two
+    cache = cache_of(rows)
+    logits = torch.empty(rows, tokens, vocab, dtype=BF16, device="cuda")
+    given = drafts(rows, 2, vocab, BF16, F32, 9)
+    logits[:, -2:] = given["logits"]
+    want = [x.tolist() for x in cache.verify(**given)]
+    assert [x.tolist() for x in cache.verify(**{**given, "logits": logits[:, -2:]})] == want
+    logits[:, -2:] = given["draft"].to(BF16)
+    assert [x.tolist() for x in cache.verify(**{**given, "draft": logits[:, -2:]})] == [x.tolist() for x in cache.verify(**{**given, "draft": given["draft"].to(BF16)})]
+    assert faults_of(cache) == 0
+
+
+def test_nothing_to_verify():
+    cache = cache_of(2)
+    for shape in ((0, 3, 10), (2, 0, 10)):
+        n, accepted, following = cache.verify(torch.zeros(shape, device="cuda"), torch.zeros(shape[:2], dtype=torch.int32, device="cuda"), torch.zeros(shape[:2], device="cuda"))
+        assert n.tolist() == [0, 0] and accepted.tolist() == [[-1] * shape[1]] * 2 and following.tolist() == [-1, -1]
+    assert faults_of(cache) == 0
+
+
+def test_arguments_that_are_refused():
+    cache = cache_of(2)
+    given = drafts(2, 3, 11, F32, F32, 0)
+    ok = dict(given, parents=ints([-1, 0, 1]))
+    cache.verify(**ok)
+    for change, error in [
+            (dict(logits=given["logits"].double()), TypeError), (dict(logits=given["logits"][0]), ValueError), (dict(logits=given["logits"].cpu()), ValueError), (dict(logits=None), TypeError),
+            (dict(logits=given["logits"][..., :0]), ValueError), (dict(tokens=given["tokens"][:, :2]), ValueError), (dict(tokens=given["tokens"].float()), TypeError),
+            (dict(tokens=given["tokens"].cpu()), ValueError), (dict(uniform=given["uniform"].double()), TypeError), (dict(uniform=given["uniform"][:1]), ValueError), (dict(uniform=None), TypeError),
+            (dict(draft=given["draft"][..., :10]), ValueError), (dict(draft=given["draft"].double()), TypeError), (dict(draft=given["draft"].cpu()), ValueError),
+            (dict(parents=ints([0, 1])), ValueError), (dict(parents=ints([[0, 1, 2]])), ValueError), (dict(parents=given["uniform"]), TypeError), (dict(counts=ints([1])), ValueError),
+            (dict(slots=ints([1, 0, 2])), ValueError), (dict(temperature=1.0), TypeError), (dict(temperature=torch.ones(3, device="cuda")), ValueError),
+            (dict(temperature=torch.ones(2, device="cuda", dtype=torch.float64)), TypeError)]:
+        with pytest.raises(error):
+            cache.verify(**{**ok, **change})
+    three = drafts(3, 1, 11, F32, None, 0)
+    with pytest.raises(ValueError):
+        cache.verify(**three)
+    long = drafts(1, 513, 4, F32, None, 0)
+    with pytest.raises(ValueError):
+        cache.verify(**long)
+    assert cache.verify(**{k: v[:, :512] if v is not None else v for k, v in long.items()})[0][0].item() > 0
+    assert faults_of(cache) == 0
+    cache.close()
+    with pytest.raises(ValueError):
+        cache.verify(**ok)
+
+
+def test_the_c_entry_refuses():
+    import ctypes as C
+
+    cache, lib = cache_of(2), _cabi.load()
+    given = drafts(2, 3, 1000, F32, F32, 0)
+    x, d = given["logits"], given["draft"]
+    n = lib.kb200_cache_verify_workspace(cache._cache, 2, 3, 1000)
+    space, out = torch.empty(n + 16, dtype=torch.uint8, device="cuda"), torch.empty(2, 5, dtype=torch.int32, device="cuda")
+    outs = (out[:, 0].contiguous(), out[:, 1:4].contiguous(), out[:, 4].contiguous())
+
+    def call(logits=_cabi.Scores(x.data_ptr(), 0, 0, x.stride()[:2]), draft=_cabi.Scores(d.data_ptr(), 0, 0, d.stride()[:2]), rows=2, tokens=3, vocab=1000, drafted=given["tokens"].data_ptr(),
+             uniform=given["uniform"].data_ptr(), a=outs[0].data_ptr(), b=outs[1].data_ptr(), f=outs[2].data_ptr(), at=space.data_ptr(), size=n):
+        return lib.kb200_cache_verify(cache._cache, C.byref(logits) if logits else None, C.byref(draft) if draft else None, rows, tokens, vocab, drafted, None, 3, uniform, None, None, None,
+                                      a, b, f, at, size, None)
+
+    assert n > 0 and call() == 0 and call(draft=None) == 0
+    assert call(logits=None) == call(logits=_cabi.Scores(None, 0, 0, (3000, 1000))) == call(logits=_cabi.Scores(x.data_ptr(), 3, 0, (3000, 1000))) == -1
+    assert call(draft=_cabi.Scores(d.data_ptr() + 2, 0, 0, (3000, 1000))) == call(rows=3) == call(rows=-1) == call(tokens=513) == call(vocab=0) == call(drafted=None) == call(uniform=None) == -1
+    assert call(a=None) == call(b=None) == call(f=None) == call(at=None) == call(size=n - 1) == call(at=space.data_ptr() + 8) == -1
+    assert lib.kb200_cache_verify_workspace(cache._cache, 2, 513, 10) == lib.kb200_cache_verify_workspace(cache._cache, 0, 3, 10) == 0
+    torch.cuda.synchronize()
+    assert faults_of(cache) == 0
+
+
+def test_calls_in_graphs_and_on_two_streams():
+    cache = cache_of(20)
+    given = drafts(20, 6, 30011, BF16, F32, 11)
+    other = drafts(20, 6, 30011, BF16, F32, 12)
+    want, want_other = ([x.tolist() for x in cache.verify(**g)] for g in (given, other))
+    static = {k: None if v is None else v.clone() for k, v in given.items()}
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        cache.verify(**static)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(cache.verify(**static))
+        graphs.append(graph)
+    for i in range(6):
+        for k, v in (given, other)[i // 2 % 2].items():
+            if v is not None:
+                static[k].copy_(v)
+        graphs[i % 2].replay()
+        assert [x.tolist() for x in outs[i % 2]] == (want, want_other)[i // 2 % 2]
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(cache.verify(**(given, other)[i]))
+    torch.cuda.synchronize()
+    assert all([x.tolist() for x in r] == (want, want_other)[i] for i in range(2) for r in got[i])
+    assert faults_of(cache) == 0
+
+
+def test_rows_by_row_and_all_at_once():
+    """As many CTAs to a row as there are few rows: the same tokens."""
+    rows = 200
+    cache = cache_of(rows)
+    given = drafts(rows, 4, 10007, BF16, F32, 13)
+    want = [x.tolist() for x in cache.verify(**given)]
+    for b in range(0, rows, 23):
+        one = cache.verify(**{k: None if v is None else v[b:b + 1] for k, v in given.items()}, slots=ints([b]))
+        assert [x[b].tolist() for x in one] == [x[b] for x in want]
