@@ -23,10 +23,10 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kStatThreads = 256, kWalkThreads = 512, kWalkWarps = kWalkThreads / 32, kMostCluster = 8;
+constexpr int kStatThreads = 256, kWalkThreads = 512, kWalkWarps = kWalkThreads / 32, kMostCluster = 16;
 constexpr int kMostTokens = 512;       // of a row
 constexpr double kLog2e = 1.4426950408889634074;
-// What float32's sums may be off by, relatively: sums of 32 at a time (2^-19 at most) of exponentials that are off by 2^-22 each.
+// What float32's sums may be off by, relatively: sums of 8 at a time (2^-20 at most, joined by pairs) of exponentials that are off by 2^-22 each, scaled once or twice.
 constexpr double kUnsure = 4e-6;
 
 struct VerifyParams {
@@ -67,17 +67,29 @@ struct RowOf {
   __device__ __forceinline__ int first(int i) const { return i * kVec - off; }
   __device__ __forceinline__ bool whole(int i) const { return first(i) >= 0 && first(i) + kVec <= n; }
   // -inf where there is none.
-  __device__ __forceinline__ void load(int i, float (&x)[kVec]) const {
+  __device__ __forceinline__ uint4 load(int i) const {
     const int at = first(i);
-    if (at >= 0 && at + kVec <= n) {
-      const uint4 v = *reinterpret_cast<const uint4*>(row + at);
-      const T* const e = reinterpret_cast<const T*>(&v);
+    if (at >= 0 && at + kVec <= n) return *reinterpret_cast<const uint4*>(row + at);
+    return load_part(at);
+  }
+  __device__ __noinline__ uint4 load_part(int at) const {
+    uint4 v;
+    T* const e = reinterpret_cast<T*>(&v);
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) x[j] = as_float(e[j]);
-    } else {
+    for (int j = 0; j < kVec; ++j) e[j] = at + j >= 0 && at + j < n ? row[at + j] : T(-CUDART_INF_F);
+    return v;
+  }
+  static __device__ __forceinline__ uint4 nothing() {
+    uint4 v;
+    T* const e = reinterpret_cast<T*>(&v);
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) x[j] = at + j >= 0 && at + j < n ? as_float(row[at + j]) : -CUDART_INF_F;
-    }
+    for (int j = 0; j < kVec; ++j) e[j] = T(-CUDART_INF_F);
+    return v;
+  }
+  static __device__ __forceinline__ void unpack(const uint4& v, float (&x)[kVec]) {
+    const T* const e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) x[j] = as_float(e[j]);
   }
 };
 
@@ -101,8 +113,9 @@ __device__ __forceinline__ int row_slot(const VerifyParams& p, int b, int* count
 
 // Maxima and sums of exponentials of a drafted token's row, by chunks.
 template <typename T>
-__global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const __grid_constant__ VerifyParams p) {
-  constexpr int VEC = RowOf<T>::kVec, AT_ONCE = 32 / VEC;
+__global__ void __launch_bounds__(kStatThreads, 4) verify_stats_kernel(const __grid_constant__ VerifyParams p) {
+  using Row = RowOf<T>;
+  constexpr int VEC = Row::kVec, AT_ONCE = 4;
   __shared__ float maxima[kStatThreads / 32];
   __shared__ double sums[kStatThreads / 32];
   __shared__ int indexes[kStatThreads / 32];
@@ -123,23 +136,15 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const __grid
     const int chunk = (int)(u % p.chunks), node = (int)(u / p.chunks % p.width), b = (int)(u / p.chunks / p.width);
     if (node >= (p.counts != nullptr ? p.counts[b] : p.width)) continue;
     const float t = p.temperature != nullptr ? p.temperature[b] : 1.0f, scale = fminf((float)(kLog2e / t), 1e38f);
-    const RowOf<T> row(static_cast<const T*>(p.logits) + b * p.logits_stride[0] + node * p.logits_stride[1], p.vocab);
+    const Row row(static_cast<const T*>(p.logits) + b * p.logits_stride[0] + node * p.logits_stride[1], p.vocab);
     const int vectors = row.vectors(), lo = (int)((int64_t)vectors * chunk / p.chunks), hi = (int)((int64_t)vectors * (chunk + 1) / p.chunks);
     float m = -CUDART_INF_F;
     double s = 0.0;
     int index = INT_MAX;
-    for (int i0 = lo + threadIdx.x; i0 < hi; i0 += kStatThreads * AT_ONCE) {
+    auto add = [&](const uint4 (&v)[AT_ONCE], int i0) {
       float x[AT_ONCE][VEC];
 #pragma unroll
-      for (int j = 0; j < AT_ONCE; ++j) {
-        const int i = i0 + j * kStatThreads;
-        if (i < hi) {
-          row.load(i, x[j]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) x[j][e] = -CUDART_INF_F;
-        }
-      }
+      for (int j = 0; j < AT_ONCE; ++j) Row::unpack(v[j], x[j]);
       if (t == 0.0f) {
 #pragma unroll
         for (int j = 0; j < AT_ONCE; ++j)
@@ -148,28 +153,49 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const __grid
             if (x[j][e] > m) m = x[j][e], index = row.first(i0 + j * kStatThreads) + e;
             if (x[j][e] != x[j][e]) s = CUDART_NAN;
           }
-        continue;
+        return;
       }
       float top = m;
 #pragma unroll
       for (int j = 0; j < AT_ONCE; ++j)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) top = fmaxf(top, x[j][e]);
-      if (top == -CUDART_INF_F) {        // (NaN alone are such a maximum too)
-#pragma unroll
-        for (int j = 0; j < AT_ONCE; ++j)
-#pragma unroll
-          for (int e = 0; e < VEC; ++e)
-            if (x[j][e] != x[j][e]) s = CUDART_NAN;
-        continue;
-      }
-      float sum = 0.0f;
+        for (int e = 0; e < VEC; e += 2) top = tc::fmax3(top, x[j][e], x[j][e + 1]);
+      const float2 behind = top == -CUDART_INF_F ? make_float2(0.0f, 0.0f) : make_float2(-top, -top), scale2 = make_float2(scale, scale);      // (nothing but -inf so far: weights of 0; NaN: NaN)
+      float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
       for (int j = 0; j < AT_ONCE; ++j)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) sum += exp2_fast((x[j][e] - top) * scale);
-      if (top > m) s *= exp2_fast((m - top) * scale), m = top;
-      s += sum;
+        for (int e = 0; e < VEC; e += 2) {
+          const float2 y = tc::fmul2(tc::fadd2(make_float2(x[j][e], x[j][e + 1]), behind), scale2);
+          sum[e >> 1 & 1] = tc::fadd2(sum[e >> 1 & 1], make_float2(exp2_fast(y.x), exp2_fast(y.y)));
+        }
+      if (top > m && m > -CUDART_INF_F) s *= exp2_fast((m - top) * scale);
+      m = top;
+      s += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+    };
+    // Whole vectors, the next of which are under way while these are summed; the row's first and last may not be whole.
+    const int from = max(lo, 1), to = min(hi, vectors - 1);
+    const uint4* const whole = reinterpret_cast<const uint4*>(row.row + row.first(1));
+    uint4 ahead[AT_ONCE];
+    auto ask = [&](int i0) {
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) ahead[j] = i0 + j * kStatThreads < to ? __ldcg(whole + i0 + j * kStatThreads - 1) : Row::nothing();
+    };
+    ask(from + threadIdx.x);
+    for (int i0 = from + threadIdx.x; i0 < to; i0 += kStatThreads * AT_ONCE) {
+      uint4 now[AT_ONCE];
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) now[j] = ahead[j];
+      ask(i0 + kStatThreads * AT_ONCE);
+      add(now, i0);
+    }
+    if ((lo == 0 || hi == vectors) && threadIdx.x < 32) {
+      const int i = threadIdx.x == 0 && lo == 0 ? 0 : threadIdx.x == 1 && hi == vectors && vectors > 1 ? vectors - 1 : -1;
+      uint4 edge[AT_ONCE];
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) edge[j] = Row::nothing();
+      if (i >= 0) edge[0] = row.load(i);
+      add(edge, max(i, 0));
     }
     // of the CTA
     float all = m;
@@ -195,19 +221,20 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const __grid
   }
 }
 
-// 2^y for y <= 0 to about 2e-16: a table of 32nds and a polynomial, 2^f = sum (f ln 2)^k / k!, |f| <= 1/64.
+// 2^y for y <= 0 to about 3e-15: a table of 32nds and a polynomial, 2^f = sum (f ln 2)^k / k!, |f| <= 1/64 (the sixth power is 2e-15).  (More 32nds would save a
+// multiplication and cost as much: 32 doubles lie two to a bank of shared memory.)
+constexpr double kLn2 = 0.69314718055994530942;
 __device__ __forceinline__ double exp2_wide(double y, const double* table) {
   if (!(y > -1000.0)) return y != y ? y : 0.0;
-  constexpr double kRound = 6755399441055744.0;      // 3 x 2^51: the sum's last bits are a whole number
-  const double t = __fma_rn(y, 32.0, kRound);
+  constexpr double kRound = 211106232532992.0;       // 3 x 2^46: the sum's last bits are 32nds
+  const double t = y + kRound, f = y - (t - kRound);
   const int n = __double2loint(t);
-  const double f = __fma_rn(t - kRound, -1.0 / 32.0, y), z = f * 0.69314718055994530942;
-  double r = __fma_rn(z, 1.0 / 720.0, 1.0 / 120.0);
-  r = __fma_rn(z, r, 1.0 / 24.0);
-  r = __fma_rn(z, r, 1.0 / 6.0);
-  r = __fma_rn(z, r, 0.5);
-  r = __fma_rn(z, r, 1.0);
-  r = __fma_rn(z, r, 1.0) * table[n & 31];
+  double r = __fma_rn(f, kLn2 * kLn2 * kLn2 * kLn2 * kLn2 / 120.0, kLn2 * kLn2 * kLn2 * kLn2 / 24.0);
+  r = __fma_rn(f, r, kLn2 * kLn2 * kLn2 / 6.0);
+  r = __fma_rn(f, r, kLn2 * kLn2 / 2.0);
+  r = __fma_rn(f, r, kLn2);
+  const double power = table[n & 31];
+  r = __fma_rn(power, f * r, power);
   return __hiloint2double(__double2hiint(r) + ((n >> 5) << 20), __double2loint(r));
 }
 
@@ -220,25 +247,254 @@ __device__ __forceinline__ float draft_at(const VerifyParams& p, int64_t at) {
 // What is known of the drafted tokens of a row.
 struct Drafted {
   double *sum, *weight;                  // a token's row: the sum; its own weight in the row of the one that it follows, 2^((logit - maximum) / T log2 e)
-  double* divisors;                      // see below
+  double* chance;                        // ... by that row's sum
+  double* divisors;                      // see Left
   float *top, *uniform, *chance_q;       // a token's row: its maximum; the random number; the draft's probability of it
   int *parent, *token, *best;            // best: the largest logit's index (temperature 0)
-  int* out;                              // followers that were refused (no draft)
+  int* out;                              // see Left
 };
-constexpr int kDraftedBytes = 3 * 8 + 3 * 4 + 4 * 4;
+constexpr int kDraftedBytes = 4 * 8 + 3 * 4 + 4 * 4;
 
+// What is left of a token's row: weights 2^(scale (logit - top)), the first of them without what was refused, or, with a draft, in units of their sum, from which the draft's
+// probabilities were taken `depth` times (divisors: the reciprocals of what was left before each time, of the first also the sum's).
+struct Left {
+  double scale, top;
+  const double *table = nullptr, *divisors = nullptr;
+  const int* out = nullptr;
+  int64_t draft = 0;                     // the row's first element in p.draft
+  int refused = 0, depth = 0;
+};
+__device__ __forceinline__ double value_of(const VerifyParams& p, const Left& left, int v, float logit) {
+  double r = exp2_wide(((double)logit - left.top) * left.scale, left.table);
+  for (int j = 0; j < left.refused; ++j)
+    if (left.out[j] == v) r = 0.0;
+  if (left.depth > 0) {
+    const double q = draft_at(p, left.draft + v);
+    for (int k = 0; k < left.depth; ++k) r = fmax(__fma_rn(r, left.divisors[k], -q), 0.0);
+  }
+  return r;
+}
+// Sums of vectors lo .. hi of a row, by a warp.
+struct Sums {
+  double left;                           // what is left
+  double all, of_left, near;             // (sum_first) the weights; those of what is left; the draft's probabilities that a weight is near
+};
+// Of whatever is left.
+template <typename T>
+__device__ __noinline__ Sums sum_any(const VerifyParams& p, const RowOf<T>& row, const Left& left, int lo, int hi) {
+  double x = 0.0;
+  for (int i = lo + (threadIdx.x & 31); i < hi; i += 32)
+    for (int j = 0; j < RowOf<T>::kVec; ++j) {
+      const int v = row.first(i) + j;
+      if (v >= 0 && v < row.n) x += value_of(p, left, v, as_float(row.row[v]));
+    }
+  return Sums{x, 0.0, 0.0, 0.0};
+}
+
+// The forms below are what nearly every call needs.  What bounds them is the instructions of an exponential, 20 (10 of float64), in sum_any 70.  They take (logit - top) scale as one
+// multiply-add, off by 2^-53 of top scale, and are for rows where that is 2^12 at most, 5e-13 of a weight; and one power of f less than exp2_wide, 1.2e-12.
+constexpr double kNearTop = 4096.0;
+struct Power {
+  double e;
+  bool any;                              // y >= -1000; if not e is nothing
+};
+__device__ __forceinline__ Power power_of(double y, uint32_t table) {
+  constexpr double kRound = 211106232532992.0;
+  const double t = y + kRound, f = y - (t - kRound);
+  const int n = __double2loint(t);
+  double r = __fma_rn(f, kLn2 * kLn2 * kLn2 * kLn2 / 24.0, kLn2 * kLn2 * kLn2 / 6.0), power;
+  r = __fma_rn(f, r, kLn2 * kLn2 / 2.0);
+  r = __fma_rn(f, r, kLn2);
+  asm("ld.shared.f64 %0, [%1];" : "=d"(power) : "r"(table + ((n & 31) << 3)));
+  r = __fma_rn(power, f * r, power);
+  return Power{__hiloint2double(__double2hiint(r) + ((n & ~31) << 15), __double2loint(r)), (unsigned)__double2hiint(y) <= 0xC08F4000u};
+}
+
+// A vector's elements, as they lie.
+template <typename T, int VEC>
+struct Vector {
+  uint32_t w[VEC * sizeof(T) / 4];
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (std::is_same<T, float>::value) return __uint_as_float(w[i]);
+    else if constexpr (std::is_same<T, __half>::value) return i & 1 ? __high2float(*reinterpret_cast<const __half2*>(&w[i / 2])) : __low2float(*reinterpret_cast<const __half2*>(&w[i / 2]));
+    else return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+  }
+};
+template <typename T>
+using Logits = Vector<T, RowOf<T>::kVec>;
+template <typename T>
+__device__ __forceinline__ Logits<T> logits_of(const RowOf<T>& row, int i, int hi) {
+  const uint4 v = i < hi ? row.load(i) : RowOf<T>::nothing();
+  return Logits<T>{{v.x, v.y, v.z, v.w}};
+}
+// As many of a draft's probabilities as a vector of logits has: in 16 bytes or twice that where they lie so, or one by one.
+template <typename T, typename Q>
+struct DraftOf {
+  static constexpr int kVec = RowOf<T>::kVec, kWords = kVec * (int)sizeof(Q) / 4, kEach = kWords < 4 ? kWords : 4;
+  using Chances = Vector<Q, kVec>;
+  struct alignas(kEach * 4) Words {
+    uint32_t w[kEach];
+  };
+  const Q* q;
+  bool aligned;
+  __device__ __forceinline__ DraftOf(const VerifyParams& p, const Left& left, const RowOf<T>& row)
+      : q(static_cast<const Q*>(p.draft) + left.draft), aligned(reinterpret_cast<uintptr_t>(q + row.first(0)) % sizeof(Words) == 0) {}
+  __device__ __forceinline__ Chances load(const RowOf<T>& row, int i, int hi) const {
+    Chances x = {};
+    if (i >= hi) return x;
+    if (!aligned || !row.whole(i)) return load_part(q, row.first(i), row.n);
+#pragma unroll
+    for (int k = 0; k < kWords; k += kEach) {
+      const Words v = *reinterpret_cast<const Words*>(q + row.first(i) + k * 4 / (int)sizeof(Q));
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) x.w[k + j] = v.w[j];
+    }
+    return x;
+  }
+  static __device__ __noinline__ Chances load_part(const Q* q, int first, int n) {
+    Chances x = {};
+    Q* const e = reinterpret_cast<Q*>(x.w);
+#pragma unroll
+    for (int j = 0; j < kVec; ++j)
+      if (first + j >= 0 && first + j < n) e[j] = q[first + j];
+    return x;
+  }
+};
+constexpr int kAhead = 4;                // vectors of a lane that are under way
+
+// Of weights, without those refused.
+template <typename T>
+__device__ __noinline__ Sums sum_weights(const VerifyParams& p, const RowOf<T>& row, const Left& left, int lo, int hi) {
+  const double scale = left.scale, shift = -left.top * left.scale;
+  const uint32_t table = tc::smem_u32(left.table);
+  const int refused = left.refused;
+  double x = 0.0;
+  int i = lo + (threadIdx.x & 31);
+  Logits<T> ahead[kAhead];
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j) ahead[j] = logits_of(row, i + 32 * j, hi);
+  for (; i < hi; i += 32) {
+    const Logits<T> now = ahead[0];                    // (-inf, a weight of 0, where there is none)
+#pragma unroll
+    for (int j = 1; j < kAhead; ++j) ahead[j - 1] = ahead[j];
+    ahead[kAhead - 1] = logits_of(row, i + 32 * kAhead, hi);
+    float logit[RowOf<T>::kVec];
+#pragma unroll
+    for (int j = 0; j < RowOf<T>::kVec; ++j) logit[j] = now[j];
+    for (int k = 0; k < refused; ++k) {
+      const int at = left.out[k] - row.first(i);
+#pragma unroll
+      for (int j = 0; j < RowOf<T>::kVec; ++j) logit[j] = at == j ? -CUDART_INF_F : logit[j];
+    }
+#pragma unroll
+    for (int j = 0; j < RowOf<T>::kVec; ++j) {
+      const Power y = power_of(__fma_rn((double)logit[j], scale, shift), table);
+      if (y.any) x += y.e;
+    }
+  }
+  return Sums{x, 0.0, 0.0, 0.0};
+}
+// Of weights, and of what the draft's probabilities leave of them when the sum is only known to float32 (its reciprocal: divisors[0]).  That is off by up to d = 4e-6; what is left is
+// then sum (e / sum' - q) = left + of_left (1 / sum' - 1 / sum), but for elements where |e / sum - q| is less than d q, which may have been counted or left out wrongly: d q at most for
+// each.  Those of 2^-16 q and less (8 d) are summed; 64 in 128000 of such logits' differences are, and where they are more than kMostNear what is left is summed again with
+// the sum that is then known.  (That always: twice the time.)
+constexpr double kMostNear = 1e-4;
+template <typename T, typename Q>
+__device__ __noinline__ Sums sum_first(const VerifyParams& p, const RowOf<T>& row, const Left& left, int lo, int hi) {
+  const DraftOf<T, Q> draft(p, left, row);
+  const double scale = left.scale, shift = -left.top * left.scale, unit = left.divisors[0];
+  const uint32_t table = tc::smem_u32(left.table);
+  Sums x{0.0, 0.0, 0.0, 0.0};
+  float near = 0.0f;
+  int i = lo + (threadIdx.x & 31);
+  Logits<T> ahead[kAhead];
+  typename DraftOf<T, Q>::Chances q_ahead[kAhead];
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j) ahead[j] = logits_of(row, i + 32 * j, hi), q_ahead[j] = draft.load(row, i + 32 * j, hi);
+  for (; i < hi; i += 32) {
+    const Logits<T> now = ahead[0];
+    const typename DraftOf<T, Q>::Chances q = q_ahead[0];
+#pragma unroll
+    for (int j = 1; j < kAhead; ++j) ahead[j - 1] = ahead[j], q_ahead[j - 1] = q_ahead[j];
+    ahead[kAhead - 1] = logits_of(row, i + 32 * kAhead, hi), q_ahead[kAhead - 1] = draft.load(row, i + 32 * kAhead, hi);
+#pragma unroll
+    for (int j = 0; j < RowOf<T>::kVec; ++j) {
+      const Power y = power_of(__fma_rn((double)now[j], scale, shift), table);
+      const double chance = (double)q[j], r = __fma_rn(y.e, unit, -chance);
+      if ((__double2hiint(r) & 0x7fffffff) + (16 << 20) < __double2hiint(chance)) near += q[j];
+      if (y.any) x.all += y.e;
+      if (y.any && r > 0.0) x.left += r, x.of_left += y.e;
+    }
+  }
+  x.near = (double)near;
+  return x;
+}
+// Of what they leave, taken off any number of times.
+template <typename T, typename Q>
+__device__ __noinline__ Sums sum_beyond(const VerifyParams& p, const RowOf<T>& row, const Left& left, int lo, int hi) {
+  const DraftOf<T, Q> draft(p, left, row);
+  const double scale = left.scale, shift = -left.top * left.scale;
+  const uint32_t table = tc::smem_u32(left.table);
+  double x = 0.0;
+  int i = lo + (threadIdx.x & 31);
+  Logits<T> ahead = logits_of(row, i, hi);
+  typename DraftOf<T, Q>::Chances q_ahead = draft.load(row, i, hi);
+  for (; i < hi; i += 32) {
+    const Logits<T> now = ahead;
+    const typename DraftOf<T, Q>::Chances q = q_ahead;
+    ahead = logits_of(row, i + 32, hi), q_ahead = draft.load(row, i + 32, hi);
+    double r[RowOf<T>::kVec];
+#pragma unroll
+    for (int j = 0; j < RowOf<T>::kVec; ++j) {
+      const Power y = power_of(__fma_rn((double)now[j], scale, shift), table);
+      r[j] = y.any ? y.e : 0.0;
+    }
+    for (int k = 0; k < left.depth; ++k) {
+      const double unit = left.divisors[k];
+#pragma unroll
+      for (int j = 0; j < RowOf<T>::kVec; ++j) r[j] = fmax(__fma_rn(r[j], unit, -(double)q[j]), 0.0);
+    }
+#pragma unroll
+    for (int j = 0; j < RowOf<T>::kVec; ++j) x += r[j];
+  }
+  return Sums{x, 0.0, 0.0, 0.0};
+}
+template <typename T, typename Q>
+__device__ __forceinline__ Sums sum_drafted(const VerifyParams& p, const RowOf<T>& row, const Left& left, int lo, int hi, bool first) {
+  return first ? sum_first<T, Q>(p, row, left, lo, hi) : sum_beyond<T, Q>(p, row, left, lo, hi);
+}
+__device__ __forceinline__ bool near_top(const Left& left) { return fabs(left.top * left.scale) <= kNearTop; }
+template <typename T>
+__device__ __forceinline__ Sums sum_of(const VerifyParams& p, const RowOf<T>& row, const Left& left, int lo, int hi, bool first) {
+  Sums x;
+  if (!near_top(left)) x = sum_any<T>(p, row, left, lo, hi);
+  else if (left.depth == 0) x = sum_weights<T>(p, row, left, lo, hi);
+  else if (p.draft_dtype == KB200_DTYPE_FP32) x = sum_drafted<T, float>(p, row, left, lo, hi, first);
+  else if (p.draft_dtype == KB200_DTYPE_BF16) x = sum_drafted<T, __nv_bfloat16>(p, row, left, lo, hi, first);
+  else x = sum_drafted<T, __half>(p, row, left, lo, hi, first);
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) {
+    x.left += __shfl_xor_sync(0xffffffffu, x.left, o);
+    if (first) {
+      x.all += __shfl_xor_sync(0xffffffffu, x.all, o);
+      x.of_left += __shfl_xor_sync(0xffffffffu, x.of_left, o);
+      x.near += __shfl_xor_sync(0xffffffffu, x.near, o);
+    }
+  }
+  return x;
+}
 template <typename T>
 __global__ void __launch_bounds__(kWalkThreads, 1) verify_walk_kernel(const __grid_constant__ VerifyParams p) {
   using Row = RowOf<T>;
   constexpr int VEC = Row::kVec;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ double table[32], shares[kWalkWarps], totals[2][kMostCluster];
-  pdl_wait();
-  pdl_launch_dependents();
+  __shared__ double table[32], shares[4][kWalkWarps], totals[2][4][kMostCluster];      // (as in Sums)
   const cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks(), b = blockIdx.x / ranks;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x < 32) table[threadIdx.x] = exp2((double)threadIdx.x / 32.0);
+  pdl_wait();
+  pdl_launch_dependents();
   int count;
   float temperature;
   const int slot = row_slot(p, b, &count, &temperature, rank == 0);
@@ -256,27 +512,45 @@ __global__ void __launch_bounds__(kWalkThreads, 1) verify_walk_kernel(const __gr
   Drafted d;
   {
     double* at = reinterpret_cast<double*>(smem);
-    d.sum = at, d.weight = at + p.width, d.divisors = at + 2 * p.width;
-    float* of = reinterpret_cast<float*>(at + 3 * p.width);
+    d.sum = at, d.weight = at + p.width, d.chance = at + 2 * p.width, d.divisors = at + 3 * p.width;
+    float* of = reinterpret_cast<float*>(at + 4 * p.width);
     d.top = of, d.uniform = of + p.width, d.chance_q = of + 2 * p.width;
     int* to = reinterpret_cast<int*>(of + 3 * p.width);
     d.parent = to, d.token = to + p.width, d.best = to + 2 * p.width, d.out = to + 3 * p.width;
   }
   __syncthreads();                       // (the table)
-  // Every row's chunks together, a warp to a row.
+  // What is given of the drafted tokens, by the last warps, and every row's chunks together, a warp to a row: at the same time, as far as there are warps.
+  for (int i = kWalkThreads - 1 - threadIdx.x; i < count; i += kWalkThreads) {
+    int parent = p.parents != nullptr ? p.parents[b * p.parents_stride + i] : i - 1;
+    const int token = p.tokens[(int64_t)b * p.width + i];
+    const float uniform = p.uniform[(int64_t)b * p.width + i];
+    if (i > 0 && (parent < -1 || parent >= i || (unsigned)token >= (unsigned)p.vocab)) {
+      if (rank == 0) cache_fault(p.c, KB200_CACHE_BAD_INDEX);
+      parent = -1;
+    }
+    if (i > 0 && parent >= 0 && !greedy) {
+      d.weight[i] = (double)as_float(logits[parent * p.logits_stride[1] + token]);
+      d.chance_q[i] = p.draft != nullptr ? draft_at(p, b * p.draft_stride[0] + parent * p.draft_stride[1] + token) : 1.0f;
+    }
+    d.parent[i] = i > 0 ? parent : -1;
+    d.token[i] = token;
+    d.uniform[i] = fmaxf(uniform, 0.0f);
+  }
   for (int i = warp; i < count; i += kWalkWarps) {
     const float2* const parts = p.partial + ((int64_t)b * p.width + i) * p.chunks;
-    float top = -CUDART_INF_F;
-    bool nan = false;
-    for (int j = lane; j < p.chunks; j += 32) top = fmaxf(top, parts[j].x), nan = nan || parts[j].x != parts[j].x;
+    const float2 none_there = make_float2(-CUDART_INF_F, 0.0f), first = lane < p.chunks ? parts[lane] : none_there, second = lane + 32 < p.chunks ? parts[lane + 32] : none_there;
+    float top = fmaxf(first.x, second.x);
+    bool nan = first.x != first.x || second.x != second.x;
 #pragma unroll
     for (int x = 16; x > 0; x /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
     nan = __any_sync(0xffffffffu, nan) != 0;
     double sum = 0.0;
     int best = INT_MAX;
-    for (int j = lane; j < p.chunks; j += 32) {
-      if (greedy && parts[j].x == top) best = min(best, __float_as_int(parts[j].y));
-      if (!greedy && parts[j].x > -CUDART_INF_F) sum += (double)parts[j].y * exp2_wide(((double)parts[j].x - (double)top) * scale, table);
+#pragma unroll 1
+    for (int j = 0; j < 2; ++j) {
+      const float2 part = j == 0 ? first : second;
+      if (greedy && part.x == top) best = min(best, __float_as_int(part.y));
+      if (!greedy && part.x > -CUDART_INF_F) sum += (double)part.y * exp2_wide(((double)part.x - (double)top) * scale, table);
     }
 #pragma unroll
     for (int x = 16; x > 0; x /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, x);
@@ -285,246 +559,190 @@ __global__ void __launch_bounds__(kWalkThreads, 1) verify_walk_kernel(const __gr
     const bool none = nan || !(top > -CUDART_INF_F) || (!greedy && !(top < CUDART_INF_F && sum > 0.0));
     if (lane == 0) d.top[i] = top, d.sum[i] = none ? -1.0 : sum, d.best[i] = best;
   }
-  for (int i = threadIdx.x; i < count; i += kWalkThreads) {
-    int parent = p.parents != nullptr ? p.parents[b * p.parents_stride + i] : i - 1;
-    const int token = p.tokens[(int64_t)b * p.width + i];
-    if (i > 0 && (parent < -1 || parent >= i || (unsigned)token >= (unsigned)p.vocab)) {
-      if (rank == 0) cache_fault(p.c, KB200_CACHE_BAD_INDEX);
-      parent = -1;
-    }
-    d.parent[i] = i > 0 ? parent : -1;
-    d.token[i] = token;
-    d.uniform[i] = fmaxf(p.uniform[(int64_t)b * p.width + i], 0.0f);
-  }
   __syncthreads();
   if (!greedy)
-    for (int i = 1 + threadIdx.x; i < count; i += kWalkThreads) {
-      if (d.parent[i] < 0) continue;
-      const int of = d.parent[i], token = d.token[i];
-      d.weight[i] = exp2_wide(((double)as_float(logits[of * p.logits_stride[1] + token]) - (double)d.top[of]) * scale, table);
-      d.chance_q[i] = p.draft != nullptr ? draft_at(p, b * p.draft_stride[0] + of * p.draft_stride[1] + token) : 1.0f;
-    }
+    for (int i = threadIdx.x; i < count; i += kWalkThreads)
+      if (d.parent[i] >= 0) {
+        const int of = d.parent[i];
+        d.weight[i] = exp2_wide((d.weight[i] - (double)d.top[of]) * scale, table);
+        d.chance[i] = d.weight[i] / d.sum[of];
+      }
   __syncthreads();
 
-  // From here on every thread of the cluster takes the same steps with the same numbers, and only the sums over the vocabulary are shared out.
-  int at = 0, steps = 1, turn = 0;
-  int depth = 0;               // how many times the draft's probabilities have been taken off the row of `at`, by which divisors
-  int refused = 0;             // (no draft) how many of the followers' tokens have been taken out of it
-  double sum = d.sum[0], left = 1.0;
+  // The first warp of every CTA of the cluster takes the same steps with the same numbers (by all threads they took 400 cycles for a token), and only the sums over the
+  // vocabulary are shared out: it says which one it needs, and goes on behind it.
+  enum { kNothing, kExactly, kFirst, kTaken, kRefused, kLast, kDone };
+  struct Plan {
+    int wants, at, steps, refused, depth;
+    bool known;
+    double total;
+  };
+  __shared__ Plan plan;
+  int at = 0, steps = 1, c = 1, wants = kNothing, refused = 0, depth = 0, turn = 0;
+  double sum = d.sum[0], left = 1.0, total = 0.0;
   bool exact = false;          // `sum` is float64's
   bool shared = false;         // shares and totals are of what is left now
-  double total = 0.0;
-  auto removed = [&](int token, int n) {
+  bool known = sum >= 0.0;
+  auto removed = [&](int token) {
     bool is = false;
-    for (int j = 0; j < n; ++j) is = is || d.out[j] == token;
+    for (int j = 0; j < refused; ++j) is = is || d.out[j] == token;
     return is;
   };
-  // What is left of element v of the row of `at`, in units of the row's sum with a draft, of its largest weight without.
-  auto value = [&](int v, float logit, int out) {
-    const double e = exp2_wide(((double)logit - (double)d.top[at]) * scale, table);
-    if (out > 0) return removed(v, out) ? 0.0 : e;
-    if (depth == 0) return e;
-    const double q = draft_at(p, b * p.draft_stride[0] + at * p.draft_stride[1] + v);
-    double r = e / sum;
-    for (int k = 0; k < depth; ++k) r = fmax(r / d.divisors[k] - q, 0.0);
-    return r;
-  };
-  auto sum_of = [&](const Row& row, int lo, int hi, int out) {      // of vectors lo .. hi, by a warp
-    double x = 0.0;
-    for (int i = lo + lane; i < hi; i += 32) {
-      float logit[VEC];
-      row.load(i, logit);
-      const int first = row.first(i);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j)
-        if (first + j >= 0 && first + j < p.vocab) x += value(first + j, logit[j], out);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o /= 2) x += __shfl_xor_sync(0xffffffffu, x, o);
-    return x;
-  };
-  auto row_at = [&]() { return Row(logits + at * p.logits_stride[1], p.vocab); };
-  auto part_of = [](int lo, int hi, int i, int n, int* from, int* to) {
-    *from = lo + (int)((int64_t)(hi - lo) * i / n);
-    *to = lo + (int)((int64_t)(hi - lo) * (i + 1) / n);
-  };
-  // The sum of what is left, over the cluster; the first `out` of the refused tokens are out of it.
-  auto sum_left = [&](int out) {
-    const Row row = row_at();
-    int lo, hi, from, to;
-    part_of(0, row.vectors(), rank, ranks, &lo, &hi);
-    part_of(lo, hi, warp, kWalkWarps, &from, &to);
-    const double mine = sum_of(row, from, to, out);
-    __syncthreads();                     // (the last shares have been read)
-    if (lane == 0) shares[warp] = mine;
-    __syncthreads();
-    if (threadIdx.x < ranks) {
-      double x = 0.0;
-      for (int w = 0; w < kWalkWarps; ++w) x += shares[w];
-      cluster.map_shared_rank(&totals[turn][0], threadIdx.x)[rank] = x;
-    }
-    cluster.sync();
-    double x = 0.0;
-    for (int r = 0; r < ranks; ++r) x += totals[turn][r];
-    turn ^= 1;
-    return x;
-  };
-  auto sum_exactly = [&]() {               // (nothing has been taken off by a draft yet)
-    if (exact) return;
-    total = sum = sum_left(0);
-    exact = true;
-    shared = refused == 0;
-  };
-
-  bool known = sum > 0.0 || greedy;
-  if (d.sum[0] < 0.0) known = false;
-  for (int c = 1; c < count && known; ++c) {
-    if (d.parent[c] != at) continue;
-    bool take;
-    if (greedy) {
-      take = d.token[c] == d.best[at];
-    } else {
-      const double u = (double)d.uniform[c] * (double)d.chance_q[c];
-      for (int pass = 0; pass < 2; ++pass) {
-        double chance = d.weight[c] / sum;
-        if (p.draft != nullptr) {
-          for (int k = 0; k < depth; ++k) chance = fmax(chance / d.divisors[k] - (double)d.chance_q[c], 0.0);
-        } else if (removed(d.token[c], refused)) {
-          chance = 0.0;
-        }
-        take = u * left < chance;
-        if (exact || pass > 0 || fabs(u * left - chance) > kUnsure * (u + chance)) break;
-        // (what is left without a draft is 1 less the refused ones' chances, which are as near as the sum)
-        const double before = sum;
-        sum_exactly();
-        if (p.draft == nullptr && refused != 0) left = 1.0 - (1.0 - left) * (before / sum);
-      }
-    }
-    if (take) {
-      at = c;
-      if (writes) accepted[steps] = c;
-      ++steps;
-      depth = 0, refused = 0, left = 1.0, exact = false, shared = false;
-      sum = d.sum[at];
-      if (d.sum[at] < 0.0) known = false;
-    } else if (!greedy) {
-      if (p.draft != nullptr) {
-        sum_exactly();
-        if (threadIdx.x == 0) d.divisors[depth] = left;
-        __syncthreads();
-        ++depth;
-        const double rest = sum_left(0);
-        shared = rest > 0.0;
-        if (shared) left = rest, total = rest;
-        else --depth;                    // (where nothing is left it stays as it was)
-      } else if (!removed(d.token[c], refused)) {
-        if (threadIdx.x == 0) d.out[refused] = d.token[c];
-        __syncthreads();
-        double rest = left - d.weight[c] / sum;
-        if (rest < 1e-3) {               // little is left: float64 says how much
-          sum_exactly();
-          rest = sum_left(refused + 1) / sum;
-        }
-        shared = false;
-        if (rest > 0.0) left = rest, ++refused;
-      }
-    }
-  }
-  if (writes) p.accepted_n[slot] = steps;
-  if (!known) {
-    if (writes) p.following[slot] = -1, cache_fault(p.c, KB200_CACHE_BAD_VALUE);
-    return;
-  }
-  if (greedy) {
-    if (writes) p.following[slot] = d.best[at];
-    return;
-  }
-  // ---- the token that follows ----
-  if (!shared) total = sum_left(refused);
-  double target = (double)d.uniform[0] * total;
-  const int last_turn = turn ^ 1;
-  int owner = -1;
-  for (int r = 0; r < ranks; ++r) {      // the first whose share reaches beyond the target; where roundings leave none, the last that has any
-    const double x = totals[last_turn][r];
-    if (x > 0.0) owner = r;
-    if (target < x) break;
-    if (r + 1 < ranks) {
-      bool more = false;
-      for (int r2 = r + 1; r2 < ranks; ++r2) more = more || totals[last_turn][r2] > 0.0;
-      if (!more) break;
-    }
-    target -= x;
-  }
-  if (owner < 0 && writes) p.following[slot] = -1;
-  if (rank != owner) return;
-  const Row row = row_at();
-  // Of parts' sums (of all warps), the one that the target falls into.
-  auto find = [&]() {
-    int found = 0;
-    for (int w = 0, had = -1; w < kWalkWarps; ++w) {
-      const double x = shares[w];
-      if (x > 0.0) {
-        had = w;
-        if (target < x) {
-          found = w;
+  while (true) {
+    if (warp == 0) {
+      while (wants == kNothing) {
+        while (c < count && (!known || d.parent[c] != at)) ++c;
+        if (c == count) {
+          wants = !known || greedy || shared ? kDone : kLast;
           break;
         }
+        bool take;
+        if (greedy) {
+          take = d.token[c] == d.best[at];
+        } else {
+          const double u = (double)d.uniform[c] * (double)d.chance_q[c];
+          const bool again = p.draft == nullptr && removed(d.token[c]);
+          double chance = again ? 0.0 : depth > 0 ? d.weight[c] : exact ? d.weight[c] / sum : d.chance[c];
+          for (int k = 0; k < depth; ++k) chance = fmax(__fma_rn(chance, d.divisors[k], -(double)d.chance_q[c]), 0.0);
+          take = u * left < chance;
+          if (!exact && fabs(u * left - chance) <= kUnsure * (u + chance)) {
+            wants = kExactly;            // (what is left without a draft is 1 less the refused ones' chances, which are as near as the sum)
+          } else if (!take && p.draft != nullptr) {
+            wants = exact ? kTaken : near_top(Left{scale, (double)d.top[at]}) ? kFirst : kExactly;
+          } else if (!take && !again) {
+            const double rest = left - chance;
+            if (rest >= 1e-3) {
+              if (lane == 0) d.out[refused] = d.token[c];
+              __syncwarp();
+              left = rest, shared = false, ++refused;
+            } else {                     // little is left: float64 says how much
+              wants = exact ? kRefused : kExactly;
+            }
+          }
+        }
+        if (wants != kNothing) break;
+        if (take) {
+          at = c;
+          if (writes) accepted[steps] = c;
+          ++steps;
+          sum = d.sum[at], left = 1.0, exact = shared = false, refused = depth = 0;
+          known = sum >= 0.0;
+        }
+        ++c;
       }
-      found = max(had, 0);
-      bool more = false;
-      for (int w2 = w + 1; w2 < kWalkWarps; ++w2) more = more || shares[w2] > 0.0;
-      if (!more) break;
-      target -= x;
+      if (lane == 0) {
+        Plan next{wants, at, steps, refused, depth, known, total};
+        if (wants == kExactly) next.refused = next.depth = 0;
+        if (wants == kTaken || wants == kFirst) d.divisors[next.depth++] = 1.0 / (depth == 0 ? sum : left);
+        if (wants == kRefused) d.out[next.refused++] = d.token[c];
+        plan = next;
+      }
     }
-    return found;
-  };
-  int lo, hi, from, to;
-  part_of(0, row.vectors(), rank, ranks, &lo, &hi);
-  const int w1 = find();
-  part_of(lo, hi, w1, kWalkWarps, &from, &to);
-  lo = from, hi = to;
-  part_of(lo, hi, warp, kWalkWarps, &from, &to);
-  const double mine = sum_of(row, from, to, refused);
-  __syncthreads();
-  if (lane == 0) shares[warp] = mine;
-  __syncthreads();
-  const int w2 = find();
-  part_of(lo, hi, w2, kWalkWarps, &from, &to);
-  if (warp != 0) return;
-  int last = -1;
-  for (int i0 = from; i0 < to; i0 += 32) {
-    const int i = i0 + lane, first = row.first(i);
-    double x[VEC], of_lane = 0.0;
-    float logit[VEC];
-    if (i < to) row.load(i, logit);
+    __syncthreads();
+    if (plan.wants == kDone) break;
+    // ---- a sum over the vocabulary ----
+    const Row row(logits + plan.at * p.logits_stride[1], p.vocab);
+    const Left of{scale, (double)d.top[plan.at], table, d.divisors, d.out, b * p.draft_stride[0] + plan.at * p.draft_stride[1], plan.refused, plan.depth};
+    const int64_t vectors = row.vectors(), of_all = ranks * kWalkWarps, mine = rank * kWalkWarps + warp;
+    const int lo = (int)(vectors * mine / of_all), hi = (int)(vectors * (mine + 1) / of_all);
+    const bool first = plan.wants == kFirst;
+    const Sums mine_of = sum_of<T>(p, row, of, lo, hi, first);
+    if (lane == 0) shares[0][warp] = mine_of.left, shares[1][warp] = mine_of.all, shares[2][warp] = mine_of.of_left, shares[3][warp] = mine_of.near;
+    __syncthreads();
+    if (warp < (first ? 4 : 1)) {
+      double x = lane < kWalkWarps ? shares[warp][lane] : 0.0;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      x[j] = i < to && first + j >= 0 && first + j < p.vocab ? value(first + j, logit[j], refused) : 0.0;
-      of_lane += x[j];
+      for (int o = 16; o > 0; o /= 2) x += __shfl_xor_sync(0xffffffffu, x, o);
+      if (lane < ranks) cluster.map_shared_rank(&totals[turn][warp][0], lane)[rank] = x;
     }
-    double before = of_lane;
+    cluster.sync();
+    if (first) {                         // with the sum as it is now known
+      double all = 0.0;
+      for (int r = 0; r < ranks; ++r) all += totals[turn][1][r];
+      const double change = 1.0 / all - d.divisors[0];
+      if (lane == 0) shares[0][warp] = fmax(__fma_rn(mine_of.of_left, change, mine_of.left), 0.0);
+      __syncthreads();
+      if (warp == 0) {
+        if (lane < ranks) totals[turn][0][lane] = fmax(__fma_rn(totals[turn][2][lane], change, totals[turn][0][lane]), 0.0);
+        if (lane == 0) d.divisors[0] = 1.0 / all;
+        sum = all, exact = true;
+      }
+    }
+    if (warp == 0) {
+      __syncwarp();
+      double all = 0.0, near = 0.0;
+      for (int r = 0; r < ranks; ++r) all += totals[turn][0][r], near += first ? totals[turn][3][r] : 0.0;
+      if (near > kMostNear) {
+        shared = false, wants = kNothing;
+      } else if (wants == kExactly) {
+        if (p.draft == nullptr) left = 1.0 - (1.0 - left) * (sum / all);
+        sum = total = all, exact = true;
+        shared = refused == 0;
+        wants = kNothing;
+      } else if (wants == kLast) {
+        total = all, wants = kDone;
+      } else {                           // (where nothing is left it stays as it was)
+        const double rest = wants == kRefused ? all / sum : all;
+        shared = rest > 0.0;
+        if (shared) left = rest, total = all, refused = plan.refused, depth = plan.depth;
+        ++c;
+        wants = kNothing;
+      }
+    }
+    turn ^= 1;
+  }
+  at = plan.at;
+  if (writes) p.accepted_n[slot] = plan.steps;
+  if (!plan.known || greedy) {
+    if (writes) p.following[slot] = plan.known ? d.best[at] : -1;
+    if (writes && !plan.known) cache_fault(p.c, KB200_CACHE_BAD_VALUE);
+    return;
+  }
+  const Left now{scale, (double)d.top[at], table, d.divisors, d.out, b * p.draft_stride[0] + at * p.draft_stride[1], plan.refused, plan.depth};
+  // ---- the token that follows: the CTA, the warp's part, a part of that, and in it the token, in whose share the target falls ----
+  const Row row(logits + at * p.logits_stride[1], p.vocab);
+  double target = (double)d.uniform[0] * plan.total;
+  // Of up to 32 shares, one in each lane, the first that reaches beyond the target, which becomes what it is beyond those before; where roundings leave none, the last
+  // that has any.
+  bool reached = false;                  // whether the one found is of the first kind
+  double below = 0.0, all = 0.0;         // the shares in front of it; all of them
+  auto find = [&](double x) {
+    double upto = x;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
-      const double y = __shfl_up_sync(0xffffffffu, before, o);
-      if (lane >= o) before += y;
+      const double y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
     }
-    const double all = __shfl_sync(0xffffffffu, before, 31);
-    before -= of_lane;
-    int mine_at = INT_MAX, mine_last = -1;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      before += x[j];
-      if (x[j] > 0.0) {
-        mine_last = first + j;
-        if (mine_at == INT_MAX && before > target) mine_at = first + j;
-      }
-    }
-    const int found = __reduce_min_sync(0xffffffffu, mine_at);
-    last = max(last, __reduce_max_sync(0xffffffffu, mine_last));
-    if (found != INT_MAX) {
-      last = found;
-      break;
-    }
+    const unsigned any = __ballot_sync(0xffffffffu, x > 0.0), beyond = __ballot_sync(0xffffffffu, x > 0.0 && target < upto);
+    const int found = beyond != 0 ? __ffs(beyond) - 1 : 31 - __clz(any);      // (-1: there are none)
+    all = __shfl_sync(0xffffffffu, upto, 31);
+    below = __shfl_sync(0xffffffffu, upto - x, max(found, 0));
+    reached = beyond != 0;
+    return found;
+  };
+  const int owner = find(lane < ranks ? totals[turn ^ 1][0][lane] : 0.0);
+  if (owner < 0 && writes) p.following[slot] = -1;
+  if (rank != owner) return;
+  target -= below;
+  const int w1 = find(lane < kWalkWarps ? shares[0][lane] : 0.0);
+  target -= below;
+  const int64_t vectors = row.vectors(), of_all = ranks * kWalkWarps, mine = rank * kWalkWarps + w1;
+  const int lo = (int)(vectors * mine / of_all), hi = (int)(vectors * (mine + 1) / of_all);
+  auto part = [&](int i) { return lo + (int)((int64_t)(hi - lo) * i / kWalkWarps); };
+  const double share = sum_of<T>(p, row, now, part(warp), part(warp + 1), false).left;
+  __syncthreads();
+  if (lane == 0) shares[0][warp] = share;
+  __syncthreads();
+  if (warp != 0) return;
+  const int w2 = find(lane < kWalkWarps ? shares[0][lane] : 0.0);
+  target -= below;
+  const int begin = max(row.first(part(w2)), 0), end = min(row.first(part(w2 + 1)), p.vocab);
+  int last = -1;
+  for (int v0 = begin; v0 < end; v0 += 32) {
+    const int v = v0 + lane;
+    const int found = find(v < end ? value_of(p, now, v, as_float(row.row[v])) : 0.0);
+    if (found >= 0) last = v0 + found;
+    if (reached) break;
     target -= all;
   }
   if (lane == 0) p.following[slot] = last;
@@ -532,14 +750,15 @@ __global__ void __launch_bounds__(kWalkThreads, 1) verify_walk_kernel(const __gr
 
 // ---- host --------------------------------------------------------------------------------------
 
-// Chunks of a row: so many CTAs that each of them has a row's part of 16 KB or so, and the GPU is full a few times over.
+// Chunks of a row: as many CTAs as an SM holds of them, four, and a row's part is 8 KB at least.  (With four times as many, of which half had a row behind its sequence's last, 8 rows of
+// 12 tokens took 14.5 us.)
 int chunks_of(const Cache& c, int rows, int tokens, int vocab) {
-  const int64_t nodes = (int64_t)rows * tokens, wanted = (16 * (int64_t)c.sm_count + nodes - 1) / nodes;
-  return (int)std::min<int64_t>(std::min<int64_t>(wanted, 64), std::max(1, vocab / 2048));
+  const int64_t nodes = (int64_t)rows * tokens, wanted = (4 * (int64_t)c.sm_count + nodes - 1) / nodes;
+  return (int)std::min<int64_t>(std::min<int64_t>(wanted, 64), std::max(1, vocab / 2048));      // (64: two to a lane)
 }
 int cluster_of(const Cache& c, int rows) {
   int n = kMostCluster;
-  while (n > 2 && rows * n > 2 * c.sm_count) n /= 2;
+  while (n > 1 && (int64_t)rows * n > c.sm_count) n /= 2;
   return n;
 }
 
@@ -565,11 +784,23 @@ cudaError_t launch_verify(const Cache& c, const VerifyParams& p, cudaStream_t s)
   return cudaLaunchKernelEx(&cfg, verify_walk_kernel<T>, p);
 }
 
+template <typename T>
+cudaError_t allow_clusters() {
+  return cudaFuncSetAttribute(verify_walk_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+}
 bool verify_ok(const Cache& c, int rows, int tokens, int vocab) {
   return rows >= 0 && rows <= (1 << 20) && tokens >= 0 && tokens <= kMostTokens && vocab >= 1 && vocab < (1 << 30);
 }
 
 }  // namespace
+
+int cache_verify_prepare() {
+  KB200_CUDA(allow_clusters<float>());
+  KB200_CUDA(allow_clusters<__nv_bfloat16>());
+  KB200_CUDA(allow_clusters<__half>());
+  return KB200_OK;
+}
+
 }  // namespace kb200
 
 using namespace kb200;
