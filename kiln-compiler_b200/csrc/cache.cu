@@ -709,6 +709,7 @@ KB200_EXPORT int kb200_cache_create(const kb200_cache_desc* d, int device, kb200
   c->view = CacheView{d->pool, d->table, d->held, d->lengths, d->refs, status, d->layers, d->sequences, d->max_pages, d->pages, d->kv_heads,
                       page_log2_of(d->page_tokens), d->head_dim, d->head_dim * c->element / 16};
   int prepared = cache_attention_prepare(*c);
+  if (prepared == KB200_OK) prepared = cache_weigh_prepare(*c);
   if (prepared == KB200_OK) prepared = cache_verify_prepare();
   if (prepared != KB200_OK) {
     cudaFree(c->scratch);

@@ -44,6 +44,7 @@ inline bool cache_attention_call_ok(const Cache& c, int rows, int tokens, int he
          (int64_t)rows * (tokens > 1 ? tokens : 1) <= (1 << 30) && (int64_t)heads * c.view.row_chunks <= (1 << 30);
 }
 int cache_verify_prepare();                  // (cache_verify.cu) the kernels' limits, on the current device
+int cache_weigh_prepare(const Cache& c);     // (cache_weigh.cu) the same
 int cache_attention_prepare(Cache& c);       // (cache_attention.cu) the pool's map and the kernels' limits, on the current device
 
 inline Cache* cache_of(const kb200_cache* c) { return reinterpret_cast<Cache*>(const_cast<kb200_cache*>(c)); }
