@@ -59,13 +59,26 @@ __device__ __forceinline__ uint32_t rank_of(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// The sum of a warp's lanes up to each.
+__device__ __forceinline__ int warp_sums(int x) {
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int below = __shfl_up_sync(0xffffffffu, x, d);
+    if ((threadIdx.x & 31) >= d) x += below;
+  }
+  return x;
+}
+
 // A CTA takes a sequence.  The least rank that stays is found digit by digit (11, 11 and 10 bits from the top), by counting the candidates of each digit; of the tokens
-// at that rank the first ones stay.  Two sweeps then give every kept token its place: a warp has neighbouring tokens, so that its places begin behind those of the
-// warps before it.
-__global__ void __launch_bounds__(kChooseThreads) evict_choose_kernel(const CacheView c, const EvictParams p) {
+// at that rank the first ones stay.  Then every kept token gets its place, 8192 tokens at a time: by ballots, how many stay of each 32, and sums of those.  The first 8192 weights are
+// read once, eight to a thread (read again for every digit, with sums over the warps one by one, a sequence of 1000 took 9.2 us and one of 4096 14.7).
+constexpr int kHeld = 8, kGroup = kHeld * kChooseThreads;
+
+__global__ void __launch_bounds__(kChooseThreads, 1) evict_choose_kernel(const CacheView c, const EvictParams p) {
   __shared__ int bins[kBins];
   __shared__ int sums[kChooseWarps];
-  __shared__ int2 counts[kChooseWarps];
+  __shared__ int2 counts[kHeld * kChooseWarps];
+  __shared__ int2 group_counts;
   __shared__ int digit, above, in_digit, first_moved, faults;
   pdl_wait();
   pdl_launch_dependents();
@@ -73,13 +86,21 @@ __global__ void __launch_bounds__(kChooseThreads) evict_choose_kernel(const Cach
   const float* const weights = p.weights + s * p.weights_stride;
   float* const out = p.out + s * p.out_stride;
   const int32_t* const row = c.table + (int64_t)s * c.max_pages;
+  float w[kHeld];                                             // (asked for before the sequence's length is known)
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) w[k] = k * kChooseThreads + (int)threadIdx.x < p.width ? weights[k * kChooseThreads + threadIdx.x] : 0.0f;
   const int held = min(max(c.held[s], 0), c.max_pages), want = p.keep[s];
   int length = max(c.lengths[s], 0);
-  if (threadIdx.x == 0) first_moved = INT_MAX, faults = 0;
-  if ((int64_t)length > (int64_t)held << c.page_log2) {
-    if (threadIdx.x == 0) cache_fault(c, KB200_CACHE_NO_ROOM);
-    length = held << c.page_log2;
-  } else if (want >= 0 && want < length) {
+  const bool has_pages = (int64_t)length <= (int64_t)held << c.page_log2;
+  if (!has_pages) length = held << c.page_log2;
+  if (threadIdx.x == 0) first_moved = INT_MAX, faults = has_pages ? 0 : KB200_CACHE_NO_ROOM;
+  if (has_pages && want >= 0 && want < length) {
+    // What is written has to be the sequence's own (as far as anything moves): the first pages are looked at meanwhile.
+    auto page_faults = [&](int k) {
+      const int page = row[k];
+      return !cache_page_ok(c, page) ? KB200_CACHE_NO_ROOM : c.refs[page] > 1 ? KB200_CACHE_SHARED : 0;
+    };
+    const int last_page = (want - 1) >> c.page_log2, my_page_faults = (int)threadIdx.x <= last_page ? page_faults(threadIdx.x) : 0;
     const int first = min(p.sinks, want), last = min(p.recent, want - first);
     const int lo = first, hi = length - last;                 // the candidates, of which `need` stay
     int need = want - first - last;
@@ -88,26 +109,21 @@ __global__ void __launch_bounds__(kChooseThreads) evict_choose_kernel(const Cach
     bool all = need == 0;                                     // every candidate of this prefix and above stays (need 0: none)
     while (shift > 0 && !all) {
       const int bits = shift > 10 ? 11 : 10;
-      for (int i = threadIdx.x; i < kBins; i += kChooseThreads) bins[i] = 0;
+      bins[threadIdx.x] = bins[threadIdx.x + kChooseThreads] = 0;
       __syncthreads();
-      for (int j = lo + threadIdx.x; j < hi; j += kChooseThreads) {
-        const uint32_t r = rank_of(weights[j]);
-        if (shift == 32 || r >> shift == prefix) atomicAdd(&bins[r >> (shift - bits) & ((1u << bits) - 1)], 1);
-      }
+      auto count = [&](int j, float x) {
+        const uint32_t r = rank_of(x);
+        if (j >= lo && j < hi && (shift == 32 || r >> shift == prefix)) atomicAdd(&bins[r >> (shift - bits) & ((1u << bits) - 1)], 1);
+      };
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k) count(k * kChooseThreads + threadIdx.x, w[k]);
+      for (int j = kGroup + threadIdx.x; j < hi; j += kChooseThreads) count(j, weights[j]);
       __syncthreads();
       // from the highest digit down: thread t has digits kBins - 1 - 2t and the one below
-      const int d = kBins - 1 - 2 * threadIdx.x, a = bins[d], b = bins[d - 1];
-      int sum = a + b;
-#pragma unroll
-      for (int i = 1; i < 32; i *= 2) {
-        const int below = __shfl_up_sync(0xffffffffu, sum, i);
-        if (lane >= i) sum += below;
-      }
-      if (lane == 31) sums[warp] = sum;
+      const int d = kBins - 1 - 2 * threadIdx.x, a = bins[d], b = bins[d - 1], upto = warp_sums(a + b);
+      if (lane == 31) sums[warp] = upto;
       __syncthreads();
-      int before = 0;
-      for (int w = 0; w < warp; ++w) before += sums[w];
-      before += sum - a - b;
+      const int of_warps = warp_sums(sums[lane]), before = __shfl_sync(0xffffffffu, of_warps - sums[lane], warp) + upto - a - b;
       if (before < need && before + a >= need) digit = d, above = before, in_digit = a;
       else if (before + a < need && before + a + b >= need) digit = d - 1, above = before + a, in_digit = b;
       __syncthreads();
@@ -118,77 +134,103 @@ __global__ void __launch_bounds__(kChooseThreads) evict_choose_kernel(const Cach
     }
     const uint32_t least = need == 0 ? 0xffffffffu : prefix << shift;
     const int ties = need == 0 ? 0 : all ? INT_MAX : need;
-    // Kept whatever the others are; kept if `ties` allow.
-    auto sure = [&](int j, uint32_t r) { return j < lo || j >= hi || (all && need > 0 ? r >= least : r > least); };
-    auto tied = [&](int j, uint32_t r) { return j >= lo && j < hi && !all && r == least; };
-    const int part = (length + kChooseThreads - 1) / kChooseThreads * 32, from = min(warp * part, length), to = min(from + part, length);
-    int2 mine = make_int2(0, 0);
-    for (int j0 = from; j0 < to; j0 += 32) {
-      const int j = j0 + lane;
-      const uint32_t r = j < to ? rank_of(weights[j]) : 0u;
-      mine.x += __popc(__ballot_sync(0xffffffffu, j < to && sure(j, r)));
-      mine.y += __popc(__ballot_sync(0xffffffffu, j < to && tied(j, r)));
-    }
-    if (lane == 0) counts[warp] = mine;
-    __syncthreads();
-    int places = 0, equal = 0;
-    for (int w = 0; w < warp; ++w) places += counts[w].x, equal += counts[w].y;
-    places += min(equal, ties);
     int64_t* const kept = p.from + (int64_t)s * p.width;
     float* const staged = p.staged + (int64_t)s * p.width;
     const unsigned below = (1u << lane) - 1;
-    int moved = INT_MAX, fault = 0;
-    for (int j0 = from; j0 < to; j0 += 32) {
-      const int j = j0 + lane;
-      const float w = j < to ? weights[j] : 0.0f;
-      const uint32_t r = rank_of(w);
-      const bool is_tied = j < to && tied(j, r);
-      const unsigned all_tied = __ballot_sync(0xffffffffu, is_tied);
-      const bool stays = j < to && (sure(j, r) || (is_tied && equal + __popc(all_tied & below) < ties));
-      const unsigned all_stay = __ballot_sync(0xffffffffu, stays);
-      if (stays) {
-        const int at = places + __popc(all_stay & below), page = row[j >> c.page_log2];
-        kept[at] = ((int64_t)page << c.page_log2) + (j & in_page);
-        staged[at] = w;
-        if (at != j) moved = min(moved, at);
-        fault |= cache_page_ok(c, page) ? 0 : KB200_CACHE_NO_ROOM;
+    const bool in_one = length <= kGroup;                     // the kept weights stay where they are until it is known that the tokens may move
+    int places[kHeld], moved = INT_MAX, fault = 0;
+    int2 base = make_int2(0, 0);                              // kept whatever the others are; at the least rank
+    for (int j0 = 0; j0 < length; j0 += kGroup) {
+      unsigned sure[kHeld], tied[kHeld];
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k) {
+        const int j = j0 + k * kChooseThreads + threadIdx.x;
+        if (j0 > 0) w[k] = j < length ? weights[j] : 0.0f;
+        const uint32_t r = rank_of(w[k]);
+        const bool in = j >= lo && j < hi;
+        sure[k] = __ballot_sync(0xffffffffu, j < length && (!in || (all && need > 0 ? r >= least : r > least)));
+        tied[k] = __ballot_sync(0xffffffffu, j < length && in && !all && r == least);
+        if (lane == k) counts[k * kChooseWarps + warp] = make_int2(__popc(sure[k]), __popc(tied[k]));
       }
-      places += __popc(all_stay);
-      equal += __popc(all_tied);
+      __syncthreads();
+      if (warp == 0) {
+        int2 mine[kHeld], sum = make_int2(0, 0);              // a lane has eight in a row
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) {
+          const int2 x = counts[lane * kHeld + k];
+          mine[k] = sum;
+          sum.x += x.x, sum.y += x.y;
+        }
+        const int x = warp_sums(sum.x), y = warp_sums(sum.y);
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) counts[lane * kHeld + k] = make_int2(mine[k].x + x - sum.x, mine[k].y + y - sum.y);
+        if (lane == 31) group_counts = make_int2(x, y);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k) {
+        const int j = j0 + k * kChooseThreads + threadIdx.x;
+        const int2 before = counts[k * kChooseWarps + warp];
+        const int equal = base.y + before.y + __popc(tied[k] & below);
+        places[k] = -1;
+        if ((sure[k] >> lane & 1) != 0 || ((tied[k] >> lane & 1) != 0 && equal < ties)) {
+          const int at = base.x + before.x + __popc(sure[k] & below) + min(equal, ties), page = row[j >> c.page_log2];
+          kept[at] = ((int64_t)page << c.page_log2) + (j & in_page);
+          places[k] = at;
+          if (!in_one) staged[at] = w[k];
+          if (at != j) moved = min(moved, at);
+          fault |= cache_page_ok(c, page) ? 0 : KB200_CACHE_NO_ROOM;
+        }
+      }
+      base.x += group_counts.x, base.y += group_counts.y;
+      __syncthreads();
     }
     if (moved != INT_MAX) atomicMin(&first_moved, moved);
     if (fault != 0) atomicOr(&faults, fault);
     __syncthreads();
-    // What is written has to be the sequence's own.
-    if (first_moved != INT_MAX)
-      for (int k = (first_moved >> c.page_log2) + threadIdx.x; k <= (want - 1) >> c.page_log2; k += kChooseThreads) {
-        const int page = row[k];
-        const int bad = !cache_page_ok(c, page) ? KB200_CACHE_NO_ROOM : c.refs[page] > 1 ? KB200_CACHE_SHARED : 0;
-        if (bad != 0) atomicOr(&faults, bad);
-      }
+    if (first_moved != INT_MAX) {
+      const int first_page = first_moved >> c.page_log2;
+      int bad = (int)threadIdx.x >= first_page ? my_page_faults : 0;
+      for (int k = threadIdx.x + kChooseThreads; k <= last_page; k += kChooseThreads) bad |= k >= first_page ? page_faults(k) : 0;
+      if (bad != 0) atomicOr(&faults, bad);
+    }
     __syncthreads();
     if (faults == 0) {
       if (threadIdx.x == 0) p.answers[s] = make_int2(want, first_moved);
-      for (int i = threadIdx.x; i < p.width; i += kChooseThreads) out[i] = i < want ? staged[i] : 0.0f;
+      if (in_one) {
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k)
+          if (places[k] >= 0) out[places[k]] = w[k];
+      }
+      for (int i = threadIdx.x; i < p.width; i += kChooseThreads)
+        if (!in_one || i >= want) out[i] = i < want ? staged[i] : 0.0f;
       return;
     }
-    if (threadIdx.x == 0) cache_fault(c, faults);
   }
-  if (threadIdx.x == 0) p.answers[s] = make_int2(-1, 0);
+  if (threadIdx.x == 0) {
+    if (faults != 0) cache_fault(c, faults);
+    p.answers[s] = make_int2(-1, 0);
+  }
   for (int i = threadIdx.x; i < p.width; i += kChooseThreads) out[i] = i < length ? weights[i] : 0.0f;
 }
 
 // ---- the tokens --------------------------------------------------------------------------------
 
-constexpr int kMoveThreads = 256, kMoveAtOnce = 8;
+constexpr int kMoveThreads = 256, kMoveWarps = kMoveThreads / 32, kMoveAtOnce = 16;
 
 // A CTA takes one sequence's tokens in one layer, head and of K or V.  Token i comes from a place behind its own or from its own: batches ascend, and a batch
-// is read before any of it is written, so nothing is overwritten that is still to be read.
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const CacheView c, const EvictParams p) {
+// is read before any of it is written, so nothing is overwritten that is still to be read.  A warp has up to 32 neighbouring tokens of a batch, whose places its lanes work out, one each, and moves
+// up to 512 chunks of 16 bytes, 16 to a lane, all under way at once.  (With a place looked up for every chunk 157 us for 390 MB, 5.0 TB/s both ways.)
+// And what is behind the kept tokens is given up, which no token moves into or out of.
+__global__ void __launch_bounds__(kMoveThreads, 2) evict_move_kernel(const CacheView c, const EvictParams p) {
   pdl_wait();
   pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, in_page = (1 << c.page_log2) - 1;
+  for (int s = gridDim.x * warp + blockIdx.x; s < c.sequences; s += gridDim.x * kMoveWarps)
+    if (p.answers[s].x >= 0) cut(c, s, p.answers[s].x);
   const int64_t planes = (int64_t)c.layers * 2 * c.kv_heads, units = planes * c.sequences;
-  const int in_page = (1 << c.page_log2) - 1;
+  const int rows = min(32, 32 * kMoveAtOnce / c.row_chunks), chunks = rows * c.row_chunks;        // of a warp (row_chunks: 64 at most)
+  const int reciprocal = ((1 << 20) + c.row_chunks - 1) / c.row_chunks;                           // chunk / row_chunks of up to 2048 = chunk * reciprocal >> 20
   uint4* const pool = static_cast<uint4*>(c.pool);
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
     const int s = (int)(u / planes);
@@ -197,41 +239,37 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const CacheVie
     const int64_t plane = u % planes;
     const int64_t half = plane / c.kv_heads * c.pages;          // K or V of a layer, in pages
     const int head = (int)(plane % c.kv_heads);
-    const int32_t* const row = c.table + (int64_t)s * c.max_pages;
+    const int32_t* const table = c.table + (int64_t)s * c.max_pages;
     const int64_t* const kept = p.from + (int64_t)s * p.width;
-    auto place = [&](int64_t page, int at) { return pool + ((((half + page) * c.kv_heads + head) << c.page_log2) + at) * c.row_chunks; };
-    const int64_t chunks = (int64_t)(answer.x - answer.y) * c.row_chunks;
-    for (int64_t i0 = 0; i0 < chunks; i0 += kMoveThreads * kMoveAtOnce) {
-      uint4 v[kMoveAtOnce];
-      uint4* to[kMoveAtOnce];
-      const int batch = (int)min((int64_t)(kMoveThreads * kMoveAtOnce), chunks - i0);
-      const int token0 = answer.y + (int)(i0 / c.row_chunks), chunk0 = (int)(i0 % c.row_chunks);
-#pragma unroll
-      for (int j = 0; j < kMoveAtOnce; ++j) {
-        const int i = threadIdx.x + kMoveThreads * j;
-        to[j] = nullptr;
-        if (i < batch) {
-          const int ahead = (chunk0 + i) / c.row_chunks, chunk = chunk0 + i - ahead * c.row_chunks, token = token0 + ahead;
-          const int64_t from = kept[token];
-          v[j] = __ldcs(place(from >> c.page_log2, (int)(from & in_page)) + chunk);
-          to[j] = place(row[token >> c.page_log2], token & in_page) + chunk;
-        }
+    auto place = [&](int64_t page, int at) { return ((((half + page) * c.kv_heads + head) << c.page_log2) + at) * c.row_chunks; };
+    for (int token0 = answer.y; token0 < answer.x; token0 += kMoveWarps * rows) {
+      const int token = token0 + warp * rows + lane, there = min(rows, answer.x - token0 - warp * rows);
+      int64_t from = 0, to = 0;
+      if (lane < there) {
+        const int64_t slot = kept[token];
+        from = place(slot >> c.page_log2, (int)(slot & in_page));
+        to = place(table[token >> c.page_log2], token & in_page);
       }
-      __syncthreads();
+      uint4 v[kMoveAtOnce];
+      auto each = [&](auto&& f) {
 #pragma unroll
-      for (int j = 0; j < kMoveAtOnce; ++j)
-        if (to[j] != nullptr) *to[j] = v[j];
+        for (int j = 0; j < kMoveAtOnce; ++j) {
+          if (32 * j >= chunks) break;
+          const int i = 32 * j + lane, r = i * reciprocal >> 20;
+          f(j, r, i - r * c.row_chunks);
+        }
+      };
+      each([&](int j, int r, int chunk) {
+        const int64_t at = __shfl_sync(0xffffffffu, from, r & 31);
+        if (r < there) v[j] = __ldcs(pool + at + chunk);
+      });
+      __syncthreads();
+      each([&](int j, int r, int chunk) {
+        const int64_t at = __shfl_sync(0xffffffffu, to, r & 31);
+        if (r < there) pool[at + chunk] = v[j];
+      });
     }
   }
-}
-
-constexpr int kSlotThreads = 128;
-
-__global__ void __launch_bounds__(kSlotThreads) evict_commit_kernel(const CacheView c, const EvictParams p) {
-  pdl_wait();
-  pdl_launch_dependents();
-  const int s = blockIdx.x * (kSlotThreads / 32) + (threadIdx.x >> 5);
-  if (s < c.sequences && p.answers[s].x >= 0) cut(c, s, p.answers[s].x);
 }
 
 // ---- host --------------------------------------------------------------------------------------
@@ -274,8 +312,6 @@ KB200_EXPORT int kb200_cache_evict(kb200_cache* handle, const float* weights, in
                 reinterpret_cast<int2*>(at + up(n * 8) + up(n * 4)), recent, sinks, (int)width};
   KB200_CUDA(launch_kernel(true, evict_choose_kernel, dim3(c.view.sequences), dim3(kChooseThreads), 0, s, c.view, p));
   const int64_t units = c.planes() * c.view.sequences;
-  KB200_CUDA(launch_kernel(true, evict_move_kernel, dim3((unsigned)std::min<int64_t>(units, 16 * c.sm_count)), dim3(kMoveThreads), 0, s, c.view, p));
-  const int per = kSlotThreads / 32;
-  KB200_CUDA(launch_kernel(true, evict_commit_kernel, dim3((c.view.sequences + per - 1) / per), dim3(kSlotThreads), 0, s, c.view, p));
+  KB200_CUDA(launch_kernel(true, evict_move_kernel, dim3((unsigned)std::min<int64_t>(units, 2 * c.sm_count)), dim3(kMoveThreads), 0, s, c.view, p));
   return KB200_OK;
 }

@@ -210,7 +210,7 @@ def test_any_operations_leave_what_the_lists_say(dtype, page_tokens, head_dim, s
     assert moved > 0
 
 
-@pytest.mark.parametrize("length", [1, 31, 33, 1000, 1024, 1025, 5000])
+@pytest.mark.parametrize("length", [1, 31, 33, 1000, 1024, 1025, 5000, 8193, 20000])
 def test_evicted_tokens(length):
     """Ties, NaN, infinities and zeros of both signs; weights in place and in rows of another tensor."""
     cache, _ = filled([length, 40], [0, 0] if length < 1 else [1, 1], dtype=BF16, kv_heads=1, head_dim=16, page_tokens=8)
