@@ -153,6 +153,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
       CacheGap gap{0, 0};
       if constexpr (WINDOW) {
         gap = gap_of<ROWS, TILE>(p, now);
+        at.sure = min(sure_keys<ROWS>(p, now), now.it.end);
         at.hidden = now.it.length + last_place<ROWS>(p, now.row_tile, at.rows_here) - p.window + 1;
       }
       auto key_of = [&](int tile) { return (WINDOW ? gap.tile(tile) : tile) * TILE; };

@@ -123,6 +123,11 @@ template <int ROWS, int TILE>
 __device__ __forceinline__ CacheGap gap_of(const CacheAttnParams& p, const CacheCursor& u) {
   return gap_of<TILE>(p, u.it.length, u.it.row_tiles > 1 && own_places(p) ? u.row_tile * ROWS / p.group : 0);
 }
+// Keys in front of which a mask hides nothing from an item's rows: without one, those up to its first row's own.
+template <int ROWS>
+__device__ __forceinline__ int sure_keys(const CacheAttnParams& p, const CacheCursor& u) {
+  return u.it.length + (p.mask == nullptr ? u.row_tile * ROWS / p.group + 1 : 0);
+}
 // To the next item.
 template <int ROWS, int TILE, bool WINDOW>
 __device__ __forceinline__ void next_item(const CacheAttnParams& p, CacheCursor& u) {

@@ -40,6 +40,11 @@ struct TcMath {
   static __device__ __forceinline__ float log_sum(float top, float sum, float scale) { return MmaMath<T, DP>::log_sum(top, sum, scale); }
 };
 
+// With a window, output rows are rescaled only when a row's maximum has grown by this power of two.  Among the first few dozen tiles one of a warp's 32 rows nearly always has a new
+// maximum, and rescaling is an eighth of a tile's time; weights up to 2^8 of the largest so far are as exact, and float16, whose largest is 2^12, has three more powers.
+template <typename T>
+constexpr float kSlack = std::is_same<T, __half>::value ? 3.0f : 8.0f;
+
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
@@ -60,6 +65,20 @@ __device__ __forceinline__ void tmem_ld8x2(uint32_t addr_a, uint32_t addr_b, flo
       : "memory");
 #pragma unroll
   for (int i = 0; i < 8; ++i) va[i] = __uint_as_float(a[i]), vb[i] = __uint_as_float(b[i]);
+}
+
+// Whether any of a group's threads says so; all of them meet.
+__device__ __forceinline__ bool any_of_group(int group, bool says) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.aligned.pred q, %2, %3, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"(says ? 1u : 0u), "r"(1 + group), "n"(kRows)
+      : "memory");
+  return any != 0;
 }
 
 // More drafted tokens than are looked up ahead: what the rows see of those in one tile, two words per token, a warp a word in four.  (64 sequences, trees of 300 tokens behind
@@ -206,7 +225,7 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
     auto meet_both = [&]() { asm volatile("bar.sync 3, %0;" ::"n"(2 * kRows) : "memory"); };
     uint32_t t0 = 0;                                 // the item's first tile
     for (int tiles; any && (tiles = run.tiles(p)) > 0; run.pass<kRows, TILE, WINDOW>(p, tiles)) {
-      const int rows_here = min(kRows, now.it.count * p.group - now.row_tile * kRows), sure = min(now.it.length, now.it.end);
+      const int rows_here = min(kRows, now.it.count * p.group - now.row_tile * kRows), sure = min(WINDOW ? sure_keys<kRows>(p, now) : now.it.length, now.it.end);
       const bool there = row < rows_here, warp_there = quad * 32 < rows_here;
       CacheGap gap{0, 0};
       int hidden = 0;                                // (a window) keys from here on are not hidden from any row
@@ -232,7 +251,25 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
         }
       }
       // half a row of Q (the products that read the last item's have been executed: its output was read); zeros for rows that are not there
-      if (warp_there) {
+      if (WINDOW && !p.q_fp32 && warp_there) {
+        // Four rows to a load of the warp.  (A row to a lane is 32 lines to a load: 4700 cycles of an item's 14000 beside its tiles.)
+        const int64_t mine = now.b * p.q_stride[0] + r.token * p.q_stride[1] + r.head * p.q_stride[2];
+        uint4 x[DP / 16];
+        constexpr int LANES = DP / 16, ROWS = 32 / LANES;              // of a row's half; rows at once
+        const int at = group * LANES + lane % LANES;
+#pragma unroll
+        for (int i = 0; i < LANES; ++i) {
+          const int of = i * ROWS + lane / LANES;
+          const int64_t from = __shfl_sync(0xffffffffu, mine, of);
+          x[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (quad * 32 + of < rows_here && at * 8 < p.c.head_dim) x[i] = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + from)[at];
+        }
+#pragma unroll
+        for (int i = 0; i < LANES; ++i) {
+          const int of = quad * 32 + i * ROWS + lane / LANES;
+          *reinterpret_cast<uint4*>(smem + at / 8 * Z::kQBlock + of * 128 + (((at % 8) ^ (of & 7)) << 4)) = x[i];
+        }
+      } else if (warp_there) {
         const int64_t from = now.b * p.q_stride[0] + r.token * p.q_stride[1] + r.head * p.q_stride[2];
         uint4 x[DP / 16];
 #pragma unroll
@@ -281,7 +318,26 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const bool hides = WINDOW && window_hides(p, key0, TILE, hidden), drafted = key0 + TILE > sure || hides, work = ok && warp_there;
         unsigned long long odd = 0ull;
-        if (drafted) {
+        // (with a window, where such tiles are a third of all: once over V, and all of that only where something in it is not finite)
+        bool look_closely = drafted;
+        if (WINDOW && drafted) {
+          uint8_t* const values = smem + Z::kQBytes + stage * G::kBytes + G::kHalf;
+          constexpr int kChunks = G::kBlocks * 8;
+          const int in_page = (1 << p.c.page_log2) - 1, last = now.it.end - key0;
+          const int from = (hides ? 0 : max(0, sure - key0)) * kChunks, to = min(TILE, ((now.it.end + in_page) & ~in_page) - key0) * kChunks;
+          uint32_t found = 0u;
+          if (wait(full + 8 * stage, (t / Z::kStages) & 1)) {
+#pragma unroll 4
+            for (int c = from + worker; c < to; c += kRows) {
+              uint4* const x = reinterpret_cast<uint4*>(G::at(values, c / kChunks, c % kChunks * 8));
+              if (c / kChunks >= last) *x = make_uint4(0u, 0u, 0u, 0u);
+              else found |= not_finite<T>(x->x) | not_finite<T>(x->y) | not_finite<T>(x->z) | not_finite<T>(x->w);
+            }
+          }
+          if (to > last * kChunks) fence_async_smem();
+          look_closely = any_of_group(group, (found & 0x80008000u) != 0u) || (MANY && p.mask != nullptr);
+        }
+        if (look_closely) {
           // V behind the sequence's end becomes zeros, and so do infinities and NaN (see look_at_values), by all rows' threads of the group together.
           uint8_t* const values = smem + Z::kQBytes + stage * G::kBytes + G::kHalf;
           constexpr int kChunks = G::kBlocks * 8;
@@ -346,7 +402,7 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
           const float mx = exponent_of_top<T>(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), p.scale_log2);
           if (done == 0) {
             m = mx;
-          } else if (__any_sync(0xffffffffu, mx > m)) {
+          } else if (__any_sync(0xffffffffu, mx > (WINDOW && fabsf(m) <= kFarScore ? m + kSlack<T> : m))) {
             const float grown = fmaxf(m, mx), alpha = grown == -CUDART_INF_F ? 1.0f : ex2(m - grown);
             m = grown;
             l *= alpha;
@@ -421,6 +477,20 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
         if constexpr (WINDOW) {
           if (whole && there && group == 0) write_lse(p, now.b, r, TcMath<T, DP>::log_sum(top, sum, p.scale_log2));
         }
+        if (WINDOW && whole) {                       // 64 bytes of a row at a time (16: 4800 cycles)
+#pragma unroll 1
+          for (int c = group * (DP / 2); c < (group + 1) * (DP / 2); c += 32) {
+            float o[32], o2[32];
+            tmem_ld32x2(lane_addr + c, lane_addr + DP + c, o, o2);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = (first ? o[j] * fa : 0.0f) + (second ? o2[j] * fb : 0.0f);
+#pragma unroll
+            for (int j = 0; j < 32; j += 8)
+              if (there && c + j < p.c.head_dim)
+                *reinterpret_cast<uint4*>(to + c + j) = make_uint4(pack<T>(o[j], o[j + 1]), pack<T>(o[j + 2], o[j + 3]), pack<T>(o[j + 4], o[j + 5]), pack<T>(o[j + 6], o[j + 7]));
+            __syncwarp();
+          }
+        } else
         // (small code: a launch meets it cold)
 #pragma unroll 1
         for (int c = group * (DP / 2); c < (group + 1) * (DP / 2); c += 8) {

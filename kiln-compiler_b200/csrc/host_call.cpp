@@ -399,9 +399,19 @@ const at::Tensor& floats_to(const CacheCaller& c, PyObject* o, const char* name,
   if (at::has_internal_overlap(t) == at::MemOverlap::Yes) REFUSE(PyExc_ValueError, "elements of %s share memory", name);
   return t;
 }
+// Whether two tensors' memory, from the first to the last element of each, has bytes in common.
+bool near_each_other(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0 || !has_memory(a) || !has_memory(b)) return false;
+  auto extent = [](const at::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);      // (strides are not negative)
+    return (last + 1) * (int64_t)t.element_size();
+  };
+  const char *const at_a = static_cast<const char*>(a.const_data_ptr()), *const at_b = static_cast<const char*>(b.const_data_ptr());
+  return at_a < at_b + extent(b) && at_b < at_a + extent(a);
+}
 void apart(const at::Tensor& a, const at::Tensor& b, const char* name_a, const char* name_b) {
-  const at::MemOverlapStatus is = at::get_overlap_status(a, b);
-  if (is == at::MemOverlapStatus::Partial || is == at::MemOverlapStatus::Full) REFUSE(PyExc_ValueError, "%s shares memory with %s", name_a, name_b);
+  if (near_each_other(a, b)) REFUSE(PyExc_ValueError, "%s shares memory with %s", name_a, name_b);
 }
 
 // cache_attend(cache, layer, q, mask, counts, slots, scale, out, window, sinks, places, lse) -> out
@@ -512,8 +522,16 @@ struct TokenWeights {
       return;
     }
     to = result = floats_to(c, out, "out", shape);
-    if (from.defined() && at::get_overlap_status(to, from) == at::MemOverlapStatus::Partial) REFUSE(PyExc_ValueError, "out shares part of the weights' memory");
+    if (from.defined() && near_each_other(to, from) && !same_or_beside(to, from)) REFUSE(PyExc_ValueError, "out shares part of the weights' memory");
     if (!by_rows(to)) to = at::detail::empty_cuda(shape, c10::kFloat, c.device, std::nullopt);
+  }
+  // The same numbers, or rows that lie side by side in a third tensor's.
+  static bool same_or_beside(const at::Tensor& a, const at::Tensor& b) {
+    if (!by_rows(a) || !by_rows(b) || (a.size(0) > 1 && a.stride(0) != b.stride(0))) return false;
+    const int64_t bytes = static_cast<const char*>(a.const_data_ptr()) - static_cast<const char*>(b.const_data_ptr());
+    if (bytes == 0) return true;
+    const int64_t row = a.stride(0) * 4, width = a.size(1) * 4, off = a.size(0) > 1 ? (bytes % row + row) % row : 0;
+    return off >= width && row - off >= width;
   }
   static bool by_rows(const at::Tensor& t) { return t.stride(1) == 1 && (t.size(0) == 1 || t.stride(0) >= t.size(1)); }
   const float* read() const { return from.defined() ? static_cast<const float*>(from.const_data_ptr()) : nullptr; }

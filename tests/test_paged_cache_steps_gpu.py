@@ -269,9 +269,9 @@ def test_released_pages_are_not_missed_by_the_window_that_left_them():
     before = [cache.attend(0, q, window=w, sinks=20) for w in (100, 64, 1)]
     free = (cache.refs == 0).sum().item()
     cache.release(100, 20)
-    o = Steps.of(cache)
     assert (cache.refs == 0).sum().item() - free == sum(max(0, (n - 99) // 8 - 3) for n in (700, 33, 512))
     cache.pool[:, :, cache.refs == 0] = float("nan")
+    o = Steps.of(cache)
     assert all(torch.equal(cache.attend(0, q, window=w, sinks=20), x) for w, x in zip((100, 64, 1), before))
     assert faults_of(cache) == 0
     out = cache.attend(0, q)                        # a call that wants them
@@ -444,6 +444,10 @@ def test_arguments_that_are_refused():
     long = torch.zeros(3, 48, device="cuda").view(-1)
     with pytest.raises(ValueError, match="part"):
         cache.evict(long[:96].view(2, 48), two, out=long[48:].view(2, 48))
+    wide = torch.zeros(2, 100, device="cuda")
+    with pytest.raises(ValueError, match="part"):
+        cache.evict(wide[:, :48], two, out=wide[:, 40:88])
+    cache.evict(wide[:, :48], two, out=wide[:, 50:98])      # (side by side)
     assert faults_of(cache) == 0 and cache.lengths.tolist() == [0, 0]
     cache.close()
     for call in (lambda: cache.release(1), lambda: cache.weigh(0, q, lse), lambda: cache.evict(weights, two)):
