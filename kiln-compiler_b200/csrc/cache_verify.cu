@@ -360,7 +360,7 @@ struct DraftOf {
     return x;
   }
 };
-constexpr int kAhead = 4;                // vectors of a lane that are under way
+constexpr int kAhead = 1;                // vectors of a lane that are under way (more are moved from register to register: 81, 82.5 and 86 us with 1, 2 and 4; 1024 threads: 100)
 
 // Of weights, without those refused.
 template <typename T>
@@ -486,7 +486,6 @@ __device__ __forceinline__ Sums sum_of(const VerifyParams& p, const RowOf<T>& ro
 template <typename T>
 __global__ void __launch_bounds__(kWalkThreads, 1) verify_walk_kernel(const __grid_constant__ VerifyParams p) {
   using Row = RowOf<T>;
-  constexpr int VEC = Row::kVec;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ double table[32], shares[4][kWalkWarps], totals[2][4][kMostCluster];      // (as in Sums)
   const cg::cluster_group cluster = cg::this_cluster();
