@@ -473,11 +473,12 @@ int kb200_cache_release(kb200_cache* cache, int window, int sinks, void* cuda_st
 
 /* The weight that the tokens of a sequence draw: out[s, j] = weights[s, j] + sum over i < counts[b] and heads h of exp(scale * q[b, i, h] . k[j, g] - lse[b, i, h]) for the tokens
  * j that token i of batch row b (s = slots[b]) sees, as in kb200_cache_attend, whose lse makes them its weights.  Rows whose lse is -inf add nothing.  All other entries of out
- * are weights'.  weights and out: float32 [sequences, max_pages * page_tokens], a row `stride` elements behind the last; weights NULL: zeros; out may be weights.
+ * are weights'.  committed: 0, the tokens are those drafted behind the committed ones, as in kb200_cache_attend; else they are the last counts[b] of the committed ones (what
+ * kb200_cache_accept has taken, in its order).  weights and out: float32 [sequences, max_pages * page_tokens], a row `stride` elements behind the last; weights NULL: zeros; out may be weights.
  * No sequence twice.  Sums are float32; every key's are taken in the same order in every call. */
 int kb200_cache_weigh(kb200_cache* cache, int layer, const kb200_rows* q, const float* lse, const int64_t* lse_stride, int rows, int tokens,
                       const uint8_t* mask, const int64_t* mask_stride, const int32_t* counts, const int32_t* slots, float scale,
-                      const float* weights, int64_t weights_stride, float* out, int64_t out_stride, void* cuda_stream);
+                      int committed, const float* weights, int64_t weights_stride, float* out, int64_t out_stride, void* cuda_stream);
 
 /* Keeps keep[s] of every sequence's committed tokens and drops the others, in all layers: the first `sinks`, of the rest the last `recent`, and of what then lacks the heaviest
  * by weights[s] (of equal ones the first; NaN is heaviest); fewer than the first and last ones where keep[s] is less.  They keep their order and become the sequence's first keep[s]

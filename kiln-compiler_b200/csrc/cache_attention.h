@@ -28,7 +28,9 @@ struct CacheAttnParams {
   const int32_t* places;                   // null: token t stands t behind the committed ones
   float* lse;                              // or null
   int64_t lse_stride[3];
+  bool committed;                          // (kOrCommitted, in the place of WINDOW) the rows are the last of the committed tokens
 };
+constexpr int kOrCommitted = 2;
 
 // Work is counted in units: a tile of keys for a tile of query rows (the drafted tokens of a sequence times the heads that share a key head), and in front of an
 // item's tiles a few for its beginning and end.  All units of a call, sequence by sequence, key head by key head, row tile by row tile, are divided into equal runs of neighbours, one
@@ -81,7 +83,7 @@ __device__ __forceinline__ int place_of(const CacheAttnParams& p, int b, int tok
 }
 __device__ __forceinline__ bool own_places(const CacheAttnParams& p) { return p.mask == nullptr && p.places == nullptr; }
 
-template <int ROWS, int TILE, bool WINDOW>
+template <int ROWS, int TILE, int WINDOW>
 __device__ __forceinline__ CacheItems cache_items(const CacheAttnParams& p, int b) {
   CacheItems r{};
   const int slot = p.slots != nullptr ? p.slots[b] : b;
@@ -92,7 +94,14 @@ __device__ __forceinline__ CacheItems cache_items(const CacheAttnParams& p, int 
     count = min(max(count, 0), p.tokens);
   }
   const int64_t room = (int64_t)min(max(p.c.held[slot], 0), p.c.max_pages) << p.c.page_log2;
-  const int length = max(p.c.lengths[slot], 0);
+  int length = max(p.c.lengths[slot], 0);
+  if constexpr (WINDOW == kOrCommitted) {
+    if (p.committed) {
+      if (count > length) cache_fault(p.c, KB200_CACHE_BAD_INDEX);
+      count = min(count, length);
+      length -= count;
+    }
+  }
   r.slot = slot;
   r.count = count;
   r.length = length;
@@ -101,7 +110,7 @@ __device__ __forceinline__ CacheItems cache_items(const CacheAttnParams& p, int 
   if (r.end < length + count) cache_fault(p.c, KB200_CACHE_NO_ROOM);
   r.row_tiles = (count * p.group + ROWS - 1) / ROWS;
   r.key_tiles = max(1, (r.end + TILE - 1) / TILE);
-  if constexpr (WINDOW) {
+  if constexpr (WINDOW == 1) {
     if (r.row_tiles > 1 && own_places(p)) {          // row tiles begin at keys of their own; all have as many tiles as any may have
       const int begin = max(0, length + count - p.window), front = (min(p.sinks, begin) + TILE - 1) / TILE;
       r.key_tiles = (int)min((int64_t)r.key_tiles, front + window_tiles<TILE>(p.window, tokens_of_tile<ROWS>(p.group)));
@@ -129,7 +138,7 @@ __device__ __forceinline__ int sure_keys(const CacheAttnParams& p, const CacheCu
   return u.it.length + (p.mask == nullptr ? u.row_tile * ROWS / p.group + 1 : 0);
 }
 // To the next item.
-template <int ROWS, int TILE, bool WINDOW>
+template <int ROWS, int TILE, int WINDOW>
 __device__ __forceinline__ void next_item(const CacheAttnParams& p, CacheCursor& u) {
   u.tile = 0;
   if (++u.row_tile < u.it.row_tiles) return;
@@ -153,7 +162,7 @@ struct CacheRun {
     if (left <= skip) return 0;
     return p.whole ? at.it.key_tiles : (int)min(left - skip, (int64_t)at.it.key_tiles - at.tile);
   }
-  template <int ROWS, int TILE, bool WINDOW = false>
+  template <int ROWS, int TILE, int WINDOW = false>
   __device__ __forceinline__ void pass(const CacheAttnParams& p, int tiles) {
     left -= p.whole ? 1 : skip + tiles;
     skip = p.item_units;
@@ -167,7 +176,7 @@ struct CacheRunShared {
 };
 
 // The run of CTA `part`, by all threads of a CTA of THREADS; false: it has none.
-template <int ROWS, int TILE, int THREADS, bool WINDOW = false>
+template <int ROWS, int TILE, int THREADS, int WINDOW = false>
 __device__ __forceinline__ bool find_run(const CacheAttnParams& p, int part, CacheRunShared& shared, CacheRun* run) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool one_round = p.rows <= THREADS;

@@ -77,7 +77,7 @@ __device__ __forceinline__ void write_rest(const WeighParams& p) {
     const int s = (int)(u / pieces), from = (int)(u % pieces) * 4 * kThreads + threadIdx.x;
     int end = 0;
     if (s < p.a.rows) {
-      const CacheItems it = cache_items<1 << 24, 8, false>(p.a, s);
+      const CacheItems it = cache_items<1 << 24, 8, kOrCommitted>(p.a, s);
       end = it.count > 0 ? it.end : 0;
     }
     float x[4];
@@ -100,12 +100,12 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_kernel(const __grid_constan
   write_rest(p);
   const int lane = threadIdx.x & 31, warp = warp_index(), g = lane >> 2, t4 = lane & 3;
   CacheRun run;
-  if (!find_run<ROWS, KEYS, kThreads>(p.a, blockIdx.x, found, &run)) return;
+  if (!find_run<ROWS, KEYS, kThreads, kOrCommitted>(p.a, blockIdx.x, found, &run)) return;
   const CacheView& c = p.a.c;
   const int beside = kWarps / p.split, mine = warp / p.split, part = warp % p.split, in_page = (1 << c.page_log2) - 1;
   const float scale = p.a.scale_log2;
   int turn = 0;
-  for (int tiles; (tiles = run.tiles(p.a)) > 0; run.pass<ROWS, KEYS>(p.a, tiles)) {
+  for (int tiles; (tiles = run.tiles(p.a)) > 0; run.pass<ROWS, KEYS, kOrCommitted>(p.a, tiles)) {
     const CacheItems& it = run.at.it;
     const int b = run.at.b, rows = it.count * p.group;
     if (p.a.slots != nullptr) {                    // a sequence that an earlier row names is that row's
@@ -272,14 +272,14 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_few_kernel(const __grid_con
   const uint32_t ring = smem_u32(smem) + warp * kStages * Ring::kTileBytes, full = smem_u32(&bars[warp * kStages]);
   uint32_t asked = 0, taken = 0;                   // tiles, over all runs
   CacheRun run;
-  if (!find_run<ROWS, KEYS, kThreads>(p.a, blockIdx.x, found, &run)) return;
+  if (!find_run<ROWS, KEYS, kThreads, kOrCommitted>(p.a, blockIdx.x, found, &run)) return;
   const CacheView& c = p.a.c;
   const int beside = kWarps / p.split, mine = warp / p.split, part = warp % p.split, in_page = (1 << c.page_log2) - 1;
   const float scale = p.a.scale_log2;
   const int64_t head_stride = (int64_t)c.head_dim << c.page_log2;
   // Of a lane's sums, one per key, those of all lanes that have the same keys: each lane is left with one key's.
   const int my_key = GROUPS == 4 ? (lane >> 3 & 1) * 16 + (lane >> 4 & 1) * 8 + 2 * t4 + (lane >> 2 & 1) : GROUPS == 2 ? (lane >> 3 & 1) * 8 + 2 * t4 + (lane >> 2 & 1) : 2 * t4 + (lane >> 2 & 1);
-  for (int tiles; (tiles = run.tiles(p.a)) > 0; run.pass<ROWS, KEYS>(p.a, tiles)) {
+  for (int tiles; (tiles = run.tiles(p.a)) > 0; run.pass<ROWS, KEYS, kOrCommitted>(p.a, tiles)) {
     const CacheItems& it = run.at.it;
     const int b = run.at.b, rows = it.count * p.group;
     if (p.a.slots != nullptr) {                    // a sequence that an earlier row names is that row's
@@ -472,7 +472,7 @@ int cache_weigh_prepare(const Cache& c) {
 using namespace kb200;
 
 KB200_EXPORT int kb200_cache_weigh(kb200_cache* handle, int layer, const kb200_rows* q, const float* lse, const int64_t* lse_stride, int rows, int tokens,
-                                   const uint8_t* mask, const int64_t* mask_stride, const int32_t* counts, const int32_t* slots, float scale, const float* weights,
+                                   const uint8_t* mask, const int64_t* mask_stride, const int32_t* counts, const int32_t* slots, float scale, int committed, const float* weights,
                                    int64_t weights_stride, float* out, int64_t out_stride, void* stream) {
   KB200_CACHE_ENTER("kb200_cache_weigh");
   if (layer < 0 || layer >= c.view.layers) return fail(KB200_ERR_ARGUMENT, "kb200_cache_weigh: layer %d of %d", layer, c.view.layers);
@@ -508,6 +508,7 @@ KB200_EXPORT int kb200_cache_weigh(kb200_cache* handle, int layer, const kb200_r
   p.a.counts = counts;
   p.a.slots = slots;
   p.a.layer = layer;
+  p.a.committed = committed != 0;
   p.a.rows = rows;
   p.a.tokens = tokens;
   p.a.heads = q->heads;

@@ -552,10 +552,10 @@ struct TokenWeights {
   }
 };
 
-// cache_weigh(cache, layer, q, lse, weights, mask, counts, slots, scale, out) -> out
+// cache_weigh(cache, layer, q, lse, weights, mask, counts, slots, scale, committed, out) -> out
 PyObject* cache_weigh(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (!n_args(n, 10)) return nullptr;
+  if (!n_args(n, 11)) return nullptr;
   try {
     CacheCaller& c = cache_of(args[0]);
     const c10::cuda::CUDAGuard guard(c.device);
@@ -571,19 +571,21 @@ PyObject* cache_weigh(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor mask = mask_of(c, args[5], rows, tokens, mask_stride);
     const at::Tensor counts = integers_or_none(c, args[6], "counts", rows), slots = integers_or_none(c, args[7], "slots", rows);
     const double scale = scale_of(c, args[8]);
-    TokenWeights w(c, args[4], args[9]);
+    const int committed = PyObject_IsTrue(args[9]);
+    if (committed < 0) return nullptr;
+    TokenWeights w(c, args[4], args[10]);
     apart(w.to, q.t, "out", "q");
     apart(w.to, lse, "out", "lse");
     const int64_t lse_stride[3] = {lse.stride(0), lse.stride(1), lse.stride(2)};
     float* const to = w.write();
     PyObject* const done = enqueue(c, [&](cudaStream_t s) {
       return kb200_cache_weigh(c.cache, layer, &q.rows, static_cast<const float*>(lse.const_data_ptr()), lse_stride, (int)rows, (int)tokens,
-                               mask.defined() ? static_cast<const uint8_t*>(mask.const_data_ptr()) : nullptr, mask_stride, at_of(counts), at_of(slots), (float)scale, w.read(),
+                               mask.defined() ? static_cast<const uint8_t*>(mask.const_data_ptr()) : nullptr, mask_stride, at_of(counts), at_of(slots), (float)scale, committed, w.read(),
                                w.read_stride(), to, w.to.stride(0), s);
     });
     if (done == nullptr) return nullptr;
     Py_DECREF(done);
-    return w.done(args[9]);
+    return w.done(args[10]);
   } catch (const Refused&) {
     return nullptr;
   }
@@ -701,7 +703,7 @@ PyMethodDef methods[] = {
     {"cache_accept", fast(cache_accept), METH_FASTCALL, "cache_accept(cache, counts, kept)"},
     {"cache_attend", fast(cache_attend), METH_FASTCALL, "cache_attend(cache, layer, q, mask, counts, slots, scale, out, window, sinks, places, lse) -> out"},
     {"cache_release", fast(cache_release), METH_FASTCALL, "cache_release(cache, window, sinks)"},
-    {"cache_weigh", fast(cache_weigh), METH_FASTCALL, "cache_weigh(cache, layer, q, lse, weights, mask, counts, slots, scale, out) -> out"},
+    {"cache_weigh", fast(cache_weigh), METH_FASTCALL, "cache_weigh(cache, layer, q, lse, weights, mask, counts, slots, scale, committed, out) -> out"},
     {"cache_evict", fast(cache_evict), METH_FASTCALL, "cache_evict(cache, weights, keep, recent, sinks, out) -> out"},
     {"cache_verify", fast(cache_verify), METH_FASTCALL,
      "cache_verify(cache, logits, tokens, uniform, draft, parents, counts, slots, temperature) -> (n_accepted, accepted, following)"},

@@ -122,8 +122,8 @@ EXPORTS = {
                                             C.POINTER(C.c_int64), C.c_void_p, C.c_uint64, C.c_void_p]),
     "kb200_cache_release": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
     "kb200_cache_weigh": (C.c_int, [C.c_void_p, C.c_int, C.POINTER(Rows), C.c_void_p, C.POINTER(C.c_int64), C.c_int, C.c_int, C.c_void_p,
-                                    C.POINTER(C.c_int64), C.c_void_p, C.c_void_p, C.c_float, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
-                                    C.c_void_p]),
+                                    C.POINTER(C.c_int64), C.c_void_p, C.c_void_p, C.c_float, C.c_int, C.c_void_p, C.c_int64, C.c_void_p,
+                                    C.c_int64, C.c_void_p]),
     "kb200_cache_evict_workspace": (C.c_uint64, [C.c_void_p]),
     "kb200_cache_evict": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_int64, C.c_void_p,
                                     C.c_uint64, C.c_void_p]),

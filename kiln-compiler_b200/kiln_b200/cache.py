@@ -138,11 +138,12 @@ class PagedCache:
         The sequences keep their lengths; ``attend`` with that window (or a smaller one) goes on as before."""
         self._call.cache_release(self._caller, window, sinks)
 
-    def weigh(self, layer, q, lse, weights=None, mask=None, counts=None, slots=None, scale=None, out=None):
+    def weigh(self, layer, q, lse, weights=None, mask=None, counts=None, slots=None, scale=None, committed=False, out=None):
         """Adds up what weight the tokens of the sequences draw: ``weights`` [sequences, max_pages * page_tokens] (float32; default: zeros) plus the sum over heads and over the first
         ``counts[b]`` rows of ``q`` of the weights that ``attend`` (without a window) gave them, whose ``lse`` this takes.  Returns ``out``, which may be ``weights``.
-        To be called before ``accept``, of tokens that are going to be accepted where they stand.  ``slots`` names no sequence twice."""
-        return self._call.cache_weigh(self._caller, layer, q, lse, weights, mask, counts, slots, scale, out)
+        The rows are the tokens drafted behind the committed ones, or, ``committed``, the last of those: what a call of ``accept`` has taken, in its order (of a
+        tree that was drafted, the rows of ``q`` and ``lse`` that ``accepted`` names).  ``slots`` names no sequence twice."""
+        return self._call.cache_weigh(self._caller, layer, q, lse, weights, mask, counts, slots, scale, committed, out)
 
     def evict(self, weights, keep, recent=0, sinks=0, out=None):
         """Keeps ``keep[s]`` committed tokens of every sequence, in all layers: the first ``sinks``, the last ``recent`` and, of the others, the heaviest (of equal ones the

@@ -360,6 +360,20 @@ def test_weights_of_rows_that_name_their_sequences(dtype):
                        cache.weigh(0, q.to(dtype), lse, start, counts=ints([3, 1, 2])))
 
 
+@pytest.mark.parametrize("dtype, tokens", [(BF16, 3), (F32, 3), (F16, 20)])
+def test_weights_of_committed_tokens(dtype, tokens):
+    """As of the same tokens before they were accepted."""
+    cache, q = filled([100, 5, 0], [tokens] * 3, dtype=dtype, kv_heads=2, group=2, head_dim=64)
+    lse, counts = torch.empty(3, tokens, 4, device="cuda"), ints([tokens, 1, tokens - 1])
+    cache.attend(0, q, counts=counts, lse=lse)
+    want = cache.weigh(0, q, lse, counts=counts)
+    cache.accept(counts)
+    assert torch.equal(cache.weigh(0, q, lse, counts=counts, committed=True), want) and faults_of(cache) == 0
+    cache.truncate(ints([-1, 2, 0]))
+    got = cache.weigh(0, q, lse, counts=ints([tokens, 3, 1]), committed=True)              # more tokens than there are
+    assert faults_of(cache) == BAD_INDEX and torch.equal(got[0], want[0]) and got[2].count_nonzero() == 0 and got[1, 2:].count_nonzero() == 0
+
+
 @pytest.mark.parametrize("dtype, head_dim", [(BF16, 64), (F32, 64), (F16, 128), (F32, 256), (BF16, 256)])
 def test_weights_beside_rows_and_keys_that_are_no_numbers(dtype, head_dim):
     cache, q = filled([100], [4], dtype=dtype, kv_heads=2, group=2, head_dim=head_dim)
@@ -480,7 +494,7 @@ def test_c_entries_refuse():
         assert evict(*[value if j == i else x for j, x in enumerate(at)], space.data_ptr(), size) == -1
     assert evict(*at, space.data_ptr(), size - 1) == evict(*at, None, size) == evict(*at, space.data_ptr() + 8, size) == -1
     weigh = lambda q_=rows, lse_=lse.data_ptr(), strides=stride, to_=weights.data_ptr(), layer=0, scale=0.125: lib.kb200_cache_weigh(  # noqa: E731
-        handle, layer, C.byref(q_), lse_, strides, 1, 2, None, None, None, None, scale, None, 0, to_, width, None)
+        handle, layer, C.byref(q_), lse_, strides, 1, 2, None, None, None, None, scale, 0, None, 0, to_, width, None)
     assert weigh() == 0 and weigh(lse_=None) == weigh(strides=None) == weigh(to_=None) == weigh(layer=1) == weigh(scale=-1.0) == -1
     assert weigh(_cabi.Rows(q.data_ptr(), 1, 3, q.stride()[:3])) == weigh(_cabi.Rows(q.data_ptr() + 2, 1, 2, q.stride()[:3])) == weigh(_cabi.Rows(q.data_ptr(), 1, 2, (256, 128, 4))) == -1
     assert lib.kb200_cache_release(handle, 0, 0, None) == lib.kb200_cache_release(handle, 1, -1, None) == -1
