@@ -224,7 +224,30 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
     auto meet_group = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(kRows) : "memory"); };
     auto meet_both = [&]() { asm volatile("bar.sync 3, %0;" ::"n"(2 * kRows) : "memory"); };
     uint32_t t0 = 0;                                 // the item's first tile
-    for (int tiles; any && (tiles = run.tiles(p)) > 0; run.pass<kRows, TILE, WINDOW>(p, tiles)) {
+    // With a window: an item's query rows, four to a load of a warp, asked for in front of the last one's end.  (A row to a lane is 32 lines to a load: 4700 cycles of an item's 14000
+    // beside its tiles; asked for at its beginning still 3500.)
+    constexpr int kLanes = DP / 16;                  // of a row's half
+    uint4 ahead[kLanes];
+    auto ask_for_query = [&](const CacheCursor& at) {
+      const int n = min(kRows, at.it.count * p.group - at.row_tile * kRows);
+      const CacheRow mine = row_of<kRows>(p, at, row < n ? row : 0);
+      const int64_t my_row = at.b * p.q_stride[0] + mine.token * p.q_stride[1] + mine.head * p.q_stride[2];
+      const int chunk = group * kLanes + lane % kLanes;
+#pragma unroll
+      for (int i = 0; i < kLanes; ++i) {
+        const int of = i * (32 / kLanes) + lane / kLanes;
+        const int64_t from = __shfl_sync(0xffffffffu, my_row, of);
+        ahead[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (quad * 32 + of < n && chunk * 8 < p.c.head_dim) ahead[i] = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + from)[chunk];
+      }
+    };
+    CacheRun after = run;
+    if (WINDOW && any && !p.q_fp32 && run.tiles(p) > 0) ask_for_query(now);
+    auto pass = [&](int tiles) {
+      if constexpr (WINDOW) run = after;
+      else run.pass<kRows, TILE, WINDOW>(p, tiles);
+    };
+    for (int tiles; any && (tiles = run.tiles(p)) > 0; pass(tiles)) {
       const int rows_here = min(kRows, now.it.count * p.group - now.row_tile * kRows), sure = min(WINDOW ? sure_keys<kRows>(p, now) : now.it.length, now.it.end);
       const bool there = row < rows_here, warp_there = quad * 32 < rows_here;
       CacheGap gap{0, 0};
@@ -251,23 +274,13 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
         }
       }
       // half a row of Q (the products that read the last item's have been executed: its output was read); zeros for rows that are not there
-      if (WINDOW && !p.q_fp32 && warp_there) {
-        // Four rows to a load of the warp.  (A row to a lane is 32 lines to a load: 4700 cycles of an item's 14000 beside its tiles.)
-        const int64_t mine = now.b * p.q_stride[0] + r.token * p.q_stride[1] + r.head * p.q_stride[2];
-        uint4 x[DP / 16];
-        constexpr int LANES = DP / 16, ROWS = 32 / LANES;              // of a row's half; rows at once
-        const int at = group * LANES + lane % LANES;
+      if (WINDOW && !p.q_fp32) {
+        if (warp_there) {
 #pragma unroll
-        for (int i = 0; i < LANES; ++i) {
-          const int of = i * ROWS + lane / LANES;
-          const int64_t from = __shfl_sync(0xffffffffu, mine, of);
-          x[i] = make_uint4(0u, 0u, 0u, 0u);
-          if (quad * 32 + of < rows_here && at * 8 < p.c.head_dim) x[i] = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + from)[at];
-        }
-#pragma unroll
-        for (int i = 0; i < LANES; ++i) {
-          const int of = quad * 32 + i * ROWS + lane / LANES;
-          *reinterpret_cast<uint4*>(smem + at / 8 * Z::kQBlock + of * 128 + (((at % 8) ^ (of & 7)) << 4)) = x[i];
+          for (int i = 0; i < kLanes; ++i) {
+            const int of = quad * 32 + i * (32 / kLanes) + lane / kLanes, at = group * kLanes + lane % kLanes;
+            *reinterpret_cast<uint4*>(smem + at / 8 * Z::kQBlock + of * 128 + (((at % 8) ^ (of & 7)) << 4)) = ahead[i];
+          }
         }
       } else if (warp_there) {
         const int64_t from = now.b * p.q_stride[0] + r.token * p.q_stride[1] + r.head * p.q_stride[2];
@@ -327,11 +340,22 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
           const int from = (hides ? 0 : max(0, sure - key0)) * kChunks, to = min(TILE, ((now.it.end + in_page) & ~in_page) - key0) * kChunks;
           uint32_t found = 0u;
           if (wait(full + 8 * stage, (t / Z::kStages) & 1)) {
-#pragma unroll 4
-            for (int c = from + worker; c < to; c += kRows) {
-              uint4* const x = reinterpret_cast<uint4*>(G::at(values, c / kChunks, c % kChunks * 8));
-              if (c / kChunks >= last) *x = make_uint4(0u, 0u, 0u, 0u);
-              else found |= not_finite<T>(x->x) | not_finite<T>(x->y) | not_finite<T>(x->z) | not_finite<T>(x->w);
+            if (last >= TILE) {                      // (no stores between the loads)
+              uint4 x[TILE * kChunks / kRows];
+#pragma unroll
+              for (int i = 0; i < TILE * kChunks / kRows; ++i) {
+                const int c = i * kRows + worker;
+                x[i] = *reinterpret_cast<const uint4*>(G::at(values, c / kChunks, c % kChunks * 8));
+              }
+#pragma unroll
+              for (int i = 0; i < TILE * kChunks / kRows; ++i)
+                if (i * kRows + worker >= from) found |= not_finite<T>(x[i].x) | not_finite<T>(x[i].y) | not_finite<T>(x[i].z) | not_finite<T>(x[i].w);
+            } else {
+              for (int c = from + worker; c < to; c += kRows) {
+                uint4* const x = reinterpret_cast<uint4*>(G::at(values, c / kChunks, c % kChunks * 8));
+                if (c / kChunks >= last) *x = make_uint4(0u, 0u, 0u, 0u);
+                else found |= not_finite<T>(x->x) | not_finite<T>(x->y) | not_finite<T>(x->z) | not_finite<T>(x->w);
+              }
             }
           }
           if (to > last * kChunks) fence_async_smem();
@@ -453,6 +477,11 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
         }
       }
       // ---- the end of the item, or of the run inside it: both groups' rows, half of the columns each ----
+      if constexpr (WINDOW) {
+        after = run;
+        after.pass<kRows, TILE, WINDOW>(p, tiles);
+        if (!p.q_fp32 && after.tiles(p) > 0) ask_for_query(after.at);
+      }
       bool ok = true;
       if (done != 0) ok = wait(o_full + 8 * group, ((done - 1) >> 1) & 1);
       if (l != l) m = 0.0f;                          // (NaN, which a maximum passes over, reaches the result)
@@ -477,17 +506,21 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
         if constexpr (WINDOW) {
           if (whole && there && group == 0) write_lse(p, now.b, r, TcMath<T, DP>::log_sum(top, sum, p.scale_log2));
         }
-        if (WINDOW && whole) {                       // 64 bytes of a row at a time (16: 4800 cycles)
+        if (WINDOW && whole) {                       // 32 bytes of a row at a time
 #pragma unroll 1
-          for (int c = group * (DP / 2); c < (group + 1) * (DP / 2); c += 32) {
-            float o[32], o2[32];
-            tmem_ld32x2(lane_addr + c, lane_addr + DP + c, o, o2);
+          for (int c = group * (DP / 2); c < (group + 1) * (DP / 2); c += 16) {
+            float o[16];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = (first ? o[j] * fa : 0.0f) + (second ? o2[j] * fb : 0.0f);
+            for (int h = 0; h < 16; h += 8) {
+              float a[8], b[8];
+              tmem_ld8x2(lane_addr + c + h, lane_addr + DP + c + h, a, b);
 #pragma unroll
-            for (int j = 0; j < 32; j += 8)
-              if (there && c + j < p.c.head_dim)
-                *reinterpret_cast<uint4*>(to + c + j) = make_uint4(pack<T>(o[j], o[j + 1]), pack<T>(o[j + 2], o[j + 3]), pack<T>(o[j + 4], o[j + 5]), pack<T>(o[j + 6], o[j + 7]));
+              for (int j = 0; j < 8; ++j) o[h + j] = (first ? a[j] * fa : 0.0f) + (second ? b[j] * fb : 0.0f);
+            }
+            if (there && c < p.c.head_dim) {
+              reinterpret_cast<uint4*>(to + c)[0] = make_uint4(pack<T>(o[0], o[1]), pack<T>(o[2], o[3]), pack<T>(o[4], o[5]), pack<T>(o[6], o[7]));
+              reinterpret_cast<uint4*>(to + c)[1] = make_uint4(pack<T>(o[8], o[9]), pack<T>(o[10], o[11]), pack<T>(o[12], o[13]), pack<T>(o[14], o[15]));
+            }
             __syncwarp();
           }
         } else
