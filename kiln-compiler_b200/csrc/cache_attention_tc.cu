@@ -40,11 +40,6 @@ struct TcMath {
   static __device__ __forceinline__ float log_sum(float top, float sum, float scale) { return MmaMath<T, DP>::log_sum(top, sum, scale); }
 };
 
-// With a window, output rows are rescaled only when a row's maximum has grown by this power of two.  Among the first few dozen tiles one of a warp's 32 rows nearly always has a new
-// maximum, and rescaling is an eighth of a tile's time; weights up to 2^8 of the largest so far are as exact, and float16, whose largest is 2^12, has three more powers.
-template <typename T>
-constexpr float kSlack = std::is_same<T, __half>::value ? 3.0f : 8.0f;
-
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
@@ -426,7 +421,7 @@ cache_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_
           const float mx = exponent_of_top<T>(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), p.scale_log2);
           if (done == 0) {
             m = mx;
-          } else if (__any_sync(0xffffffffu, mx > (WINDOW && fabsf(m) <= kFarScore ? m + kSlack<T> : m))) {
+          } else if (__any_sync(0xffffffffu, mx > m)) {
             const float grown = fmaxf(m, mx), alpha = grown == -CUDART_INF_F ? 1.0f : ex2(m - grown);
             m = grown;
             l *= alpha;
