@@ -710,7 +710,7 @@ KB200_EXPORT int kb200_cache_create(const kb200_cache_desc* d, int device, kb200
                       page_log2_of(d->page_tokens), d->head_dim, d->head_dim * c->element / 16};
   int prepared = cache_attention_prepare(*c);
   if (prepared == KB200_OK) prepared = cache_weigh_prepare(*c);
-  if (prepared == KB200_OK) prepared = cache_verify_prepare();
+  if (prepared == KB200_OK) prepared = cache_verify_prepare(*c);
   if (prepared != KB200_OK) {
     cudaFree(c->scratch);
     delete c;

@@ -26,6 +26,7 @@ struct Cache {
   int device = 0;
   int sm_count = 148;
   int element = 2;         // bytes
+  int verify_cluster = 8;  // CTAs of the largest cluster (cache_verify.cu)
   int64_t planes() const { return (int64_t)view.layers * 2 * view.kv_heads; }      // of a page
   // scratch of the operations that change the cache, one allocation
   void* scratch = nullptr;
@@ -43,7 +44,7 @@ inline bool cache_attention_call_ok(const Cache& c, int rows, int tokens, int he
   return rows >= 0 && tokens >= 0 && heads >= 1 && heads % c.view.kv_heads == 0 && (int64_t)tokens * (heads / c.view.kv_heads) < (1 << 24) &&
          (int64_t)rows * (tokens > 1 ? tokens : 1) <= (1 << 30) && (int64_t)heads * c.view.row_chunks <= (1 << 30);
 }
-int cache_verify_prepare();                  // (cache_verify.cu) the kernels' limits, on the current device
+int cache_verify_prepare(Cache& c);          // (cache_verify.cu) the kernels' limits, on the current device
 int cache_weigh_prepare(const Cache& c);     // (cache_weigh.cu) the same
 int cache_attention_prepare(Cache& c);       // (cache_attention.cu) the pool's map and the kernels' limits, on the current device
 

@@ -756,7 +756,7 @@ int chunks_of(const Cache& c, int rows, int tokens, int vocab) {
   return (int)std::min<int64_t>(std::min<int64_t>(wanted, 64), std::max(1, vocab / 2048));      // (64: two to a lane)
 }
 int cluster_of(const Cache& c, int rows) {
-  int n = kMostCluster;
+  int n = c.verify_cluster;
   while (n > 1 && (int64_t)rows * n > c.sm_count) n /= 2;
   return n;
 }
@@ -783,9 +783,26 @@ cudaError_t launch_verify(const Cache& c, const VerifyParams& p, cudaStream_t s)
   return cudaLaunchKernelEx(&cfg, verify_walk_kernel<T>, p);
 }
 
+// The largest cluster, of up to kMostCluster CTAs, that the device takes.
 template <typename T>
-cudaError_t allow_clusters() {
-  return cudaFuncSetAttribute(verify_walk_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+cudaError_t most_of_cluster(int* most) {
+  cudaError_t e = cudaFuncSetAttribute(verify_walk_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  for (; e == cudaSuccess && *most > 8; *most /= 2) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(*most);
+    cfg.blockDim = dim3(kWalkThreads);
+    cfg.dynamicSmemBytes = (size_t)kMostTokens * kDraftedBytes;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = *most;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int fit = 0;
+    if (cudaOccupancyMaxActiveClusters(&fit, verify_walk_kernel<T>, &cfg) == cudaSuccess && fit > 0) break;
+    cudaGetLastError();
+  }
+  return e;
 }
 bool verify_ok(const Cache& c, int rows, int tokens, int vocab) {
   return rows >= 0 && rows <= (1 << 20) && tokens >= 0 && tokens <= kMostTokens && vocab >= 1 && vocab < (1 << 30);
@@ -793,10 +810,11 @@ bool verify_ok(const Cache& c, int rows, int tokens, int vocab) {
 
 }  // namespace
 
-int cache_verify_prepare() {
-  KB200_CUDA(allow_clusters<float>());
-  KB200_CUDA(allow_clusters<__nv_bfloat16>());
-  KB200_CUDA(allow_clusters<__half>());
+int cache_verify_prepare(Cache& c) {
+  c.verify_cluster = kMostCluster;
+  KB200_CUDA(most_of_cluster<float>(&c.verify_cluster));
+  KB200_CUDA(most_of_cluster<__nv_bfloat16>(&c.verify_cluster));
+  KB200_CUDA(most_of_cluster<__half>(&c.verify_cluster));
   return KB200_OK;
 }
 

@@ -1,9 +1,9 @@
 // What weight the tokens of a sequence draw (kb200_cache_weigh): for every key the sum, over query rows and heads, of exp(scale q k - lse).
 //
-// What bounds it: the bytes of K, which is read once; nothing comes back but a number per key.  A warp takes 8 to 32 keys of one head at a time straight into
-// registers, all of them under way at once, and keeps the keys' sums there over the query rows and its heads.  No ring and no shared memory are needed in front of
-// the products: a key's 16-byte chunks go to the four lanes that hold it in mma.sync's second operand, and since the order in which a dot product's elements are
-// summed is free, the query rows are read in the same order.  (Which chunks a lane has: tc, tc + 4, ... where four lanes share a key.)
+// What bounds it: the bytes of K, which is read once; nothing comes back but a number per key.  K needs no layout but its own: a key's 16-byte chunks go to the four lanes that hold it in
+// mma.sync's second operand, and since the order in which a dot product's elements are summed is free, the query rows are read in the same order.  (Which chunks a lane has: t4, t4 + 4, ...)
+// Few rows (weigh_few_kernel): a warp walks a run of keys for query rows that stay.  Many rows, and float32 (weigh_kernel): a warp takes 8 to 32 keys of a head straight into
+// registers and walks the rows.
 //
 // Every key belongs to one CTA, whose warps share out the heads and are added up in their order: no atomics, the same bits every time.
 #include <algorithm>
