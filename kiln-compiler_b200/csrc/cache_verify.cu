@@ -491,9 +491,11 @@ __global__ void __launch_bounds__(kWalkThreads, 1) verify_walk_kernel(const __gr
   const cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks(), b = blockIdx.x / ranks;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  tc::cluster_arrive_relaxed();
   if (threadIdx.x < 32) table[threadIdx.x] = exp2((double)threadIdx.x / 32.0);
   pdl_wait();
   pdl_launch_dependents();
+  tc::cluster_wait();                    // (all of the cluster's CTAs have started: what they write into each other's shared memory finds it)
   int count;
   float temperature;
   const int slot = row_slot(p, b, &count, &temperature, rank == 0);

@@ -90,6 +90,24 @@ def test_pieces_of_prompts(dtype, head_dim, group, page_tokens, window, sinks):
     look(cache, q, None, [260, 130, 1], window=window, sinks=sinks)
 
 
+@pytest.mark.parametrize("dtype, head_dim, group, tokens", [(BF16, 128, 4, 200), (F16, 64, 4, 200), (BF16, 80, 3, 200), (F16, 112, 8, 20), (BF16, 256, 1, 40), (F32, 64, 1, 70), (BF16, 64, 2, 3)])
+def test_queries_of_the_caches_type(dtype, head_dim, group, tokens):
+    """As they lie, in part of another tensor, and overwritten by their results; many sequences, so that a CTA goes from one item to the next."""
+    counts = [tokens, 1, tokens // 2, tokens - 1] * 6
+    cache, q = filled([300, 0, 77, 1000] * 6, counts, dtype=dtype, kv_heads=2, group=group, head_dim=head_dim, page_tokens=16)
+    q = q.to(dtype)
+    want, lse = look(cache, q, None, counts, window=100, sinks=5)
+    rounded = cache.attend(0, q.float(), counts=ints(counts), window=100, sinks=5)
+    assert torch.equal(rounded, want)
+    wide = torch.full((tokens, 24, 2 * group + 3, head_dim + 16), float("nan"), dtype=dtype, device="cuda")
+    part = wide.transpose(0, 1)[:, :, 2:-1, 8:-8]
+    part.copy_(q)
+    got = torch.empty_like(lse)
+    assert torch.equal(cache.attend(0, part, counts=ints(counts), window=100, sinks=5, lse=got), want) and torch.equal(got, lse)
+    assert cache.attend(0, part, counts=ints(counts), window=100, sinks=5, out=part) is part and torch.equal(part, want)
+    assert torch.isnan(wide[:, :, :2]).all() and torch.isnan(wide[..., :8]).all() and faults_of(cache) == 0
+
+
 @pytest.mark.parametrize("dtype, tokens, head_dim", [(BF16, 1, 64), (BF16, 9, 128), (F16, 40, 64), (F32, 3, 64), (F32, 20, 128), (BF16, 3, 256), (F16, 90, 128)])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 def test_what_a_window_hides_does_not_reach_a_row(dtype, tokens, head_dim, bad):
