@@ -150,7 +150,8 @@ __global__ void __launch_bounds__(kStatThreads, 4) verify_stats_kernel(const __g
         for (int j = 0; j < AT_ONCE; ++j)
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
-            if (x[j][e] > m) m = x[j][e], index = row.first(i0 + j * kStatThreads) + e;
+            const int at = row.first(i0 + j * kStatThreads) + e;
+            if (x[j][e] > m || (x[j][e] == m && at < index)) m = x[j][e], index = at;      // (a row's first vector comes last)
             if (x[j][e] != x[j][e]) s = CUDART_NAN;
           }
         return;

@@ -84,6 +84,24 @@ def test_tokens_that_follow_the_same_one():
     assert any(x == 1 and v != 2 for x, v in zip(n, following))
 
 
+@pytest.mark.parametrize("dtype, vocab", [(F32, 5), (BF16, 4001), (F16, 50257), (F32, 131072), (BF16, 131072)])
+def test_equal_logits_at_temperature_zero(dtype, vocab):
+    """The first of the largest ones counts, wherever they lie: all equal, a few values only, and two of them anywhere."""
+    rows = 12
+    cache = cache_of(rows)
+    given = drafts(rows, 4, vocab, dtype, None, 4)
+    x = given["logits"]
+    x[:4] = 1.5
+    x[4:8] = (x[4:8] / 4).round()
+    dice = random.Random(vocab)
+    for b in range(8, rows):
+        for i in range(4):
+            x[b, i, [0, dice.randrange(vocab)] if i < 2 else [dice.randrange(vocab), vocab - 1 - dice.randrange(min(vocab, 9))]] = 60.0
+    given["tokens"] = torch.zeros_like(given["tokens"])
+    n, _, following = check(cache, temperature=torch.zeros(rows, device="cuda"), **given)
+    assert n[:4] == [4] * 4 and following[:4] == [0] * 4
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_numbers_next_to_a_border(dtype):
     """Random numbers one step of float32 to either side of a token's chance and of the border between two tokens that may follow: float32's sums cannot tell them."""
