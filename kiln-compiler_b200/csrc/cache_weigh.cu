@@ -323,15 +323,15 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_few_kernel(const __grid_con
       for (int head = part; head < p.kv_heads; head += p.split) {
         uint4 q[2][CHUNKS];
         float shift[2];
+        bool adds[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int of = head * p.group + in_group[h];
           const float lse = g + 8 * h < rows ? p.lse[b * p.lse_stride[0] + token[h] * p.lse_stride[1] + of * p.lse_stride[2]] : -CUDART_INF_F;
-          // (no row, or one that sees nothing: 2^-inf)
-          load_row<T, DP>(p, b, token[h], of, lse != -CUDART_INF_F, t4, q[h]);
-          shift[h] = lse == -CUDART_INF_F ? -CUDART_INF_F : lse * -1.4426950408889634f;
+          adds[h] = lse != -CUDART_INF_F;          // (a row, and one that sees something)
+          load_row<T, DP>(p, b, token[h], of, adds[h], t4, q[h]);
+          shift[h] = lse * -1.4426950408889634f;
         }
-        const bool any = __any_sync(0xffffffffu, shift[0] != -CUDART_INF_F || shift[1] != -CUDART_INF_F) != 0;
         const T* const base = static_cast<const T*>(c.pool) + head * head_stride;
         const uint32_t row_bytes = c.row_chunks * 16;
         auto ask = [&](int tile) {                 // by a lane for each eight keys
@@ -372,21 +372,23 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_few_kernel(const __grid_con
             }
           }
           __syncwarp();                            // (the tile has been read; its stage is the next one's)
+          // What a row does not add is left out behind the exponential: a key with an infinity makes NaN even of a row of zeros, and a row's lse may be NaN.
           const int key0 = (run.at.tile + tile) * KEYS;
-          if (key0 + KEYS > it.length) {           // drafted tokens, or what is behind them
+          float sum[2 * GROUPS];
+          auto add = [&](auto&& sees) {
 #pragma unroll
             for (int i = 0; i < GROUPS; ++i)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int key = key0 + 8 * i + 2 * t4 + (e & 1);
-                if (!(key < it.end && g + 8 * (e >> 1) < rows && (key < it.length || sees_key(p, b, token[e >> 1], key - it.length)))) s[i][e] = -CUDART_INF_F;
+              for (int e = 0; e < 2; ++e) {
+                const int key = key0 + 8 * i + 2 * t4 + e;
+                const float x = ex2(fmaf(s[i][e], scale, shift[0])), y = ex2(fmaf(s[i][2 + e], scale, shift[1]));
+                sum[2 * i + e] = (adds[0] && sees(0, key) ? x : 0.0f) + (adds[1] && sees(1, key) ? y : 0.0f);
               }
-          }
-          float sum[2 * GROUPS];
-#pragma unroll
-          for (int i = 0; i < GROUPS; ++i)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) sum[2 * i + e] = ex2(fmaf(s[i][e], scale, shift[0])) + ex2(fmaf(s[i][2 + e], scale, shift[1]));
+          };
+          if (key0 + KEYS <= it.length)
+            add([](int, int) { return true; });
+          else                                     // drafted tokens, or what is behind them
+            add([&](int h, int key) { return key < it.end && (key < it.length || sees_key(p, b, token[h], key - it.length)); });
           // over the lanes with other rows: as many sums as there are halve at every step
 #pragma unroll
           for (int d = 4, m = GROUPS; d < 32; d *= 2, m /= 2) {
@@ -405,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_few_kernel(const __grid_con
           }
           if (GROUPS == 4 || (lane & (GROUPS == 2 ? 16 : 24)) == 0) {
             float* const to = &sums[warp * kRunKeys + (tile - first) * KEYS + my_key];
-            *to = (head == part ? 0.0f : *to) + (any ? sum[0] : 0.0f);
+            *to = (head == part ? 0.0f : *to) + sum[0];
           }
         }
       }

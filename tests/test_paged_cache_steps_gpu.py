@@ -409,6 +409,37 @@ def test_weights_beside_rows_and_keys_that_are_no_numbers(dtype, head_dim):
     assert faults_of(cache) == 0
 
 
+@pytest.mark.parametrize("dtype, head_dim, tokens, group", [(BF16, 64, 1, 1), (F16, 128, 3, 2), (BF16, 256, 4, 2), (F16, 80, 16, 1), (BF16, 128, 17, 1), (F32, 64, 1, 1), (F32, 128, 5, 3)])
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf")])
+def test_weights_of_a_key_that_holds_an_infinity(dtype, head_dim, tokens, group, bad):
+    """Which leaves real rows a score of -inf, a weight of 0 exactly, as a score of -10000 does; beside rows that are not there, and one that saw nothing."""
+    cache, q = filled([100, 30], [tokens, 1], dtype=dtype, kv_heads=2, group=group, head_dim=head_dim)
+    page, counts = cache.table[0, 2].long(), ints([tokens, 1])
+    size = 20000.0 * head_dim**0.5
+    q[0, :, :group, 3] = -1.0 if bad > 0 else 1.0
+    got = []
+    for value in (bad, size if bad > 0 else -size):
+        cache.pool[0, 0, page, 0, 5, 3] = value                            # (key 37, of one of the two key heads)
+        lse = torch.empty(2, tokens, 2 * group, device="cuda")
+        assert torch.isfinite(cache.attend(0, q, counts=counts, lse=lse)).all() and torch.isfinite(lse[0]).all()
+        got.append(cache.weigh(0, q, lse, counts=counts))
+        lse[0, 0], lse[1, 0, 0] = -float("inf"), -float("inf")
+        got.append(cache.weigh(0, q, lse, counts=counts))
+    assert torch.equal(got[0], got[2]) and torch.equal(got[1], got[3])
+    assert torch.isfinite(torch.stack(got)).all() and faults_of(cache) == 0
+
+
+@pytest.mark.parametrize("dtype, tokens", [(BF16, 3), (F16, 16), (BF16, 20), (F32, 3)])
+def test_a_row_whose_lse_is_no_number_reaches_only_what_it_sees(dtype, tokens):
+    cache, q = filled([90], [tokens], dtype=dtype, kv_heads=2, head_dim=64)
+    lse = torch.empty(1, tokens, 2, device="cuda")
+    cache.attend(0, q, lse=lse)
+    rest = lse.clone()
+    lse[0, 1], rest[0, 1] = float("nan"), -float("inf")
+    got, want = cache.weigh(0, q, lse), cache.weigh(0, q, rest)
+    assert torch.isnan(got[0, :92]).all() and torch.equal(got[0, 92:], want[0, 92:]) and faults_of(cache) == 0
+
+
 def test_no_rows_and_no_tokens():
     cache, q = filled([30, 20], [2, 2], dtype=BF16, kv_heads=1, head_dim=64)
     start = torch.rand(2, cache.max_pages * 16, device="cuda")
