@@ -475,7 +475,7 @@ int kb200_cache_release(kb200_cache* cache, int window, int sinks, void* cuda_st
  * j that token i of batch row b (s = slots[b]) sees, as in kb200_cache_attend, whose lse makes them its weights.  Rows whose lse is -inf add nothing.  All other entries of out
  * are weights'.  committed: 0, the tokens are those drafted behind the committed ones, as in kb200_cache_attend; else they are the last counts[b] of the committed ones (what
  * kb200_cache_accept has taken, in its order).  weights and out: float32 [sequences, max_pages * page_tokens], a row `stride` elements behind the last; weights NULL: zeros; out may be weights.
- * No sequence twice.  Sums are float32; every key's are taken in the same order in every call. */
+ * No sequence twice.  Tokens whose page is missing (kb200_cache_release) draw nothing and are told KB200_CACHE_BAD_INDEX.  Sums are float32; every key's are taken in the same order in every call. */
 int kb200_cache_weigh(kb200_cache* cache, int layer, const kb200_rows* q, const float* lse, const int64_t* lse_stride, int rows, int tokens,
                       const uint8_t* mask, const int64_t* mask_stride, const int32_t* counts, const int32_t* slots, float scale,
                       int committed, const float* weights, int64_t weights_stride, float* out, int64_t out_stride, void* cuda_stream);

@@ -95,6 +95,7 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_kernel(const __grid_constan
   constexpr int KEYS = W::kKeys, GROUPS = W::kGroups, CHUNKS = W::kChunks, ROWS = 1 << 24;
   __shared__ CacheRunShared found;
   __shared__ float sums[2][kWarps][KEYS];
+  __shared__ bool gone[2][kWarps][GROUPS];         // of a tile's groups of eight keys, which no page's border cuts: their page is missing
   pdl_wait();
   pdl_launch_dependents();
   write_rest(p);
@@ -132,6 +133,7 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_kernel(const __grid_constan
             page = c.table[(int64_t)it.slot * c.max_pages + (key >> c.page_log2)];
             if (!cache_page_ok(c, page)) cache_fault(c, KB200_CACHE_BAD_INDEX), page = -1;
           }
+          if (lane == 0) gone[turn][warp][i] = page < 0;
           keys[i] = page < 0 ? nullptr : static_cast<const T*>(c.pool) + (((((int64_t)p.a.layer * 2 * c.pages + page) * p.kv_heads) << c.page_log2) + (key & in_page)) * c.head_dim;
         }
         const bool drafted = key0 + KEYS > it.length;
@@ -226,7 +228,7 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_kernel(const __grid_constan
       if (there && part == 0 && lane < KEYS && key0 + lane < it.end) {
         float x = 0.0f;
         for (int w = 0; w < p.split; ++w) x += sums[turn][warp + w][lane];
-        p.out[it.slot * p.out_stride + key0 + lane] = added_to(p, it.slot, key0 + lane) + x;
+        p.out[it.slot * p.out_stride + key0 + lane] = added_to(p, it.slot, key0 + lane) + (gone[turn][warp][lane >> 3] ? 0.0f : x);
       }
       turn ^= 1;
     }
@@ -259,6 +261,7 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_few_kernel(const __grid_con
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ CacheRunShared found;
   __shared__ __align__(8) uint64_t bars[kWarps * kStages];
+  __shared__ unsigned gone[kWarps][2];             // of a warp's run: groups of eight keys whose page is missing
   __shared__ int gave_up;
   float* const sums = reinterpret_cast<float*>(smem + kWarps * kStages * Ring::kTileBytes);      // [kWarps][kRunKeys]
   const int lane = threadIdx.x & 31, warp = warp_index(), g = lane >> 2, t4 = lane & 3;
@@ -301,19 +304,23 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_few_kernel(const __grid_con
     for (int i0 = 0; i0 < tiles; i0 += kRunTiles * beside) {
       const int n = min(tiles - i0, kRunTiles * beside), per = (n + beside - 1) / beside;
       const int first = i0 + mine * per, last = min(i0 + n, first + per);
-      // Where the run's groups of eight keys are, which no page's border cuts: one or two to a lane.  (What is behind the keys, and where a page is missing, is the last key's, or the
-      // first page's: it is not seen.)
-      constexpr int PLACES = GROUPS * kRunTiles / 32 > 1 ? GROUPS * kRunTiles / 32 : 1;
+      // Where the run's groups of eight keys are, which no page's border cuts: two to a lane.  (Behind the keys there are the last ones again, which no row sees, and where a page is
+      // missing the pool's first page, whose sums are left out.)
+      constexpr int PLACES = GROUPS * kRunTiles / 32;
+      static_assert(PLACES == 2, "a bit of `gone` to a group");
       int64_t places[PLACES];
 #pragma unroll
       for (int i = 0; i < PLACES; ++i) {
         const int key = (run.at.tile + first) * KEYS + 8 * (lane + 32 * i), there = max(min(key, (it.end - 1) & ~7), 0);
         int page = first < last ? table[there >> c.page_log2] : 0;
-        if (!cache_page_ok(c, page)) {
+        const bool missing = !cache_page_ok(c, page);
+        if (missing) {
           if (key < it.end && key < (run.at.tile + last) * KEYS) cache_fault(c, KB200_CACHE_BAD_INDEX);
           page = 0;
         }
         places[i] = (((((int64_t)p.a.layer * 2 * c.pages + page) * p.kv_heads) << c.page_log2) + (there & in_page)) * c.head_dim;
+        const unsigned lacks = __ballot_sync(0xffffffffu, missing);
+        if (lane == 0) gone[warp][i] = lacks;
       }
       // (what the first of the keys' sums are added to is asked for in front of them)
       const int key_first = (run.at.tile + i0) * KEYS + threadIdx.x;
@@ -416,8 +423,10 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_few_kernel(const __grid_con
       for (int k = threadIdx.x; k < n * KEYS; k += kThreads) {
         const int tile = k / KEYS, of = tile / per, key = (run.at.tile + i0) * KEYS + k;
         if (key >= it.end) continue;
+        const int in_run = k - of * per * KEYS;
         float x = 0.0f;
-        for (int w = 0; w < min(p.split, p.kv_heads); ++w) x += sums[(of * p.split + w) * kRunKeys + k - of * per * KEYS];
+        for (int w = 0; w < min(p.split, p.kv_heads); ++w) x += sums[(of * p.split + w) * kRunKeys + in_run];
+        if (gone[of * p.split][in_run >> 8] >> (in_run >> 3 & 31) & 1u) x = 0.0f;
         p.out[it.slot * p.out_stride + key] = (k < kThreads ? before[0] : k < 2 * kThreads ? before[1] : added_to(p, it.slot, key)) + x;
       }
       __syncthreads();

@@ -440,6 +440,25 @@ def test_a_row_whose_lse_is_no_number_reaches_only_what_it_sees(dtype, tokens):
     assert torch.isnan(got[0, :92]).all() and torch.equal(got[0, 92:], want[0, 92:]) and faults_of(cache) == 0
 
 
+@pytest.mark.parametrize("dtype, tokens, group, page_tokens", [(BF16, 1, 1, 8), (F16, 4, 4, 16), (BF16, 12, 1, 64), (BF16, 20, 2, 8), (F16, 9, 4, 32), (F32, 1, 1, 8), (F32, 6, 2, 64)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_keys_without_a_page_draw_nothing(dtype, tokens, group, page_tokens, in_place):
+    """Whatever the pool's pages hold, and as many rows as there are: what is left of the weights is what they would have been."""
+    cache, q = filled([700, 33], [tokens, 1], dtype=dtype, kv_heads=2, group=group, head_dim=64, page_tokens=page_tokens)
+    lse, counts = torch.empty(2, tokens, 2 * group, device="cuda"), ints([tokens, 1])
+    cache.attend(0, q, counts=counts, lse=lse)
+    start = torch.rand(2, cache.max_pages * page_tokens, device="cuda")
+    want = cache.weigh(0, q, lse, start, counts=counts)
+    assert faults_of(cache) == 0
+    cache.release(100, 20)
+    lost = torch.zeros_like(want, dtype=torch.bool)
+    lost[0, :cache.table.shape[1] * page_tokens] = (cache.table[0] < 0).repeat_interleave(page_tokens) & (torch.arange(want.shape[1], device="cuda") < 700)
+    assert 400 < lost.sum().item() < 600
+    got = cache.weigh(0, q, lse, start, counts=counts, out=start.clone() if in_place else None)
+    assert faults_of(cache) == BAD_INDEX
+    assert torch.equal(got, torch.where(lost, start, want))
+
+
 def test_no_rows_and_no_tokens():
     cache, q = filled([30, 20], [2, 2], dtype=BF16, kv_heads=1, head_dim=64)
     start = torch.rand(2, cache.max_pages * 16, device="cuda")
