@@ -26,8 +26,12 @@ namespace cg = cooperative_groups;
 constexpr int kStatThreads = 256, kWalkThreads = 512, kWalkWarps = kWalkThreads / 32, kMostCluster = 16;
 constexpr int kMostTokens = 512;       // of a row
 constexpr double kLog2e = 1.4426950408889634074;
-// What float32's sums may be off by, relatively: sums of 8 at a time (2^-20 at most, joined by pairs) of exponentials that are off by 2^-22 each, scaled once or twice.
-constexpr double kUnsure = 4e-6;
+// What float32's sums may be off by, relatively.  A thread sums weights 2^(scale (x - m)) for a reference m that its maximum is kSlack above at most, and follows it by a factor in
+// float64, however often.  A weight is off by 2^-22, and by ln 2 of what its exponent is: three roundings (difference, scale, product) of 2^-24 of the way from x to m and on to
+// the largest of the CTA's m.  On the average over the weights that way is 2 kSlack longer at most than the distance to the row's maximum, and that is the entropy at most, log2 of the
+// vocabulary: 1.24e-7 x (30 + 8) = 4.8e-6.  The factor from m to the largest: 2^-22.  Sums of eight, three joins and what is stored: 11 x 2^-24.  Together 6e-6.
+constexpr double kUnsure = 8e-6;
+constexpr float kSlack = 4.0f;         // log2 of a weight
 
 struct VerifyParams {
   CacheView c;
@@ -39,7 +43,7 @@ struct VerifyParams {
   const int32_t *counts, *slots;
   int rows, width, vocab, chunks;
   int draft_dtype;
-  float2* partial;         // [rows, width, chunks]: maximum and sum (temperature 0: maximum and, as bits, its index)
+  float2* partial;         // [rows, width, chunks]: what a sum is relative to, and the sum (temperature 0: the maximum and, as bits, its index)
   int32_t *accepted_n, *accepted, *following;
 };
 
@@ -138,7 +142,7 @@ __global__ void __launch_bounds__(kStatThreads, 4) verify_stats_kernel(const __g
     const float t = p.temperature != nullptr ? p.temperature[b] : 1.0f, scale = fminf((float)(kLog2e / t), 1e38f);
     const Row row(static_cast<const T*>(p.logits) + b * p.logits_stride[0] + node * p.logits_stride[1], p.vocab);
     const int vectors = row.vectors(), lo = (int)((int64_t)vectors * chunk / p.chunks), hi = (int)((int64_t)vectors * (chunk + 1) / p.chunks);
-    float m = -CUDART_INF_F;
+    float m = -CUDART_INF_F;             // what the sum's weights are relative to (temperature 0: the maximum)
     double s = 0.0;
     int index = INT_MAX;
     auto add = [&](const uint4 (&v)[AT_ONCE], int i0) {
@@ -161,6 +165,7 @@ __global__ void __launch_bounds__(kStatThreads, 4) verify_stats_kernel(const __g
       for (int j = 0; j < AT_ONCE; ++j)
 #pragma unroll
         for (int e = 0; e < VEC; e += 2) top = tc::fmax3(top, x[j][e], x[j][e + 1]);
+      if (!((top - m) * scale > kSlack)) top = m;
       const float2 behind = top == -CUDART_INF_F ? make_float2(0.0f, 0.0f) : make_float2(-top, -top), scale2 = make_float2(scale, scale);      // (nothing but -inf so far: weights of 0; NaN: NaN)
       float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
@@ -170,7 +175,7 @@ __global__ void __launch_bounds__(kStatThreads, 4) verify_stats_kernel(const __g
           const float2 y = tc::fmul2(tc::fadd2(make_float2(x[j][e], x[j][e + 1]), behind), scale2);
           sum[e >> 1 & 1] = tc::fadd2(sum[e >> 1 & 1], make_float2(exp2_fast(y.x), exp2_fast(y.y)));
         }
-      if (top > m && m > -CUDART_INF_F) s *= exp2_fast((m - top) * scale);
+      if (top > m && m > -CUDART_INF_F) s *= exp2(((double)m - (double)top) * (double)scale);
       m = top;
       s += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
     };
@@ -395,9 +400,9 @@ __device__ __noinline__ Sums sum_weights(const VerifyParams& p, const RowOf<T>& 
   }
   return Sums{x, 0.0, 0.0, 0.0};
 }
-// Of weights, and of what the draft's probabilities leave of them when the sum is only known to float32 (its reciprocal: divisors[0]).  That is off by up to d = 4e-6; what is left is
+// Of weights, and of what the draft's probabilities leave of them when the sum is only known to float32 (its reciprocal: divisors[0]).  That is off by up to d = kUnsure; what is left is
 // then sum (e / sum' - q) = left + of_left (1 / sum' - 1 / sum), but for elements where |e / sum - q| is less than d q, which may have been counted or left out wrongly: d q at most for
-// each.  Those of 2^-16 q and less (8 d) are summed; 64 in 128000 of such logits' differences are, and where they are more than kMostNear what is left is summed again with
+// each.  Those of 2^-16 q and less (1.9 d) are summed; 64 in 128000 of such logits' differences are, and where they are more than kMostNear what is left is summed again with
 // the sum that is then known.  (That always: twice the time.)
 constexpr double kMostNear = 1e-4;
 template <typename T, typename Q>

@@ -129,6 +129,27 @@ def test_numbers_next_to_a_border(dtype):
     check(cache, **given)
 
 
+@pytest.mark.parametrize("rise", [0.25, 0.5, 0.75, 1.0, 1.5, 2.5, 4.0, 7.0, 40.0])
+def test_logits_that_ascend(rise):
+    """By as much in every 4096 of four million, so that a running maximum grows a thousand times: a row's sum is still near enough to tell which random numbers are next to a token's
+    chance (from 4 x 10^-8 of it on, to either side)."""
+    vocab, rows = 1 << 22, 640
+    cache = cache_of(rows)
+    row = (torch.arange(vocab, device="cuda") // 4096).float() * (rise / 1024)
+    p = torch.softmax(row.double(), 0)
+    token = vocab - 5000
+    chance = p[token].item()
+    near = torch.tensor(chance, device="cuda").float().view(torch.int32) + (torch.arange(rows, device="cuda") - rows // 2).int()      # (a step is 2^-24 to 2^-23 of it)
+    uniform = torch.stack([torch.full((rows,), 0.37, device="cuda"), near.view(F32)], 1)
+    n, accepted, following = cache.verify(row.expand(rows, 2, vocab), ints([[0, token]] * rows), uniform)
+    taken = uniform[:, 1].double() < chance
+    assert n.tolist() == (1 + taken.int()).tolist() and {1, 2} == set(n.tolist())
+    rest = p.clone()
+    rest[token] = 0
+    first = [int(torch.searchsorted(x.cumsum(0), uniform[0, 0].double() * x.sum(), right=True)) for x in (rest, p)]
+    assert following.tolist() == [first[int(x)] for x in taken] and faults_of(cache) == 0
+
+
 def test_what_is_returned_is_distributed_as_the_models_samples():
     """The first token that a step adds, over 32768 rows each: of a chain, of several drafts of one token, with probabilities of a draft and without.  A count is off by its standard
     deviation sqrt(n p (1 - p)) five times at most (24 counts: one in 70000 would be)."""
