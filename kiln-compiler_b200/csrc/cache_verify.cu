@@ -400,11 +400,11 @@ __device__ __noinline__ Sums sum_weights(const VerifyParams& p, const RowOf<T>& 
   }
   return Sums{x, 0.0, 0.0, 0.0};
 }
-// Of weights, and of what the draft's probabilities leave of them when the sum is only known to float32 (its reciprocal: divisors[0]).  That is off by up to d = kUnsure; what is left is
-// then sum (e / sum' - q) = left + of_left (1 / sum' - 1 / sum), but for elements where |e / sum - q| is less than d q, which may have been counted or left out wrongly: d q at most for
-// each.  Those of 2^-16 q and less (1.9 d) are summed; 64 in 128000 of such logits' differences are, and where they are more than kMostNear what is left is summed again with
-// the sum that is then known.  (That always: twice the time.)
-constexpr double kMostNear = 1e-4;
+// Of weights, and of what the draft's probabilities leave of them when the sum is only known to float32 (its reciprocal: divisors[0]).  Where that turns out to be off by d, kUnsure at
+// most, what is left is sum (e / sum' - q) = left + of_left (1 / sum' - 1 / sum), but for elements where |e / sum - q| is less than d q, which may have been counted or left out wrongly: d q
+// at most for each.  Those of 2^-16 q and less are summed (near); 64 in 128000 of such logits' differences are.  Where d near is more than kMostOff of what is left, that is summed again
+// with the sum that is then known.  (That always: twice the time.)
+constexpr double kMostOff = 1e-10;
 template <typename T, typename Q>
 __device__ __noinline__ Sums sum_first(const VerifyParams& p, const RowOf<T>& row, const Left& left, int lo, int hi) {
   const DraftOf<T, Q> draft(p, left, row);
@@ -663,6 +663,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) verify_walk_kernel(const __gr
       if (lane < ranks) cluster.map_shared_rank(&totals[turn][warp][0], lane)[rank] = x;
     }
     cluster.sync();
+    double off = 0.0;
     if (first) {                         // with the sum as it is now known
       double all = 0.0;
       for (int r = 0; r < ranks; ++r) all += totals[turn][1][r];
@@ -672,6 +673,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) verify_walk_kernel(const __gr
       if (warp == 0) {
         if (lane < ranks) totals[turn][0][lane] = fmax(__fma_rn(totals[turn][2][lane], change, totals[turn][0][lane]), 0.0);
         if (lane == 0) d.divisors[0] = 1.0 / all;
+        off = fabs(change) * sum;
         sum = all, exact = true;
       }
     }
@@ -679,7 +681,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) verify_walk_kernel(const __gr
       __syncwarp();
       double all = 0.0, near = 0.0;
       for (int r = 0; r < ranks; ++r) all += totals[turn][0][r], near += first ? totals[turn][3][r] : 0.0;
-      if (near > kMostNear) {
+      if (near * off > kMostOff * all) {
         shared = false, wants = kNothing;
       } else if (wants == kExactly) {
         if (p.draft == nullptr) left = 1.0 - (1.0 - left) * (sum / all);

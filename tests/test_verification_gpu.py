@@ -150,6 +150,34 @@ def test_logits_that_ascend(rise):
     assert following.tolist() == [first[int(x)] for x in taken] and faults_of(cache) == 0
 
 
+def test_little_that_a_draft_leaves():
+    """Ten-millionths of the model's chances, and beside them a draft that is right to float32's last bit for tokens of a thousand times as much: of those what is left changes its sign with a
+    sum that is off by as little.  Random numbers next to the borders of what may follow."""
+    rows, vocab = 64, 20011
+    cache = cache_of(rows)
+    generator = torch.Generator("cuda").manual_seed(17)
+    order = torch.rand(rows, vocab, device="cuda", generator=generator).argsort(-1)
+    size = torch.ones(rows, vocab, dtype=torch.float64, device="cuda")              # most tokens: equal ones, of which a draft has too much
+    size[:, 0] = torch.linspace(0.3, 4.0, rows, device="cuda").double().exp()       # the largest, by which a row's weights are scaled
+    rand = lambda n: 0.5 + torch.rand(rows, n, device="cuda", generator=generator).double()  # noqa: E731
+    size[:, 1:801] = rand(800) * 1e-7 * vocab                                       # a draft that is nearly right: 8e-5
+    size[:, 801:841] = rand(40) * 5e-9 * vocab                                      # half of it is left: 1e-7
+    logits = torch.empty(rows, 2, vocab, device="cuda")
+    logits[:] = size.log().float().gather(1, order.argsort(-1))[:, None]
+    p = torch.softmax(logits[:, 0].double(), -1)
+    factor = torch.full((rows, vocab), 1.01, dtype=torch.float64, device="cuda")
+    factor[:, 1:801], factor[:, 801:841] = 1.0, 0.5
+    draft = (p * factor.gather(1, order.argsort(-1))).float()
+    left = (p - draft.double()).clamp_min(0)
+    assert (left.sum(-1) < 2e-7).all() and (left.sum(-1) > 5e-8).all()
+    sums, at = left.cumsum(-1), torch.arange(rows, device="cuda")
+    border = (sums / sums[:, -1:])[at, order[at, 801 + at % 40]].float().clamp_max(0.999)
+    steps = torch.tensor([-2, -1, 1, 2], dtype=torch.int32, device="cuda")[at % 4]
+    uniform = torch.stack([(border.view(torch.int32) + steps).view(F32), torch.full((rows,), 0.9999, device="cuda")], 1)
+    n, *_ = check(cache, logits=logits, tokens=order[:, [0, 5000]].int(), uniform=uniform, draft=draft[:, None].expand(rows, 2, vocab))
+    assert n == [1] * rows
+
+
 def test_what_is_returned_is_distributed_as_the_models_samples():
     """The first token that a step adds, over 32768 rows each: of a chain, of several drafts of one token, with probabilities of a draft and without.  A count is off by its standard
     deviation sqrt(n p (1 - p)) five times at most (24 counts: one in 70000 would be)."""
