@@ -426,10 +426,10 @@ __device__ __noinline__ Sums sum_first(const VerifyParams& p, const RowOf<T>& ro
 #pragma unroll
     for (int j = 0; j < RowOf<T>::kVec; ++j) {
       const Power y = power_of(__fma_rn((double)now[j], scale, shift), table);
-      const double chance = (double)q[j], r = __fma_rn(y.e, unit, -chance);
-      if ((__double2hiint(r) & 0x7fffffff) + (16 << 20) < __double2hiint(chance)) near += q[j];
-      if (y.any) x.all += y.e;
-      if (y.any && r > 0.0) x.left += r, x.of_left += y.e;
+      const double e = y.any ? y.e : 0.0, chance = (double)q[j], r = __fma_rn(e, unit, -chance);
+      if ((__double2hiint(r) & 0x7fffffff) < (int)((unsigned)__double2hiint(chance) - (16u << 20))) near += q[j];      // (16 of the exponent)
+      x.all += e;
+      if (r > 0.0) x.left += r, x.of_left += e;
     }
   }
   x.near = (double)near;

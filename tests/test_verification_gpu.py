@@ -178,6 +178,19 @@ def test_little_that_a_draft_leaves():
     assert n == [1] * rows
 
 
+@pytest.mark.parametrize("mask", [-float("inf"), -1e9, -30000.0])
+@pytest.mark.parametrize("dtype, draft_dtype, vocab, rows, trees", [(F32, F32, 20011, 9, False), (BF16, F32, 50257, 6, False), (F16, F16, 30000, 6, True), (BF16, None, 20011, 6, True)])
+def test_masked_logits(dtype, draft_dtype, vocab, rows, trees, mask):
+    """All but a few logits of every row, as a grammar or the top 50 leave them, and a draft that knows nothing of it."""
+    cache = cache_of(rows)
+    for seed, kept in enumerate((1, 50, 999)):
+        given = drafts(rows, 6, vocab, dtype, draft_dtype, 30 + seed, trees)
+        x = given["logits"]
+        least = x.topk(kept, -1).values[..., -1:]
+        x.masked_fill_(x < least, mask if dtype != F16 else max(mask, -60000.0) if mask > -float("inf") else mask)
+        check(cache, temperature=None if seed else torch.full((rows,), 0.6, device="cuda"), **given)
+
+
 def test_what_is_returned_is_distributed_as_the_models_samples():
     """The first token that a step adds, over 32768 rows each: of a chain, of several drafts of one token, with probabilities of a draft and without.  A count is off by its standard
     deviation sqrt(n p (1 - p)) five times at most (24 counts: one in 70000 would be)."""
