@@ -455,7 +455,8 @@ int kb200_cache_attend(kb200_cache* cache, int layer, const kb200_rows* q, const
                        void* workspace, uint64_t workspace_bytes, void* cuda_stream);
 
 /* kb200_cache_attend to a sliding window and a few first tokens, with the logarithms of the rows' sums.  Token i of a batch row stands `place` behind the committed
- * ones: places[b * tokens + i], or i where places is NULL (the depth in a tree, for masks of trees).  Of the committed tokens j it sees those with
+ * ones: places[b * tokens + i], or i where places is NULL (the depth in a tree, for masks of trees).  Places are from 0 to tokens - 1; one outside counts as the nearest of
+ * these, and nothing is told: a tree goes into one call, not into several by pieces.  Of the committed tokens j it sees those with
  * j < sinks or j > lengths + place - window.  Of the drafted ones it sees what `mask` shows, whatever the window is; with mask NULL those t <= i that are
  * in the window or among the first `sinks` tokens in the same way.  window: 1 or more, 0: all tokens (sinks and places then change nothing).
  * Pages of which no row sees a token may be missing from the table (kb200_cache_release).

@@ -117,7 +117,8 @@ class PagedCache:
         itself, but not share part of its memory.
 
         ``window``: a token sees itself and the ``window - 1`` tokens before it, and the sequence's first ``sinks``.  Which of the drafted tokens a mask shows
-        is the mask's matter; a token of a tree stands ``places[b, i]`` (its depth, from 0 to ``tokens - 1``; default: ``i``) behind the committed ones.
+        is the mask's matter; a token of a tree stands ``places[b, i]`` (its depth, from 0 to ``tokens - 1``; what is outside counts as the nearest of these; default: ``i``)
+        behind the committed ones.
         ``lse``: a float32 tensor [rows, tokens, heads] that gets the logarithm of each row's sum of exponentials (-inf where a row sees nothing)."""
         return self._call.cache_attend(self._caller, layer, q, mask, counts, slots, scale, out, window, sinks, places, lse)
 
