@@ -282,6 +282,33 @@ def test_sequences_that_cannot_be_evicted_stay():
     assert faults_of(cache) == 0
 
 
+def test_evictions_that_would_write_into_shared_pages_are_refused():
+    """Each fault by itself, and both together: told once, with the pages, the tables and the weights as they were."""
+    def three(keep, release=None):
+        cache, _ = filled([100, 100, 100], [1, 1, 1], dtype=F16, kv_heads=1, head_dim=16, page_tokens=8)
+        cache.fork(ints([0, 0, 2]))                 # the first two share their pages, all of which are there
+        if release is not None:
+            cache.release(*release)
+        o = Steps.of(cache)
+        weights = torch.arange(3 * cache.max_pages * 8, device="cuda").view(3, -1).float()
+        want = o.evict(weights.cpu().numpy(), keep, 0, 0)
+        got = cache.evict(weights, ints(keep))
+        told = faults_of(cache)
+        assert np.array_equal(got.cpu().numpy(), want) and told == o.faults and faults_of(cache) == 0
+        same(cache, o)
+        return told, cache.lengths.tolist(), weights, got
+
+    told, lengths, weights, got = three([50, 99, 40])
+    assert told == SHARED and lengths == [100, 100, 40]
+    assert torch.equal(got[:2, :100], weights[:2, :100]) and got[:2, 100:].count_nonzero() == 0
+    told, lengths, *_ = three([-1, -1, 50], (10, 0))                   # the third's first pages are gone, into which tokens would move
+    assert told == NO_ROOM and lengths == [100, 100, 100]
+    told, lengths, *_ = three([50, 40, -1], (10, 40))                  # the first pages are shared, and of the heaviest tokens some are gone
+    assert told == NO_ROOM | SHARED and lengths == [100, 100, 100]
+    told, lengths, *_ = three([100, -1, 0])                            # nothing moves
+    assert told == 0 and lengths == [100, 100, 0]
+
+
 def test_released_pages_are_not_missed_by_the_window_that_left_them():
     cache, q = filled([700, 33, 512], [3, 3, 3], dtype=BF16, kv_heads=2, group=2, head_dim=64, page_tokens=8)
     before = [cache.attend(0, q, window=w, sinks=20) for w in (100, 64, 1)]
