@@ -122,8 +122,9 @@ struct Place {
 __device__ __forceinline__ bool window_hides(const CacheAttnParams& p, int key0, int keys, int hidden) { return key0 < hidden && key0 + keys > p.sinks; }
 // ... the bits of those that are hidden from a row of place `place`; drafted tokens are the mask's matter where there is one.
 __device__ __forceinline__ unsigned long long hidden_keys(const CacheAttnParams& p, int length, int place, int key0) {
-  const int begin = length + place - p.window + 1;
-  const int from = max(0, p.sinks - key0), to = (p.mask != nullptr ? min(begin, length) : begin) - key0;
+  const int begin = length + place - p.window + 1, end = p.mask != nullptr ? min(begin, length) : begin;
+  if (end <= key0) return 0ull;            // (first: with a window of 2^31 - 1, end - key0 may be below -2^31)
+  const int from = max(0, p.sinks - key0), to = end - key0;
   if (to <= from || from >= 64) return 0ull;
   return (to >= 64 ? ~0ull : (1ull << to) - 1) & ~((1ull << from) - 1);
 }

@@ -152,6 +152,23 @@ def test_places_without_a_mask_and_out_of_range(places):
     look(cache, q, np.ones((3, 3), bool), [3], window=2, places=np.array(places, np.int32))
 
 
+@pytest.mark.parametrize("dtype, lengths, tokens, head_dim, group", [
+    (F32, [0, 20, 300], 5, 64, 1), (F32, [60], 70, 64, 2), (BF16, [3, 62, 190], 12, 64, 1), (F16, [0, 50], 40, 256, 1), (BF16, [60, 200], 40, 128, 1), (F16, [1, 58, 700], 64, 64, 4),
+    (BF16, [0, 60], 90, 64, 3), (F16, [26, 1], 138, 128, 1)])
+@pytest.mark.parametrize("window", [None, 2**31 - 1, 2**31 - 60])
+def test_masks_that_show_later_tokens_through_windows_that_hide_nothing(dtype, lengths, tokens, head_dim, group, window):
+    """What a mask shows is seen wherever it stands, and how far places are in front of a key is no matter."""
+    cache, q = filled(lengths, [tokens] * len(lengths), dtype=dtype, kv_heads=2, group=group, head_dim=head_dim, page_tokens=8)
+    dice = np.random.default_rng(tokens)
+    mask = dice.random((len(lengths), tokens, tokens)) < 0.2
+    mask[:, 0] = np.arange(tokens) == tokens - 1            # the first sees the last of them only
+    places = None if window is None else np.minimum(dice.integers(0, 4, (len(lengths), tokens)), tokens - 1).astype(np.int32)
+    look(cache, q, mask, None, window=window, places=places)
+    look(cache, q, mask[0], None, window=window, sinks=0 if window is None else 3)
+    if window is not None:
+        look(cache, q, None, None, window=window, places=places)
+
+
 def test_strides_and_types_of_what_a_window_asks_for():
     cache, q = filled([90, 200], [3, 5], dtype=BF16, kv_heads=2, group=2, head_dim=64)
     mask = np.stack([tree(random.Random(b), 5) for b in range(2)])
