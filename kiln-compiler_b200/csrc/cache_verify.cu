@@ -270,8 +270,36 @@ struct Left {
   int64_t draft = 0;                     // the row's first element in p.draft
   int refused = 0, depth = 0;
 };
+// What nearly every row needs: sums over the vocabulary are bounded by the instructions of an exponential, 20 here (10 of float64).  (logit - top) scale is one multiply-add, off by 2^-53 of
+// top scale, for rows where that is 2^12 at most, 5e-13 of a weight; and there is one power of f less than in exp2_wide, 1.2e-12.
+constexpr double kNearTop = 4096.0;
+struct Power {
+  double e;
+  bool any;                              // y >= -1000; if not e is nothing
+};
+__device__ __forceinline__ Power power_of(double y, uint32_t table) {
+  constexpr double kRound = 211106232532992.0;
+  const double t = y + kRound, f = y - (t - kRound);
+  const int n = __double2loint(t);
+  double r = __fma_rn(f, kLn2 * kLn2 * kLn2 * kLn2 / 24.0, kLn2 * kLn2 * kLn2 / 6.0), power;
+  r = __fma_rn(f, r, kLn2 * kLn2 / 2.0);
+  r = __fma_rn(f, r, kLn2);
+  asm("ld.shared.f64 %0, [%1];" : "=d"(power) : "r"(table + ((n & 31) << 3)));
+  r = __fma_rn(power, f * r, power);
+  return Power{__hiloint2double(__double2hiint(r) + ((n & ~31) << 15), __double2loint(r)), (unsigned)__double2hiint(y) <= 0xC08F4000u};
+}
+
+__device__ __forceinline__ bool near_top(const Left& left) { return fabs(left.top * left.scale) <= kNearTop; }
+// A token's weight, by the same steps wherever it is needed: what a draft leaves of one is a difference that is divided by what is left, refusal by refusal, and where a quarter is left each
+// time a weight that is off by 10^-12 of itself is another number after twenty.
+__device__ __forceinline__ double weight_of(const Left& left, double logit) {
+  if (!near_top(left)) return exp2_wide((logit - left.top) * left.scale, left.table);
+  const double shift = -left.top * left.scale;
+  const Power y = power_of(__fma_rn(logit, left.scale, shift), tc::smem_u32(left.table));
+  return y.any ? y.e : 0.0;
+}
 __device__ __forceinline__ double value_of(const VerifyParams& p, const Left& left, int v, float logit) {
-  double r = exp2_wide(((double)logit - left.top) * left.scale, left.table);
+  double r = weight_of(left, (double)logit);
   for (int j = 0; j < left.refused; ++j)
     if (left.out[j] == v) r = 0.0;
   if (left.depth > 0) {
@@ -295,25 +323,6 @@ __device__ __noinline__ Sums sum_any(const VerifyParams& p, const RowOf<T>& row,
       if (v >= 0 && v < row.n) x += value_of(p, left, v, as_float(row.row[v]));
     }
   return Sums{x, 0.0, 0.0, 0.0};
-}
-
-// The forms below are what nearly every call needs.  What bounds them is the instructions of an exponential, 20 (10 of float64), in sum_any 70.  They take (logit - top) scale as one
-// multiply-add, off by 2^-53 of top scale, and are for rows where that is 2^12 at most, 5e-13 of a weight; and one power of f less than exp2_wide, 1.2e-12.
-constexpr double kNearTop = 4096.0;
-struct Power {
-  double e;
-  bool any;                              // y >= -1000; if not e is nothing
-};
-__device__ __forceinline__ Power power_of(double y, uint32_t table) {
-  constexpr double kRound = 211106232532992.0;
-  const double t = y + kRound, f = y - (t - kRound);
-  const int n = __double2loint(t);
-  double r = __fma_rn(f, kLn2 * kLn2 * kLn2 * kLn2 / 24.0, kLn2 * kLn2 * kLn2 / 6.0), power;
-  r = __fma_rn(f, r, kLn2 * kLn2 / 2.0);
-  r = __fma_rn(f, r, kLn2);
-  asm("ld.shared.f64 %0, [%1];" : "=d"(power) : "r"(table + ((n & 31) << 3)));
-  r = __fma_rn(power, f * r, power);
-  return Power{__hiloint2double(__double2hiint(r) + ((n & ~31) << 15), __double2loint(r)), (unsigned)__double2hiint(y) <= 0xC08F4000u};
 }
 
 // A vector's elements, as they lie.
@@ -469,7 +478,6 @@ template <typename T, typename Q>
 __device__ __forceinline__ Sums sum_drafted(const VerifyParams& p, const RowOf<T>& row, const Left& left, int lo, int hi, bool first) {
   return first ? sum_first<T, Q>(p, row, left, lo, hi) : sum_beyond<T, Q>(p, row, left, lo, hi);
 }
-__device__ __forceinline__ bool near_top(const Left& left) { return fabs(left.top * left.scale) <= kNearTop; }
 template <typename T>
 __device__ __forceinline__ Sums sum_of(const VerifyParams& p, const RowOf<T>& row, const Left& left, int lo, int hi, bool first) {
   Sums x;
@@ -571,7 +579,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) verify_walk_kernel(const __gr
     for (int i = threadIdx.x; i < count; i += kWalkThreads)
       if (d.parent[i] >= 0) {
         const int of = d.parent[i];
-        d.weight[i] = exp2_wide((d.weight[i] - (double)d.top[of]) * scale, table);
+        d.weight[i] = weight_of(Left{scale, (double)d.top[of], table}, d.weight[i]);
         d.chance[i] = d.weight[i] / d.sum[of];
       }
   __syncthreads();

@@ -191,6 +191,27 @@ def test_masked_logits(dtype, draft_dtype, vocab, rows, trees, mask):
         check(cache, temperature=None if seed else torch.full((rows,), 0.6, device="cuda"), **given)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_token_that_every_refusal_leaves(dtype):
+    """Of two hundred drafts of one token none is accepted, and each time one token is left, by as much: 1 less the draft's chance of it, of 1.  What it is divided by is what it was, bit by
+    bit, or nothing is left of it in the end."""
+    rows, tokens, vocab = 200, 200, 90
+    cache = cache_of(rows)
+    generator = torch.Generator("cuda").manual_seed(23)
+    logits = torch.randn(rows, 1, vocab, device="cuda", generator=generator)
+    one = torch.randint(vocab, (rows, 1, 1), device="cuda", generator=generator)
+    logits.scatter_(2, one, 14.0 + torch.rand(rows, 1, 1, device="cuda", generator=generator))         # 0.999 and more
+    draft = torch.rand(rows, 1, vocab, device="cuda", generator=generator) + 0.1
+    draft.scatter_(2, one, 0.0)
+    share = torch.linspace(0.03, 0.97, rows, device="cuda")[:, None, None]
+    draft = (draft / draft.sum(-1, keepdim=True) * (1 - share)).scatter(2, one, share)
+    drawn = (one[:, :, 0] + torch.randint(1, vocab, (rows, tokens), device="cuda", generator=generator)) % vocab
+    uniform = 0.5 + torch.rand(rows, tokens, device="cuda", generator=generator) / 2
+    n, _, following = check(cache, logits=logits.to(dtype).expand(rows, tokens, vocab), tokens=drawn.int(), uniform=uniform, draft=draft.expand(rows, tokens, vocab),
+                            parents=ints([-1] + [0] * (tokens - 1)))
+    assert n == [1] * rows and following == one.flatten().tolist()
+
+
 def test_what_is_returned_is_distributed_as_the_models_samples():
     """The first token that a step adds, over 32768 rows each: of a chain, of several drafts of one token, with probabilities of a draft and without.  A count is off by its standard
     deviation sqrt(n p (1 - p)) five times at most (24 counts: one in 70000 would be)."""
