@@ -407,6 +407,33 @@ def test_weights(shape, masked):
     assert torch.equal(apart[:, ::2], fresh) and (apart[:, 1::2] == 0).all()
 
 
+@pytest.mark.parametrize("dtype, head_dim, group, tokens, page_tokens", [(BF16, 128, 4, 200, 64), (F16, 64, 2, 130, 8), (F32, 64, 2, 90, 16), (BF16, 256, 1, 150, 32), (F32, 128, 8, 33, 16)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_weights_of_pieces_of_prompts(dtype, head_dim, group, tokens, page_tokens, masked):
+    """Hundreds of rows to a key head, and masks of more than 64 tokens; the same when they have been accepted."""
+    counts = [tokens, tokens // 2, 1]
+    cache, q = filled([500, 0, 70], counts, dtype=dtype, kv_heads=1, group=group, head_dim=head_dim, page_tokens=page_tokens)
+    mask = np.random.default_rng(tokens).random((3, tokens, tokens)) < 0.3 if masked else None
+    got, lse = weigh(cache, q, mask, counts)
+    cache.accept(ints(counts))
+    given = dict(mask=None if mask is None else torch.from_numpy(mask).cuda(), counts=ints(counts))
+    assert torch.equal(cache.weigh(0, q, lse, committed=True, **given), got) and faults_of(cache) == 0
+
+
+@pytest.mark.parametrize("dtype, group, tokens", [(BF16, 1, 2), (F16, 4, 5), (F32, 2, 1)])
+def test_weights_of_hundreds_of_sequences(dtype, group, tokens):
+    """More than a CTA has threads; by their own numbers, and in any order."""
+    dice = random.Random(tokens)
+    lengths = [dice.choice([1, dice.randint(1, 60)]) for _ in range(600)]
+    counts = [dice.choice([0, tokens, tokens]) for _ in range(600)]
+    cache, q = filled(lengths, counts, dtype=dtype, kv_heads=1, group=group, head_dim=64, page_tokens=8)
+    start = torch.rand(600, cache.max_pages * 8, device="cuda")
+    got, lse = weigh(cache, q, None, counts, weights=start)
+    order = list(range(600))
+    dice.shuffle(order)
+    assert torch.equal(cache.weigh(0, q[order], lse[order], start, counts=ints([counts[s] for s in order]), slots=ints(order)), got) and faults_of(cache) == 0
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 def test_weights_of_rows_that_name_their_sequences(dtype):
     cache, q = filled([100, 5, 300, 41], [3, 3, 3, 3], dtype=dtype, kv_heads=2, group=2, head_dim=64)
