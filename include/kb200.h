@@ -483,7 +483,7 @@ int kb200_cache_weigh(kb200_cache* cache, int layer, const kb200_rows* q, const 
 
 /* Keeps keep[s] of every sequence's committed tokens and drops the others, in all layers: the first `sinks`, of the rest the last `recent`, and of what then lacks the heaviest
  * by weights[s] (of equal ones the first; NaN is heaviest); fewer than the first and last ones where keep[s] is less.  They keep their order and become the sequence's first keep[s]
- * tokens; the pages behind them are free, what was reserved too.  A negative entry, or one of lengths[s] and more, leaves the sequence as it is.
+ * tokens (whose indexes are then no positions in a text: lengths, windows and places count what is left); the pages behind them are free, what was reserved too.  A negative entry, or one of lengths[s] and more, leaves the sequence as it is.
  * out[s]: the weights of the tokens that the sequence then has, zeros behind them.  weights and out: as in kb200_cache_weigh; out may be weights.
  * A sequence whose tokens would move within pages that were shared before the call, or that would keep tokens of pages that it does not have (kb200_cache_release), stays
  * as it is.
@@ -511,7 +511,9 @@ typedef struct kb200_scores {
  * uniform[b, c] * draft[b, a, x] * R < r(x) (without draft: uniform[b, c] * R < r(x)); then it takes a's place.  If not, r becomes max(r / R - draft[b, a], 0) (without: r(x)
  * becomes 0) and R its sum, unless that is 0.  In the end following[s] is the first v at which r, summed up, exceeds uniform[b, 0] times its sum.
  * n_accepted [sequences], accepted [sequences, tokens] (-1 behind): as kb200_cache_accept takes them; sequences without a row, or with counts[b] 0: 0, and -1 in following.
- * Numbers are compared as if computed in float64.  If the logits of an accepted token are no distribution the row ends there, with -1 in following.  tokens: 512 at most.
+ * Numbers are compared as if computed in float64, with probabilities that are off by 4e-12 of themselves at most (below 2^-1000 of a row's largest they are 0) and sums of what a draft leaves by
+ * 1e-10.  (Where a draft leaves no more than such errors, because it is the model itself, the token that follows is one that the model may draw.)  If the logits of an accepted token are
+ * no distribution the row ends there, with -1 in following.  tokens: 512 at most.
  * workspace: kb200_cache_verify_workspace bytes, 16-byte aligned, used by this call alone until it has run. */
 uint64_t kb200_cache_verify_workspace(const kb200_cache* cache, int rows, int tokens, int vocab);
 int kb200_cache_verify(kb200_cache* cache, const kb200_scores* logits, const kb200_scores* draft, int rows, int tokens, int vocab, const int32_t* drafted,

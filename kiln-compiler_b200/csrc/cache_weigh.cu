@@ -463,6 +463,8 @@ Variant variant_of(int head_dim) {
   return head_dim <= 64 ? Variant{weigh_kernel<T, 64>, WeighTile<T, 64>::kKeys, 0} : head_dim <= 128 ? Variant{weigh_kernel<T, 128>, WeighTile<T, 128>::kKeys, 0}
                                                                                                   : Variant{weigh_kernel<T, 256>, WeighTile<T, 256>::kKeys, 0};
 }
+// 16 rows are what a product of weigh_few_kernel has and all that its warps keep.  (32 sequences of up to 8192, heads of 128, four to a key head, BF16: 4 tokens take 48.8 us by it and 80.7 by weigh_kernel; of
+// 8192 each 96 and 167, and there 5 tokens, 20 rows, take 236 by weigh_kernel.)
 Variant variant_for(const Cache& c, int rows) {
   if (rows <= 16 && c.dtype != KB200_DTYPE_FP32) return c.dtype == KB200_DTYPE_BF16 ? few_variant_of<__nv_bfloat16>(c.view.head_dim) : few_variant_of<__half>(c.view.head_dim);
   return c.dtype == KB200_DTYPE_FP32 ? variant_of<float>(c.view.head_dim)

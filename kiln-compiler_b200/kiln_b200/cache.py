@@ -15,7 +15,9 @@ prompt, and the attention of new tokens over them.  One step of a server that dr
 Ordinary decoding drafts one token and accepts it; a prompt is a chain of tokens (no mask) that are all accepted.
 
 A sequence need not keep all of its tokens.  With a sliding window and a few first tokens (``attend(..., window=, sinks=)``) ``release`` gives the pages behind the window
-back; or ``weigh`` adds up what weight its tokens draw (from ``attend(..., lse=)``), and ``evict`` keeps the heaviest.
+back; or ``weigh`` adds up what weight its tokens draw (from ``attend(..., lse=)``), and ``evict`` keeps the heaviest.  The two do not go together: ``weigh`` knows no window
+and misses pages that were released.  After an eviction a token's index in its sequence is no longer its position in the text: ``lengths``, windows, first tokens and
+places count the tokens that are left, and a model whose keys and queries carry positions takes those of new tokens from its caller's own count.
 
 All arguments and all of the cache's state are tensors on the GPU, every call is enqueued on the current stream, and none waits for the GPU: a step can be
 captured into a CUDA graph whose replays follow what the tensors hold then; the cache has to live until the last of them has run.  Calls that change the cache are
@@ -143,12 +145,14 @@ class PagedCache:
         """Adds up what weight the tokens of the sequences draw: ``weights`` [sequences, max_pages * page_tokens] (float32; default: zeros) plus the sum over heads and over the first
         ``counts[b]`` rows of ``q`` of the weights that ``attend`` (without a window) gave them, whose ``lse`` this takes.  Returns ``out``, which may be ``weights``.
         The rows are the tokens drafted behind the committed ones, or, ``committed``, the last of those: what a call of ``accept`` has taken, in its order (of a
-        tree that was drafted, the rows of ``q`` and ``lse`` that ``accepted`` names).  ``slots`` names no sequence twice."""
+        tree that was drafted, the rows of ``q`` and ``lse`` that ``accepted`` names).  ``slots`` names no sequence twice.  Tokens whose page was released draw nothing, and ``status``
+        tells of them."""
         return self._call.cache_weigh(self._caller, layer, q, lse, weights, mask, counts, slots, scale, committed, out)
 
     def evict(self, weights, keep, recent=0, sinks=0, out=None):
         """Keeps ``keep[s]`` committed tokens of every sequence, in all layers: the first ``sinks``, the last ``recent`` and, of the others, the heaviest (of equal ones the
-        first).  They become its first tokens, in their order, and its other pages are free.  A negative entry, or a sequence of no more tokens, changes nothing.
+        first).  They become its first tokens, in their order (their indexes are then no positions in the text), and its other pages are free.  A negative entry, or a sequence of no
+        more tokens, changes nothing.
         Returns ``out`` (which may be ``weights``): the weights of the tokens that are left, zeros behind them."""
         return self._call.cache_evict(self._caller, weights, keep, recent, sinks, out)
 
